@@ -125,6 +125,24 @@ _SIGS = {
 
 EXPORTED = tuple(_SIGS)
 
+# the row operators (include/tace_rows.h), with a version of their own
+ROWS_ABI_VERSION = 1
+_ROW_SIGS = {
+    "tace_rows_abi_version": (_c_int, []),
+    "tace_embed_fwd": (_c_int, [_c_int, _c_int, _vp, _vp, _c_i64, _c_i64, _c_i32, _c_dbl, _vp, _vp]),
+    "tace_embed_grad_work": (_c_i64, [_c_int, _c_i64, _c_i64, _c_i32]),
+    "tace_embed_grad_scans": (_c_int, [_c_i64, _c_i64, _c_i32]),
+    "tace_embed_grad": (_c_int, [_c_int, _c_int, _vp, _vp, _vp, _vp, _c_i64, _c_i64, _c_i32, _c_dbl, _vp, _vp, _c_i64,
+                                 _vp]),
+    "tace_route_place": (_c_int, [_vp, _c_i64, _vp, _vp]),
+    "tace_route_dispatch": (_c_int, [_c_int, _vp, _vp, _vp, _vp, _c_i64, _c_i32, _c_i32, _vp, _vp, _vp]),
+    "tace_route_combine": (_c_int, [_c_int, _vp, _vp, _vp, _vp, _c_i64, _c_i32, _c_i32, _vp, _vp, _vp]),
+    "tace_route_dots": (_c_int, [_c_int, _vp, _vp, _vp, _vp, _vp, _c_i64, _c_i32, _c_i32, _vp, _vp, _vp, _vp]),
+    "tace_dropout": (_c_int, [_c_int, _vp, _vp, _vp, _c_i64, _c_i64, ctypes.c_uint32, _c_i32, _c_i64, _c_i32, _c_i32,
+                              _vp, _vp, _vp]),
+}
+ROWS_EXPORTED = tuple(_ROW_SIGS)
+
 
 class NativeError(RuntimeError):
     pass
@@ -145,7 +163,11 @@ def lib() -> ctypes.CDLL:
                 if got != ABI_VERSION:
                     raise NativeError(f"{LIB_PATH} has ABI version {got}, these bindings are for {ABI_VERSION}; "
                                       "build it again with `python -m tace_amd.build`")
-                for name, (res, args) in _SIGS.items():
+                got = L.tace_rows_abi_version() if hasattr(L, "tace_rows_abi_version") else None
+                if got != ROWS_ABI_VERSION:
+                    raise NativeError(f"{LIB_PATH} has row operators of version {got}, these bindings are for "
+                                      f"{ROWS_ABI_VERSION}; build it again with `python -m tace_amd.build`")
+                for name, (res, args) in (*_SIGS.items(), *_ROW_SIGS.items()):
                     f = getattr(L, name)
                     f.restype = res
                     f.argtypes = args

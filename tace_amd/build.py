@@ -32,6 +32,9 @@ HIP_FLAGS = [
     "-munsafe-fp-atomics", "-Wno-unused-variable", "-Wno-unused-parameter",
 ]
 
+# the row operators (include/tace_rows.h)
+ROW_SRCS = ("rows.hip", "dropout.hip")
+
 
 def generate():
     sys.path.insert(0, ROOT)
@@ -46,6 +49,8 @@ def _compile(src: str, force: bool) -> str:
             os.path.join(CSRC, "scan.h"),
             os.path.join(ROOT, "include", "tace_hip.h")]
     deps += glob.glob(os.path.join(GEN, "*.inc"))
+    if os.path.basename(src) in ROW_SRCS:
+        deps += [os.path.join(CSRC, "row_types.h"), os.path.join(ROOT, "include", "tace_rows.h")]
     if not force and os.path.exists(obj) and os.path.getmtime(obj) >= max(os.path.getmtime(d) for d in deps):
         return obj
     tmp = obj + ".tmp.o"
@@ -60,7 +65,7 @@ def build(verbose: bool = True, force: bool = True, jobs: int = 0) -> str:
     # the longest translation units first
     srcs = [os.path.join(CSRC, n) for n in ("tece_rotin.hip", "tece_rotout.hip", "tece_ace.hip", "linear.hip",
                                             "tace_hip.hip", "tece_score.hip", "tece_wigner.hip", "mlp.hip",
-                                            "so2_gemm.hip", "nodewise.hip", "group.hip")] + generate()
+                                            "so2_gemm.hip", "nodewise.hip", "group.hip", *ROW_SRCS)] + generate()
     os.makedirs(OBJ, exist_ok=True)
     os.makedirs(LIBDIR, exist_ok=True)
     jobs = jobs or min(16, os.cpu_count() or 4)

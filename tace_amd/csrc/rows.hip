@@ -1,0 +1,557 @@
+// Row operators: table lookup by token with its gradient, rows sorted by
+// expert and back.  All of them move rows once and are bound by HBM.
+#include "row_types.h"
+
+#include <type_traits>
+
+namespace {
+
+// ------------------------------------------------------------- embedding ----
+constexpr int WG = 256;
+constexpr int MAX_ROW = 1 << 15;   // elements: RowDiv's range
+
+// Work of a workgroup that goes through `rows * chunks` chunks in order, U per
+// thread: row and chunk of its u-th.
+struct RowChunks {
+  int64_t total;      // rows * chunks
+  RowDiv chunks;      // chunks a row
+
+  template <int U, typename F>
+  __device__ __forceinline__ void each(F&& f) const {
+    const int64_t q0 = (int64_t)blockIdx.x * (WG * U);
+    const int64_t r0 = q0 / chunks.d;
+    const unsigned rem = (unsigned)(q0 - r0 * chunks.d);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const unsigned q = rem + u * WG + threadIdx.x;
+      if (q0 - rem + q < total) {
+        const unsigned r = chunks.div(q);
+        f(u, r0 + r, q - r * chunks.d);
+      }
+    }
+  }
+};
+
+template <typename T, int V, typename I, int U>
+__global__ __launch_bounds__(WG) void k_embed_fwd(const T* __restrict__ table, const I* __restrict__ tokens,
+                                                  RowChunks rc, int64_t vocab, row_sum_t<T> scale,
+                                                  T* __restrict__ out) {
+  typedef row_vec_t<T, V> Vec;
+  const Vec* tab = (const Vec*)table;
+  Vec* o = (Vec*)out;
+  rc.each<U>([&](int, int64_t r, unsigned c) {
+    const I t = tokens[r];
+    row_sum_t<T> a[V];
+    if (t >= 0 && t < (I)vocab) {
+      row_widen<T, V>(tab[(int64_t)t * rc.chunks.d + c], a);
+#pragma unroll
+      for (int i = 0; i < V; ++i) a[i] *= scale;
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i) a[i] = 0;
+    }
+    o[r * rc.chunks.d + c] = row_round<T, V>(a);
+  });
+}
+
+// Sorted positions in pieces of `per`; `cw` lanes hold a piece's row sums.  A
+// token whose rows all lie in one piece is written at once; of another token a
+// piece writes its share into part [piece][2][channels]: slot 0 if the
+// token's rows reach the piece's first position, else slot 1.
+template <typename T, int V, typename I>
+__global__ __launch_bounds__(WG) void k_embed_grad_part(const T* __restrict__ g, const I* __restrict__ tokens,
+                                                        const int* __restrict__ order, const int* __restrict__ rowptr,
+                                                        int vocab, int channels, int per, int pieces, int lanes,
+                                                        row_sum_t<T> scale, T* __restrict__ grad,
+                                                        row_sum_t<T>* __restrict__ part) {
+  typedef row_vec_t<T, V> Vec;
+  typedef row_sum_t<T> S;
+  constexpr int U = 8;
+  const int cw = channels / V, groups = WG / lanes;
+  const int grp = (int)threadIdx.x / lanes, c = (int)threadIdx.x % lanes + (int)blockIdx.y * lanes;
+  const int piece = (int)blockIdx.x * groups + grp;
+  if (grp >= groups || piece >= pieces || c >= cw) return;
+  const int end = rowptr[vocab];   // (padding comes after it)
+  const int64_t first = (int64_t)piece * per;
+  if (first >= end) return;
+  const int p0 = (int)first, p1 = (int)min(first + per, (int64_t)end);
+  const Vec* rows = (const Vec*)g;
+  S sum[V];
+  int cur = -1;
+  auto flush = [&]() {
+    const int b = rowptr[cur], e = rowptr[cur + 1];
+    if (b >= p0 && e <= p1) {
+      S a[V];
+#pragma unroll
+      for (int i = 0; i < V; ++i) a[i] = sum[i] * scale;
+      ((Vec*)grad)[(int64_t)cur * cw + c] = row_round<T, V>(a);
+    } else {
+      S* o = part + ((int64_t)piece * 2 + (b > p0 ? 1 : 0)) * channels + (int64_t)c * V;
+#pragma unroll
+      for (int i = 0; i < V; ++i) o[i] = sum[i];
+    }
+  };
+  for (int p = p0; p < p1; p += U) {
+    int at[U], key[U];
+    Vec v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) at[u] = order[min(p + u, p1 - 1)];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      key[u] = (int)tokens[at[u]];
+      v[u] = rows[(int64_t)at[u] * cw + c];
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (p + u >= p1) break;
+      S a[V];
+      row_widen<T, V>(v[u], a);
+      if (key[u] != cur) {
+        if (cur >= 0) flush();
+        cur = key[u];
+#pragma unroll
+        for (int i = 0; i < V; ++i) sum[i] = a[i];
+      } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) sum[i] += a[i];
+      }
+    }
+  }
+  flush();
+}
+
+// The tokens that no piece wrote: zeros without rows, else the sum of the
+// pieces' shares, 16 of them at a time and then across.
+constexpr int JOIN_COLS = 64, JOIN_ROWS = 4;
+template <typename T>
+__global__ __launch_bounds__(JOIN_COLS * JOIN_ROWS) void k_embed_grad_join(const int* __restrict__ rowptr, int vocab,
+                                                                         int channels, int per, row_sum_t<T> scale,
+                                                                         const row_sum_t<T>* __restrict__ part,
+                                                                         T* __restrict__ grad) {
+  typedef row_sum_t<T> S;
+  __shared__ S red[JOIN_ROWS][JOIN_COLS];
+  const int x = (int)threadIdx.x % JOIN_COLS, y = (int)threadIdx.x / JOIN_COLS;
+  const int c = (int)blockIdx.y * JOIN_COLS + x;
+  for (int v = (int)blockIdx.x; v < vocab; v += (int)gridDim.x) {
+    const int b = rowptr[v], e = rowptr[v + 1];
+    const int c0 = b / per, c1 = (e - 1) / per;
+    if (e > b && c0 == c1) continue;
+    S sum = 0;
+    if (e > b && c < channels) {
+      for (int q = c0 + y; q <= c1; q += JOIN_ROWS)
+        sum += part[((int64_t)q * 2 + (q == c0 && b != c0 * per ? 1 : 0)) * channels + c];
+    }
+    red[y][x] = sum;
+    __syncthreads();
+    if (y == 0 && c < channels) {
+#pragma unroll
+      for (int k = 1; k < JOIN_ROWS; ++k) sum += red[k][x];
+      grad[(int64_t)v * channels + c] = (T)(sum * scale);
+    }
+    __syncthreads();
+  }
+}
+
+// Few rows: a workgroup per token (and tile of columns) lists the token's rows
+// in LDS and sums them; no grouping, one launch.
+constexpr int SCAN_N = 4096;
+template <typename T, int V, typename I>
+__global__ __launch_bounds__(WG) void k_embed_grad_scan(const T* __restrict__ g, const I* __restrict__ tokens, int n,
+                                                        int channels, int lanes, row_sum_t<T> scale,
+                                                        T* __restrict__ grad) {
+  typedef row_vec_t<T, V> Vec;
+  typedef row_sum_t<T> S;
+  __shared__ int list[SCAN_N], found[WG / 64];
+  __shared__ S red[WG * V];
+  const int t = (int)threadIdx.x, lane = t & 63, w = t >> 6;
+  const I v = (I)blockIdx.x;
+  int count = 0;
+  for (int base = 0; base < n; base += WG) {
+    const int i = base + t;
+    const bool hit = i < n && tokens[i] == v;
+    const unsigned long long m = __ballot(hit);
+    if (lane == 0) found[w] = __popcll(m);
+    __syncthreads();
+    int at = count;
+#pragma unroll
+    for (int k = 0; k < WG / 64; ++k) {
+      if (k < w) at += found[k];
+      count += found[k];
+    }
+    if (hit) list[at + __popcll(m & ((1ull << lane) - 1))] = i;
+    __syncthreads();
+  }
+  const int cw = channels / V, groups = WG / lanes, grp = t / lanes, c = t % lanes + (int)blockIdx.y * lanes;
+  S sum[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) sum[i] = 0;
+  if (grp < groups && c < cw) {
+    const Vec* rows = (const Vec*)g;
+#pragma unroll 4
+    for (int k = grp; k < count; k += groups) {
+      S a[V];
+      row_widen<T, V>(rows[(int64_t)list[k] * cw + c], a);
+#pragma unroll
+      for (int i = 0; i < V; ++i) sum[i] += a[i];
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < V; ++i) red[i * WG + t] = sum[i];
+  __syncthreads();
+  if (grp == 0 && c < cw) {
+    for (int k = 1; k < groups; ++k)
+#pragma unroll
+      for (int i = 0; i < V; ++i) sum[i] += red[i * WG + t + k * lanes];
+#pragma unroll
+    for (int i = 0; i < V; ++i) sum[i] *= scale;
+    ((Vec*)grad)[(int64_t)v * cw + c] = row_round<T, V>(sum);
+  }
+}
+
+int embed_lanes(int cw) { return cw < WG ? cw : WG; }
+
+// positions a piece: enough pieces to fill the GPU, few enough that a token
+// with most of the rows is joined quickly
+int embed_per(int64_t n) {
+  const int64_t per = (n + 4095) / 4096;
+  return (int)(per < 32 ? 32 : per);
+}
+
+// --------------------------------------------------------------- routing ----
+// A row's chunks in blocks that lie apart: block b of R rows starts at R *
+// start[b] chunks and holds start[b + 1] - start[b] of each row.
+struct Blocks {
+  int count;
+  unsigned start[TACE_ROW_MAX_BLOCKS + 1];
+
+  __device__ __forceinline__ int64_t at(int64_t rows, int64_t row, unsigned c) const {
+    unsigned lo = 0, hi = start[1];
+#pragma unroll
+    for (int b = 1; b < TACE_ROW_MAX_BLOCKS; ++b)
+      if (b < count && c >= start[b]) {
+        lo = start[b];
+        hi = start[b + 1];
+      }
+    return rows * lo + row * (hi - lo) + (c - lo);
+  }
+};
+
+__global__ __launch_bounds__(WG) void k_route_place(const int* __restrict__ order, int n, int* __restrict__ place) {
+  const int64_t i = (int64_t)blockIdx.x * WG + threadIdx.x;
+  if (i < n) place[order[i]] = (int)i;
+}
+
+template <typename T, int V, int U>
+__global__ __launch_bounds__(WG) void k_route_dispatch(const T* __restrict__ x, const row_sum_t<T>* __restrict__ w,
+                                                       const int* __restrict__ place, const int* __restrict__ rows_end,
+                                                       RowChunks rc, int64_t tokens, int k, Blocks bl,
+                                                       T* __restrict__ out) {
+  typedef row_vec_t<T, V> Vec;
+  typedef row_sum_t<T> S;
+  const int end = *rows_end;
+  const int64_t n = tokens * k;
+  rc.each<U>([&](int, int64_t t, unsigned c) {
+    const Vec v = ((const Vec*)x)[bl.at(tokens, t, c)];
+    for (int j = 0; j < k; ++j) {
+      const int64_t s = t * k + j;
+      const int p = place[s];
+      Vec o = v;
+      if (p >= end || w) {
+        S a[V];
+        row_widen<T, V>(v, a);
+#pragma unroll
+        for (int i = 0; i < V; ++i) a[i] = p >= end ? (S)0 : a[i] * w[s];
+        o = row_round<T, V>(a);
+      }
+      ((Vec*)out)[bl.at(n, p, c)] = o;
+    }
+  });
+}
+
+template <typename T, int V, int U>
+__global__ __launch_bounds__(WG) void k_route_combine(const T* __restrict__ y, const row_sum_t<T>* __restrict__ w,
+                                                      const int* __restrict__ place, const int* __restrict__ rows_end,
+                                                      RowChunks rc, int64_t tokens, int k, Blocks bl,
+                                                      T* __restrict__ out) {
+  typedef row_vec_t<T, V> Vec;
+  typedef row_sum_t<T> S;
+  const int end = *rows_end;
+  const int64_t n = tokens * k;
+  rc.each<U>([&](int, int64_t t, unsigned c) {
+    S sum[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) sum[i] = 0;
+    for (int j = 0; j < k; ++j) {
+      const int64_t s = t * k + j;
+      const int p = place[s];
+      if (p >= end) continue;
+      S a[V];
+      row_widen<T, V>(((const Vec*)y)[bl.at(n, p, c)], a);
+      const S f = w ? w[s] : (S)1;
+#pragma unroll
+      for (int i = 0; i < V; ++i) sum[i] += f * a[i];
+    }
+    ((Vec*)out)[bl.at(tokens, t, c)] = row_round<T, V>(sum);
+  });
+}
+
+// `lanes` (a power of two, at most 64) lanes a token
+template <typename T, int V>
+__global__ __launch_bounds__(WG) void k_route_dots(const T* __restrict__ x, const T* __restrict__ y,
+                                                   const row_sum_t<T>* __restrict__ w, const int* __restrict__ place,
+                                                   const int* __restrict__ rows_end, int64_t tokens, int k, int lanes,
+                                                   unsigned cw, Blocks bl, T* __restrict__ g_y,
+                                                   row_sum_t<T>* __restrict__ dots) {
+  typedef row_vec_t<T, V> Vec;
+  typedef row_sum_t<T> S;
+  const int end = *rows_end, groups = WG / lanes;
+  const int64_t t = (int64_t)blockIdx.x * groups + (int)threadIdx.x / lanes, n = tokens * k;
+  if (t >= tokens) return;   // (whole groups; the shuffles stay inside a group)
+  const int lane = (int)threadIdx.x % lanes;
+  for (int j = 0; j < k; ++j) {
+    const int64_t s = t * k + j;
+    const int p = place[s];
+    const bool kept = p < end;
+    const S f = w ? w[s] : (S)1;
+    S dot = 0;
+    for (unsigned c = lane; c < cw; c += lanes) {
+      S a[V] = {}, b[V];
+      if (kept) {
+        row_widen<T, V>(((const Vec*)x)[bl.at(tokens, t, c)], a);
+        row_widen<T, V>(((const Vec*)y)[bl.at(n, p, c)], b);
+#pragma unroll
+        for (int i = 0; i < V; ++i) dot += a[i] * b[i];
+      }
+      if (g_y) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) a[i] = kept ? f * a[i] : (S)0;
+        ((Vec*)g_y)[bl.at(n, p, c)] = row_round<T, V>(a);
+      }
+    }
+    for (int o = lanes >> 1; o > 0; o >>= 1) dot += __shfl_xor(dot, o, 64);
+    if (lane == 0) dots[s] = dot;
+  }
+}
+
+// (a launch holds less than 2^32 threads)
+constexpr int64_t MAX_GRID = (1 << 24) - 1;
+bool grid_ok(int64_t blocks) { return blocks <= MAX_GRID; }
+
+// the blocks in chunks of V elements; false if a width has a remainder
+bool make_blocks(int32_t blocks, const int64_t* widths, int V, Blocks* bl) {
+  bl->count = blocks;
+  int64_t s = 0;
+  for (int b = 0; b <= TACE_ROW_MAX_BLOCKS; ++b) {
+    bl->start[b] = (unsigned)(s / V);
+    if (b < blocks) {
+      if (widths[b] % V) return false;
+      s += widths[b];
+    }
+  }
+  return true;
+}
+
+const char* route_bad(int type, int64_t tokens, int32_t k, int32_t blocks, const int64_t* widths) {
+  if (type < 0 || type > TACE_ROW_F16) return "tace_route: unknown row type";
+  if (tokens < 0 || k < 1 || tokens > (INT32_MAX - 8192) / k) return "tace_route: bad sizes";
+  if (blocks < 1 || blocks > TACE_ROW_MAX_BLOCKS || !widths) return "tace_route: 1 to 8 blocks";
+  int64_t D = 0;
+  for (int b = 0; b < blocks; ++b) {
+    if (widths[b] < 1 || widths[b] > (1 << 24)) return "tace_route: bad block width";
+    D += widths[b];
+  }
+  if (D > MAX_ROW) return "tace_route: rows of over 32768 elements";
+  return nullptr;
+}
+
+}  // namespace
+
+extern "C" int tace_rows_abi_version(void) { return TACE_ROWS_ABI_VERSION; }
+
+extern "C" int tace_embed_fwd(int type, int index_bytes, const void* table, const void* tokens, int64_t n,
+                              int64_t vocab, int32_t channels, double scale, void* out, void* stream) {
+  if (n < 0 || vocab < 0 || vocab > INT32_MAX || channels < 1 || channels > MAX_ROW)
+    return tace_fail_msg("tace_embed_fwd: bad sizes");
+  if (index_bytes != 4 && index_bytes != 8) return tace_fail_msg("tace_embed_fwd: indices of 4 or 8 bytes");
+  if (n == 0) return 0;
+  if ((vocab && !table) || !tokens || !out) return tace_fail_msg("tace_embed_fwd: null pointer");
+  bool fits = true;
+  const bool known = row_dispatch(type, [&](auto z) {
+    typedef decltype(z) T;
+    constexpr int W = 16 / sizeof(T), U = 4;
+    const bool vec = channels % W == 0 && row_aligned(table) && row_aligned(out);
+    const RowChunks rc{n * (channels / (vec ? W : 1)), row_div((unsigned)(channels / (vec ? W : 1)))};
+    const int64_t grid = (rc.total + WG * U - 1) / (WG * U);
+    fits = grid_ok(grid);
+    if (!fits) return;
+    auto go = [&](auto i) {
+      typedef decltype(i) I;
+      if (vec)
+        hipLaunchKernelGGL((k_embed_fwd<T, W, I, U>), dim3((unsigned)grid), dim3(WG), 0, (hipStream_t)stream,
+                           (const T*)table, (const I*)tokens, rc, vocab, (row_sum_t<T>)scale, (T*)out);
+      else
+        hipLaunchKernelGGL((k_embed_fwd<T, 1, I, U>), dim3((unsigned)grid), dim3(WG), 0, (hipStream_t)stream,
+                           (const T*)table, (const I*)tokens, rc, vocab, (row_sum_t<T>)scale, (T*)out);
+    };
+    if (index_bytes == 4) go(int32_t());
+    else go(int64_t());
+  });
+  if (!known) return tace_fail_msg("tace_embed_fwd: unknown row type");
+  if (!fits) return tace_fail_msg("tace_embed_fwd: too many rows");
+  return tace_check_launch("tace_embed_fwd");
+}
+
+extern "C" int tace_embed_grad_scans(int64_t n, int64_t vocab, int32_t channels) {
+  (void)channels;
+  return n <= SCAN_N && vocab <= 1024 ? 1 : 0;
+}
+
+extern "C" int64_t tace_embed_grad_work(int type, int64_t n, int64_t vocab, int32_t channels) {
+  (void)vocab;
+  if (n < 1) return 16;
+  const int64_t pieces = (n + embed_per(n) - 1) / embed_per(n);
+  return pieces * 2 * channels * (type == TACE_ROW_F64 ? 8 : 4);
+}
+
+extern "C" int tace_embed_grad(int type, int index_bytes, const void* g, const void* tokens, const int32_t* order,
+                               const int32_t* rowptr, int64_t n, int64_t vocab, int32_t channels, double scale,
+                               void* grad, void* work, int64_t work_bytes, void* stream) {
+  if (n < 0 || vocab < 0 || n > INT32_MAX - 8192 || vocab > INT32_MAX - 8192 || channels < 1 || channels > MAX_ROW)
+    return tace_fail_msg("tace_embed_grad: bad sizes");
+  if (index_bytes != 4 && index_bytes != 8) return tace_fail_msg("tace_embed_grad: indices of 4 or 8 bytes");
+  if (type < 0 || type > TACE_ROW_F16) return tace_fail_msg("tace_embed_grad: unknown row type");
+  if (vocab == 0) return 0;
+  const bool scans = order == nullptr;
+  if (!grad || (n && (!g || !tokens))) return tace_fail_msg("tace_embed_grad: null pointer");
+  if (scans) {
+    if (!tace_embed_grad_scans(n, vocab, channels))
+      return tace_fail_msg("tace_embed_grad: too many rows or tokens without a grouping");
+  } else {
+    if (!rowptr || (n && !work)) return tace_fail_msg("tace_embed_grad: null pointer");
+    if (n && (work_bytes < tace_embed_grad_work(type, n, vocab, channels) || !row_aligned(work)))
+      return tace_fail_msg("tace_embed_grad: workspace too small or not 16-byte aligned");
+  }
+  row_dispatch(type, [&](auto z) {
+    typedef decltype(z) T;
+    typedef row_sum_t<T> S;
+    constexpr int W = 16 / sizeof(T);
+    const bool vec = channels % W == 0 && row_aligned(g) && row_aligned(grad);
+    const int cw = vec ? channels / W : channels, lanes = embed_lanes(cw), tiles = (cw + lanes - 1) / lanes;
+    hipStream_t s = (hipStream_t)stream;
+    const int per = embed_per(n), pieces = (int)((n + per - 1) / per), groups = WG / lanes;
+    auto go = [&](auto i) {
+      typedef decltype(i) I;
+      auto run = [&](auto vc) {
+        constexpr int V = decltype(vc)::value;
+        if (scans)
+          hipLaunchKernelGGL((k_embed_grad_scan<T, V, I>), dim3((unsigned)vocab, (unsigned)tiles), dim3(WG), 0, s,
+                             (const T*)g, (const I*)tokens, (int)n, channels, lanes, (S)scale, (T*)grad);
+        else if (n)
+          hipLaunchKernelGGL((k_embed_grad_part<T, V, I>), dim3((unsigned)((pieces + groups - 1) / groups), tiles),
+                             dim3(WG), 0, s, (const T*)g, (const I*)tokens, order, rowptr, (int)vocab, channels, per,
+                             pieces, lanes, (S)scale, (T*)grad, (S*)work);
+      };
+      if (vec) run(std::integral_constant<int, W>());
+      else run(std::integral_constant<int, 1>());
+    };
+    if (index_bytes == 4) go(int32_t());
+    else go(int64_t());
+    if (!scans)
+      hipLaunchKernelGGL((k_embed_grad_join<T>),
+                         dim3((unsigned)(vocab < 65536 ? vocab : 65536), (unsigned)((channels + JOIN_COLS - 1) / JOIN_COLS)),
+                         dim3(JOIN_COLS * JOIN_ROWS), 0, s, rowptr, (int)vocab, channels, per, (S)scale, (const S*)work,
+                         (T*)grad);
+  });
+  return tace_check_launch("tace_embed_grad");
+}
+
+extern "C" int tace_route_place(const int32_t* order, int64_t n, int32_t* place, void* stream) {
+  if (n < 0 || n > INT32_MAX - 8192) return tace_fail_msg("tace_route_place: bad sizes");
+  if (n == 0) return 0;
+  if (!order || !place) return tace_fail_msg("tace_route_place: null pointer");
+  hipLaunchKernelGGL(k_route_place, dim3((unsigned)((n + WG - 1) / WG)), dim3(WG), 0, (hipStream_t)stream, order,
+                     (int)n, place);
+  return tace_check_launch("tace_route_place");
+}
+
+namespace {
+
+// f(row type, elements a chunk, blocks in chunks, chunks a row)
+template <typename F>
+void route_go(int type, int32_t blocks, const int64_t* widths, bool aligned, F&& f) {
+  row_dispatch(type, [&](auto z) {
+    typedef decltype(z) T;
+    constexpr int W = 16 / sizeof(T);
+    Blocks bl;
+    if (aligned && make_blocks(blocks, widths, W, &bl)) {
+      f(z, std::integral_constant<int, W>(), bl, bl.start[blocks]);
+    } else {
+      make_blocks(blocks, widths, 1, &bl);
+      f(z, std::integral_constant<int, 1>(), bl, bl.start[blocks]);
+    }
+  });
+}
+
+}  // namespace
+
+extern "C" int tace_route_dispatch(int type, const void* x, const void* weights, const int32_t* place,
+                                   const int32_t* rows_end, int64_t tokens, int32_t k, int32_t blocks,
+                                   const int64_t* widths, void* out, void* stream) {
+  if (const char* bad = route_bad(type, tokens, k, blocks, widths)) return tace_fail_msg(bad);
+  if (tokens == 0) return 0;
+  if (!x || !place || !rows_end || !out) return tace_fail_msg("tace_route_dispatch: null pointer");
+  bool fits = true;
+  route_go(type, blocks, widths, row_aligned(x) && row_aligned(out), [&](auto z, auto vc, const Blocks& bl, unsigned cw) {
+    typedef decltype(z) T;
+    constexpr int V = decltype(vc)::value, U = 2;
+    const RowChunks rc{tokens * cw, row_div(cw)};
+    const int64_t grid = (rc.total + WG * U - 1) / (WG * U);
+    fits = grid_ok(grid);
+    if (fits)
+      hipLaunchKernelGGL((k_route_dispatch<T, V, U>), dim3((unsigned)grid), dim3(WG), 0, (hipStream_t)stream,
+                         (const T*)x, (const row_sum_t<T>*)weights, place, rows_end, rc, tokens, k, bl, (T*)out);
+  });
+  if (!fits) return tace_fail_msg("tace_route_dispatch: too many rows");
+  return tace_check_launch("tace_route_dispatch");
+}
+
+extern "C" int tace_route_combine(int type, const void* y, const void* weights, const int32_t* place,
+                                  const int32_t* rows_end, int64_t tokens, int32_t k, int32_t blocks,
+                                  const int64_t* widths, void* out, void* stream) {
+  if (const char* bad = route_bad(type, tokens, k, blocks, widths)) return tace_fail_msg(bad);
+  if (tokens == 0) return 0;
+  if (!y || !place || !rows_end || !out) return tace_fail_msg("tace_route_combine: null pointer");
+  bool fits = true;
+  route_go(type, blocks, widths, row_aligned(y) && row_aligned(out), [&](auto z, auto vc, const Blocks& bl, unsigned cw) {
+    typedef decltype(z) T;
+    constexpr int V = decltype(vc)::value, U = 2;
+    const RowChunks rc{tokens * cw, row_div(cw)};
+    const int64_t grid = (rc.total + WG * U - 1) / (WG * U);
+    fits = grid_ok(grid);
+    if (fits)
+      hipLaunchKernelGGL((k_route_combine<T, V, U>), dim3((unsigned)grid), dim3(WG), 0, (hipStream_t)stream,
+                         (const T*)y, (const row_sum_t<T>*)weights, place, rows_end, rc, tokens, k, bl, (T*)out);
+  });
+  if (!fits) return tace_fail_msg("tace_route_combine: too many rows");
+  return tace_check_launch("tace_route_combine");
+}
+
+extern "C" int tace_route_dots(int type, const void* x, const void* y, const void* weights, const int32_t* place,
+                               const int32_t* rows_end, int64_t tokens, int32_t k, int32_t blocks,
+                               const int64_t* widths, void* g_y, void* dots, void* stream) {
+  if (const char* bad = route_bad(type, tokens, k, blocks, widths)) return tace_fail_msg(bad);
+  if (tokens == 0) return 0;
+  if (!x || !y || !place || !rows_end || !dots) return tace_fail_msg("tace_route_dots: null pointer");
+  route_go(type, blocks, widths, row_aligned(x) && row_aligned(y) && (!g_y || row_aligned(g_y)),
+           [&](auto z, auto vc, const Blocks& bl, unsigned cw) {
+             typedef decltype(z) T;
+             constexpr int V = decltype(vc)::value;
+             int lanes = 1;
+             while (lanes < 64 && (unsigned)lanes < cw) lanes *= 2;
+             const int groups = WG / lanes;
+             hipLaunchKernelGGL((k_route_dots<T, V>), dim3((unsigned)((tokens + groups - 1) / groups)), dim3(WG), 0,
+                                (hipStream_t)stream, (const T*)x, (const T*)y, (const row_sum_t<T>*)weights, place,
+                                rows_end, tokens, k, lanes, cw, bl, (T*)g_y, (row_sum_t<T>*)dots);
+           });
+  return tace_check_launch("tace_route_dots");
+}
