@@ -175,6 +175,36 @@ def lib() -> ctypes.CDLL:
     return _lib
 
 
+_rows_mod = None
+
+
+def rows():
+    """The row operators on torch tensors (``_lib/_rows.so``), loaded once."""
+    global _rows_mod
+    if _rows_mod is None:
+        lib()   # (checks the versions)
+        import importlib.machinery
+        import importlib.util
+
+        import torch  # noqa: F401  (its libraries first)
+
+        path = os.path.join(_HERE, "_lib", "_rows.so")
+        if not os.path.exists(path):
+            raise NativeError(f"_rows.so not found at {path}; build it with `python -m tace_amd.build`")
+        loader = importlib.machinery.ExtensionFileLoader("_rows", path)
+        mod = importlib.util.module_from_spec(importlib.util.spec_from_loader("_rows", loader))
+        loader.exec_module(mod)
+        if mod.abi_version() != ROWS_ABI_VERSION:
+            raise NativeError(f"{path} has row operators of version {mod.abi_version()}, these bindings are for "
+                              f"{ROWS_ABI_VERSION}; build it again with `python -m tace_amd.build`")
+        with _lock:
+            if _rows_mod is None:
+                from . import ops
+                mod.timer(ops._t0, ops._t1)
+                _rows_mod = mod
+    return _rows_mod
+
+
 def check(rc: int, what: str = "") -> None:
     if rc != 0:
         msg = lib().tace_last_error()

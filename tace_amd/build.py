@@ -3,7 +3,8 @@
 ``python -m tace_amd.build`` (or ``__graft_entry__.build()``) regenerates the
 tensor-product kernels from ``csrc/codegen.py`` (one translation unit per
 variant), compiles every translation unit with hipcc in parallel and links
-``tace_amd/_lib/libtace_hip.so``.  Packed-FP32 VALU instructions are disabled
+``tace_amd/_lib/libtace_hip.so``, and beside it ``_rows.so``, the row operators
+on torch tensors (host C++).  Packed-FP32 VALU instructions are disabled
 for every HIP translation unit.  Objects whose source and headers are older
 than the object are reused unless ``force=True``.
 """
@@ -60,6 +61,31 @@ def _compile(src: str, force: bool) -> str:
     return obj
 
 
+ROWS_LIB = os.path.join(LIBDIR, "_rows.so")
+
+
+def _build_rows(force: bool) -> None:
+    """The row operators' torch binding (host code only), linked to the library beside it."""
+    import sysconfig
+
+    import torch
+
+    src = os.path.join(CSRC, "rows_torch.cpp")
+    deps = [src] + [os.path.join(ROOT, "include", h) for h in ("tace_hip.h", "tace_rows.h")]
+    if not force and os.path.exists(ROWS_LIB) and os.path.getmtime(ROWS_LIB) >= max(os.path.getmtime(d) for d in deps):
+        return
+    top = os.path.dirname(torch.__file__)
+    inc = [os.path.join(top, "include"), os.path.join(top, "include", "torch", "csrc", "api", "include"),
+           sysconfig.get_paths()["include"], os.path.join(os.path.dirname(os.path.dirname(HIPCC)), "include")]
+    tmp = ROWS_LIB + ".tmp"
+    subprocess.run([os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-D__HIP_PLATFORM_AMD__",
+                    f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *("-I" + d for d in inc), src,
+                    "-o", tmp, "-L" + LIBDIR, "-ltace_hip", "-L" + os.path.join(top, "lib"), "-lc10", "-lc10_hip",
+                    "-ltorch_cpu", "-ltorch_python", "-Wl,-rpath,$ORIGIN"], check=True, stdout=subprocess.PIPE,
+                   stderr=subprocess.STDOUT)
+    os.replace(tmp, ROWS_LIB)
+
+
 def build(verbose: bool = True, force: bool = True, jobs: int = 0) -> str:
     t0 = time.time()
     # the longest translation units first
@@ -84,6 +110,11 @@ def build(verbose: bool = True, force: bool = True, jobs: int = 0) -> str:
     tmp = LIB + ".tmp"
     subprocess.check_call([HIPCC, "--offload-arch=gfx950", "-shared", "-fPIC", *objs, "-o", tmp])
     os.replace(tmp, LIB)
+    try:
+        _build_rows(force)
+    except subprocess.CalledProcessError as e:
+        sys.stderr.write(e.stdout.decode(errors="replace"))
+        raise
     if verbose:
         print(f"[tace_amd.build] {LIB} in {time.time() - t0:.1f}s", flush=True)
     return LIB

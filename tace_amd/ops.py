@@ -1500,129 +1500,21 @@ def sender_csr(rows_src: torch.Tensor, n_rows: int) -> Tuple[torch.Tensor, torch
 
 
 # -------------------------------------------------------- rows of atoms ----
-# Lookups, routed rows and dropout (include/tace_rows.h): float64, float32,
+# Lookups, routed rows and dropout (csrc/rows_torch.cpp): float64, float32,
 # bfloat16 and float16 rows, sums in float64 for float64 rows and in float32
 # for the others.  Every backward is made of the same operators, so each can be
 # differentiated any number of times.
-_ROW_TYPES = {torch.float32: 0, torch.float64: 1, torch.bfloat16: 2, torch.float16: 3}
-_ROW_MAX = 32768       # elements a row
-_ROW_BLOCKS = 8
-
-
-def _row_code(t: torch.Tensor, name: str) -> int:
-    if not isinstance(t, torch.Tensor) or not t.is_cuda:
-        raise ValueError(f"{name} must be a GPU tensor (got {getattr(t, 'device', type(t).__name__)})")
-    code = _ROW_TYPES.get(t.dtype)
-    if code is None:
-        raise ValueError(f"{name} has dtype {t.dtype}, expected float32, float64, bfloat16 or float16")
-    return code
-
-
-def _same_device(a: torch.Tensor, b: torch.Tensor, name: str):
-    if b.device != a.device:
-        raise ValueError(f"{name} is on {b.device}, expected {a.device}")
-
-
-def _indices(t: torch.Tensor, name: str):
-    if t.dtype not in (torch.int32, torch.int64):
-        raise ValueError(f"{name} has dtype {t.dtype}, expected int32 or int64")
-
-
-def _on(t: torch.Tensor):
-    """The tensor's device as the current one, for the launches on it."""
-    if torch.cuda.current_device() == t.device.index:
-        return contextlib.nullcontext()
-    return torch.cuda.device(t.device)
-
-
-def _sum_dtype(dt) -> torch.dtype:
-    return torch.float64 if dt == torch.float64 else torch.float32
-
-
-def _embed_fwd(table, tokens, scale: float) -> torch.Tensor:
-    V, C = table.shape
-    out = torch.empty(tokens.shape[0], C, dtype=table.dtype, device=table.device)
-    with _on(table):
-        tok = _t0("embed_fwd")
-        N.check(N.lib().tace_embed_fwd(_ROW_TYPES[table.dtype], tokens.element_size(), table.data_ptr(),
-                                       tokens.data_ptr(), tokens.shape[0], V, C, scale, out.data_ptr(),
-                                       N.stream_ptr(table.device)), "tace_embed_fwd")
-        _t1(tok, (tokens.shape[0], C))
-    return out
-
-
-def _embed_grad(g, tokens, V: int, scale: float, groups) -> torch.Tensor:
-    n, C = g.shape
-    if n == 0:
-        return torch.zeros(V, C, dtype=g.dtype, device=g.device)
-    L = N.lib()
-    code = _ROW_TYPES[g.dtype]
-    grad = torch.empty(V, C, dtype=g.dtype, device=g.device)
-    with _on(g):
-        rowptr = order = work = None
-        nbytes = 0
-        if not L.tace_embed_grad_scans(n, V, C):
-            rowptr, order = groups if groups is not None else group_by_key(tokens, V)
-            nbytes = L.tace_embed_grad_work(code, n, V, C)
-            work = torch.empty(nbytes, dtype=torch.uint8, device=g.device)
-        tok = _t0("embed_grad")
-        N.check(L.tace_embed_grad(code, tokens.element_size(), g.data_ptr(), tokens.data_ptr(), N.ptr(order),
-                                  N.ptr(rowptr), n, V, C, scale, grad.data_ptr(), N.ptr(work), nbytes,
-                                  N.stream_ptr(g.device)), "tace_embed_grad")
-        _t1(tok, (n, V, C))
-    return grad
-
-
-class _Embedding(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, table, tokens, scale: float, groups):
-        ctx.save_for_backward(tokens)
-        ctx.args = (table.shape[0], scale, groups)
-        return _embed_fwd(table, tokens, scale)
-
-    @staticmethod
-    def backward(ctx, g):
-        (tokens,) = ctx.saved_tensors
-        return _EmbeddingGrad.apply(g.contiguous(), tokens, *ctx.args), None, None, None
-
-
-class _EmbeddingGrad(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, g, tokens, V: int, scale: float, groups):
-        ctx.save_for_backward(tokens)
-        ctx.args = (scale, groups)
-        return _embed_grad(g, tokens, V, scale, groups)
-
-    @staticmethod
-    def backward(ctx, gg):
-        (tokens,) = ctx.saved_tensors
-        return _Embedding.apply(gg.contiguous(), tokens, *ctx.args), None, None, None, None
-
-
 def embedding(table: torch.Tensor, tokens: torch.Tensor, scale: float = 1.0,
               groups: Optional[Tuple[torch.Tensor, torch.Tensor]] = None) -> torch.Tensor:
     """``scale * table[tokens]``: rows of ``table`` [V, C] for integer
     ``tokens`` of any shape.  A token outside [0, V) (padding) gives a row of
     zeros and takes no gradient.  The table's gradient sums each token's rows in
     an order that depends on the sizes alone (the same bits on every run) and
-    rounds once.  ``groups``: ``group_by_key(tokens, V)`` where the caller has
-    it already (several lookups of the same tokens); made when needed otherwise.
-    Differentiable any number of times."""
-    _row_code(table, "table")
-    if table.dim() != 2 or not 1 <= table.shape[1] <= _ROW_MAX:
-        raise ValueError(f"table has shape {tuple(table.shape)}, expected [V, C] with C of 1 to {_ROW_MAX}")
-    _indices(tokens, "tokens")
-    _same_device(table, tokens, "tokens")
-    n, V = tokens.numel(), table.shape[0]
-    if max(n, V) >= 2 ** 31 - 8192:
-        raise ValueError("embedding: tokens or table rows exceed 32-bit indices")
-    if groups is not None:
-        _req(groups[0], "groups[0] (rowptr)", torch.int32, (V + 1,))
-        _req(groups[1], "groups[1] (order)", torch.int32, (n,))
-        _same_device(table, groups[0], "groups[0] (rowptr)")
-        _same_device(table, groups[1], "groups[1] (order)")
-    out = _Embedding.apply(table.contiguous(), tokens.reshape(-1).contiguous(), float(scale), groups)
-    return out.view(*tokens.shape, table.shape[1])
+    rounds once.  ``groups``: ``group_by_key(tokens.reshape(-1), V)`` where the
+    caller has it already (several lookups of the same tokens); made when needed
+    otherwise.  Differentiable any number of times."""
+    rowptr, order = (None, None) if groups is None else groups
+    return N.rows().embedding(table, tokens, scale, rowptr, order, TIMER is not None)
 
 
 class RoutePlan:
@@ -1631,10 +1523,15 @@ class RoutePlan:
     expert, the dropped ones last; ``place`` (int32 [n]) the sorted row of each
     slot; ``rowptr`` (int32 [n_experts + 1]) each expert's range of rows."""
 
-    def __init__(self, n_tokens: int, k: int, n_experts: int, rowptr, order, place):
-        self.n_tokens, self.k, self.n_experts = n_tokens, k, n_experts
-        self.rowptr, self.order, self.place = rowptr, order, place
+    __slots__ = ("rowptr", "order", "place", "n_tokens", "k", "_ranges")
+
+    def __init__(self, rowptr, order, place, n_tokens: int, k: int):
+        self.rowptr, self.order, self.place, self.n_tokens, self.k = rowptr, order, place, n_tokens, k
         self._ranges = None
+
+    @property
+    def n_experts(self) -> int:
+        return self.rowptr.shape[0] - 1
 
     @property
     def n_rows(self) -> int:
@@ -1663,134 +1560,7 @@ def route_plan(experts: torch.Tensor, n_experts: int) -> RoutePlan:
     """Tokens sorted by expert.  ``experts`` [T] or [T, k] (int32 or int64): the
     experts of each token; a choice outside [0, n_experts) is dropped.  No host
     synchronisation."""
-    if not experts.is_cuda:
-        raise ValueError(f"experts must be a GPU tensor (got {experts.device})")
-    _indices(experts, "experts")
-    if experts.dim() not in (1, 2) or (experts.dim() == 2 and experts.shape[1] < 1):
-        raise ValueError(f"experts has shape {tuple(experts.shape)}, expected [T] or [T, k]")
-    T, k = experts.shape[0], 1 if experts.dim() == 1 else experts.shape[1]
-    n = T * k
-    if n_experts < 0 or max(n, n_experts) >= 2 ** 31 - 8192:
-        raise ValueError("route_plan: slots or experts exceed 32-bit indices")
-    flat = experts.reshape(-1)
-    with _on(experts):
-        _, rowptr, order, _ = _group_keys(flat, n_experts)
-        place = torch.empty(n, dtype=torch.int32, device=experts.device)
-        N.check(N.lib().tace_route_place(order.data_ptr(), n, place.data_ptr(), N.stream_ptr(experts.device)),
-                "tace_route_place")
-    return RoutePlan(T, k, n_experts, rowptr, order, place)
-
-
-def _route_args(plan: RoutePlan, widths, weights):
-    """The arguments all routing entries share, from place on."""
-    w = np.asarray(widths, dtype=np.int64)
-    return (plan.place.data_ptr(), plan.rowptr.data_ptr() + 4 * plan.n_experts, plan.n_tokens, plan.k, len(w),
-            w.ctypes.data), w
-
-
-def _route_call(name: str, x, weights, plan: RoutePlan, widths, rows: int) -> torch.Tensor:
-    out = torch.empty(rows, x.shape[1], dtype=x.dtype, device=x.device)
-    args, keep = _route_args(plan, widths, weights)
-    with _on(x):
-        tok = _t0(name)
-        N.check(getattr(N.lib(), "tace_" + name)(_ROW_TYPES[x.dtype], x.data_ptr(), N.ptr(weights), *args,
-                                                 out.data_ptr(), N.stream_ptr(x.device)), "tace_" + name)
-        _t1(tok, (plan.n_tokens, plan.k, x.shape[1]))
-    return out
-
-
-def _route_dots(x, y, weights, plan: RoutePlan, widths, want_gy: bool):
-    """(weights[s] x rows at place[s] or None, <x row, y row> per slot [T, k])."""
-    gy = torch.empty_like(y) if want_gy else None
-    dots = torch.empty(plan.n_tokens, plan.k, dtype=_sum_dtype(x.dtype), device=x.device)
-    args, keep = _route_args(plan, widths, weights)
-    with _on(x):
-        tok = _t0("route_dots")
-        N.check(N.lib().tace_route_dots(_ROW_TYPES[x.dtype], x.data_ptr(), y.data_ptr(), N.ptr(weights), *args,
-                                        N.ptr(gy), dots.data_ptr(), N.stream_ptr(x.device)), "tace_route_dots")
-        _t1(tok, (plan.n_tokens, plan.k, x.shape[1]))
-    return gy, dots
-
-
-class _Dispatch(torch.autograd.Function):
-    """xs[place[s]] = w_s x[t(s)]."""
-
-    @staticmethod
-    def forward(ctx, x, weights, plan, widths):
-        # (x only for the weights' gradient)
-        ctx.save_for_backward(x if weights is not None else None, weights)
-        ctx.plan, ctx.widths = plan, widths
-        return _route_call("route_dispatch", x, weights, plan, widths, plan.n_rows)
-
-    @staticmethod
-    def backward(ctx, g):
-        x, w = ctx.saved_tensors
-        g = g.contiguous()
-        gx = _Combine.apply(g, w, ctx.plan, ctx.widths) if ctx.needs_input_grad[0] else None
-        gw = _RowDots.apply(x, g, ctx.plan, ctx.widths) if ctx.needs_input_grad[1] else None
-        return gx, gw, None, None
-
-
-class _Combine(torch.autograd.Function):
-    """out[t] = sum over t's kept slots of w_s y[place[s]]."""
-
-    @staticmethod
-    def forward(ctx, y, weights, plan, widths):
-        ctx.save_for_backward(y if weights is not None else None, weights)
-        ctx.plan, ctx.widths = plan, widths
-        return _route_call("route_combine", y, weights, plan, widths, plan.n_tokens)
-
-    @staticmethod
-    def backward(ctx, g):
-        y, w = ctx.saved_tensors
-        g = g.contiguous()
-        need_y, need_w = ctx.needs_input_grad[:2]
-        if need_w and not torch.is_grad_enabled():   # both gradients in one pass
-            return (*_route_dots(g, y, w, ctx.plan, ctx.widths, need_y), None, None)
-        gy = _Dispatch.apply(g, w, ctx.plan, ctx.widths) if need_y else None
-        gw = _RowDots.apply(g, y, ctx.plan, ctx.widths) if need_w else None
-        return gy, gw, None, None
-
-
-class _RowDots(torch.autograd.Function):
-    """d[t, j] = <x[t], y[place[t k + j]]>, 0 for a dropped slot."""
-
-    @staticmethod
-    def forward(ctx, x, y, plan, widths):
-        ctx.save_for_backward(x, y)
-        ctx.plan, ctx.widths = plan, widths
-        return _route_dots(x, y, None, plan, widths, False)[1]
-
-    @staticmethod
-    def backward(ctx, g):
-        x, y = ctx.saved_tensors
-        g = g.contiguous()
-        gx = _Combine.apply(y, g, ctx.plan, ctx.widths) if ctx.needs_input_grad[0] else None
-        gy = _Dispatch.apply(x, g, ctx.plan, ctx.widths) if ctx.needs_input_grad[1] else None
-        return gx, gy, None, None
-
-
-def _routed(x, plan: RoutePlan, weights, widths, name: str):
-    """Checked (rows, weights in the sums' type, plan, block widths) of token
-    rows "x" or experts' rows "y"."""
-    _row_code(x, name)
-    if not isinstance(plan, RoutePlan):
-        raise ValueError("plan must be a RoutePlan (route_plan)")
-    rows = plan.n_tokens if name == "x" else plan.n_rows
-    if x.dim() != 2 or x.shape[0] != rows or not 1 <= x.shape[1] <= _ROW_MAX:
-        raise ValueError(f"{name} has shape {tuple(x.shape)}, expected [{rows}, D] with D of 1 to {_ROW_MAX}")
-    _same_device(plan.place, x, name)
-    widths = (x.shape[1],) if widths is None else tuple(int(w) for w in widths)
-    if not 1 <= len(widths) <= _ROW_BLOCKS or min(widths) < 1 or sum(widths) != x.shape[1]:
-        raise ValueError(f"widths {widths} are not 1 to {_ROW_BLOCKS} blocks of {x.shape[1]} elements")
-    if weights is not None:
-        if not weights.is_floating_point() or tuple(weights.shape) not in {
-                (plan.n_tokens, plan.k), (plan.n_tokens,) if plan.k == 1 else None}:
-            raise ValueError(f"weights must be floating point [{plan.n_tokens}, {plan.k}], got {weights.dtype} "
-                             f"{tuple(weights.shape)}")
-        _same_device(x, weights, "weights")
-        weights = weights.reshape(plan.n_tokens, plan.k).to(_sum_dtype(x.dtype)).contiguous()
-    return x.contiguous(), weights, plan, widths
+    return RoutePlan(*N.rows().route_plan(experts, n_experts))
 
 
 def expert_dispatch(x: torch.Tensor, plan: RoutePlan, weights: Optional[torch.Tensor] = None,
@@ -1801,7 +1571,7 @@ def expert_dispatch(x: torch.Tensor, plan: RoutePlan, weights: Optional[torch.Te
     (``model.GMLayout``), the element counts of their blocks, each of which
     lies in memory as [rows, width] after the one before; None: ordinary rows.
     Differentiable any number of times in x and weights."""
-    return _Dispatch.apply(*_routed(x, plan, weights, widths, "x"))
+    return N.rows().route(False, x, plan.place, plan.rowptr, plan.n_tokens, plan.k, weights, widths, TIMER is not None)
 
 
 def expert_combine(y: torch.Tensor, plan: RoutePlan, weights: Optional[torch.Tensor] = None,
@@ -1811,30 +1581,7 @@ def expert_combine(y: torch.Tensor, plan: RoutePlan, weights: Optional[torch.Ten
     ``plan.place[s]``, in slot order; zeros for a token without kept slots,
     whatever the rows behind ``plan.rowptr[-1]`` hold.  ``widths`` as in
     ``expert_dispatch``.  Differentiable any number of times in y and weights."""
-    return _Combine.apply(*_routed(y, plan, weights, widths, "y"))
-
-
-class _Dropout(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, residual, state, seed: int, offset: int, site: int, threshold: int, channels: int, comps):
-        ctx.save_for_backward(state)
-        ctx.args = (seed, offset, site, threshold, channels, comps)
-        out = torch.empty_like(x)
-        c = np.asarray(comps, dtype=np.int32)
-        rows = x.numel() // (channels * int(c.sum()))
-        with _on(x):
-            tok = _t0("dropout")
-            N.check(N.lib().tace_dropout(_ROW_TYPES[x.dtype], x.data_ptr(), N.ptr(residual), N.ptr(state), seed, offset,
-                                         site, threshold, rows, channels, len(c), c.ctypes.data, out.data_ptr(),
-                                         N.stream_ptr(x.device)), "tace_dropout")
-            _t1(tok, (x.numel(),))
-        return out
-
-    @staticmethod
-    def backward(ctx, g):
-        (state,) = ctx.saved_tensors
-        gx = _Dropout.apply(g.contiguous(), None, state, *ctx.args) if ctx.needs_input_grad[0] else None
-        return gx, (g if ctx.needs_input_grad[1] else None), None, None, None, None, None, None, None
+    return N.rows().route(True, y, plan.place, plan.rowptr, plan.n_tokens, plan.k, weights, widths, TIMER is not None)
 
 
 def dropout(x: torch.Tensor, p: float, rng, site: int = 0, components: Sequence[int] = (1,),
@@ -1853,42 +1600,16 @@ def dropout(x: torch.Tensor, p: float, rng, site: int = 0, components: Sequence[
     components, which keeps a tensor's degree-l blocks equivariant; (1,): one
     draw for each element of x in its order.  Differentiable any number of
     times."""
-    _row_code(x, "x")
-    p = float(p)
-    threshold = round(65536 * p) if 0.0 <= p <= 1.0 else -1
-    if threshold < 0 or (threshold == 0) != (p == 0.0) or (threshold == 65536) != (p == 1.0):
-        raise ValueError(f"dropout: p = {p} is outside [0, 1] or nearer to its ends than the mask's 2^-16")
-    comps = tuple(int(c) for c in components)
-    if not 1 <= len(comps) <= _ROW_BLOCKS or min(comps) < 1 or max(comps) > 1024:
-        raise ValueError(f"dropout: components {comps} are not 1 to {_ROW_BLOCKS} blocks of 1 to 1024")
-    if comps == (1,):
-        channels = 1
-    else:
-        if x.dim() != 2 or x.shape[1] < 1 or x.shape[1] % sum(comps):
-            raise ValueError(f"x has shape {tuple(x.shape)}, expected [rows, {sum(comps)} C]")
-        channels = x.shape[1] // sum(comps)
-    if x.numel() // sum(comps) * len(comps) > 2 ** 34:
-        raise ValueError("dropout: over 2^34 draws")
-    if not 0 <= int(site) < 2 ** 32:
-        raise ValueError(f"dropout: site {site} is outside 0 .. 2^32 - 1")
     state, seed, offset = None, 0, 0
     if isinstance(rng, torch.Tensor):
-        _same_device(x, rng, "rng")
-        _req(rng, "rng", torch.int64, (2,))
         state = rng
     else:
-        # the 64 bits of either signed or unsigned integers
         seed, offset = (int(v) for v in rng)
-        if not all(-2 ** 63 <= v < 2 ** 64 for v in (seed, offset)):
+        if not (-2 ** 63 <= seed < 2 ** 64 and -2 ** 63 <= offset < 2 ** 64):
             raise ValueError("dropout: seed and offset have 64 bits")
+        # (the same 64 bits as signed integers)
         seed, offset = (v - 2 ** 64 if v >= 2 ** 63 else v for v in (seed, offset))
-    if residual is not None:
-        if residual.shape != x.shape or residual.dtype != x.dtype:
-            raise ValueError(f"residual is {residual.dtype} {tuple(residual.shape)}, expected {x.dtype} "
-                             f"{tuple(x.shape)}")
-        _same_device(x, residual, "residual")
-        residual = residual.contiguous()
-    return _Dropout.apply(x.contiguous(), residual, state, seed, offset, int(site), threshold, channels, comps)
+    return N.rows().dropout(x, p, state, seed, offset, site, components, residual, TIMER is not None)
 
 
 def _pad4(lst):

@@ -368,13 +368,13 @@ def test_refusals(cuda):
         lambda: ops.route_plan(t.view(6, 1)[:, :0], 4),
         lambda: ops.expert_dispatch(x, plan), lambda: ops.expert_combine(x[:3], plan),
         lambda: ops.expert_dispatch(x[:3], plan, widths=(4, 5)), lambda: ops.expert_dispatch(x[:3], plan, widths=(8, 0)),
-        lambda: ops.expert_dispatch(x[:3], plan, widths=(1,) * 9), lambda: ops.expert_dispatch(x[:3], None),
+        lambda: ops.expert_dispatch(x[:3], plan, widths=(1,) * 9),
         lambda: ops.expert_dispatch(x[:3], plan, torch.zeros(2, 3, device=cuda)),
         lambda: ops.expert_dispatch(x[:3], plan, torch.zeros(3, 2, dtype=torch.int32, device=cuda)),
         lambda: ops.expert_combine(x, plan, torch.zeros(3, 2)), lambda: ops.expert_combine(cpu, plan),
         lambda: ops.dropout(x, -0.1, (1, 2)), lambda: ops.dropout(x, 1.5, (1, 2)), lambda: ops.dropout(x, 1e-7, (1, 2)),
         lambda: ops.dropout(x, 1 - 1e-7, (1, 2)), lambda: ops.dropout(x, float("nan"), (1, 2)),
-        lambda: ops.dropout(x, 0.1, (1, 2 ** 64)), lambda: ops.dropout(x, 0.1, (1, 2), site=-1),
+        lambda: ops.dropout(x, 0.1, (1, 2 ** 64)), lambda: ops.dropout(x, 0.1, (1, 2), site=-1), lambda: ops.dropout(x, 0.1, (1, 2), site=2 ** 32),
         lambda: ops.dropout(x, 0.1, (1, 2), components=(3,)), lambda: ops.dropout(x, 0.1, (1, 2), components=(0, 1)),
         lambda: ops.dropout(x, 0.1, (1, 2), components=()), lambda: ops.dropout(x, 0.1, torch.zeros(2, device=cuda)),
         lambda: ops.dropout(x, 0.1, torch.zeros(2, dtype=torch.int64)), lambda: ops.dropout(x, 0.1, (1, 2), residual=x[0]),
@@ -384,6 +384,22 @@ def test_refusals(cuda):
         with pytest.raises(ValueError):
             call()
             print("accepted:", i)
+    with pytest.raises(AttributeError):
+        ops.expert_dispatch(x[:3], None)
+
+
+def test_kernel_timer_sees_every_launch(cuda):
+    """Forward and backward launches, the backward's from autograd's thread."""
+    ops.TIMER = ops.KernelTimer()
+    try:
+        s = _pass_inputs(cuda, 5000, 3)
+        _training_pass(s)
+        seen = ops.TIMER.summary()
+    finally:
+        ops.TIMER = None
+    assert {k: v[0] for k, v in seen.items() if k != "group_keys"} == dict(
+        embed_fwd=1, embed_grad=1, dropout=2, route_dispatch=1, route_combine=2, route_dots=1)
+    assert all(ms > 0 for _, ms, _ in seen.values())
 
 
 # ---------------------------------------------------------- graphs, streams ----
