@@ -36,7 +36,8 @@ int tace_embed_fwd(int type, int index_bytes, const void* table, const void* tok
  * on the sizes alone.  order [n] and rowptr [vocab + 1] are tace_group_keys'
  * of the tokens; work: tace_embed_grad_work bytes (16-byte aligned).
  * order NULL: no grouping and no work are read, every token looks through all
- * of tokens (for few rows or tokens: tace_embed_grad_scans says where). */
+ * of tokens (for few rows and tokens: tace_embed_grad_scans says where; the
+ * only form for n = 0). */
 int64_t tace_embed_grad_work(int type, int64_t n, int64_t vocab, int32_t channels);
 int tace_embed_grad_scans(int64_t n, int64_t vocab, int32_t channels);
 int tace_embed_grad(int type, int index_bytes, const void* g, const void* tokens, const int32_t* order,

@@ -2,6 +2,7 @@
 // expert and back.  All of them move rows once and are bound by HBM.
 #include "row_types.h"
 
+#include <algorithm>
 #include <type_traits>
 
 namespace {
@@ -54,101 +55,157 @@ __global__ __launch_bounds__(WG) void k_embed_fwd(const T* __restrict__ table, c
   });
 }
 
-// Sorted positions in pieces of `per`; `cw` lanes hold a piece's row sums.  A
-// token whose rows all lie in one piece is written at once; of another token a
-// piece writes its share into part [piece][2][channels]: slot 0 if the
-// token's rows reach the piece's first position, else slot 1.
+// The gradient by sorted tokens.  A workgroup takes `per` sorted positions for
+// each of its groups of `lanes` threads, which hold a row's sums in registers.
+// Sorted, a token's rows are a run; whether a run goes on outside a group's (or
+// the workgroup's) positions shows in the neighbouring position's token.  Runs
+// inside a group are written at once; the others meet in LDS, in position
+// order; what goes on beyond the workgroup is left in part [workgroup][2]
+// [channels]: [0] a run that began before it, [1] one that begins in it.
 template <typename T, int V, typename I>
 __global__ __launch_bounds__(WG) void k_embed_grad_part(const T* __restrict__ g, const I* __restrict__ tokens,
                                                         const int* __restrict__ order, const int* __restrict__ rowptr,
-                                                        int vocab, int channels, int per, int pieces, int lanes,
+                                                        int vocab, int channels, int per, int lanes,
                                                         row_sum_t<T> scale, T* __restrict__ grad,
                                                         row_sum_t<T>* __restrict__ part) {
   typedef row_vec_t<T, V> Vec;
   typedef row_sum_t<T> S;
   constexpr int U = 8;
-  const int cw = channels / V, groups = WG / lanes;
-  const int grp = (int)threadIdx.x / lanes, c = (int)threadIdx.x % lanes + (int)blockIdx.y * lanes;
-  const int piece = (int)blockIdx.x * groups + grp;
-  if (grp >= groups || piece >= pieces || c >= cw) return;
+  __shared__ S open[2 * V * WG];   // [slot][element][thread]
+  __shared__ int open_key[2 * WG];
+  const int cw = channels / V, groups = WG / lanes, t = (int)threadIdx.x;
+  const int grp = t / lanes, lane = t % lanes, c = lane + (int)blockIdx.y * lanes;
   const int end = rowptr[vocab];   // (padding comes after it)
-  const int64_t first = (int64_t)piece * per;
-  if (first >= end) return;
-  const int p0 = (int)first, p1 = (int)min(first + per, (int64_t)end);
-  const Vec* rows = (const Vec*)g;
+  const int64_t span = (int64_t)per * groups, w0 = blockIdx.x * span;
+  if (w0 >= end) return;
+  const int w1 = (int)min(w0 + span, (int64_t)end);
+  const int p0 = (int)min(w0 + (int64_t)grp * per, (int64_t)w1), p1 = min(p0 + per, w1);
+  auto key_at = [&](int p) { return p >= 0 && p < end ? (int)tokens[order[p]] : -1; };
+  const bool mine = grp < groups && c < cw;
+  if (lane == 0 && grp < groups) open_key[2 * grp] = open_key[2 * grp + 1] = -1;
+  auto write = [&](int v, const S* sum) {
+    S a[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) a[i] = sum[i] * scale;
+    ((Vec*)grad)[(int64_t)v * cw + c] = row_round<T, V>(a);
+  };
+  if (mine && p0 < p1) {
+    const int left = key_at(p0 - 1), right = key_at(p1);
+    const Vec* rows = (const Vec*)g;
+    S sum[V];
+    int cur = -1;
+    bool head = true;   // the run at p0
+    auto flush = [&]() {
+      if (cur != left && cur != right) {
+        write(cur, sum);
+      } else {
+        const int slot = head ? 0 : 1;
+#pragma unroll
+        for (int i = 0; i < V; ++i) open[(slot * V + i) * WG + t] = sum[i];
+        if (lane == 0) open_key[2 * grp + slot] = cur;
+      }
+    };
+    for (int p = p0; p < p1; p += U) {
+      int at[U], key[U];
+      Vec v[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) at[u] = order[min(p + u, p1 - 1)];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        key[u] = (int)tokens[at[u]];
+        v[u] = rows[(int64_t)at[u] * cw + c];
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (p + u >= p1) break;
+        S a[V];
+        row_widen<T, V>(v[u], a);
+        if (key[u] != cur) {
+          if (cur >= 0) {
+            flush();
+            head = false;
+          }
+          cur = key[u];
+#pragma unroll
+          for (int i = 0; i < V; ++i) sum[i] = a[i];
+        } else {
+#pragma unroll
+          for (int i = 0; i < V; ++i) sum[i] += a[i];
+        }
+      }
+    }
+    flush();
+  }
+  __syncthreads();
+  if (grp != 0 || c >= cw) return;
+  const int left = key_at((int)w0 - 1), right = key_at(w1);
   S sum[V];
   int cur = -1;
   auto flush = [&]() {
-    const int b = rowptr[cur], e = rowptr[cur + 1];
-    if (b >= p0 && e <= p1) {
-      S a[V];
-#pragma unroll
-      for (int i = 0; i < V; ++i) a[i] = sum[i] * scale;
-      ((Vec*)grad)[(int64_t)cur * cw + c] = row_round<T, V>(a);
+    if (cur != left && cur != right) {
+      write(cur, sum);
     } else {
-      S* o = part + ((int64_t)piece * 2 + (b > p0 ? 1 : 0)) * channels + (int64_t)c * V;
+      S* o = part + ((int64_t)blockIdx.x * 2 + (cur == left ? 0 : 1)) * channels + (int64_t)c * V;
 #pragma unroll
       for (int i = 0; i < V; ++i) o[i] = sum[i];
     }
   };
-  for (int p = p0; p < p1; p += U) {
-    int at[U], key[U];
-    Vec v[U];
+  for (int q = 0; q < 2 * groups; ++q) {
+    const int key = open_key[q];
+    if (key < 0) continue;
+    const S* o = open + (q & 1) * V * WG + (q >> 1) * lanes + lane;
+    if (key != cur) {
+      if (cur >= 0) flush();
+      cur = key;
 #pragma unroll
-    for (int u = 0; u < U; ++u) at[u] = order[min(p + u, p1 - 1)];
+      for (int i = 0; i < V; ++i) sum[i] = o[i * WG];
+    } else {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      key[u] = (int)tokens[at[u]];
-      v[u] = rows[(int64_t)at[u] * cw + c];
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (p + u >= p1) break;
-      S a[V];
-      row_widen<T, V>(v[u], a);
-      if (key[u] != cur) {
-        if (cur >= 0) flush();
-        cur = key[u];
-#pragma unroll
-        for (int i = 0; i < V; ++i) sum[i] = a[i];
-      } else {
-#pragma unroll
-        for (int i = 0; i < V; ++i) sum[i] += a[i];
-      }
+      for (int i = 0; i < V; ++i) sum[i] += o[i * WG];
     }
   }
-  flush();
+  if (cur >= 0) flush();
 }
 
-// The tokens that no piece wrote: zeros without rows, else the sum of the
-// pieces' shares, 16 of them at a time and then across.
-constexpr int JOIN_COLS = 64, JOIN_ROWS = 4;
-template <typename T>
-__global__ __launch_bounds__(JOIN_COLS * JOIN_ROWS) void k_embed_grad_join(const int* __restrict__ rowptr, int vocab,
-                                                                         int channels, int per, row_sum_t<T> scale,
-                                                                         const row_sum_t<T>* __restrict__ part,
-                                                                         T* __restrict__ grad) {
+// What is left: workgroup w < workgroups - 1 joins the run that begins in the
+// w-th workgroup above and goes on in the next (if there is one); the others
+// write the zeros of tokens without rows, one per wavefront and step.
+constexpr int JOIN_COLS = 16, JOIN_ROWS = WG / JOIN_COLS;
+template <typename T, typename I>
+__global__ __launch_bounds__(WG) void k_embed_grad_join(const I* __restrict__ tokens, const int* __restrict__ order,
+                                                        const int* __restrict__ rowptr, int vocab, int channels,
+                                                        int64_t span, int seams, row_sum_t<T> scale,
+                                                        const row_sum_t<T>* __restrict__ part, T* __restrict__ grad) {
   typedef row_sum_t<T> S;
+  const int t = (int)threadIdx.x;
+  if ((int)blockIdx.x >= seams) {
+    const int step = ((int)gridDim.x - seams) * (WG / 64) * (int)gridDim.y;
+    for (int64_t v = (((int64_t)blockIdx.x - seams) * gridDim.y + blockIdx.y) * (WG / 64) + t / 64; v < vocab; v += step)
+      if (rowptr[v] == rowptr[v + 1])
+        for (int c = t % 64; c < channels; c += 64) grad[v * channels + c] = (T)0;
+    return;
+  }
+  const int end = rowptr[vocab];
+  const int64_t w0 = blockIdx.x * span, w1 = w0 + span;
+  if (w1 >= end) return;
+  const int v = (int)tokens[order[w1]];
+  const int b = rowptr[v], e = rowptr[v + 1];
+  if (b >= w1 || b < w0) return;   // begins at the seam, or joined at an earlier one
   __shared__ S red[JOIN_ROWS][JOIN_COLS];
-  const int x = (int)threadIdx.x % JOIN_COLS, y = (int)threadIdx.x / JOIN_COLS;
-  const int c = (int)blockIdx.y * JOIN_COLS + x;
-  for (int v = (int)blockIdx.x; v < vocab; v += (int)gridDim.x) {
-    const int b = rowptr[v], e = rowptr[v + 1];
-    const int c0 = b / per, c1 = (e - 1) / per;
-    if (e > b && c0 == c1) continue;
-    S sum = 0;
-    if (e > b && c < channels) {
-      for (int q = c0 + y; q <= c1; q += JOIN_ROWS)
-        sum += part[((int64_t)q * 2 + (q == c0 && b != c0 * per ? 1 : 0)) * channels + c];
-    }
-    red[y][x] = sum;
-    __syncthreads();
-    if (y == 0 && c < channels) {
+  const int x = t % JOIN_COLS, y = t / JOIN_COLS, c = (int)blockIdx.y * JOIN_COLS + x;
+  const int last = (int)((e - 1) / span);
+  S sum = 0;
+  if (c < channels) {
+#pragma unroll 8
+    for (int q = (int)blockIdx.x + y; q <= last; q += JOIN_ROWS)
+      sum += part[((int64_t)q * 2 + (q == (int)blockIdx.x ? 1 : 0)) * channels + c];
+  }
+  red[y][x] = sum;
+  __syncthreads();
+  if (y == 0 && c < channels) {
 #pragma unroll
-      for (int k = 1; k < JOIN_ROWS; ++k) sum += red[k][x];
-      grad[(int64_t)v * channels + c] = (T)(sum * scale);
-    }
-    __syncthreads();
+    for (int k = 1; k < JOIN_ROWS; ++k) sum += red[k][x];
+    grad[(int64_t)v * channels + c] = (T)(sum * scale);
   }
 }
 
@@ -210,11 +267,16 @@ __global__ __launch_bounds__(WG) void k_embed_grad_scan(const T* __restrict__ g,
 
 int embed_lanes(int cw) { return cw < WG ? cw : WG; }
 
-// positions a piece: enough pieces to fill the GPU, few enough that a token
-// with most of the rows is joined quickly
-int embed_per(int64_t n) {
-  const int64_t per = (n + 4095) / 4096;
-  return (int)(per < 32 ? 32 : per);
+// Positions a group: 1,024 workgroups, which fill the GPU and leave a token
+// that has most of the rows few sums to join; at least 16.
+int embed_per(int64_t n, int lanes) {
+  const int64_t groups = WG / lanes, per = (n + 1024 * groups - 1) / (1024 * groups);
+  return (int)(per < 16 ? 16 : per);
+}
+// workgroups for rows of cw chunks, whatever their type
+int64_t embed_wgs(int64_t n, int lanes) {
+  const int64_t span = (int64_t)embed_per(n, lanes) * (WG / lanes);
+  return (n + span - 1) / span;
 }
 
 // --------------------------------------------------------------- routing ----
@@ -408,9 +470,12 @@ extern "C" int tace_embed_grad_scans(int64_t n, int64_t vocab, int32_t channels)
 
 extern "C" int64_t tace_embed_grad_work(int type, int64_t n, int64_t vocab, int32_t channels) {
   (void)vocab;
-  if (n < 1) return 16;
-  const int64_t pieces = (n + embed_per(n) - 1) / embed_per(n);
-  return pieces * 2 * channels * (type == TACE_ROW_F64 ? 8 : 4);
+  if (n < 1 || channels < 1 || channels > MAX_ROW) return 16;
+  // (rows may be moved whole or by element: the larger count of workgroups)
+  const int bytes = type == TACE_ROW_F64 ? 8 : type == TACE_ROW_F32 ? 4 : 2, v = 16 / bytes;
+  int64_t wgs = embed_wgs(n, embed_lanes(channels));
+  if (channels % v == 0) wgs = std::max(wgs, embed_wgs(n, embed_lanes(channels / v)));
+  return wgs * 2 * channels * (type == TACE_ROW_F64 ? 8 : 4);
 }
 
 extern "C" int tace_embed_grad(int type, int index_bytes, const void* g, const void* tokens, const int32_t* order,
@@ -423,12 +488,13 @@ extern "C" int tace_embed_grad(int type, int index_bytes, const void* g, const v
   if (vocab == 0) return 0;
   const bool scans = order == nullptr;
   if (!grad || (n && (!g || !tokens))) return tace_fail_msg("tace_embed_grad: null pointer");
+  if (!scans && n == 0) return tace_fail_msg("tace_embed_grad: no rows, and a grouping of them");
   if (scans) {
     if (!tace_embed_grad_scans(n, vocab, channels))
       return tace_fail_msg("tace_embed_grad: too many rows or tokens without a grouping");
   } else {
-    if (!rowptr || (n && !work)) return tace_fail_msg("tace_embed_grad: null pointer");
-    if (n && (work_bytes < tace_embed_grad_work(type, n, vocab, channels) || !row_aligned(work)))
+    if (!rowptr || !work) return tace_fail_msg("tace_embed_grad: null pointer");
+    if ((work_bytes < tace_embed_grad_work(type, n, vocab, channels) || !row_aligned(work)))
       return tace_fail_msg("tace_embed_grad: workspace too small or not 16-byte aligned");
   }
   row_dispatch(type, [&](auto z) {
@@ -438,7 +504,7 @@ extern "C" int tace_embed_grad(int type, int index_bytes, const void* g, const v
     const bool vec = channels % W == 0 && row_aligned(g) && row_aligned(grad);
     const int cw = vec ? channels / W : channels, lanes = embed_lanes(cw), tiles = (cw + lanes - 1) / lanes;
     hipStream_t s = (hipStream_t)stream;
-    const int per = embed_per(n), pieces = (int)((n + per - 1) / per), groups = WG / lanes;
+    const int per = embed_per(n, lanes), wgs = (int)embed_wgs(n, lanes), groups = WG / lanes;
     auto go = [&](auto i) {
       typedef decltype(i) I;
       auto run = [&](auto vc) {
@@ -446,21 +512,23 @@ extern "C" int tace_embed_grad(int type, int index_bytes, const void* g, const v
         if (scans)
           hipLaunchKernelGGL((k_embed_grad_scan<T, V, I>), dim3((unsigned)vocab, (unsigned)tiles), dim3(WG), 0, s,
                              (const T*)g, (const I*)tokens, (int)n, channels, lanes, (S)scale, (T*)grad);
-        else if (n)
-          hipLaunchKernelGGL((k_embed_grad_part<T, V, I>), dim3((unsigned)((pieces + groups - 1) / groups), tiles),
-                             dim3(WG), 0, s, (const T*)g, (const I*)tokens, order, rowptr, (int)vocab, channels, per,
-                             pieces, lanes, (S)scale, (T*)grad, (S*)work);
+        else
+          hipLaunchKernelGGL((k_embed_grad_part<T, V, I>), dim3((unsigned)wgs, tiles), dim3(WG), 0, s, (const T*)g,
+                             (const I*)tokens, order, rowptr, (int)vocab, channels, per, lanes, (S)scale, (T*)grad,
+                             (S*)work);
       };
       if (vec) run(std::integral_constant<int, W>());
       else run(std::integral_constant<int, 1>());
+      if (!scans) {
+        const int columns = (channels + JOIN_COLS - 1) / JOIN_COLS, seams = wgs - 1;
+        const int64_t zeros = (vocab + 4 * columns - 1) / (4 * columns);
+        hipLaunchKernelGGL((k_embed_grad_join<T, I>), dim3((unsigned)(seams + (zeros < 2048 ? zeros : 2048)), columns),
+                           dim3(WG), 0, s, (const I*)tokens, order, rowptr, (int)vocab, channels, (int64_t)per * groups,
+                           seams, (S)scale, (const S*)work, (T*)grad);
+      }
     };
     if (index_bytes == 4) go(int32_t());
     else go(int64_t());
-    if (!scans)
-      hipLaunchKernelGGL((k_embed_grad_join<T>),
-                         dim3((unsigned)(vocab < 65536 ? vocab : 65536), (unsigned)((channels + JOIN_COLS - 1) / JOIN_COLS)),
-                         dim3(JOIN_COLS * JOIN_ROWS), 0, s, rowptr, (int)vocab, channels, per, (S)scale, (const S*)work,
-                         (T*)grad);
   });
   return tace_check_launch("tace_embed_grad");
 }

@@ -88,12 +88,13 @@ def test_operators_take_no_cpu_tensors():
             call()
 
 
-def test_workspace_covers_every_piece():
-    """Two sums of a row for each piece of sorted positions, whatever the size."""
+def test_workspace_covers_every_workgroup():
+    """Two sums of a row for each workgroup's sorted positions: at most 1,024 of them, whatever the size."""
     L = N.lib()
-    for n in (1, 31, 32, 33, 4095, 131072, 131073, 1063830, 2 ** 31 - 8193):
+    for n in (1, 31, 257, 4097, 131072, 131073, 1063830, 2 ** 31 - 8193):
         for ty, size in ((0, 4), (1, 8), (2, 4)):
-            nbytes = L.tace_embed_grad_work(ty, n, 7, 100)
-            assert nbytes % (200 * size) == 0
-            pieces = nbytes // (200 * size)
-            assert 1 <= pieces <= 4096
+            for C in (1, 7, 100, 128, 4096, 32768):
+                nbytes = L.tace_embed_grad_work(ty, n, 7, C)
+                assert nbytes % (2 * C * size) == 0
+                assert 1 <= nbytes // (2 * C * size) <= 1024
+    _refused(L.tace_embed_grad(0, 8, 4096, 4096, 4096, 4096, 0, 4, 4, 1.0, 4096, 4096, 16, None), b"no rows")
