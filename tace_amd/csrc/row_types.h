@@ -3,6 +3,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "../../include/tace_rows.h"
 
 int tace_fail_msg(const char* msg);   // tace_hip.hip
@@ -56,6 +58,16 @@ inline RowDiv row_div(unsigned d) {
 }
 
 inline bool row_aligned(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+// Calls f with the elements a move takes, as a constant: 16 bytes, else 8, that
+// `fits` (an element count, bytes) allows, else one.
+template <typename T, typename Fits, typename F>
+void row_moves(Fits&& fits, F&& f) {
+  constexpr int W = 16 / sizeof(T), H = W > 2 ? W / 2 : W;
+  if (fits(W, 16)) f(std::integral_constant<int, W>());
+  else if (H < W && fits(H, 8)) f(std::integral_constant<int, H>());
+  else f(std::integral_constant<int, 1>());
+}
 
 // calls f with a zero of the row type; false for another code
 template <typename F>

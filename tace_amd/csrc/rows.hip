@@ -3,7 +3,6 @@
 #include "row_types.h"
 
 #include <algorithm>
-#include <type_traits>
 
 namespace {
 
@@ -11,36 +10,30 @@ namespace {
 constexpr int WG = 256;
 constexpr int MAX_ROW = 1 << 15;   // elements: RowDiv's range
 
-// Work of a workgroup that goes through `rows * chunks` chunks in order, U per
-// thread: row and chunk of its u-th.
+// A chunk of a row for each thread, in order.
 struct RowChunks {
   int64_t total;      // rows * chunks
   RowDiv chunks;      // chunks a row
 
-  template <int U, typename F>
+  template <typename F>
   __device__ __forceinline__ void each(F&& f) const {
-    const int64_t q0 = (int64_t)blockIdx.x * (WG * U);
-    const int64_t r0 = q0 / chunks.d;
-    const unsigned rem = (unsigned)(q0 - r0 * chunks.d);
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const unsigned q = rem + u * WG + threadIdx.x;
-      if (q0 - rem + q < total) {
-        const unsigned r = chunks.div(q);
-        f(u, r0 + r, q - r * chunks.d);
-      }
+    const int64_t q0 = (int64_t)blockIdx.x * WG, r0 = q0 / chunks.d;
+    const unsigned rem = (unsigned)(q0 - r0 * chunks.d), q = rem + threadIdx.x;
+    if (q0 + threadIdx.x < total) {
+      const unsigned r = chunks.div(q);
+      f(r0 + r, q - r * chunks.d);
     }
   }
 };
 
-template <typename T, int V, typename I, int U>
+template <typename T, int V, typename I>
 __global__ __launch_bounds__(WG) void k_embed_fwd(const T* __restrict__ table, const I* __restrict__ tokens,
                                                   RowChunks rc, int64_t vocab, row_sum_t<T> scale,
                                                   T* __restrict__ out) {
   typedef row_vec_t<T, V> Vec;
   const Vec* tab = (const Vec*)table;
   Vec* o = (Vec*)out;
-  rc.each<U>([&](int, int64_t r, unsigned c) {
+  rc.each([&](int64_t r, unsigned c) {
     const I t = tokens[r];
     row_sum_t<T> a[V];
     if (t >= 0 && t < (I)vocab) {
@@ -51,7 +44,7 @@ __global__ __launch_bounds__(WG) void k_embed_fwd(const T* __restrict__ table, c
 #pragma unroll
       for (int i = 0; i < V; ++i) a[i] = 0;
     }
-    o[r * rc.chunks.d + c] = row_round<T, V>(a);
+    __builtin_nontemporal_store(row_round<T, V>(a), &o[r * rc.chunks.d + c]);
   });
 }
 
@@ -62,40 +55,49 @@ __global__ __launch_bounds__(WG) void k_embed_fwd(const T* __restrict__ table, c
 // inside a group are written at once; the others meet in LDS, in position
 // order; what goes on beyond the workgroup is left in part [workgroup][2]
 // [channels]: [0] a run that began before it, [1] one that begins in it.
+constexpr int TEAM = 8;   // groups whose open runs one of them joins
 template <typename T, int V, typename I>
 __global__ __launch_bounds__(WG) void k_embed_grad_part(const T* __restrict__ g, const I* __restrict__ tokens,
-                                                        const int* __restrict__ order, const int* __restrict__ rowptr,
-                                                        int vocab, int channels, int per, int lanes,
+                                                        const int* __restrict__ order, int n, int vocab, int channels,
+                                                        int per, int lanes,
                                                         row_sum_t<T> scale, T* __restrict__ grad,
                                                         row_sum_t<T>* __restrict__ part) {
   typedef row_vec_t<T, V> Vec;
   typedef row_sum_t<T> S;
   constexpr int U = 8;
   __shared__ S open[2 * V * WG];   // [slot][element][thread]
-  __shared__ int open_key[2 * WG];
+  __shared__ int open_key[2 * WG], team_key[2 * WG / TEAM], outer[2 * WG / TEAM];
   const int cw = channels / V, groups = WG / lanes, t = (int)threadIdx.x;
   const int grp = t / lanes, lane = t % lanes, c = lane + (int)blockIdx.y * lanes;
-  const int end = rowptr[vocab];   // (padding comes after it)
-  const int64_t span = (int64_t)per * groups, w0 = blockIdx.x * span;
-  if (w0 >= end) return;
-  const int w1 = (int)min(w0 + span, (int64_t)end);
-  const int p0 = (int)min(w0 + (int64_t)grp * per, (int64_t)w1), p1 = min(p0 + per, w1);
-  auto key_at = [&](int p) { return p >= 0 && p < end ? (int)tokens[order[p]] : -1; };
-  const bool mine = grp < groups && c < cw;
-  if (lane == 0 && grp < groups) open_key[2 * grp] = open_key[2 * grp + 1] = -1;
+  const int64_t w0 = blockIdx.x * (int64_t)per * groups;
+  const int p0 = (int)min(w0 + (int64_t)grp * per, (int64_t)n), p1 = min(p0 + per, n);
+  // (padding, sorted last, has no key)
+  auto key_of = [&](I v) { return v >= 0 && v < (I)vocab ? (int)v : -1; };
   auto write = [&](int v, const S* sum) {
     S a[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) a[i] = sum[i] * scale;
     ((Vec*)grad)[(int64_t)v * cw + c] = row_round<T, V>(a);
   };
-  if (mine && p0 < p1) {
-    const int left = key_at(p0 - 1), right = key_at(p1);
-    const Vec* rows = (const Vec*)g;
+  if (grp < groups) {
+    int next[U];
+    auto ahead = [&](int p) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) next[u] = order[min(p + u, n - 1)];
+    };
+    ahead(p0);
+    const int left = p0 > 0 ? key_of(tokens[order[p0 - 1]]) : -1, right = p1 < n ? key_of(tokens[order[p1]]) : -1;
+    if (lane == 0) {
+      const int team = grp / TEAM;
+      open_key[2 * grp] = open_key[2 * grp + 1] = -1;
+      if (grp % TEAM == 0) outer[2 * team] = left, team_key[2 * team] = team_key[2 * team + 1] = -1;
+      if (grp % TEAM == TEAM - 1 || grp == groups - 1) outer[2 * team + 1] = right;
+    }
     S sum[V];
     int cur = -1;
     bool head = true;   // the run at p0
     auto flush = [&]() {
+      if (cur < 0 || c >= cw) return;
       if (cur != left && cur != right) {
         write(cur, sum);
       } else {
@@ -105,30 +107,28 @@ __global__ __launch_bounds__(WG) void k_embed_grad_part(const T* __restrict__ g,
         if (lane == 0) open_key[2 * grp + slot] = cur;
       }
     };
+    const Vec* rows = (const Vec*)g + min(c, cw - 1);
     for (int p = p0; p < p1; p += U) {
-      int at[U], key[U];
+      I tok[U];
       Vec v[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u) at[u] = order[min(p + u, p1 - 1)];
-#pragma unroll
       for (int u = 0; u < U; ++u) {
-        key[u] = (int)tokens[at[u]];
-        v[u] = rows[(int64_t)at[u] * cw + c];
+        tok[u] = tokens[next[u]];
+        v[u] = __builtin_nontemporal_load(rows + (int64_t)next[u] * cw);   // (read once)
       }
+      ahead(p + U);
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        if (p + u >= p1) break;
+        const int key = p + u < p1 ? key_of(tok[u]) : cur;
         S a[V];
         row_widen<T, V>(v[u], a);
-        if (key[u] != cur) {
-          if (cur >= 0) {
-            flush();
-            head = false;
-          }
-          cur = key[u];
+        if (key != cur) {
+          flush();
+          head = head && cur < 0;
+          cur = key;
 #pragma unroll
           for (int i = 0; i < V; ++i) sum[i] = a[i];
-        } else {
+        } else if (p + u < p1) {
 #pragma unroll
           for (int i = 0; i < V; ++i) sum[i] += a[i];
         }
@@ -137,34 +137,53 @@ __global__ __launch_bounds__(WG) void k_embed_grad_part(const T* __restrict__ g,
     flush();
   }
   __syncthreads();
-  if (grp != 0 || c >= cw) return;
-  const int left = key_at((int)w0 - 1), right = key_at(w1);
-  S sum[V];
-  int cur = -1;
-  auto flush = [&]() {
-    if (cur != left && cur != right) {
-      write(cur, sum);
-    } else {
-      S* o = part + ((int64_t)blockIdx.x * 2 + (cur == left ? 0 : 1)) * channels + (int64_t)c * V;
+  // the open runs of `count` groups, `step` apart, from g0 on
+  auto merge = [&](int g0, int count, int step, const int* keys, int left, int right, auto&& leave) {
+    S sum[V];
+    int cur = -1;
+    auto flush = [&]() {
+      if (cur != left && cur != right) write(cur, sum);
+      else leave(cur == left ? 0 : 1, cur, sum);
+    };
+    for (int q = 0; q < 2 * count; ++q) {
+      const int key = keys[q];
+      if (key < 0) continue;
+      const S* o = open + (q & 1) * V * WG + (g0 + (q >> 1) * step) * lanes + lane;
+      if (key != cur) {
+        if (cur >= 0) flush();
+        cur = key;
 #pragma unroll
-      for (int i = 0; i < V; ++i) o[i] = sum[i];
+        for (int i = 0; i < V; ++i) sum[i] = o[i * WG];
+      } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) sum[i] += o[i * WG];
+      }
     }
+    if (cur >= 0) flush();
   };
-  for (int q = 0; q < 2 * groups; ++q) {
-    const int key = open_key[q];
-    if (key < 0) continue;
-    const S* o = open + (q & 1) * V * WG + (q >> 1) * lanes + lane;
-    if (key != cur) {
-      if (cur >= 0) flush();
-      cur = key;
+  const int teams = (groups + TEAM - 1) / TEAM;
+  auto leave_part = [&](int slot, int, const S* sum) {
+    S* o = part + ((int64_t)blockIdx.x * 2 + slot) * channels + (int64_t)c * V;
 #pragma unroll
-      for (int i = 0; i < V; ++i) sum[i] = o[i * WG];
-    } else {
-#pragma unroll
-      for (int i = 0; i < V; ++i) sum[i] += o[i * WG];
-    }
+    for (int i = 0; i < V; ++i) o[i] = sum[i];
+  };
+  if (teams == 1) {
+    if (grp == 0 && c < cw) merge(0, groups, 1, open_key, outer[0], outer[1], leave_part);
+    return;
   }
-  if (cur >= 0) flush();
+  // teams of groups first (a thread reads and writes its own sums here, and
+  // those of its column in its team)
+  if (grp < groups && grp % TEAM == 0 && c < cw) {
+    const int team = grp / TEAM;
+    merge(grp, min(TEAM, groups - grp), 1, open_key + 2 * grp, outer[2 * team], outer[2 * team + 1],
+          [&](int slot, int key, const S* sum) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) open[(slot * V + i) * WG + t] = sum[i];
+            if (lane == 0) team_key[2 * team + slot] = key;
+          });
+  }
+  __syncthreads();
+  if (grp == 0 && c < cw) merge(0, teams, TEAM, team_key, outer[0], outer[2 * teams - 1], leave_part);
 }
 
 // What is left: workgroup w < workgroups - 1 joins the run that begins in the
@@ -180,7 +199,8 @@ __global__ __launch_bounds__(WG) void k_embed_grad_join(const I* __restrict__ to
   const int t = (int)threadIdx.x;
   if ((int)blockIdx.x >= seams) {
     const int step = ((int)gridDim.x - seams) * (WG / 64) * (int)gridDim.y;
-    for (int64_t v = (((int64_t)blockIdx.x - seams) * gridDim.y + blockIdx.y) * (WG / 64) + t / 64; v < vocab; v += step)
+    const int first = (((int)blockIdx.x - seams) * (int)gridDim.y + (int)blockIdx.y) * (WG / 64) + t / 64;
+    for (int64_t v = first; v < vocab; v += step)
       if (rowptr[v] == rowptr[v + 1])
         for (int c = t % 64; c < channels; c += 64) grad[v * channels + c] = (T)0;
     return;
@@ -267,11 +287,13 @@ __global__ __launch_bounds__(WG) void k_embed_grad_scan(const T* __restrict__ g,
 
 int embed_lanes(int cw) { return cw < WG ? cw : WG; }
 
-// Positions a group: 1,024 workgroups, which fill the GPU and leave a token
-// that has most of the rows few sums to join; at least 16.
+// Positions a group: 512 workgroups, at least 8.  (us of 256, 512, 1,024
+// workgroups: 1.06 M rows of 64 float32 73, 63, 69; 200,000 of 256 49, 43, 48;
+// 60,000 of 1,000 float16 47, 48, 62: fewer leave CUs idle, more spend their time
+// on their first loads and their seams.)
 int embed_per(int64_t n, int lanes) {
-  const int64_t groups = WG / lanes, per = (n + 1024 * groups - 1) / (1024 * groups);
-  return (int)(per < 16 ? 16 : per);
+  const int64_t groups = WG / lanes, per = (n + 512 * groups - 1) / (512 * groups);
+  return (int)(per < 8 ? 8 : per);
 }
 // workgroups for rows of cw chunks, whatever their type
 int64_t embed_wgs(int64_t n, int lanes) {
@@ -303,7 +325,15 @@ __global__ __launch_bounds__(WG) void k_route_place(const int* __restrict__ orde
   if (i < n) place[order[i]] = (int)i;
 }
 
-template <typename T, int V, int U>
+// STREAM: stores that do not stay in the caches
+template <bool STREAM, typename Vec>
+__device__ __forceinline__ void put(Vec* p, const Vec& v) {
+  if constexpr (STREAM) __builtin_nontemporal_store(v, p);
+  else *p = v;
+}
+
+// a row is read once and stored k times
+template <typename T, int V, bool STREAM>
 __global__ __launch_bounds__(WG) void k_route_dispatch(const T* __restrict__ x, const row_sum_t<T>* __restrict__ w,
                                                        const int* __restrict__ place, const int* __restrict__ rows_end,
                                                        RowChunks rc, int64_t tokens, int k, Blocks bl,
@@ -312,8 +342,9 @@ __global__ __launch_bounds__(WG) void k_route_dispatch(const T* __restrict__ x, 
   typedef row_sum_t<T> S;
   const int end = *rows_end;
   const int64_t n = tokens * k;
-  rc.each<U>([&](int, int64_t t, unsigned c) {
+  rc.each([&](int64_t t, unsigned c) {
     const Vec v = ((const Vec*)x)[bl.at(tokens, t, c)];
+#pragma unroll 2
     for (int j = 0; j < k; ++j) {
       const int64_t s = t * k + j;
       const int p = place[s];
@@ -325,12 +356,14 @@ __global__ __launch_bounds__(WG) void k_route_dispatch(const T* __restrict__ x, 
         for (int i = 0; i < V; ++i) a[i] = p >= end ? (S)0 : a[i] * w[s];
         o = row_round<T, V>(a);
       }
-      ((Vec*)out)[bl.at(n, p, c)] = o;
+      put<STREAM>((Vec*)out + bl.at(n, p, c), o);
     }
   });
 }
 
-template <typename T, int V, int U>
+// K slots' rows are loaded before the first is added (the dropped ones too:
+// they have a row, which is not added)
+template <typename T, int V, int K>
 __global__ __launch_bounds__(WG) void k_route_combine(const T* __restrict__ y, const row_sum_t<T>* __restrict__ w,
                                                       const int* __restrict__ place, const int* __restrict__ rows_end,
                                                       RowChunks rc, int64_t tokens, int k, Blocks bl,
@@ -339,26 +372,39 @@ __global__ __launch_bounds__(WG) void k_route_combine(const T* __restrict__ y, c
   typedef row_sum_t<T> S;
   const int end = *rows_end;
   const int64_t n = tokens * k;
-  rc.each<U>([&](int, int64_t t, unsigned c) {
+  rc.each([&](int64_t t, unsigned c) {
     S sum[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) sum[i] = 0;
-    for (int j = 0; j < k; ++j) {
-      const int64_t s = t * k + j;
-      const int p = place[s];
-      if (p >= end) continue;
-      S a[V];
-      row_widen<T, V>(((const Vec*)y)[bl.at(n, p, c)], a);
-      const S f = w ? w[s] : (S)1;
+    for (int j = 0; j < k; j += K) {
+      int p[K];
+      S f[K];
+      Vec v[K];
 #pragma unroll
-      for (int i = 0; i < V; ++i) sum[i] += f * a[i];
+      for (int q = 0; q < K; ++q) {
+        const int64_t s = t * k + min(j + q, k - 1);
+        p[q] = place[s];
+        f[q] = w ? w[s] : (S)1;
+      }
+#pragma unroll
+      for (int q = 0; q < K; ++q) v[q] = ((const Vec*)y)[bl.at(n, p[q], c)];
+#pragma unroll
+      for (int q = 0; q < K; ++q) {
+        if (p[q] >= end || j + q >= k) continue;
+        S a[V];
+        row_widen<T, V>(v[q], a);
+#pragma unroll
+        for (int i = 0; i < V; ++i) sum[i] += f[q] * a[i];
+      }
     }
-    ((Vec*)out)[bl.at(tokens, t, c)] = row_round<T, V>(sum);
+    put<true>((Vec*)out + bl.at(tokens, t, c), row_round<T, V>(sum));
   });
 }
 
-// `lanes` (a power of two, at most 64) lanes a token
-template <typename T, int V>
+// `lanes` (a power of two, at most 64) lanes a slot, the slots of a token side
+// by side: its row of x comes from memory once.  U chunks of both rows are
+// loaded before the first is multiplied.
+template <typename T, int V, int U>
 __global__ __launch_bounds__(WG) void k_route_dots(const T* __restrict__ x, const T* __restrict__ y,
                                                    const row_sum_t<T>* __restrict__ w, const int* __restrict__ place,
                                                    const int* __restrict__ rows_end, int64_t tokens, int k, int lanes,
@@ -366,33 +412,40 @@ __global__ __launch_bounds__(WG) void k_route_dots(const T* __restrict__ x, cons
                                                    row_sum_t<T>* __restrict__ dots) {
   typedef row_vec_t<T, V> Vec;
   typedef row_sum_t<T> S;
-  const int end = *rows_end, groups = WG / lanes;
-  const int64_t t = (int64_t)blockIdx.x * groups + (int)threadIdx.x / lanes, n = tokens * k;
-  if (t >= tokens) return;   // (whole groups; the shuffles stay inside a group)
-  const int lane = (int)threadIdx.x % lanes;
-  for (int j = 0; j < k; ++j) {
-    const int64_t s = t * k + j;
-    const int p = place[s];
-    const bool kept = p < end;
-    const S f = w ? w[s] : (S)1;
-    S dot = 0;
-    for (unsigned c = lane; c < cw; c += lanes) {
-      S a[V] = {}, b[V];
-      if (kept) {
-        row_widen<T, V>(((const Vec*)x)[bl.at(tokens, t, c)], a);
-        row_widen<T, V>(((const Vec*)y)[bl.at(n, p, c)], b);
+  const int64_t s = (int64_t)blockIdx.x * (WG / lanes) + (int)threadIdx.x / lanes, n = tokens * k;
+  if (s >= n) return;   // (whole groups of lanes; the shuffles stay inside one)
+  const unsigned lane = threadIdx.x % lanes;
+  const int64_t t = (uint64_t)s / (unsigned)k;
+  const int p = place[s];
+  const bool kept = p < *rows_end;
+  const S f = w ? w[s] : (S)1;
+  S dot = 0;
+  for (unsigned c0 = lane; c0 < cw; c0 += U * lanes) {
+    Vec xv[U], yv[U];
 #pragma unroll
-        for (int i = 0; i < V; ++i) dot += a[i] * b[i];
-      }
+    for (int u = 0; u < U; ++u) {
+      const unsigned c = min(c0 + u * lanes, cw - 1);
+      xv[u] = ((const Vec*)x)[bl.at(tokens, t, c)];
+      yv[u] = ((const Vec*)y)[bl.at(n, p, c)];
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const unsigned c = c0 + u * lanes;
+      if (c >= cw) break;
+      S a[V], b[V];
+      row_widen<T, V>(xv[u], a);
+      row_widen<T, V>(yv[u], b);
+#pragma unroll
+      for (int i = 0; i < V; ++i) dot += kept ? a[i] * b[i] : (S)0;
       if (g_y) {
 #pragma unroll
         for (int i = 0; i < V; ++i) a[i] = kept ? f * a[i] : (S)0;
-        ((Vec*)g_y)[bl.at(n, p, c)] = row_round<T, V>(a);
+        put<true>((Vec*)g_y + bl.at(n, p, c), row_round<T, V>(a));
       }
     }
-    for (int o = lanes >> 1; o > 0; o >>= 1) dot += __shfl_xor(dot, o, 64);
-    if (lane == 0) dots[s] = dot;
   }
+  for (int o = lanes >> 1; o > 0; o >>= 1) dot += __shfl_xor(dot, o, 64);
+  if (lane == 0) dots[s] = dot;
 }
 
 // (a launch holds less than 2^32 threads)
@@ -440,23 +493,22 @@ extern "C" int tace_embed_fwd(int type, int index_bytes, const void* table, cons
   bool fits = true;
   const bool known = row_dispatch(type, [&](auto z) {
     typedef decltype(z) T;
-    constexpr int W = 16 / sizeof(T), U = 4;
-    const bool vec = channels % W == 0 && row_aligned(table) && row_aligned(out);
-    const RowChunks rc{n * (channels / (vec ? W : 1)), row_div((unsigned)(channels / (vec ? W : 1)))};
-    const int64_t grid = (rc.total + WG * U - 1) / (WG * U);
-    fits = grid_ok(grid);
-    if (!fits) return;
-    auto go = [&](auto i) {
-      typedef decltype(i) I;
-      if (vec)
-        hipLaunchKernelGGL((k_embed_fwd<T, W, I, U>), dim3((unsigned)grid), dim3(WG), 0, (hipStream_t)stream,
-                           (const T*)table, (const I*)tokens, rc, vocab, (row_sum_t<T>)scale, (T*)out);
-      else
-        hipLaunchKernelGGL((k_embed_fwd<T, 1, I, U>), dim3((unsigned)grid), dim3(WG), 0, (hipStream_t)stream,
-                           (const T*)table, (const I*)tokens, rc, vocab, (row_sum_t<T>)scale, (T*)out);
-    };
-    if (index_bytes == 4) go(int32_t());
-    else go(int64_t());
+    row_moves<T>(
+        [&](int v, int bytes) { return channels % v == 0 && ((uintptr_t)table | (uintptr_t)out) % bytes == 0; },
+        [&](auto vc) {
+          constexpr int V = decltype(vc)::value;
+          const RowChunks rc{n * (channels / V), row_div((unsigned)(channels / V))};
+          const int64_t grid = (rc.total + WG - 1) / WG;
+          fits = grid_ok(grid);
+          if (!fits) return;
+          auto go = [&](auto i) {
+            typedef decltype(i) I;
+            hipLaunchKernelGGL((k_embed_fwd<T, V, I>), dim3((unsigned)grid), dim3(WG), 0, (hipStream_t)stream,
+                               (const T*)table, (const I*)tokens, rc, vocab, (row_sum_t<T>)scale, (T*)out);
+          };
+          if (index_bytes == 4) go(int32_t());
+          else go(int64_t());
+        });
   });
   if (!known) return tace_fail_msg("tace_embed_fwd: unknown row type");
   if (!fits) return tace_fail_msg("tace_embed_fwd: too many rows");
@@ -471,10 +523,11 @@ extern "C" int tace_embed_grad_scans(int64_t n, int64_t vocab, int32_t channels)
 extern "C" int64_t tace_embed_grad_work(int type, int64_t n, int64_t vocab, int32_t channels) {
   (void)vocab;
   if (n < 1 || channels < 1 || channels > MAX_ROW) return 16;
-  // (rows may be moved whole or by element: the larger count of workgroups)
-  const int bytes = type == TACE_ROW_F64 ? 8 : type == TACE_ROW_F32 ? 4 : 2, v = 16 / bytes;
-  int64_t wgs = embed_wgs(n, embed_lanes(channels));
-  if (channels % v == 0) wgs = std::max(wgs, embed_wgs(n, embed_lanes(channels / v)));
+  // (rows may be moved by 16 bytes, 8, or one element: the largest count of workgroups)
+  const int bytes = type == TACE_ROW_F64 ? 8 : type == TACE_ROW_F32 ? 4 : 2;
+  int64_t wgs = 0;
+  for (int v : {1, 8 / bytes, 16 / bytes})
+    if (channels % v == 0) wgs = std::max(wgs, embed_wgs(n, embed_lanes(channels / v)));
   return wgs * 2 * channels * (type == TACE_ROW_F64 ? 8 : 4);
 }
 
@@ -500,35 +553,33 @@ extern "C" int tace_embed_grad(int type, int index_bytes, const void* g, const v
   row_dispatch(type, [&](auto z) {
     typedef decltype(z) T;
     typedef row_sum_t<T> S;
-    constexpr int W = 16 / sizeof(T);
-    const bool vec = channels % W == 0 && row_aligned(g) && row_aligned(grad);
-    const int cw = vec ? channels / W : channels, lanes = embed_lanes(cw), tiles = (cw + lanes - 1) / lanes;
-    hipStream_t s = (hipStream_t)stream;
-    const int per = embed_per(n, lanes), wgs = (int)embed_wgs(n, lanes), groups = WG / lanes;
-    auto go = [&](auto i) {
-      typedef decltype(i) I;
-      auto run = [&](auto vc) {
-        constexpr int V = decltype(vc)::value;
-        if (scans)
-          hipLaunchKernelGGL((k_embed_grad_scan<T, V, I>), dim3((unsigned)vocab, (unsigned)tiles), dim3(WG), 0, s,
-                             (const T*)g, (const I*)tokens, (int)n, channels, lanes, (S)scale, (T*)grad);
-        else
-          hipLaunchKernelGGL((k_embed_grad_part<T, V, I>), dim3((unsigned)wgs, tiles), dim3(WG), 0, s, (const T*)g,
-                             (const I*)tokens, order, rowptr, (int)vocab, channels, per, lanes, (S)scale, (T*)grad,
-                             (S*)work);
-      };
-      if (vec) run(std::integral_constant<int, W>());
-      else run(std::integral_constant<int, 1>());
-      if (!scans) {
-        const int columns = (channels + JOIN_COLS - 1) / JOIN_COLS, seams = wgs - 1;
-        const int64_t zeros = (vocab + 4 * columns - 1) / (4 * columns);
-        hipLaunchKernelGGL((k_embed_grad_join<T, I>), dim3((unsigned)(seams + (zeros < 2048 ? zeros : 2048)), columns),
-                           dim3(WG), 0, s, (const I*)tokens, order, rowptr, (int)vocab, channels, (int64_t)per * groups,
-                           seams, (S)scale, (const S*)work, (T*)grad);
-      }
-    };
-    if (index_bytes == 4) go(int32_t());
-    else go(int64_t());
+    row_moves<T>(
+        [&](int v, int bytes) { return channels % v == 0 && ((uintptr_t)g | (uintptr_t)grad) % bytes == 0; },
+        [&](auto vc) {
+          constexpr int V = decltype(vc)::value;
+          const int cw = channels / V, lanes = embed_lanes(cw), tiles = (cw + lanes - 1) / lanes;
+          const int per = embed_per(n, lanes), wgs = (int)embed_wgs(n, lanes), groups = WG / lanes;
+          hipStream_t s = (hipStream_t)stream;
+          auto go = [&](auto i) {
+            typedef decltype(i) I;
+            if (scans) {
+              hipLaunchKernelGGL((k_embed_grad_scan<T, V, I>), dim3((unsigned)vocab, (unsigned)tiles), dim3(WG), 0, s,
+                                 (const T*)g, (const I*)tokens, (int)n, channels, lanes, (S)scale, (T*)grad);
+              return;
+            }
+            hipLaunchKernelGGL((k_embed_grad_part<T, V, I>), dim3((unsigned)wgs, (unsigned)tiles), dim3(WG), 0, s,
+                               (const T*)g, (const I*)tokens, order, (int)n, (int)vocab, channels, per, lanes,
+                               (S)scale, (T*)grad, (S*)work);
+            const int columns = (channels + JOIN_COLS - 1) / JOIN_COLS, seams = wgs - 1;
+            const int64_t zeros = (vocab + 4 * columns - 1) / (4 * columns);
+            hipLaunchKernelGGL((k_embed_grad_join<T, I>),
+                               dim3((unsigned)(seams + (zeros < 2048 ? zeros : 2048)), (unsigned)columns), dim3(WG), 0,
+                               s, (const I*)tokens, order, rowptr, (int)vocab, channels, (int64_t)per * groups, seams,
+                               (S)scale, (const S*)work, (T*)grad);
+          };
+          if (index_bytes == 4) go(int32_t());
+          else go(int64_t());
+        });
   });
   return tace_check_launch("tace_embed_grad");
 }
@@ -544,19 +595,33 @@ extern "C" int tace_route_place(const int32_t* order, int64_t n, int32_t* place,
 
 namespace {
 
-// f(row type, elements a chunk, blocks in chunks, chunks a row)
+// Rows that go to scattered places are stored past the caches where they are
+// whole 128-byte lines (12,288 x 2 rows of 2,048 float32 50 us instead of 58),
+// not where two rows meet in a line (20,000 x 4 rows of 400 float16 27 instead
+// of 16).
+bool whole_lines(int32_t blocks, const int64_t* widths, int size) {
+  for (int b = 0; b < blocks; ++b)
+    if (widths[b] * size % 128) return false;
+  return true;
+}
+
 template <typename F>
-void route_go(int type, int32_t blocks, const int64_t* widths, bool aligned, F&& f) {
+void route_flag(bool on, F&& f) {
+  if (on) f(std::true_type());
+  else f(std::false_type());
+}
+
+// f(row type, elements a chunk, blocks in chunks, chunks a row); at: the rows'
+// addresses, or-ed
+template <typename F>
+void route_go(int type, int32_t blocks, const int64_t* widths, uintptr_t at, F&& f) {
   row_dispatch(type, [&](auto z) {
-    typedef decltype(z) T;
-    constexpr int W = 16 / sizeof(T);
     Blocks bl;
-    if (aligned && make_blocks(blocks, widths, W, &bl)) {
-      f(z, std::integral_constant<int, W>(), bl, bl.start[blocks]);
-    } else {
-      make_blocks(blocks, widths, 1, &bl);
-      f(z, std::integral_constant<int, 1>(), bl, bl.start[blocks]);
-    }
+    row_moves<decltype(z)>([&](int v, int bytes) { return at % bytes == 0 && make_blocks(blocks, widths, v, &bl); },
+                           [&](auto vc) {
+                             make_blocks(blocks, widths, decltype(vc)::value, &bl);
+                             f(z, vc, bl, bl.start[blocks]);
+                           });
   });
 }
 
@@ -569,15 +634,18 @@ extern "C" int tace_route_dispatch(int type, const void* x, const void* weights,
   if (tokens == 0) return 0;
   if (!x || !place || !rows_end || !out) return tace_fail_msg("tace_route_dispatch: null pointer");
   bool fits = true;
-  route_go(type, blocks, widths, row_aligned(x) && row_aligned(out), [&](auto z, auto vc, const Blocks& bl, unsigned cw) {
+  route_go(type, blocks, widths, (uintptr_t)x | (uintptr_t)out, [&](auto z, auto vc, const Blocks& bl, unsigned cw) {
     typedef decltype(z) T;
-    constexpr int V = decltype(vc)::value, U = 2;
+    constexpr int V = decltype(vc)::value;
     const RowChunks rc{tokens * cw, row_div(cw)};
-    const int64_t grid = (rc.total + WG * U - 1) / (WG * U);
+    const int64_t grid = (rc.total + WG - 1) / WG;
     fits = grid_ok(grid);
-    if (fits)
-      hipLaunchKernelGGL((k_route_dispatch<T, V, U>), dim3((unsigned)grid), dim3(WG), 0, (hipStream_t)stream,
-                         (const T*)x, (const row_sum_t<T>*)weights, place, rows_end, rc, tokens, k, bl, (T*)out);
+    if (!fits) return;
+    route_flag(whole_lines(blocks, widths, sizeof(T)), [&](auto st) {
+      hipLaunchKernelGGL((k_route_dispatch<T, V, decltype(st)::value>), dim3((unsigned)grid), dim3(WG), 0,
+                         (hipStream_t)stream, (const T*)x, (const row_sum_t<T>*)weights, place, rows_end, rc, tokens, k,
+                         bl, (T*)out);
+    });
   });
   if (!fits) return tace_fail_msg("tace_route_dispatch: too many rows");
   return tace_check_launch("tace_route_dispatch");
@@ -590,15 +658,21 @@ extern "C" int tace_route_combine(int type, const void* y, const void* weights, 
   if (tokens == 0) return 0;
   if (!y || !place || !rows_end || !out) return tace_fail_msg("tace_route_combine: null pointer");
   bool fits = true;
-  route_go(type, blocks, widths, row_aligned(y) && row_aligned(out), [&](auto z, auto vc, const Blocks& bl, unsigned cw) {
+  route_go(type, blocks, widths, (uintptr_t)y | (uintptr_t)out, [&](auto z, auto vc, const Blocks& bl, unsigned cw) {
     typedef decltype(z) T;
-    constexpr int V = decltype(vc)::value, U = 2;
+    constexpr int V = decltype(vc)::value;
     const RowChunks rc{tokens * cw, row_div(cw)};
-    const int64_t grid = (rc.total + WG * U - 1) / (WG * U);
+    const int64_t grid = (rc.total + WG - 1) / WG;
     fits = grid_ok(grid);
-    if (fits)
-      hipLaunchKernelGGL((k_route_combine<T, V, U>), dim3((unsigned)grid), dim3(WG), 0, (hipStream_t)stream,
-                         (const T*)y, (const row_sum_t<T>*)weights, place, rows_end, rc, tokens, k, bl, (T*)out);
+    if (!fits) return;
+    auto go = [&](auto kc) {
+      hipLaunchKernelGGL((k_route_combine<T, V, decltype(kc)::value>), dim3((unsigned)grid), dim3(WG), 0,
+                         (hipStream_t)stream, (const T*)y, (const row_sum_t<T>*)weights, place, rows_end, rc, tokens, k,
+                         bl, (T*)out);
+    };
+    if (k == 1) go(std::integral_constant<int, 1>());
+    else if (k == 2) go(std::integral_constant<int, 2>());
+    else go(std::integral_constant<int, 4>());
   });
   if (!fits) return tace_fail_msg("tace_route_combine: too many rows");
   return tace_check_launch("tace_route_combine");
@@ -610,16 +684,25 @@ extern "C" int tace_route_dots(int type, const void* x, const void* y, const voi
   if (const char* bad = route_bad(type, tokens, k, blocks, widths)) return tace_fail_msg(bad);
   if (tokens == 0) return 0;
   if (!x || !y || !place || !rows_end || !dots) return tace_fail_msg("tace_route_dots: null pointer");
-  route_go(type, blocks, widths, row_aligned(x) && row_aligned(y) && (!g_y || row_aligned(g_y)),
+  bool fits = true;
+  route_go(type, blocks, widths, (uintptr_t)x | (uintptr_t)y | (uintptr_t)g_y,
            [&](auto z, auto vc, const Blocks& bl, unsigned cw) {
              typedef decltype(z) T;
              constexpr int V = decltype(vc)::value;
              int lanes = 1;
              while (lanes < 64 && (unsigned)lanes < cw) lanes *= 2;
-             const int groups = WG / lanes;
-             hipLaunchKernelGGL((k_route_dots<T, V>), dim3((unsigned)((tokens + groups - 1) / groups)), dim3(WG), 0,
-                                (hipStream_t)stream, (const T*)x, (const T*)y, (const row_sum_t<T>*)weights, place,
-                                rows_end, tokens, k, lanes, cw, bl, (T*)g_y, (row_sum_t<T>*)dots);
+             const int64_t groups = WG / lanes, grid = (tokens * k + groups - 1) / groups;
+             fits = grid_ok(grid);
+             if (!fits) return;
+             auto go = [&](auto uc) {
+               hipLaunchKernelGGL((k_route_dots<T, V, decltype(uc)::value>), dim3((unsigned)grid), dim3(WG), 0,
+                                  (hipStream_t)stream, (const T*)x, (const T*)y, (const row_sum_t<T>*)weights, place,
+                                  rows_end, tokens, k, lanes, cw, bl, (T*)g_y, (row_sum_t<T>*)dots);
+             };
+             if (cw <= (unsigned)lanes) go(std::integral_constant<int, 1>());
+             else if (cw <= 2u * lanes) go(std::integral_constant<int, 2>());
+             else go(std::integral_constant<int, 4>());
            });
+  if (!fits) return tace_fail_msg("tace_route_dots: too many rows");
   return tace_check_launch("tace_route_dots");
 }
