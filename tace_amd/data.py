@@ -86,7 +86,10 @@ def gpu_graph(structs: List[Dict], atomic_numbers: Sequence[int], cutoff: float,
     g["edge_shifts"] = g["edge_shifts"].to(dtype)
     # per-species node counts (columns of node_attrs), known here on the host
     g["_species_counts"] = attrs_h.sum(0).to(torch.int64).tolist()
-    return dict(positions=p64.to(dtype), node_attrs=up(attrs_h), lattice=lat, batch=batch, ptr=up(ptr), **g)
+    attrs = up(attrs_h)
+    # these rows (as they are now) are one-hot: what reads them may look up instead of multiplying
+    g["_one_hot"] = (attrs, attrs._version)
+    return dict(positions=p64.to(dtype), node_attrs=attrs, lattice=lat, batch=batch, ptr=up(ptr), **g)
 
 
 _CELLS: Dict = {}

@@ -303,9 +303,9 @@ uuu_backward.register_autograd(_uuu_bwd_backward, setup_context=_uuu_bwd_setup)
 # ------------------------------------------------------- per-species linear ----
 # ``e3nnElementLinear`` (tace/models/linear.py:377-481) for the exported model:
 # features in node order (group-major), the species of every node as an int64
-# tensor.  Inside the operator the rows are grouped by species and the
-# segmented GEMM runs (what the eager model does once per forward with its
-# species plan); the operator's backward gives the input gradient (exported
+# tensor.  Inside the operator the rows are sorted by species (each atom has one
+# "expert") and the segmented GEMM runs (what the eager model does once per
+# forward with its species plan); the operator's backward gives the input gradient (exported
 # models are evaluated with frozen parameters).
 _LIN_LAYOUTS = {}
 
@@ -318,29 +318,30 @@ def _lin_layout(irreps_in: str, irreps_out: str):
     return _LIN_LAYOUTS[key]
 
 
-def _gm_take(x: Tensor, gm, idx: Tensor) -> Tensor:
-    """Rows ``idx`` of group-major features (every block gathered by node)."""
-    Z = x.shape[0]
-    flat = x.reshape(-1)
-    out = [flat[Z * s:Z * (s + m * d)].view(Z, d * m).index_select(0, idx).reshape(-1) for (s, m, d) in gm.blocks]
-    return torch.cat(out).view(idx.shape[0], -1)
-
-
-def _element_linear_sorted(x, weight, bias, species, irreps_in, irreps_out, alpha):
-    from .model import SpeciesPlan, _LinearFn
-    lay = _lin_layout(irreps_in, irreps_out)
-    sp = SpeciesPlan(torch.nn.functional.one_hot(species, weight.shape[0]).to(x.dtype))
-    xs = _gm_take(x, lay.gin, sp.perm).contiguous()
-    return lay, sp, xs
+def _gm_route(route, x: Tensor, gm, plan: ops.RoutePlan) -> Tensor:
+    """``ops.expert_dispatch`` or ``ops.expert_combine`` of group-major
+    features, as many blocks at a time as one call takes."""
+    widths = [m * d for (s, m, d) in gm.blocks]
+    if len(widths) <= ops.ROW_BLOCKS and gm.dim <= ops.ROW_MAX:
+        return route(x, plan, widths=widths)
+    Z, flat, out = x.shape[0], x.reshape(-1), []
+    for (s, m, d) in gm.blocks:
+        # (a block's columns are rows of their own beyond the widest call)
+        cols = flat[Z * s:Z * (s + m * d)].view(Z, m * d).split(ops.ROW_MAX, 1)
+        out += [torch.cat([route(c, plan) for c in cols], 1).reshape(-1)]
+    return torch.cat(out).view(Z, -1)
 
 
 @torch.library.custom_op("tace_amd::element_linear", mutates_args=(), device_types="cuda")
 def element_linear(x: Tensor, weight: Tensor, bias: Optional[Tensor], species: Tensor, irreps_in: str,
                    irreps_out: str, alpha: float) -> Tensor:
     from .model import _LinearFn
-    lay, sp, xs = _element_linear_sorted(x, weight, bias, species, irreps_in, irreps_out, alpha)
-    ys = _LinearFn.apply(xs, weight, bias, lay, sp.ranges, alpha)
-    return _gm_take(ys, lay.gout, sp.inv)
+    lay = _lin_layout(irreps_in, irreps_out)
+    with torch.no_grad():
+        plan = ops.route_plan(species, weight.shape[0])
+        xs = _gm_route(ops.expert_dispatch, x, lay.gin, plan)
+        ys = _LinearFn.apply(xs, weight, bias, lay, plan.ranges, alpha)
+        return _gm_route(ops.expert_combine, ys, lay.gout, plan)
 
 
 @element_linear.register_fake
@@ -352,13 +353,17 @@ def _element_linear_fake(x, weight, bias, species, irreps_in, irreps_out, alpha)
 def element_linear_backward(x: Tensor, weight: Tensor, species: Tensor, grad_out: Tensor, irreps_in: str,
                             irreps_out: str, alpha: float) -> Tensor:
     from .model import _LinearFn
-    lay, sp, xs = _element_linear_sorted(x, weight, None, species, irreps_in, irreps_out, alpha)
-    gs = _gm_take(grad_out.contiguous(), lay.gout, sp.perm)
+    lay = _lin_layout(irreps_in, irreps_out)
+    with torch.no_grad():
+        plan = ops.route_plan(species, weight.shape[0])
+        xs = _gm_route(ops.expert_dispatch, x, lay.gin, plan)
+        gs = _gm_route(ops.expert_dispatch, grad_out.contiguous(), lay.gout, plan)
     with torch.enable_grad():
         xs = xs.detach().requires_grad_(True)
-        ys = _LinearFn.apply(xs, weight.detach(), None, lay, sp.ranges, alpha)
+        ys = _LinearFn.apply(xs, weight.detach(), None, lay, plan.ranges, alpha)
         (gx,) = torch.autograd.grad(ys, xs, gs)
-    return _gm_take(gx, lay.gin, sp.inv)
+    with torch.no_grad():
+        return _gm_route(ops.expert_combine, gx, lay.gin, plan)
 
 
 @element_linear_backward.register_fake

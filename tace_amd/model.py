@@ -24,6 +24,7 @@ from __future__ import annotations
 
 import collections
 import copy
+import functools
 import math
 import random
 from typing import Dict, List, Optional, Sequence, Tuple
@@ -49,10 +50,14 @@ class SpeciesPlan:
     _last = None
 
     def __init__(self, attrs: torch.Tensor, exchange=None, pairs: Optional[ops.EdgePairs] = None,
-                 natural: bool = False, counts: Optional[List[int]] = None):
+                 natural: bool = False, counts: Optional[List[int]] = None, one_hot: bool = False, masks=None):
         """counts: the number of nodes of each species (attrs column), when
-        the caller knows them on the host; else they are read back from attrs."""
+        the caller knows them on the host; else they are read back from attrs.
+        one_hot: attrs is known to be one-hot.  masks: this forward's dropout
+        (``_Masks``), or None."""
         self.attrs = attrs
+        self.one_hot = one_hot
+        self.masks = masks
         # LAMMPS ML-IAP data whose forward_exchange fills ghost rows before
         # every interaction layer >= 1 (several domains), or None
         self.exchange = exchange
@@ -792,6 +797,8 @@ class O3CgtpInteraction(torch.nn.Module):
         # linear_down(m) / avg_num_neighbors, the division in the GEMM scale
         m = self.linear_down(m, alpha=1.0 / self.avg_num_neighbors)
         m = self.linear_nonlinearity(_gate(m, *self._gate_lay, self.C))
+        if sp.masks is not None:
+            m = sp.masks.features(m, self.irreps_out, self.layer)
         return m, sc
 
 
@@ -841,7 +848,9 @@ class TeceInteraction(torch.nn.Module):
         x = _exchange_ghosts(self.linear_up(x), self.linear_up.irreps_out, sp, self.layer)
         if ops.MODE.double:
             # training: the whole convolution as torch operations (twice differentiable)
-            msg = self.rejector(x, self.edge_info(R), plan, sp.node_map, src, dst, wigner, R)
+            drop = None if sp.masks is None else functools.partial(sp.masks.attention, layer=self.layer)
+            msg = self.rejector(x, self.edge_info(R), plan, sp.node_map, src, dst, wigner, R,
+                                *(() if drop is None else (drop,)))
         elif tece.FUSED and tece.fused_supported(self.rejector, self.edge_info):
             msg = tece.tece_fused(self.rejector, self.edge_info, x, sp.node_map, R, plan, src, dst, wigner,
                                   self.chunk_edges)
@@ -851,6 +860,8 @@ class TeceInteraction(torch.nn.Module):
             msg = self._chunked(x, sp, R, plan, src, dst, wigner)
         m = self.linear_down(msg)
         m = self.linear_nonlinearity(_gate(m, *self._gate_lay, self.C))
+        if sp.masks is not None:
+            m = sp.masks.features(m, self.irreps_out, self.layer)
         return m, sc
 
 
@@ -1153,12 +1164,23 @@ class _Buffers(torch.nn.Module):
 
 
 class LinearNodeEmbedding(torch.nn.Module):
+    """A linear of the one-hot species (``tace/models/_e3nn/node.py:22-55``).
+    Training looks its rows up where the attributes are known to be one-hot:
+    the same rows without a product, and a weight gradient that sums each
+    species' rows in a fixed order."""
+
     def __init__(self, S, C):
         super().__init__()
         self.elem_emb1 = e3nnLinear(f"{S}x0e", f"{C}x0e", bias=False)
 
-    def forward(self, attrs):
-        return self.elem_emb1(attrs)
+    def forward(self, attrs, species=None):
+        """attrs [N, S]; species [N]: their columns, where attrs is one-hot."""
+        lin = self.elem_emb1
+        if species is not None and type(lin) is e3nnLinear and "forward" not in vars(lin) and not _hooked(lin):
+            S, C = lin.lay.dim_in, lin.lay.dim_out
+            if C <= ops.ROW_MAX and lin.weight.dtype in (torch.float32, torch.float64):
+                return ops.embedding(lin.weight.view(S, C), species, lin.lay.ins[0][5])
+        return lin(attrs)
 
 
 class RadialBasis(torch.nn.Module):
@@ -1286,7 +1308,11 @@ class Representation(torch.nn.Module):
         """Node features (group-major, rows in ``sp``'s species-sorted order)."""
         R, Y = self.edge_features(edge_vector)
         wigner = ops.edge_wigner(edge_vector, self.lmax) if self.use_so2 else None
-        x = self.node_embedding(attrs.index_select(0, sp.perm))
+        if (sp.one_hot and ops.MODE.double and not ops.MODE.export and not attrs.requires_grad
+                and type(self.node_embedding) is LinearNodeEmbedding and not _hooked(self.node_embedding)):
+            x = self.node_embedding(attrs.index_select(0, sp.perm), sp.species.index_select(0, sp.perm))
+        else:
+            x = self.node_embedding(attrs.index_select(0, sp.perm))
         for inter, prod in zip(self.interactions, self.products):
             if isinstance(inter, TeceInteraction):
                 x, sc = inter(x, sp, R, plan, edge_index[0], edge_index[1], wigner)
@@ -1298,6 +1324,8 @@ class Representation(torch.nn.Module):
 
 class TACE(torch.nn.Module):
     """MI355X ``e3nnTACE`` (energy readout; ``tace/models/_e3nn/tace.py:28-790``)."""
+
+    dropout: Optional["Dropout"] = None   # of the training mode (``set_dropout``)
 
     def __init__(self, **cfg):
         super().__init__()
@@ -1364,7 +1392,12 @@ class TACE(torch.nn.Module):
         so callers that want per-edge gradients pass None)."""
         attrs, batch, ptr = data["node_attrs"], data["batch"], data["ptr"]
         num_graphs = ptr.numel() - 1
-        sp = SpeciesPlan(attrs, exchange, pairs, natural=ops.MODE.export, counts=_opt(data, "_species_counts"))
+        hot = _opt(data, "_one_hot")
+        masks = None
+        if self.dropout is not None and self.training and ops.MODE.double and not ops.MODE.export:
+            masks = self.dropout.step_masks()
+        sp = SpeciesPlan(attrs, exchange, pairs, natural=ops.MODE.export, counts=_opt(data, "_species_counts"),
+                         one_hot=hot is not None and hot[0] is attrs and hot[1] == attrs._version, masks=masks)
         x = self.representation(attrs, plan, edge_vector, sp, data["edge_index"])
         if self._head_fits(x, attrs, plan, sp):
             l1, l2 = self.energy_readouts[0].linear2
@@ -1414,6 +1447,63 @@ def set_tece_channel_mixing(model: torch.nn.Module, dtype: Optional[torch.dtype]
         if isinstance(m, TeceConvolution):
             m.mixing = dtype
             n += 1
+    return n
+
+
+class Dropout:
+    """Dropout of the training mode (``set_dropout``): probabilities, seed, and
+    the number of forwards drawn for, which is the mask's counter.  ``step`` may
+    be set to repeat or resume a run's masks."""
+
+    def __init__(self, features: float, attention: float, seed: int):
+        self.features, self.attention, self.seed, self.step = float(features), float(attention), int(seed), 0
+
+    def step_masks(self) -> "_Masks":
+        self.step += 1
+        return _Masks(self, (self.seed, self.step))
+
+
+class _Masks:
+    """One forward's dropout: every layer draws at a site of its own."""
+
+    def __init__(self, drop: Dropout, rng):
+        self.drop, self.rng = drop, rng
+
+    def features(self, x: torch.Tensor, irreps, layer: int) -> torch.Tensor:
+        """Group-major node features: one draw per (node, irrep, channel), all
+        its components kept or dropped together."""
+        if self.drop.features == 0.0:
+            return x
+        assert len({m for m, _ in irreps}) == 1, irreps
+        return ops.dropout(x, self.drop.features, self.rng, site=2 * layer, components=[ir.dim for _, ir in irreps])
+
+    def attention(self, alpha: torch.Tensor, layer: int) -> torch.Tensor:
+        """Attention weights [E, H] of a TECE layer."""
+        if self.drop.attention == 0.0:
+            return alpha
+        return ops.dropout(alpha, self.drop.attention, self.rng, site=2 * layer + 1)
+
+
+def set_dropout(model: torch.nn.Module, features: float = 0.0, attention: float = 0.0, seed: int = 0) -> int:
+    """Dropout in the training mode of ``model`` (a TensorModel or TACE):
+    ``features`` the probability that a channel of an irrep of an atom is dropped
+    from an interaction's output (all 2l+1 components together, so rotated
+    structures give rotated outputs under the same mask), ``attention`` that of
+    an (edge, head) attention weight of the TECE layers.  Energies, forces and
+    stress of one forward are derivatives of the same masked energy.  The masks
+    are functions of (seed, forward, layer, index), ``ops.dropout``; give every
+    rank of a data-parallel run a seed of its own.  Zeros switch it off;
+    evaluation never drops.  Returns the number of interactions it applies to."""
+    for name, p in (("features", features), ("attention", attention)):
+        if not (p == 0.0 or 2.0 ** -17 < p < 1.0 - 2.0 ** -17):
+            raise ValueError(f"dropout of {name}: {p} is not 0 or a probability inside (0, 1) of the mask's 2^-16")
+    top = [m for m in model.modules() if isinstance(m, TACE)]
+    if not top:
+        raise ValueError("set_dropout needs a TensorModel or TACE")
+    n = 0
+    for m in top:
+        m.dropout = Dropout(features, attention, seed) if features or attention else None
+        n += sum(bool(features or (attention and isinstance(i, TeceInteraction))) for i in m.representation.interactions)
     return n
 
 

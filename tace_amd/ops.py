@@ -1504,10 +1504,14 @@ def sender_csr(rows_src: torch.Tensor, n_rows: int) -> Tuple[torch.Tensor, torch
 # bfloat16 and float16 rows, sums in float64 for float64 rows and in float32
 # for the others.  Every backward is made of the same operators, so each can be
 # differentiated any number of times.
+ROW_MAX = 32768   # elements a row
+ROW_BLOCKS = 8    # blocks a row
+
+
 def embedding(table: torch.Tensor, tokens: torch.Tensor, scale: float = 1.0,
               groups: Optional[Tuple[torch.Tensor, torch.Tensor]] = None) -> torch.Tensor:
     """``scale * table[tokens]``: rows of ``table`` [V, C] for integer
-    ``tokens`` of any shape.  A token outside [0, V) (padding) gives a row of
+    ``tokens`` of any shape, C up to ``ROW_MAX``.  A token outside [0, V) (padding) gives a row of
     zeros and takes no gradient.  The table's gradient sums each token's rows in
     an order that depends on the sizes alone (the same bits on every run) and
     rounds once.  ``groups``: ``group_by_key(tokens.reshape(-1), V)`` where the
@@ -1568,8 +1572,9 @@ def expert_dispatch(x: torch.Tensor, plan: RoutePlan, weights: Optional[torch.Te
     """Rows ``x`` [T, D] sorted by expert: [T k, D], row ``plan.place[s]`` =
     (``weights[s]`` times) the row of slot s's token; rows of dropped slots
     (from ``plan.rowptr[-1]`` on) are zeros.  ``widths``: group-major features
-    (``model.GMLayout``), the element counts of their blocks, each of which
-    lies in memory as [rows, width] after the one before; None: ordinary rows.
+    (``model.GMLayout``), the element counts of their blocks (at most
+    ``ROW_BLOCKS``), each of which lies in memory as [rows, width] after the one
+    before; None: ordinary rows.  D is at most ``ROW_MAX``.
     Differentiable any number of times in x and weights."""
     return N.rows().route(False, x, plan.place, plan.rowptr, plan.n_tokens, plan.k, weights, widths, TIMER is not None)
 

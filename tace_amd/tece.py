@@ -276,7 +276,7 @@ class TeceConvolution(torch.nn.Module):
         T = self.tmin + (self.tmax - self.tmin) * torch.sigmoid(self.temperature_logit)
         return s * (self.attention_scale * T) + bias
 
-    def _forward_autograd(self, x_gm, w, node_map, src, dst, wigner, R):
+    def _forward_autograd(self, x_gm, w, node_map, src, dst, wigner, R, drop=None):
         """The whole convolution as torch operations (the per-edge kernels'
         arithmetic; ``oam_2026_07_05.py:756-823``): what training with a force
         loss differentiates twice.  Same inputs and output as ``forward``."""
@@ -305,13 +305,15 @@ class TeceConvolution(torch.nn.Module):
             0, rd.view(-1, 1).expand(-1, H), score.detach(), reduce="amax", include_self=True)
         ex = torch.exp(score - mx[rd])
         alpha = ex / (torch.zeros(Nn, H, dtype=score.dtype, device=dev).index_add(0, rd, ex) + 1e-16)[rd]
+        if drop is not None:
+            alpha = drop(alpha)
         m = (m.view(E, K, H, self.Ch) * alpha.view(E, 1, H, 1)).view(E, K, C)
         m = torch.bmm(wigner.transpose(1, 2), m)
         out = torch.zeros(Nn, K, C, dtype=m.dtype, device=dev).index_add(0, rd, m)
         # [rows, K, C] (l layout) -> group-major C x (0..lmax)
         return torch.cat([out[:, l * l:(l + 1) ** 2].reshape(-1) for l in range(self.lmax + 1)]).view(Nn, K * C)
 
-    def _forward_train(self, x_gm, w, plan: ops.EdgePlan, node_map, src, dst, wigner, R):
+    def _forward_train(self, x_gm, w, plan: ops.EdgePlan, node_map, src, dst, wigner, R, drop=None):
         """Training (twice differentiable): the rotate-in and the rotate-out
         (gathers, rotations, radial weighting, attention weighting and
         receiver sums) on their HIP kernels through operators whose backward is
@@ -337,6 +339,8 @@ class TeceConvolution(torch.nn.Module):
             0, rd.view(-1, 1).expand(-1, H), score.detach(), reduce="amax", include_self=True)
         ex = torch.exp(score - mx[rd])
         alpha = ex / (torch.zeros(Nn, H, dtype=score.dtype, device=w.device).index_add(0, rd, ex) + 1e-16)[rd]
+        if drop is not None:
+            alpha = drop(alpha)
         return ops.tece_rotate_out_twice(ops.so2_to_blocks(m, L), alpha, wigner, plan, node_map, dst, L, H)
 
     def _forward_library(self, x_gm, w, plan, src, dst, wigner, R):
@@ -357,18 +361,19 @@ class TeceConvolution(torch.nn.Module):
         m = self.linear_down.blocks(o, self.mixing)
         return library.tece_rotate_out(m, alpha, wigner, rowptr, eid, dst, L, H)
 
-    def forward(self, x_gm, w, plan: ops.EdgePlan, node_map, src, dst, wigner, R):
+    def forward(self, x_gm, w, plan: ops.EdgePlan, node_map, src, dst, wigner, R, drop=None):
         """x_gm: node features, group-major C x (0..lmax) in feature-row order;
         w: radial weights [E, weight_numel]; node_map[n] = feature row of node
         n; src/dst: edge endpoints (node ids); wigner [E, K, K] from
-        ``ops.edge_wigner``; R: radial basis [E, num_radial].  Returns the
-        receiver sums, group-major, in feature-row order."""
+        ``ops.edge_wigner``; R: radial basis [E, num_radial]; drop (training):
+        applied to the attention weights [E, H].  Returns the receiver sums,
+        group-major, in feature-row order."""
         if ops.MODE.export:
             return self._forward_library(x_gm, w, plan, src, dst, wigner, R)
         if ops.MODE.double:
             if TRAIN_ON_KERNELS and isinstance(plan, ops.EdgePlan):
-                return self._forward_train(x_gm, w, plan, node_map, src, dst, wigner, R)
-            return self._forward_autograd(x_gm, w, node_map, src, dst, wigner, R)
+                return self._forward_train(x_gm, w, plan, node_map, src, dst, wigner, R, drop)
+            return self._forward_autograd(x_gm, w, node_map, src, dst, wigner, R, drop)
         rows = node_map.long()
         return self.edges(self.node_components(x_gm), w, rows[src], rows[dst], plan, node_map, dst, wigner, R)
 

@@ -4,7 +4,6 @@ import ctypes
 import os
 import re
 
-import numpy as np
 import pytest
 import torch
 
@@ -98,3 +97,18 @@ def test_workspace_covers_every_workgroup():
                 assert nbytes % (2 * C * size) == 0
                 assert 1 <= nbytes // (2 * C * size) <= 512
     _refused(L.tace_embed_grad(0, 8, 4096, 4096, 4096, 4096, 0, 4, 4, 1.0, 4096, 4096, 16, None), b"no rows")
+
+
+def test_set_dropout_arguments():
+    from tace_amd import configs, model as pm
+
+    m = pm.create_model(configs.model_cfg("tece", [26], 58.0, num_channel=16, num_head=2, edge_ace_hidden=8))
+    before = set(m.state_dict())
+    assert pm.set_dropout(m, features=0.1) == 2 and pm.set_dropout(m, attention=0.1) == 1   # (layer 0 has none)
+    assert m.readout_fn.dropout.attention == 0.1 and set(m.state_dict()) == before
+    for bad in (dict(features=-0.1), dict(features=1.0), dict(attention=1e-7), dict(features=float("nan"))):
+        with pytest.raises(ValueError, match="dropout of"):
+            pm.set_dropout(m, **bad)
+    with pytest.raises(ValueError, match="TensorModel"):
+        pm.set_dropout(torch.nn.Linear(2, 2), 0.1)
+    assert pm.set_dropout(m) == 0 and m.readout_fn.dropout is None
