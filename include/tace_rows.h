@@ -17,7 +17,7 @@
 extern "C" {
 #endif
 
-#define TACE_ROWS_ABI_VERSION 1
+#define TACE_ROWS_ABI_VERSION 2
 #define TACE_ROW_F32 0
 #define TACE_ROW_F64 1
 #define TACE_ROW_BF16 2
@@ -33,7 +33,7 @@ int tace_embed_fwd(int type, int index_bytes, const void* table, const void* tok
 
 /* grad [vocab, channels]: row v is scale * the sum of g's rows (g [n,
  * channels]) whose token is v, zeros without any; the order of the sum depends
- * on the sizes alone.  order [n] and rowptr [vocab + 1] are tace_group_keys'
+ * on the sizes alone.  order [n] and rowptr [vocab + 1] are tace_route_group's
  * of the tokens; work: tace_embed_grad_work bytes (16-byte aligned).
  * order NULL: no grouping and no work are read, every token looks through all
  * of tokens (for few rows and tokens: tace_embed_grad_scans says where; the
@@ -44,13 +44,19 @@ int tace_embed_grad(int type, int index_bytes, const void* g, const void* tokens
                     const int32_t* rowptr, int64_t n, int64_t vocab, int32_t channels, double scale, void* grad,
                     void* work, int64_t work_bytes, void* stream);
 
-/* Tokens sorted by expert.  Slot s = t k + j is choice j of token t; order [n
- * = tokens k] and rowptr [experts + 1] are tace_group_keys' of the slots'
- * experts, place[order[r]] = r.  rows_end points to rowptr[experts]: rows from
- * there on belong to dropped slots.  Rows are `blocks` blocks of widths[b]
- * elements (host array); a batch of R rows holds block after block, each [R,
- * widths[b]] (blocks = 1: ordinary rows). */
-int tace_route_place(const int32_t* order, int64_t n, int32_t* place, void* stream);
+/* Positions 0 .. n-1 grouped by key, as tace_group_keys orders them (order
+ * [n], rowptr [n_keys + 1]; positions with a key outside [0, n_keys) last), and
+ * place [n] (may be NULL), place[order[r]] = r.  Key i is keys[i * stride], of
+ * index_bytes 4 or 8.  work: tace_route_group_work int32.
+ *
+ * Tokens sorted by expert: slot s = t k + j is choice j of token t, its key the
+ * expert; n = tokens k.  rows_end points to rowptr[experts]: rows from there on
+ * belong to dropped slots.  Rows are `blocks` blocks of widths[b] elements (host
+ * array); a batch of R rows holds block after block, each [R, widths[b]]
+ * (blocks = 1: ordinary rows). */
+int64_t tace_route_group_work(int64_t n, int64_t n_keys);
+int tace_route_group(int index_bytes, const void* keys, int64_t stride, int64_t n, int64_t n_keys, int32_t* rowptr,
+                     int32_t* order, int32_t* place, int32_t* work, void* stream);
 /* out row place[s] = weights[s] x row t(s) (weights NULL: 1), zeros where s is dropped */
 int tace_route_dispatch(int type, const void* x, const void* weights, const int32_t* place, const int32_t* rows_end,
                         int64_t tokens, int32_t k, int32_t blocks, const int64_t* widths, void* out, void* stream);

@@ -1,5 +1,6 @@
 // Row operators: table lookup by token with its gradient, rows sorted by
 // expert and back.  All of them move rows once and are bound by HBM.
+#include "../../include/tace_hip.h"
 #include "row_types.h"
 
 #include <algorithm>
@@ -325,6 +326,153 @@ __global__ __launch_bounds__(WG) void k_route_place(const int* __restrict__ orde
   if (i < n) place[order[i]] = (int)i;
 }
 
+// Stable grouping by few keys (at most 255, and one for keys outside them): a
+// workgroup of 16 wavefronts has 1,024 `steps` positions in runs of 64 `steps`
+// a wavefront.  k_few_count leaves its counts of every key; k_few_place adds up
+// those of the workgroups before it and of all, ranks its own positions by
+// ballots and writes their places.  One workgroup (n <= 8,192) counts for
+// itself.  us, with the launches' gaps: 24,576 slots of 8 experts 11 instead of
+// 29 by the general grouping (tace_group_keys: any keys, four launches a digit
+// and one for the places).
+constexpr int FEW_WG = 1024, FEW_STEPS = 8, FEW_KEYS = 256, FEW_WGS = 128;
+
+template <typename I>
+__device__ __forceinline__ int few_key(I e, int n_keys) { return e >= 0 && e < (I)n_keys ? (int)e : n_keys; }
+
+template <typename I>
+__global__ __launch_bounds__(FEW_WG) void k_few_count(const I* __restrict__ keys, int64_t stride, int n, int n_keys,
+                                                      int steps, int* __restrict__ hist) {
+  __shared__ int cnt[FEW_KEYS];
+  const int t = (int)threadIdx.x;
+  if (t < FEW_KEYS) cnt[t] = 0;
+  __syncthreads();
+  const int64_t i0 = (int64_t)blockIdx.x * FEW_WG * steps + t;
+  I e[FEW_STEPS];
+#pragma unroll
+  for (int u = 0; u < FEW_STEPS; ++u)
+    if (u < steps) e[u] = keys[min(i0 + FEW_WG * u, (int64_t)n - 1) * stride];
+#pragma unroll
+  for (int u = 0; u < FEW_STEPS; ++u)
+    if (u < steps && i0 + FEW_WG * u < n) atomicAdd(cnt + few_key(e[u], n_keys), 1);
+  __syncthreads();
+  if (t <= n_keys) hist[(int64_t)blockIdx.x * (n_keys + 1) + t] = cnt[t];
+}
+
+template <typename I>
+__global__ __launch_bounds__(FEW_WG) void k_few_place(const I* __restrict__ keys, int64_t stride, int n, int n_keys,
+                                                      int steps, int bits, const int* __restrict__ hist,
+                                                      int* __restrict__ rowptr, int* __restrict__ order,
+                                                      int* __restrict__ place) {
+  constexpr int WAVES = FEW_WG / 64;
+  __shared__ int cnt[WAVES][FEW_KEYS], red[FEW_WG], before[FEW_KEYS], total[FEW_KEYS], wsum[4];
+  const int t = (int)threadIdx.x, lane = t & 63, w = t >> 6, nwg = (int)gridDim.x, K = n_keys + 1;
+  for (int q = t; q < WAVES * FEW_KEYS; q += FEW_WG) cnt[q / FEW_KEYS][q % FEW_KEYS] = 0;
+  const int64_t i0 = ((int64_t)blockIdx.x * WAVES + w) * 64 * steps + lane;
+  I e[FEW_STEPS];
+#pragma unroll
+  for (int u = 0; u < FEW_STEPS; ++u)
+    if (u < steps) e[u] = keys[min(i0 + 64 * u, (int64_t)n - 1) * stride];
+  // counts of the workgroups before this one, and of all: 2^bits keys side by
+  // side, the workgroups dealt to the threads of a key
+  int bef = 0, all = 0;
+  if (nwg > 1) {
+    const int wide = 1 << bits, key = t & (wide - 1);
+    if (key < K)
+      for (int g = t >> bits; g < nwg; g += FEW_WG >> bits) {
+        const int c = hist[(int64_t)g * K + key];
+        all += c;
+        bef += g < (int)blockIdx.x ? c : 0;
+      }
+    for (int o = FEW_WG / 2; o >= wide; o >>= 1) {   // (two sums, one after the other)
+      red[t] = bef;
+      __syncthreads();
+      if (t < o) bef += red[t + o];
+      __syncthreads();
+      red[t] = all;
+      __syncthreads();
+      if (t < o) all += red[t + o];
+      __syncthreads();
+    }
+    if (t < K) {
+      before[t] = bef;
+      total[t] = all;
+    }
+  }
+  __syncthreads();
+  int key[FEW_STEPS], rank[FEW_STEPS];
+#pragma unroll
+  for (int u = 0; u < FEW_STEPS; ++u) {
+    const bool in = u < steps && i0 + 64 * u < n;
+    key[u] = in ? few_key(e[u], n_keys) : -1;
+    if (u >= steps) continue;   // (all lanes alike)
+    const int k = key[u];
+    // this lane's place among its wavefront's equal keys so far
+    unsigned long long m = __ballot(in);
+    for (int b = 0; b < bits; ++b) {
+      const bool one = (k >> b) & 1;
+      const unsigned long long v = __ballot(one);
+      m &= one ? v : ~v;
+    }
+    const int r = __popcll(m & ((1ull << lane) - 1));
+    int had = 0;
+    if (in && r == 0) had = atomicAdd(&cnt[w][k], __popcll(m));
+    rank[u] = r + __shfl(had, in ? __ffsll((long long)m) - 1 : lane, 64);
+  }
+  __syncthreads();
+  // a key's first place: all smaller keys, its own in the workgroups and in the
+  // wavefronts before
+  int own = 0;
+  if (t < FEW_KEYS)
+    for (int k = 0; k < WAVES; ++k) own += cnt[k][t];
+  const int sum = t < K ? (nwg > 1 ? total[t] : own) : 0;
+  int inc = sum;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int v = __shfl_up(inc, o, 64);
+    if (lane >= o) inc += v;
+  }
+  if (w < 4 && lane == 63) wsum[w] = inc;
+  __syncthreads();
+  if (t < FEW_KEYS) {
+    int at = inc - sum;
+    for (int k = 0; k < w; ++k) at += wsum[k];
+    if (t < K && blockIdx.x == 0) rowptr[t] = at;   // (key n_keys: the end of the others)
+    if (nwg > 1 && t < K) at += before[t];
+    for (int k = 0; k < WAVES; ++k) {
+      const int c = cnt[k][t];
+      cnt[k][t] = at;
+      at += c;
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int u = 0; u < FEW_STEPS; ++u) {
+    if (key[u] < 0) continue;
+    const int i = (int)(i0 + 64 * u), at = cnt[w][key[u]] + rank[u];
+    order[at] = i;
+    if (place) place[i] = at;
+  }
+}
+
+// whether few_group takes it, and its workgroups and steps
+bool few_fits(int64_t n, int64_t n_keys, int* wgs, int* steps) {
+  const int64_t most = n <= FEW_WG * FEW_STEPS ? 1 : FEW_WGS;
+  *steps = (int)std::min<int64_t>((n + FEW_WG * most - 1) / (FEW_WG * most), FEW_STEPS + 1);
+  *wgs = *steps ? (int)((n + FEW_WG * *steps - 1) / (FEW_WG * *steps)) : 0;
+  return n >= 1 && n_keys < FEW_KEYS && *steps <= FEW_STEPS;
+}
+
+template <typename I>
+void few_group(const I* keys, int64_t stride, int n, int n_keys, int wgs, int steps, int32_t* rowptr, int32_t* order,
+               int32_t* place, int32_t* work, hipStream_t s) {
+  int bits = 1;
+  while ((1 << bits) < n_keys + 1) ++bits;
+  if (wgs > 1)
+    hipLaunchKernelGGL((k_few_count<I>), dim3((unsigned)wgs), dim3(FEW_WG), 0, s, keys, stride, n, n_keys, steps, work);
+  hipLaunchKernelGGL((k_few_place<I>), dim3((unsigned)wgs), dim3(FEW_WG), 0, s, keys, stride, n, n_keys, steps, bits,
+                     work, rowptr, order, place);
+}
+
 // STREAM: stores that do not stay in the caches
 template <bool STREAM, typename Vec>
 __device__ __forceinline__ void put(Vec* p, const Vec& v) {
@@ -584,13 +732,34 @@ extern "C" int tace_embed_grad(int type, int index_bytes, const void* g, const v
   return tace_check_launch("tace_embed_grad");
 }
 
-extern "C" int tace_route_place(const int32_t* order, int64_t n, int32_t* place, void* stream) {
-  if (n < 0 || n > INT32_MAX - 8192) return tace_fail_msg("tace_route_place: bad sizes");
-  if (n == 0) return 0;
-  if (!order || !place) return tace_fail_msg("tace_route_place: null pointer");
-  hipLaunchKernelGGL(k_route_place, dim3((unsigned)((n + WG - 1) / WG)), dim3(WG), 0, (hipStream_t)stream, order,
-                     (int)n, place);
-  return tace_check_launch("tace_route_place");
+extern "C" int64_t tace_route_group_work(int64_t n, int64_t n_keys) {
+  int wgs, steps;
+  if (n < 0 || n_keys < 0 || n > INT32_MAX - 8192 || n_keys > INT32_MAX - 8192) return 0;
+  if (few_fits(n, n_keys, &wgs, &steps)) return (int64_t)wgs * (n_keys + 1);
+  return tace_group_keys_work(n, n_keys) + n;   // (and the keys in 32 bits)
+}
+
+extern "C" int tace_route_group(int index_bytes, const void* keys, int64_t stride, int64_t n, int64_t n_keys,
+                                int32_t* rowptr, int32_t* order, int32_t* place, int32_t* work, void* stream) {
+  if (n < 0 || n_keys < 0 || n > INT32_MAX - 8192 || n_keys > INT32_MAX - 8192)
+    return tace_fail_msg("tace_route_group: bad sizes");
+  if (index_bytes != 4 && index_bytes != 8) return tace_fail_msg("tace_route_group: indices of 4 or 8 bytes");
+  if (!rowptr || !work || (n && (!keys || !order))) return tace_fail_msg("tace_route_group: null pointer");
+  hipStream_t s = (hipStream_t)stream;
+  int wgs, steps;
+  if (few_fits(n, n_keys, &wgs, &steps)) {
+    if (index_bytes == 4)
+      few_group((const int32_t*)keys, stride, (int)n, (int)n_keys, wgs, steps, rowptr, order, place, work, s);
+    else
+      few_group((const int64_t*)keys, stride, (int)n, (int)n_keys, wgs, steps, rowptr, order, place, work, s);
+    return tace_check_launch("tace_route_group");
+  }
+  int32_t* k32 = work + tace_group_keys_work(n, n_keys);
+  const int rc = tace_group_keys(index_bytes, keys, stride, nullptr, n, n_keys, k32, rowptr, order, nullptr, 0, nullptr,
+                                 work, nullptr, stream);
+  if (rc || !place || n == 0) return rc;
+  hipLaunchKernelGGL(k_route_place, dim3((unsigned)((n + WG - 1) / WG)), dim3(WG), 0, s, order, (int)n, place);
+  return tace_check_launch("tace_route_group");
 }
 
 namespace {

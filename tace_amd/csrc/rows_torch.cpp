@@ -110,16 +110,19 @@ const T& held(AutogradContext* ctx) {
   return static_cast<Held<T>*>(ctx->saved_data["args"].toCapsule().get())->v;
 }
 
-// positions grouped by key: (rowptr [n_keys + 1], order [n])
-std::pair<Tensor, Tensor> group(const Tensor& keys, int64_t n_keys) {
+// positions grouped by key: rowptr [n_keys + 1], order [n] and, where wanted, place [n]
+struct Groups {
+  Tensor rowptr, order, place;
+};
+Groups group(const Tensor& keys, int64_t n_keys, bool want_place, bool timed) {
   const int64_t n = keys.numel();
   const auto opt = keys.options().dtype(at::kInt);
-  Tensor k32 = at::empty({n}, opt), order = at::empty({n}, opt), rowptr = at::empty({n_keys + 1}, opt);
-  Tensor work = at::empty({tace_group_keys_work(n, n_keys)}, opt);
-  Launch l(keys, "group_keys", false);
-  l.done(tace_group_keys((int)keys.element_size(), ptr(keys), n ? keys.stride(0) : 1, nullptr, n, n_keys, ints(k32),
-                         ints(rowptr), ints(order), nullptr, 0, nullptr, ints(work), nullptr, l.stream), {});
-  return {rowptr, order};
+  Groups g{at::empty({n_keys + 1}, opt), at::empty({n}, opt), want_place ? at::empty({n}, opt) : Tensor()};
+  Tensor work = at::empty({tace_route_group_work(n, n_keys)}, opt);
+  Launch l(keys, "route_group", timed);
+  l.done(tace_route_group((int)keys.element_size(), ptr(keys), n ? keys.stride(0) : 1, n, n_keys, ints(g.rowptr),
+                          ints(g.order), ints(g.place), work.data_ptr<int>(), l.stream), {n, n_keys});
+  return g;
 }
 
 // ----------------------------------------------------------------- embedding ----
@@ -146,7 +149,14 @@ Tensor embed_grad(const Tensor& g, const Tensor& tokens, const Lookup& a) {
   Tensor grad = at::empty({a.vocab, C}, g.options()), rowptr, order, work;
   int64_t bytes = 0;
   if (!tace_embed_grad_scans(n, a.vocab, (int)C)) {
-    std::tie(rowptr, order) = a.order.defined() ? std::make_pair(a.rowptr, a.order) : group(tokens, a.vocab);
+    if (a.order.defined()) {
+      rowptr = a.rowptr;
+      order = a.order;
+    } else {
+      const Groups by = group(tokens, a.vocab, false, a.timed);
+      rowptr = by.rowptr;
+      order = by.order;
+    }
     bytes = tace_embed_grad_work(code, n, a.vocab, (int)C);
     work = at::empty({bytes}, g.options().dtype(at::kByte));
   }
@@ -323,7 +333,8 @@ Tensor dots_op(const Tensor& x, const Tensor& y, const Routed& r) {
 }
 
 // (rowptr, order, place, tokens, k)
-std::tuple<Tensor, Tensor, Tensor, int64_t, int64_t> route_plan(const Tensor& experts, int64_t n_experts) {
+std::tuple<Tensor, Tensor, Tensor, int64_t, int64_t> route_plan(const Tensor& experts, int64_t n_experts,
+                                                                bool timed) {
   TORCH_CHECK_VALUE(experts.is_cuda(), "experts must be a GPU tensor (got ", experts.device(), ")");
   want_indices(experts, "experts");
   TORCH_CHECK_VALUE(experts.dim() == 1 || (experts.dim() == 2 && experts.size(1) >= 1), "experts has shape ",
@@ -331,12 +342,8 @@ std::tuple<Tensor, Tensor, Tensor, int64_t, int64_t> route_plan(const Tensor& ex
   const int64_t T = experts.size(0), k = experts.dim() == 1 ? 1 : experts.size(1);
   TORCH_CHECK_VALUE(n_experts >= 0 && n_experts <= MAX_INDEX && T * k <= MAX_INDEX,
                     "route_plan: slots or experts exceed 32-bit indices");
-  const Tensor flat = experts.reshape({-1});
-  auto [rowptr, order] = group(flat, n_experts);
-  Tensor place = at::empty_like(order);
-  Launch l(experts, "route_place", false);
-  l.done(tace_route_place(ints(order), T * k, ints(place), l.stream), {});
-  return {rowptr, order, place, T, k};
+  const Groups g = group(experts.reshape({-1}), n_experts, true, timed);
+  return {g.rowptr, g.order, g.place, T, k};
 }
 
 Tensor route(bool combine, const Tensor& x, const Tensor& place, const Tensor& rowptr, int64_t tokens, int64_t k,

@@ -1564,7 +1564,7 @@ def route_plan(experts: torch.Tensor, n_experts: int) -> RoutePlan:
     """Tokens sorted by expert.  ``experts`` [T] or [T, k] (int32 or int64): the
     experts of each token; a choice outside [0, n_experts) is dropped.  No host
     synchronisation."""
-    return RoutePlan(*N.rows().route_plan(experts, n_experts))
+    return RoutePlan(*N.rows().route_plan(experts, n_experts, TIMER is not None))
 
 
 def expert_dispatch(x: torch.Tensor, plan: RoutePlan, weights: Optional[torch.Tensor] = None,

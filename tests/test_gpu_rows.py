@@ -139,6 +139,25 @@ def test_embedding_differentiates_again(cuda):
 
 
 # ----------------------------------------------------------------- routing ----
+# one workgroup and its last position; several, with 1 .. 8 positions a thread; the general grouping behind that
+@pytest.mark.parametrize("n", [1, 64, 1023, 1025, 8191, 8192, 8193, 131072, 131073, 300001, 1048576, 1048577, 2000003])
+@pytest.mark.parametrize("E", [1, 2, 7, 64, 127, 128, 254, 255, 256, 1000])
+def test_route_plan_is_the_stable_sort(cuda, n, E):
+    g = torch.Generator().manual_seed(n + E)
+    e = torch.randint(-1, E + 1, (n,), generator=g)
+    e[torch.rand(n, generator=g) < 0.5] = E // 2
+    if n % 2:
+        e = e.sort(descending=True)[0]
+    wide = torch.stack([e, -e], 1).to(cuda)   # (read with a stride)
+    for t in (wide[:, 0], wide[:, 0].int()):
+        plan = ops.route_plan(t, E)
+        key = torch.where((t >= 0) & (t < E), t, E)
+        order = torch.argsort(key, stable=True)
+        assert torch.equal(plan.order.long(), order)
+        assert torch.equal(plan.place.long()[order], torch.arange(n, device=cuda))
+        assert torch.equal(plan.rowptr.long(), torch.searchsorted(key[order], torch.arange(E + 1, device=cuda)))
+
+
 def _experts(T, k, E, drop, seed):
     g = torch.Generator().manual_seed(seed)
     e = torch.rand(T, E, generator=g).argsort(1)[:, :k] if E >= k else torch.randint(0, max(E, 1), (T, k), generator=g)
@@ -397,8 +416,8 @@ def test_kernel_timer_sees_every_launch(cuda):
         seen = ops.TIMER.summary()
     finally:
         ops.TIMER = None
-    assert {k: v[0] for k, v in seen.items() if k != "group_keys"} == dict(
-        embed_fwd=1, embed_grad=1, dropout=2, route_dispatch=1, route_combine=2, route_dots=1)
+    assert {k: v[0] for k, v in seen.items()} == dict(
+        embed_fwd=1, embed_grad=1, dropout=2, route_group=2, route_dispatch=1, route_combine=2, route_dots=1)
     assert all(ms > 0 for _, ms, _ in seen.values())
 
 

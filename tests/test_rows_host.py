@@ -72,7 +72,9 @@ def test_entries_refuse_bad_arguments():
         _refused(f(0, p, None, p, None, 4, 2, 1, w, p, None), b"null")
         assert f(0, None, None, None, None, 0, 2, 1, w, None, None) == 0
     _refused(L.tace_route_dots(0, p, p, None, p, p, 4, 2, 1, w, None, None, None), b"null")
-    _refused(L.tace_route_place(None, 4, p, None), b"null")
+    _refused(L.tace_route_group(4, None, 1, 4, 4, p, p, p, p, None), b"null")
+    _refused(L.tace_route_group(3, p, 1, 4, 4, p, p, p, p, None), b"4 or 8 bytes")
+    _refused(L.tace_route_group(4, p, 1, 2 ** 31, 4, p, p, p, p, None), b"bad sizes")
     _refused(L.tace_dropout(0, p, None, None, 0, 0, 0, 65537, 4, 4, 1, one, p, None), b"threshold")
     _refused(L.tace_dropout(0, p, None, None, 0, 0, 0, 5, 4, 4, 9, one, p, None), b"bad sizes")
     _refused(L.tace_dropout(0, p, None, None, 0, 0, 0, 5, 2 ** 34, 2, 1, one, p, None), b"2^34")
