@@ -17,7 +17,7 @@
 extern "C" {
 #endif
 
-#define TACE_ROWS_ABI_VERSION 2
+#define TACE_ROWS_ABI_VERSION 3
 #define TACE_ROW_F32 0
 #define TACE_ROW_F64 1
 #define TACE_ROW_BF16 2
@@ -34,12 +34,11 @@ int tace_embed_fwd(int type, int index_bytes, const void* table, const void* tok
 /* grad [vocab, channels]: row v is scale * the sum of g's rows (g [n,
  * channels]) whose token is v, zeros without any; the order of the sum depends
  * on the sizes alone.  order [n] and rowptr [vocab + 1] are tace_route_group's
- * of the tokens; work: tace_embed_grad_work bytes (16-byte aligned).
- * order NULL: no grouping and no work are read, every token looks through all
- * of tokens (for few rows and tokens: tace_embed_grad_scans says where; the
- * only form for n = 0). */
-int64_t tace_embed_grad_work(int type, int64_t n, int64_t vocab, int32_t channels);
-int tace_embed_grad_scans(int64_t n, int64_t vocab, int32_t channels);
+ * of the tokens; NULL where tace_embed_grad_grouped is 0 (few rows or tokens,
+ * always for n = 0).  work: tace_embed_grad_work bytes (16-byte aligned) of the
+ * same choice, grouped or not. */
+int tace_embed_grad_grouped(int64_t n, int64_t vocab);
+int64_t tace_embed_grad_work(int type, int64_t n, int64_t vocab, int32_t channels, int grouped);
 int tace_embed_grad(int type, int index_bytes, const void* g, const void* tokens, const int32_t* order,
                     const int32_t* rowptr, int64_t n, int64_t vocab, int32_t channels, double scale, void* grad,
                     void* work, int64_t work_bytes, void* stream);

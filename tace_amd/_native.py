@@ -126,12 +126,12 @@ _SIGS = {
 EXPORTED = tuple(_SIGS)
 
 # the row operators (include/tace_rows.h), with a version of their own
-ROWS_ABI_VERSION = 2
+ROWS_ABI_VERSION = 3
 _ROW_SIGS = {
     "tace_rows_abi_version": (_c_int, []),
     "tace_embed_fwd": (_c_int, [_c_int, _c_int, _vp, _vp, _c_i64, _c_i64, _c_i32, _c_dbl, _vp, _vp]),
-    "tace_embed_grad_work": (_c_i64, [_c_int, _c_i64, _c_i64, _c_i32]),
-    "tace_embed_grad_scans": (_c_int, [_c_i64, _c_i64, _c_i32]),
+    "tace_embed_grad_grouped": (_c_int, [_c_i64, _c_i64]),
+    "tace_embed_grad_work": (_c_i64, [_c_int, _c_i64, _c_i64, _c_i32, _c_int]),
     "tace_embed_grad": (_c_int, [_c_int, _c_int, _vp, _vp, _vp, _vp, _c_i64, _c_i64, _c_i32, _c_dbl, _vp, _vp, _c_i64,
                                  _vp]),
     "tace_route_group_work": (_c_i64, [_c_i64, _c_i64]),

@@ -53,138 +53,272 @@ __global__ __launch_bounds__(WG) void k_embed_fwd(const T* __restrict__ table, c
 // each of its groups of `lanes` threads, which hold a row's sums in registers.
 // Sorted, a token's rows are a run; whether a run goes on outside a group's (or
 // the workgroup's) positions shows in the neighbouring position's token.  Runs
-// inside a group are written at once; the others meet in LDS, in position
-// order; what goes on beyond the workgroup is left in part [workgroup][2]
-// [channels]: [0] a run that began before it, [1] one that begins in it.
+// inside a group are written at once; the others meet in LDS, in position order,
+// a team of groups first.
+//
+// `Src` says what the sorted positions are:
+//   at(p)        the row of sorted position p (any p; the nearest one outside)
+//   key(p, row)  its token, -1 behind the last (padding)
+//   left(), right()  the tokens before and behind the workgroup's positions, -1: none
+//   whole(v, c, sum), open(v, slot, c, sum)  where the sum of a run goes that
+//       ends inside the workgroup, and of one that goes on (slot 0: began before it)
 constexpr int TEAM = 8;   // groups whose open runs one of them joins
+template <typename T, int V>
+struct RunSums {
+  typedef row_vec_t<T, V> Vec;
+  typedef row_sum_t<T> S;
+  S open[2 * V * WG];   // [slot][element][thread]
+  int open_key[2 * WG], team_key[2 * WG / TEAM], outer[2 * WG / TEAM];
+
+  template <typename Src>
+  __device__ __forceinline__ void run(const Src& src, const T* __restrict__ g, int cw, int lanes, int p_begin,
+                                      int p_end, int per) {
+    constexpr int U = 8;
+    const int groups = WG / lanes, t = (int)threadIdx.x;
+    const int grp = t / lanes, lane = t % lanes, c = lane + (int)blockIdx.y * lanes;
+    const int p0 = (int)min(p_begin + (int64_t)grp * per, (int64_t)p_end);
+    const int p1 = (int)min((int64_t)p0 + per, (int64_t)p_end);
+    if (grp < groups) {
+      int next[U];
+      auto ahead = [&](int p) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) next[u] = src.at(p + u);
+      };
+      ahead(p0);
+      const int left = p0 > p_begin ? src.key(p0 - 1, src.at(p0 - 1)) : src.left();
+      const int right = p1 < p_end ? src.key(p1, src.at(p1)) : src.right();
+      if (lane == 0) {
+        const int team = grp / TEAM;
+        open_key[2 * grp] = open_key[2 * grp + 1] = -1;
+        if (grp % TEAM == 0) outer[2 * team] = left, team_key[2 * team] = team_key[2 * team + 1] = -1;
+        if (grp % TEAM == TEAM - 1 || grp == groups - 1) outer[2 * team + 1] = right;
+      }
+      S sum[V];
+      int cur = -1;
+      bool head = true;   // the run at p0
+      auto flush = [&]() {
+        if (cur < 0 || c >= cw) return;
+        if (cur != left && cur != right) {
+          src.whole(cur, c, sum);
+        } else {
+          const int slot = head ? 0 : 1;
+#pragma unroll
+          for (int i = 0; i < V; ++i) open[(slot * V + i) * WG + t] = sum[i];
+          if (lane == 0) open_key[2 * grp + slot] = cur;
+        }
+      };
+      const Vec* rows = (const Vec*)g + min(c, cw - 1);
+      for (int p = p0; p < p1; p += U) {
+        int at[U];
+        Vec v[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          at[u] = next[u];
+          v[u] = __builtin_nontemporal_load(rows + (int64_t)at[u] * cw);   // (read once)
+        }
+        int key[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) key[u] = src.key(p + u, at[u]);
+        ahead(p + U);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int k = p + u < p1 ? key[u] : cur;
+          S a[V];
+          row_widen<T, V>(v[u], a);
+          if (k != cur) {
+            flush();
+            head = head && cur < 0;
+            cur = k;
+#pragma unroll
+            for (int i = 0; i < V; ++i) sum[i] = a[i];
+          } else if (p + u < p1) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) sum[i] += a[i];
+          }
+        }
+      }
+      flush();
+    }
+    __syncthreads();
+    // the open runs of `count` groups, `step` apart, from g0 on
+    auto merge = [&](int g0, int count, int step, const int* keys, int left, int right, auto&& leave) {
+      S sum[V];
+      int cur = -1;
+      auto flush = [&]() {
+        if (cur != left && cur != right) src.whole(cur, c, sum);
+        else leave(cur == left ? 0 : 1, cur, sum);
+      };
+      for (int q = 0; q < 2 * count; ++q) {
+        const int key = keys[q];
+        if (key < 0) continue;
+        const S* o = open + (q & 1) * V * WG + (g0 + (q >> 1) * step) * lanes + lane;
+        if (key != cur) {
+          if (cur >= 0) flush();
+          cur = key;
+#pragma unroll
+          for (int i = 0; i < V; ++i) sum[i] = o[i * WG];
+        } else {
+#pragma unroll
+          for (int i = 0; i < V; ++i) sum[i] += o[i * WG];
+        }
+      }
+      if (cur >= 0) flush();
+    };
+    const int teams = (groups + TEAM - 1) / TEAM;
+    auto leave_open = [&](int slot, int v, const S* sum) { src.open(v, slot, c, sum); };
+    if (teams == 1) {
+      if (grp == 0 && c < cw) merge(0, groups, 1, open_key, outer[0], outer[1], leave_open);
+      return;
+    }
+    // (a thread reads and writes its own sums here, and those of its column in its team)
+    if (grp < groups && grp % TEAM == 0 && c < cw) {
+      const int team = grp / TEAM;
+      merge(grp, min(TEAM, groups - grp), 1, open_key + 2 * grp, outer[2 * team], outer[2 * team + 1],
+            [&](int slot, int key, const S* sum) {
+#pragma unroll
+              for (int i = 0; i < V; ++i) open[(slot * V + i) * WG + t] = sum[i];
+              if (lane == 0) team_key[2 * team + slot] = key;
+            });
+    }
+    __syncthreads();
+    if (grp == 0 && c < cw) merge(0, teams, TEAM, team_key, outer[0], outer[2 * teams - 1], leave_open);
+  }
+};
+
+// Positions sorted ahead (order): a run that goes on beyond the workgroup is
+// left in part [workgroup][slot][channels], for k_embed_grad_join.
+template <typename T, int V, typename I>
+struct SortedRows {
+  const I* tokens;
+  const int* order;
+  int n, vocab, channels, p_begin, p_end;
+  row_sum_t<T> scale;
+  T* grad;
+  row_sum_t<T>* part;
+
+  __device__ __forceinline__ int at(int p) const { return order[min(max(p, 0), n - 1)]; }
+  __device__ __forceinline__ int key(int, int row) const {
+    const I v = tokens[row];
+    return v >= 0 && v < (I)vocab ? (int)v : -1;
+  }
+  __device__ __forceinline__ int left() const { return p_begin > 0 ? key(0, at(p_begin - 1)) : -1; }
+  __device__ __forceinline__ int right() const { return p_end < n ? key(0, at(p_end)) : -1; }
+  __device__ __forceinline__ void whole(int v, int c, const row_sum_t<T>* sum) const {
+    row_sum_t<T> a[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) a[i] = sum[i] * scale;
+    ((row_vec_t<T, V>*)grad)[(int64_t)v * (channels / V) + c] = row_round<T, V>(a);
+  }
+  __device__ __forceinline__ void open(int, int slot, int c, const row_sum_t<T>* sum) const {
+    row_sum_t<T>* o = part + ((int64_t)blockIdx.x * 2 + slot) * channels + (int64_t)c * V;
+#pragma unroll
+    for (int i = 0; i < V; ++i) o[i] = sum[i];
+  }
+};
+
 template <typename T, int V, typename I>
 __global__ __launch_bounds__(WG) void k_embed_grad_part(const T* __restrict__ g, const I* __restrict__ tokens,
                                                         const int* __restrict__ order, int n, int vocab, int channels,
-                                                        int per, int lanes,
-                                                        row_sum_t<T> scale, T* __restrict__ grad,
+                                                        int per, int lanes, row_sum_t<T> scale, T* __restrict__ grad,
                                                         row_sum_t<T>* __restrict__ part) {
-  typedef row_vec_t<T, V> Vec;
-  typedef row_sum_t<T> S;
-  constexpr int U = 8;
-  __shared__ S open[2 * V * WG];   // [slot][element][thread]
-  __shared__ int open_key[2 * WG], team_key[2 * WG / TEAM], outer[2 * WG / TEAM];
-  const int cw = channels / V, groups = WG / lanes, t = (int)threadIdx.x;
-  const int grp = t / lanes, lane = t % lanes, c = lane + (int)blockIdx.y * lanes;
-  const int64_t w0 = blockIdx.x * (int64_t)per * groups;
-  const int p0 = (int)min(w0 + (int64_t)grp * per, (int64_t)n), p1 = min(p0 + per, n);
-  // (padding, sorted last, has no key)
-  auto key_of = [&](I v) { return v >= 0 && v < (I)vocab ? (int)v : -1; };
-  auto write = [&](int v, const S* sum) {
-    S a[V];
-#pragma unroll
-    for (int i = 0; i < V; ++i) a[i] = sum[i] * scale;
-    ((Vec*)grad)[(int64_t)v * cw + c] = row_round<T, V>(a);
-  };
-  if (grp < groups) {
-    int next[U];
-    auto ahead = [&](int p) {
-#pragma unroll
-      for (int u = 0; u < U; ++u) next[u] = order[min(p + u, n - 1)];
-    };
-    ahead(p0);
-    const int left = p0 > 0 ? key_of(tokens[order[p0 - 1]]) : -1, right = p1 < n ? key_of(tokens[order[p1]]) : -1;
-    if (lane == 0) {
-      const int team = grp / TEAM;
-      open_key[2 * grp] = open_key[2 * grp + 1] = -1;
-      if (grp % TEAM == 0) outer[2 * team] = left, team_key[2 * team] = team_key[2 * team + 1] = -1;
-      if (grp % TEAM == TEAM - 1 || grp == groups - 1) outer[2 * team + 1] = right;
-    }
-    S sum[V];
-    int cur = -1;
-    bool head = true;   // the run at p0
-    auto flush = [&]() {
-      if (cur < 0 || c >= cw) return;
-      if (cur != left && cur != right) {
-        write(cur, sum);
-      } else {
-        const int slot = head ? 0 : 1;
-#pragma unroll
-        for (int i = 0; i < V; ++i) open[(slot * V + i) * WG + t] = sum[i];
-        if (lane == 0) open_key[2 * grp + slot] = cur;
-      }
-    };
-    const Vec* rows = (const Vec*)g + min(c, cw - 1);
-    for (int p = p0; p < p1; p += U) {
-      I tok[U];
-      Vec v[U];
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        tok[u] = tokens[next[u]];
-        v[u] = __builtin_nontemporal_load(rows + (int64_t)next[u] * cw);   // (read once)
-      }
-      ahead(p + U);
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int key = p + u < p1 ? key_of(tok[u]) : cur;
-        S a[V];
-        row_widen<T, V>(v[u], a);
-        if (key != cur) {
-          flush();
-          head = head && cur < 0;
-          cur = key;
-#pragma unroll
-          for (int i = 0; i < V; ++i) sum[i] = a[i];
-        } else if (p + u < p1) {
-#pragma unroll
-          for (int i = 0; i < V; ++i) sum[i] += a[i];
-        }
-      }
-    }
-    flush();
-  }
-  __syncthreads();
-  // the open runs of `count` groups, `step` apart, from g0 on
-  auto merge = [&](int g0, int count, int step, const int* keys, int left, int right, auto&& leave) {
-    S sum[V];
-    int cur = -1;
-    auto flush = [&]() {
-      if (cur != left && cur != right) write(cur, sum);
-      else leave(cur == left ? 0 : 1, cur, sum);
-    };
-    for (int q = 0; q < 2 * count; ++q) {
-      const int key = keys[q];
-      if (key < 0) continue;
-      const S* o = open + (q & 1) * V * WG + (g0 + (q >> 1) * step) * lanes + lane;
-      if (key != cur) {
-        if (cur >= 0) flush();
-        cur = key;
-#pragma unroll
-        for (int i = 0; i < V; ++i) sum[i] = o[i * WG];
-      } else {
-#pragma unroll
-        for (int i = 0; i < V; ++i) sum[i] += o[i * WG];
-      }
-    }
-    if (cur >= 0) flush();
-  };
-  const int teams = (groups + TEAM - 1) / TEAM;
-  auto leave_part = [&](int slot, int, const S* sum) {
-    S* o = part + ((int64_t)blockIdx.x * 2 + slot) * channels + (int64_t)c * V;
+  __shared__ RunSums<T, V> sums;
+  const int64_t span = (int64_t)per * (WG / lanes), w0 = blockIdx.x * span;
+  const int p0 = (int)min(w0, (int64_t)n), p1 = (int)min(w0 + span, (int64_t)n);
+  const SortedRows<T, V, I> src{tokens, order, n, vocab, channels, p0, p1, scale, grad, part};
+  sums.run(src, g, channels / V, lanes, p0, p1, per);
+}
+
+// Few tokens (at most 128): a workgroup sorts its own `count` rows' tokens in
+// LDS, so no grouping of all of them is needed; each token's sum goes to part
+// [workgroup][token][channels] and its presence to seen [workgroup][token], for
+// k_embed_grad_total.  Two launches instead of four.
+constexpr int FEW_TOKENS = 128, LOCAL_STEPS = 4, LOCAL_ROWS = WG * LOCAL_STEPS;
+template <typename T, int V>
+struct LocalRows {
+  const int* list;   // token << 16 | row in the workgroup, sorted
+  int64_t row0;
+  int count, vocab, channels;
+  row_sum_t<T>* part;
+
+  __device__ __forceinline__ int packed(int p) const { return list[min(max(p, 0), count - 1)]; }
+  __device__ __forceinline__ int at(int p) const { return (int)(row0 + (packed(p) & 0xffff)); }
+  __device__ __forceinline__ int key(int p, int) const { return p < count ? packed(p) >> 16 : -1; }
+  __device__ __forceinline__ int left() const { return -1; }
+  __device__ __forceinline__ int right() const { return -1; }
+  __device__ __forceinline__ void whole(int v, int c, const row_sum_t<T>* sum) const {
+    row_sum_t<T>* o = part + ((int64_t)blockIdx.x * vocab + v) * channels + (int64_t)c * V;
 #pragma unroll
     for (int i = 0; i < V; ++i) o[i] = sum[i];
-  };
-  if (teams == 1) {
-    if (grp == 0 && c < cw) merge(0, groups, 1, open_key, outer[0], outer[1], leave_part);
-    return;
   }
-  // teams of groups first (a thread reads and writes its own sums here, and
-  // those of its column in its team)
-  if (grp < groups && grp % TEAM == 0 && c < cw) {
-    const int team = grp / TEAM;
-    merge(grp, min(TEAM, groups - grp), 1, open_key + 2 * grp, outer[2 * team], outer[2 * team + 1],
-          [&](int slot, int key, const S* sum) {
+  __device__ __forceinline__ void open(int, int, int, const row_sum_t<T>*) const {}   // (no run goes on)
+};
+
+template <typename T, int V, typename I>
+__global__ __launch_bounds__(WG) void k_embed_grad_local(const T* __restrict__ g, const I* __restrict__ tokens, int n,
+                                                         int vocab, int channels, int rows, int lanes,
+                                                         int* __restrict__ seen, row_sum_t<T>* __restrict__ part) {
+  constexpr int WAVES = WG / 64;
+  __shared__ RunSums<T, V> sums;
+  __shared__ int list[LOCAL_ROWS], cnt[WAVES][FEW_TOKENS], wsum[2], kept;
+  const int t = (int)threadIdx.x, lane = t & 63, w = t >> 6, steps = rows / WG;
+  const int64_t row0 = (int64_t)blockIdx.x * rows;
+  for (int q = t; q < WAVES * FEW_TOKENS; q += WG) cnt[q / FEW_TOKENS][q % FEW_TOKENS] = 0;
+  const int i0 = 64 * steps * w + lane;   // (of the workgroup's rows; a run of 64 `steps` a wavefront)
+  I tok[LOCAL_STEPS];
 #pragma unroll
-            for (int i = 0; i < V; ++i) open[(slot * V + i) * WG + t] = sum[i];
-            if (lane == 0) team_key[2 * team + slot] = key;
-          });
+  for (int u = 0; u < LOCAL_STEPS; ++u)
+    if (u < steps) tok[u] = tokens[min(row0 + i0 + 64 * u, (int64_t)n - 1)];
+  __syncthreads();
+  int key[LOCAL_STEPS], rank[LOCAL_STEPS];
+#pragma unroll
+  for (int u = 0; u < LOCAL_STEPS; ++u) {
+    const bool in = u < steps && row0 + i0 + 64 * u < n && tok[u] >= 0 && tok[u] < (I)vocab;
+    key[u] = in ? (int)tok[u] : -1;
+    if (u >= steps) continue;   // (all lanes alike)
+    unsigned long long m = __ballot(in);
+#pragma unroll
+    for (int b = 0; (1 << b) < FEW_TOKENS; ++b) {
+      const bool one = (key[u] >> b) & 1;
+      const unsigned long long v = __ballot(one);
+      m &= one ? v : ~v;
+    }
+    const int r = __popcll(m & ((1ull << lane) - 1));
+    int had = 0;
+    if (in && r == 0) had = atomicAdd(&cnt[w][key[u]], __popcll(m));
+    rank[u] = r + __shfl(had, in ? __ffsll((long long)m) - 1 : lane, 64);
   }
   __syncthreads();
-  if (grp == 0 && c < cw) merge(0, teams, TEAM, team_key, outer[0], outer[2 * teams - 1], leave_part);
+  int sum = 0;
+  if (t < FEW_TOKENS)
+    for (int k = 0; k < WAVES; ++k) sum += cnt[k][t];
+  int inc = sum;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int v = __shfl_up(inc, o, 64);
+    if (lane >= o) inc += v;
+  }
+  if (w < 2 && lane == 63) wsum[w] = inc;
+  __syncthreads();
+  if (t < FEW_TOKENS) {
+    int at = inc - sum + (w == 1 ? wsum[0] : 0);
+    if (t == FEW_TOKENS - 1) kept = at + sum;
+    if (t < vocab && blockIdx.y == 0) seen[(int64_t)blockIdx.x * vocab + t] = sum;
+    for (int k = 0; k < WAVES; ++k) {
+      const int c = cnt[k][t];
+      cnt[k][t] = at;
+      at += c;
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int u = 0; u < LOCAL_STEPS; ++u)
+    if (key[u] >= 0) list[cnt[w][key[u]] + rank[u]] = key[u] << 16 | (i0 + 64 * u);
+  __syncthreads();
+  const int count = kept;
+  if (count == 0) return;
+  const LocalRows<T, V> src{list, row0, count, vocab, channels, part};
+  const int groups = WG / lanes;
+  sums.run(src, g, channels / V, lanes, 0, count, (count + groups - 1) / groups);
 }
 
 // What is left: workgroup w < workgroups - 1 joins the run that begins in the
@@ -220,6 +354,33 @@ __global__ __launch_bounds__(WG) void k_embed_grad_join(const I* __restrict__ to
 #pragma unroll 8
     for (int q = (int)blockIdx.x + y; q <= last; q += JOIN_ROWS)
       sum += part[((int64_t)q * 2 + (q == (int)blockIdx.x ? 1 : 0)) * channels + c];
+  }
+  red[y][x] = sum;
+  __syncthreads();
+  if (y == 0 && c < channels) {
+#pragma unroll
+    for (int k = 1; k < JOIN_ROWS; ++k) sum += red[k][x];
+    grad[(int64_t)v * channels + c] = (T)(sum * scale);
+  }
+}
+
+// grad of k_embed_grad_local's sums: 16 columns of a token a workgroup
+template <typename T>
+__global__ __launch_bounds__(WG) void k_embed_grad_total(const int* __restrict__ seen, int workgroups, int vocab,
+                                                         int channels, row_sum_t<T> scale,
+                                                         const row_sum_t<T>* __restrict__ part, T* __restrict__ grad) {
+  typedef row_sum_t<T> S;
+  __shared__ S red[JOIN_ROWS][JOIN_COLS];
+  const int t = (int)threadIdx.x, x = t % JOIN_COLS, y = t / JOIN_COLS, v = (int)blockIdx.x;
+  const int c = (int)blockIdx.y * JOIN_COLS + x;
+  S sum = 0;
+  if (c < channels) {
+#pragma unroll 8
+    for (int q = y; q < workgroups; q += JOIN_ROWS) {
+      const int64_t at = (int64_t)q * vocab + v;
+      const S p = part[at * channels + c];   // (holds nothing where the token was not seen)
+      sum += seen[at] ? p : (S)0;
+    }
   }
   red[y][x] = sum;
   __syncthreads();
@@ -301,6 +462,22 @@ int64_t embed_wgs(int64_t n, int lanes) {
   const int64_t span = (int64_t)embed_per(n, lanes) * (WG / lanes);
   return (n + span - 1) / span;
 }
+
+// Which form the gradient takes without a grouping of the tokens: looking
+// through all of them, sorting them workgroup by workgroup, or none.
+enum { SCANS = 1, SORTS = 2, GROUPED = 0 };
+int embed_form(int64_t n, int64_t vocab) {
+  return n <= SCAN_N && vocab <= 1024 ? SCANS : vocab <= FEW_TOKENS ? SORTS : GROUPED;
+}
+
+// SORTS: rows a workgroup (256 .. 1,024: about 256 workgroups), their number,
+// and the threads a row: 16 where that leaves the GPU few workgroups
+int local_rows(int64_t n) {
+  const int64_t steps = (n + 256 * WG - 1) / (256 * WG);
+  return WG * (int)std::min<int64_t>(std::max<int64_t>(steps, 1), LOCAL_STEPS);
+}
+int64_t local_wgs(int64_t n) { return (n + local_rows(n) - 1) / local_rows(n); }
+int64_t local_seen(int64_t n, int64_t vocab) { return (local_wgs(n) * vocab * 4 + 15) / 16 * 16; }   // bytes
 
 // --------------------------------------------------------------- routing ----
 // A row's chunks in blocks that lie apart: block b of R rows starts at R *
@@ -663,20 +840,18 @@ extern "C" int tace_embed_fwd(int type, int index_bytes, const void* table, cons
   return tace_check_launch("tace_embed_fwd");
 }
 
-extern "C" int tace_embed_grad_scans(int64_t n, int64_t vocab, int32_t channels) {
-  (void)channels;
-  return n <= SCAN_N && vocab <= 1024 ? 1 : 0;
-}
+extern "C" int tace_embed_grad_grouped(int64_t n, int64_t vocab) { return embed_form(n, vocab) == GROUPED; }
 
-extern "C" int64_t tace_embed_grad_work(int type, int64_t n, int64_t vocab, int32_t channels) {
-  (void)vocab;
-  if (n < 1 || channels < 1 || channels > MAX_ROW) return 16;
+extern "C" int64_t tace_embed_grad_work(int type, int64_t n, int64_t vocab, int32_t channels, int grouped) {
+  if (n < 1 || vocab < 1 || channels < 1 || channels > MAX_ROW) return 16;
+  const int64_t row = (int64_t)channels * (type == TACE_ROW_F64 ? 8 : 4);
+  if (!grouped) return embed_form(n, vocab) == SORTS ? local_seen(n, vocab) + local_wgs(n) * vocab * row : 16;
   // (rows may be moved by 16 bytes, 8, or one element: the largest count of workgroups)
   const int bytes = type == TACE_ROW_F64 ? 8 : type == TACE_ROW_F32 ? 4 : 2;
   int64_t wgs = 0;
   for (int v : {1, 8 / bytes, 16 / bytes})
     if (channels % v == 0) wgs = std::max(wgs, embed_wgs(n, embed_lanes(channels / v)));
-  return wgs * 2 * channels * (type == TACE_ROW_F64 ? 8 : 4);
+  return wgs * 2 * row;
 }
 
 extern "C" int tace_embed_grad(int type, int index_bytes, const void* g, const void* tokens, const int32_t* order,
@@ -687,17 +862,16 @@ extern "C" int tace_embed_grad(int type, int index_bytes, const void* g, const v
   if (index_bytes != 4 && index_bytes != 8) return tace_fail_msg("tace_embed_grad: indices of 4 or 8 bytes");
   if (type < 0 || type > TACE_ROW_F16) return tace_fail_msg("tace_embed_grad: unknown row type");
   if (vocab == 0) return 0;
-  const bool scans = order == nullptr;
+  const bool grouped = order != nullptr;
+  const int form = grouped ? GROUPED : embed_form(n, vocab);
   if (!grad || (n && (!g || !tokens))) return tace_fail_msg("tace_embed_grad: null pointer");
-  if (!scans && n == 0) return tace_fail_msg("tace_embed_grad: no rows, and a grouping of them");
-  if (scans) {
-    if (!tace_embed_grad_scans(n, vocab, channels))
-      return tace_fail_msg("tace_embed_grad: too many rows or tokens without a grouping");
-  } else {
-    if (!rowptr || !work) return tace_fail_msg("tace_embed_grad: null pointer");
-    if ((work_bytes < tace_embed_grad_work(type, n, vocab, channels) || !row_aligned(work)))
-      return tace_fail_msg("tace_embed_grad: workspace too small or not 16-byte aligned");
-  }
+  if (grouped && n == 0) return tace_fail_msg("tace_embed_grad: no rows, and a grouping of them");
+  if (!grouped && form == GROUPED)
+    return tace_fail_msg("tace_embed_grad: too many rows and tokens without a grouping");
+  if (grouped && !rowptr) return tace_fail_msg("tace_embed_grad: null pointer");
+  if (form != SCANS && (!work || work_bytes < tace_embed_grad_work(type, n, vocab, channels, grouped) ||
+                        !row_aligned(work)))
+    return tace_fail_msg("tace_embed_grad: workspace too small or not 16-byte aligned");
   row_dispatch(type, [&](auto z) {
     typedef decltype(z) T;
     typedef row_sum_t<T> S;
@@ -710,15 +884,28 @@ extern "C" int tace_embed_grad(int type, int index_bytes, const void* g, const v
           hipStream_t s = (hipStream_t)stream;
           auto go = [&](auto i) {
             typedef decltype(i) I;
-            if (scans) {
+            if (form == SCANS) {
               hipLaunchKernelGGL((k_embed_grad_scan<T, V, I>), dim3((unsigned)vocab, (unsigned)tiles), dim3(WG), 0, s,
                                  (const T*)g, (const I*)tokens, (int)n, channels, lanes, (S)scale, (T*)grad);
+              return;
+            }
+            const int columns = (channels + JOIN_COLS - 1) / JOIN_COLS;
+            if (form == SORTS) {
+              const int64_t locals = local_wgs(n);
+              const int ln = locals < 512 && cw > 16 ? 16 : lanes;
+              int* seen = (int*)work;
+              S* sums = (S*)((char*)work + local_seen(n, vocab));
+              hipLaunchKernelGGL((k_embed_grad_local<T, V, I>), dim3((unsigned)locals, (unsigned)((cw + ln - 1) / ln)),
+                                 dim3(WG), 0, s, (const T*)g, (const I*)tokens, (int)n, (int)vocab, channels,
+                                 local_rows(n), ln, seen, sums);
+              hipLaunchKernelGGL((k_embed_grad_total<T>), dim3((unsigned)vocab, (unsigned)columns), dim3(WG), 0, s,
+                                 seen, (int)locals, (int)vocab, channels, (S)scale, sums, (T*)grad);
               return;
             }
             hipLaunchKernelGGL((k_embed_grad_part<T, V, I>), dim3((unsigned)wgs, (unsigned)tiles), dim3(WG), 0, s,
                                (const T*)g, (const I*)tokens, order, (int)n, (int)vocab, channels, per, lanes,
                                (S)scale, (T*)grad, (S*)work);
-            const int columns = (channels + JOIN_COLS - 1) / JOIN_COLS, seams = wgs - 1;
+            const int seams = wgs - 1;
             const int64_t zeros = (vocab + 4 * columns - 1) / (4 * columns);
             hipLaunchKernelGGL((k_embed_grad_join<T, I>),
                                dim3((unsigned)(seams + (zeros < 2048 ? zeros : 2048)), (unsigned)columns), dim3(WG), 0,

@@ -147,19 +147,16 @@ Tensor embed_grad(const Tensor& g, const Tensor& tokens, const Lookup& a) {
   if (n == 0) return at::zeros({a.vocab, C}, g.options());
   const int code = type_code(g.scalar_type());
   Tensor grad = at::empty({a.vocab, C}, g.options()), rowptr, order, work;
-  int64_t bytes = 0;
-  if (!tace_embed_grad_scans(n, a.vocab, (int)C)) {
-    if (a.order.defined()) {
-      rowptr = a.rowptr;
-      order = a.order;
-    } else {
-      const Groups by = group(tokens, a.vocab, false, a.timed);
-      rowptr = by.rowptr;
-      order = by.order;
-    }
-    bytes = tace_embed_grad_work(code, n, a.vocab, (int)C);
-    work = at::empty({bytes}, g.options().dtype(at::kByte));
+  if (a.order.defined()) {
+    rowptr = a.rowptr;
+    order = a.order;
+  } else if (tace_embed_grad_grouped(n, a.vocab)) {
+    const Groups by = group(tokens, a.vocab, false, a.timed);
+    rowptr = by.rowptr;
+    order = by.order;
   }
+  const int64_t bytes = tace_embed_grad_work(code, n, a.vocab, (int)C, order.defined());
+  if (bytes > 16) work = at::empty({bytes}, g.options().dtype(at::kByte));
   Launch l(g, "embed_grad", a.timed);
   l.done(tace_embed_grad(code, (int)tokens.element_size(), ptr(g), ptr(tokens), ints(order), ints(rowptr), n, a.vocab,
                          (int)C, a.scale, ptr(grad), ptr(work), bytes, l.stream), {n, a.vocab, C});

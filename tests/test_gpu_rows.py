@@ -67,7 +67,8 @@ def _check_embedding(cuda, table, tokens, scale, g, index=torch.int64, groups=Fa
 
 @pytest.mark.parametrize("kind", ["even", "one", "hub", "sorted", "outside", "none"])
 @pytest.mark.parametrize("n,V,C", [(1, 1, 1), (7, 3, 4), (63, 89, 128), (4096, 1024, 8), (4097, 5, 64), (4096, 1025, 16),
-                                   (5000, 89, 100), (20001, 2, 128), (9000, 7921, 64)])
+                                   (5000, 89, 100), (20001, 2, 128), (9000, 7921, 64),
+                                   (70000, 128, 40), (70000, 129, 40), (262145, 7, 12)])
 def test_embedding(cuda, kind, n, V, C):
     _check_embedding(cuda, _rand((V, C), torch.float32, 1), _tokens(kind, n, V, n + V), 0.37,
                      _rand((n, C), torch.float32, 2))
@@ -417,7 +418,7 @@ def test_kernel_timer_sees_every_launch(cuda):
     finally:
         ops.TIMER = None
     assert {k: v[0] for k, v in seen.items()} == dict(
-        embed_fwd=1, embed_grad=1, dropout=2, route_group=2, route_dispatch=1, route_combine=2, route_dots=1)
+        embed_fwd=1, embed_grad=1, dropout=2, route_group=1, route_dispatch=1, route_combine=2, route_dots=1)
     assert all(ms > 0 for _, ms, _ in seen.values())
 
 

@@ -58,9 +58,10 @@ def test_entries_refuse_bad_arguments():
     _refused(L.tace_embed_fwd(0, 8, p, p, 4, 2 ** 31, 4, 1.0, p, None), b"bad sizes")
     _refused(L.tace_embed_fwd(0, 8, None, p, 4, 4, 4, 1.0, p, None), b"null")
     assert L.tace_embed_fwd(0, 8, None, None, 0, 4, 4, 1.0, None, None) == 0
-    _refused(L.tace_embed_grad(0, 8, p, p, None, None, 5000, 4, 4, 1.0, p, None, 0, None), b"without a grouping")
+    _refused(L.tace_embed_grad(0, 8, p, p, None, None, 5000, 400, 4, 1.0, p, None, 0, None), b"without a grouping")
+    _refused(L.tace_embed_grad(0, 8, p, p, None, None, 5000, 4, 4, 1.0, p, None, 0, None), b"workspace")
     _refused(L.tace_embed_grad(0, 8, p, p, p, p, 5000, 4, 4, 1.0, p, p, 16, None), b"workspace")
-    need = L.tace_embed_grad_work(0, 5000, 4, 4)
+    need = L.tace_embed_grad_work(0, 5000, 4, 4, 1)
     _refused(L.tace_embed_grad(0, 8, p, p, p, p, 5000, 4, 4, 1.0, p, p + 8, need, None), b"workspace")
     _refused(L.tace_embed_grad(0, 8, p, p, p, p, 2 ** 31, 4, 4, 1.0, p, p, need, None), b"bad sizes")
     for f in (L.tace_route_dispatch, L.tace_route_combine):
@@ -95,9 +96,14 @@ def test_workspace_covers_every_workgroup():
     for n in (1, 31, 257, 4097, 131072, 131073, 1063830, 2 ** 31 - 8193):
         for ty, size in ((0, 4), (1, 8), (2, 4)):
             for C in (1, 7, 100, 128, 4096, 32768):
-                nbytes = L.tace_embed_grad_work(ty, n, 7, C)
+                nbytes = L.tace_embed_grad_work(ty, n, 7, C, 1)
                 assert nbytes % (2 * C * size) == 0
                 assert 1 <= nbytes // (2 * C * size) <= 512
+                # ungrouped: a sum for each of 128 tokens and at least 256 rows
+                nbytes = L.tace_embed_grad_work(ty, n, 128, C, 0)
+                assert nbytes <= 16 + (n / 256 + 1) * 128 * (C * size + 4)
+    assert [L.tace_embed_grad_grouped(*a) for a in ((4096, 1024), (4097, 128), (4097, 129), (4096, 1025), (0, 9))] == [
+        0, 0, 1, 1, 0]
     _refused(L.tace_embed_grad(0, 8, 4096, 4096, 4096, 4096, 0, 4, 4, 1.0, 4096, 4096, 16, None), b"no rows")
 
 
