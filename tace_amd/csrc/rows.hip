@@ -1,5 +1,7 @@
 // Row operators: table lookup by token with its gradient, rows sorted by
-// expert and back.  All of them move rows once and are bound by HBM.
+// expert and back.  All of them move rows once and are bound by HBM (a copy of
+// 4 GiB reaches 4.8 TB/s here, one of 64 MiB 6.9, a fill 6.9), small ones by
+// their launches.
 #include "../../include/tace_hip.h"
 #include "row_types.h"
 
@@ -27,6 +29,10 @@ struct RowChunks {
   }
 };
 
+// out[i] = scale table[tokens[i]], zeros outside the table.  The table stays in
+// L2; bound by the stores, which go past the caches: 1.06 M rows of 64 float32
+// (272 MB) 43 us, 6.3 TB/s (57 with four chunks a thread and stores that stay
+// in the caches, 47 with two and stores past them).
 template <typename T, int V, typename I>
 __global__ __launch_bounds__(WG) void k_embed_fwd(const T* __restrict__ table, const I* __restrict__ tokens,
                                                   RowChunks rc, int64_t vocab, row_sum_t<T> scale,
@@ -62,6 +68,11 @@ __global__ __launch_bounds__(WG) void k_embed_fwd(const T* __restrict__ table, c
 //   left(), right()  the tokens before and behind the workgroup's positions, -1: none
 //   whole(v, c, sum), open(v, slot, c, sum)  where the sum of a run goes that
 //       ends inside the workgroup, and of one that goes on (slot 0: began before it)
+// Bound by rows read in no order, past the caches, eight in flight a thread while
+// the next eight positions are looked up: 1.06 M rows of 64 float32 of 7,921
+// tokens 61 us, 4.5 TB/s (70 through the caches; 166 with sixteen in flight, which
+// leave a SIMD too few wavefronts).  Joining all groups' runs by one group, not by
+// teams, made 1 M rows of 16 float32 47 us instead of 37: 128 sums in sequence.
 constexpr int TEAM = 8;   // groups whose open runs one of them joins
 template <typename T, int V>
 struct RunSums {
@@ -196,7 +207,10 @@ struct SortedRows {
   T* grad;
   row_sum_t<T>* part;
 
-  __device__ __forceinline__ int at(int p) const { return order[min(max(p, 0), n - 1)]; }
+  // (positions of another grouping than these tokens' stay inside the rows)
+  __device__ __forceinline__ int at(int p) const {
+    return (int)min((unsigned)order[min(max(p, 0), n - 1)], (unsigned)n - 1);
+  }
   __device__ __forceinline__ int key(int, int row) const {
     const I v = tokens[row];
     return v >= 0 && v < (I)vocab ? (int)v : -1;
@@ -231,7 +245,9 @@ __global__ __launch_bounds__(WG) void k_embed_grad_part(const T* __restrict__ g,
 // Few tokens (at most 128): a workgroup sorts its own `count` rows' tokens in
 // LDS, so no grouping of all of them is needed; each token's sum goes to part
 // [workgroup][token][channels] and its presence to seen [workgroup][token], for
-// k_embed_grad_total.  Two launches instead of four.
+// k_embed_grad_total.  Two launches instead of four; bound by the chain of loads
+// of a workgroup: 101,306 rows of 128 bfloat16 of two tokens 13.4 us and 3.8 for
+// the total.
 constexpr int FEW_TOKENS = 128, LOCAL_STEPS = 4, LOCAL_ROWS = WG * LOCAL_STEPS;
 template <typename T, int V>
 struct LocalRows {
@@ -327,8 +343,8 @@ __global__ __launch_bounds__(WG) void k_embed_grad_local(const T* __restrict__ g
 constexpr int JOIN_COLS = 16, JOIN_ROWS = WG / JOIN_COLS;
 template <typename T, typename I>
 __global__ __launch_bounds__(WG) void k_embed_grad_join(const I* __restrict__ tokens, const int* __restrict__ order,
-                                                        const int* __restrict__ rowptr, int vocab, int channels,
-                                                        int64_t span, int seams, row_sum_t<T> scale,
+                                                        const int* __restrict__ rowptr, int n, int vocab,
+                                                        int channels, int64_t span, int seams, row_sum_t<T> scale,
                                                         const row_sum_t<T>* __restrict__ part, T* __restrict__ grad) {
   typedef row_sum_t<T> S;
   const int t = (int)threadIdx.x;
@@ -340,11 +356,10 @@ __global__ __launch_bounds__(WG) void k_embed_grad_join(const I* __restrict__ to
         for (int c = t % 64; c < channels; c += 64) grad[v * channels + c] = (T)0;
     return;
   }
-  const int end = rowptr[vocab];
-  const int64_t w0 = blockIdx.x * span, w1 = w0 + span;
-  if (w1 >= end) return;
-  const int v = (int)tokens[order[w1]];
-  const int b = rowptr[v], e = rowptr[v + 1];
+  const int64_t w0 = blockIdx.x * span, w1 = w0 + span;   // (w1 < n)
+  const I tok = tokens[min((unsigned)order[w1], (unsigned)n - 1)];
+  if (tok < 0 || tok >= (I)vocab) return;   // padding
+  const int v = (int)tok, b = rowptr[v], e = min(rowptr[v + 1], n);
   if (b >= w1 || b < w0) return;   // begins at the seam, or joined at an earlier one
   __shared__ S red[JOIN_ROWS][JOIN_COLS];
   const int x = t % JOIN_COLS, y = t / JOIN_COLS, c = (int)blockIdx.y * JOIN_COLS + x;
@@ -392,7 +407,8 @@ __global__ __launch_bounds__(WG) void k_embed_grad_total(const int* __restrict__
 }
 
 // Few rows: a workgroup per token (and tile of columns) lists the token's rows
-// in LDS and sums them; no grouping, one launch.
+// in LDS and sums them; no grouping, one launch.  Bound by latency: 1,024 rows of
+// 128 float32 of 4 tokens 4.7 us.
 constexpr int SCAN_N = 4096;
 template <typename T, int V, typename I>
 __global__ __launch_bounds__(WG) void k_embed_grad_scan(const T* __restrict__ g, const I* __restrict__ tokens, int n,
@@ -464,7 +480,10 @@ int64_t embed_wgs(int64_t n, int lanes) {
 }
 
 // Which form the gradient takes without a grouping of the tokens: looking
-// through all of them, sorting them workgroup by workgroup, or none.
+// through all of them, sorting them workgroup by workgroup, or none (it needs
+// one).  us, this form | grouping and sums: SCANS 1,024 rows of 4 tokens 4.7 |
+// 11.8, 4,096 of 1,000 tokens 7.5 | 21.8; SORTS 5,000 of 89 13 | 18, 101,306 of 2
+// 18 | 30, 1 M of 89 71 | 76, 1 M of 128 tokens (512 MB) 125 | 115.
 enum { SCANS = 1, SORTS = 2, GROUPED = 0 };
 int embed_form(int64_t n, int64_t vocab) {
   return n <= SCAN_N && vocab <= 1024 ? SCANS : vocab <= FEW_TOKENS ? SORTS : GROUPED;
@@ -508,9 +527,9 @@ __global__ __launch_bounds__(WG) void k_route_place(const int* __restrict__ orde
 // a wavefront.  k_few_count leaves its counts of every key; k_few_place adds up
 // those of the workgroups before it and of all, ranks its own positions by
 // ballots and writes their places.  One workgroup (n <= 8,192) counts for
-// itself.  us, with the launches' gaps: 24,576 slots of 8 experts 11 instead of
-// 29 by the general grouping (tace_group_keys: any keys, four launches a digit
-// and one for the places).
+// itself.  Bound by latency; us, with places | general grouping (tace_group_keys:
+// any keys, four launches or more), without: 8,192 slots of 8 experts 9 | 11,
+// 24,576 of 8 8 | 17, 200,000 of 255 15 | 24, 1 M of 89 22 | 31.
 constexpr int FEW_WG = 1024, FEW_STEPS = 8, FEW_KEYS = 256, FEW_WGS = 128;
 
 template <typename I>
@@ -657,7 +676,8 @@ __device__ __forceinline__ void put(Vec* p, const Vec& v) {
   else *p = v;
 }
 
-// a row is read once and stored k times
+// A row is read once and stored k times: 12,288 x 2 rows of 2,048 float32 53 us
+// (5.7 TB/s), 101,306 x 2 of 1,152 bfloat16 119 (5.9).
 template <typename T, int V, bool STREAM>
 __global__ __launch_bounds__(WG) void k_route_dispatch(const T* __restrict__ x, const row_sum_t<T>* __restrict__ w,
                                                        const int* __restrict__ place, const int* __restrict__ rows_end,
@@ -687,7 +707,8 @@ __global__ __launch_bounds__(WG) void k_route_dispatch(const T* __restrict__ x, 
 }
 
 // K slots' rows are loaded before the first is added (the dropped ones too:
-// they have a row, which is not added)
+// they have a row, which is not added): 12,288 x 2 rows of 2,048 float32 53 us (5.7
+// TB/s; 60 one after the other), 101,306 x 2 of 1,152 bfloat16 112 (6.2; 131).
 template <typename T, int V, int K>
 __global__ __launch_bounds__(WG) void k_route_combine(const T* __restrict__ y, const row_sum_t<T>* __restrict__ w,
                                                       const int* __restrict__ place, const int* __restrict__ rows_end,
@@ -728,7 +749,9 @@ __global__ __launch_bounds__(WG) void k_route_combine(const T* __restrict__ y, c
 
 // `lanes` (a power of two, at most 64) lanes a slot, the slots of a token side
 // by side: its row of x comes from memory once.  U chunks of both rows are
-// loaded before the first is multiplied.
+// loaded before the first is multiplied.  12,288 x 2 rows of 2,048 float32 79 us
+// (6.4 TB/s; 103 with lanes that take a token's slots one after the other), 1,024
+// x 2 of them 9.3 (15), 101,306 x 2 of 1,152 bfloat16 214 (5.5).
 template <typename T, int V, int U>
 __global__ __launch_bounds__(WG) void k_route_dots(const T* __restrict__ x, const T* __restrict__ y,
                                                    const row_sum_t<T>* __restrict__ w, const int* __restrict__ place,
@@ -885,8 +908,10 @@ extern "C" int tace_embed_grad(int type, int index_bytes, const void* g, const v
           auto go = [&](auto i) {
             typedef decltype(i) I;
             if (form == SCANS) {
-              hipLaunchKernelGGL((k_embed_grad_scan<T, V, I>), dim3((unsigned)vocab, (unsigned)tiles), dim3(WG), 0, s,
-                                 (const T*)g, (const I*)tokens, (int)n, channels, lanes, (S)scale, (T*)grad);
+              const int ln = std::min(lanes, vocab < 64 ? 8 : 64);
+              hipLaunchKernelGGL((k_embed_grad_scan<T, V, I>), dim3((unsigned)vocab, (unsigned)((cw + ln - 1) / ln)),
+                                 dim3(WG), 0, s, (const T*)g, (const I*)tokens, (int)n, channels, ln, (S)scale,
+                                 (T*)grad);
               return;
             }
             const int columns = (channels + JOIN_COLS - 1) / JOIN_COLS;
@@ -909,8 +934,8 @@ extern "C" int tace_embed_grad(int type, int index_bytes, const void* g, const v
             const int64_t zeros = (vocab + 4 * columns - 1) / (4 * columns);
             hipLaunchKernelGGL((k_embed_grad_join<T, I>),
                                dim3((unsigned)(seams + (zeros < 2048 ? zeros : 2048)), (unsigned)columns), dim3(WG), 0,
-                               s, (const I*)tokens, order, rowptr, (int)vocab, channels, (int64_t)per * groups, seams,
-                               (S)scale, (const S*)work, (T*)grad);
+                               s, (const I*)tokens, order, rowptr, (int)n, (int)vocab, channels,
+                               (int64_t)per * groups, seams, (S)scale, (const S*)work, (T*)grad);
           };
           if (index_bytes == 4) go(int32_t());
           else go(int64_t());
