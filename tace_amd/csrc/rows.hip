@@ -242,58 +242,116 @@ __global__ __launch_bounds__(WG) void k_embed_grad_part(const T* __restrict__ g,
   sums.run(src, g, channels / V, lanes, p0, p1, per);
 }
 
-// Few tokens (at most 128): a workgroup sorts its own `count` rows' tokens in
+// Few tokens (at most 128): a workgroup sorts its own `rows` rows' tokens in
 // LDS, so no grouping of all of them is needed; each token's sum goes to part
 // [workgroup][token][channels] and its presence to seen [workgroup][token], for
 // k_embed_grad_total.  Two launches instead of four; bound by the chain of loads
 // of a workgroup: 101,306 rows of 128 bfloat16 of two tokens 13.4 us and 3.8 for
 // the total.
-constexpr int FEW_TOKENS = 128, LOCAL_STEPS = 4, LOCAL_ROWS = WG * LOCAL_STEPS;
-template <typename T, int V>
+//
+// More tokens in buckets of 128: the rows are grouped by bucket first (order,
+// bptr [buckets + 1]; few keys, two launches) and a workgroup has rows of one
+// bucket.  first [buckets + 1]: each bucket's first workgroup.  1.06 M rows of 64
+// float32 of 7,921 tokens: 20 us to group them, 77 here, 14 for the total.
+constexpr int FEW_TOKENS = 128, BUCKET_BITS = 7, LOCAL_STEPS = 8, LOCAL_ROWS = WG * LOCAL_STEPS, MAX_BUCKETS = 255;
+template <typename T, int V, bool BUCKETS>
 struct LocalRows {
-  const int* list;   // token << 16 | row in the workgroup, sorted
+  const int* list;    // token << 16 | row in the workgroup, sorted
+  const int* rowid;   // BUCKETS: the rows
   int64_t row0;
-  int count, vocab, channels;
+  int count, width, channels;
   row_sum_t<T>* part;
 
   __device__ __forceinline__ int packed(int p) const { return list[min(max(p, 0), count - 1)]; }
-  __device__ __forceinline__ int at(int p) const { return (int)(row0 + (packed(p) & 0xffff)); }
+  __device__ __forceinline__ int at(int p) const {
+    const int i = packed(p) & 0xffff;
+    return BUCKETS ? rowid[i] : (int)(row0 + i);
+  }
   __device__ __forceinline__ int key(int p, int) const { return p < count ? packed(p) >> 16 : -1; }
   __device__ __forceinline__ int left() const { return -1; }
   __device__ __forceinline__ int right() const { return -1; }
   __device__ __forceinline__ void whole(int v, int c, const row_sum_t<T>* sum) const {
-    row_sum_t<T>* o = part + ((int64_t)blockIdx.x * vocab + v) * channels + (int64_t)c * V;
+    row_sum_t<T>* o = part + ((int64_t)blockIdx.x * width + v) * channels + (int64_t)c * V;
 #pragma unroll
     for (int i = 0; i < V; ++i) o[i] = sum[i];
   }
   __device__ __forceinline__ void open(int, int, int, const row_sum_t<T>*) const {}   // (no run goes on)
 };
 
-template <typename T, int V, typename I>
-__global__ __launch_bounds__(WG) void k_embed_grad_local(const T* __restrict__ g, const I* __restrict__ tokens, int n,
-                                                         int vocab, int channels, int rows, int lanes,
-                                                         int* __restrict__ seen, row_sum_t<T>* __restrict__ part) {
+// Bucket of this workgroup and its first and last position: the buckets' counts
+// of workgroups are summed by every workgroup (at most 255 of them).  False for
+// a workgroup too many.
+__device__ __forceinline__ bool bucket_of(const int* __restrict__ bptr, int buckets, int rows, int* __restrict__ first,
+                                          int* found, int* wsum, int* bucket, int* begin, int* end) {
+  const int t = (int)threadIdx.x, lane = t & 63, w = t >> 6;
+  const int a = t < buckets ? bptr[t] : 0, z = t < buckets ? bptr[t + 1] : 0;
+  const int wgs = (z - a + rows - 1) / rows;
+  int inc = wgs;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int v = __shfl_up(inc, o, 64);
+    if (lane >= o) inc += v;
+  }
+  if (lane == 63) wsum[w] = inc;
+  if (t == 0) found[0] = -1;
+  __syncthreads();
+  for (int k = 0; k < w; ++k) inc += wsum[k];
+  const int at = inc - wgs;   // this bucket's first workgroup
+  if (blockIdx.x == 0 && blockIdx.y == 0 && t <= buckets) first[t] = at;   // (t = buckets: all of them)
+  if ((int)blockIdx.x >= at && (int)blockIdx.x < inc) {
+    found[0] = t;
+    found[1] = a + ((int)blockIdx.x - at) * rows;
+    found[2] = min(found[1] + rows, z);
+  }
+  __syncthreads();
+  *bucket = found[0];
+  *begin = found[1];
+  *end = found[2];
+  return *bucket >= 0;
+}
+
+template <typename T, int V, typename I, bool BUCKETS>
+__global__ __launch_bounds__(WG) void k_embed_grad_local(const T* __restrict__ g, const I* __restrict__ tokens,
+                                                         const int* __restrict__ order, const int* __restrict__ bptr,
+                                                         int buckets, int n, int vocab, int channels, int rows,
+                                                         int lanes, int* __restrict__ first, int* __restrict__ seen,
+                                                         row_sum_t<T>* __restrict__ part) {
   constexpr int WAVES = WG / 64;
   __shared__ RunSums<T, V> sums;
-  __shared__ int list[LOCAL_ROWS], cnt[WAVES][FEW_TOKENS], wsum[2], kept;
+  __shared__ int list[LOCAL_ROWS], rowid[BUCKETS ? LOCAL_ROWS : 1], cnt[WAVES][FEW_TOKENS], wsum[WAVES], found[3], kept;
   const int t = (int)threadIdx.x, lane = t & 63, w = t >> 6, steps = rows / WG;
-  const int64_t row0 = (int64_t)blockIdx.x * rows;
+  int bucket = 0, begin = 0, end = 0;
+  if constexpr (BUCKETS) {
+    if (!bucket_of(bptr, buckets, rows, first, found, wsum, &bucket, &begin, &end)) return;
+  }
+  const int64_t row0 = BUCKETS ? begin : (int64_t)blockIdx.x * rows, stop = BUCKETS ? end : n;
+  const int width = BUCKETS ? FEW_TOKENS : vocab, base = bucket << BUCKET_BITS;
   for (int q = t; q < WAVES * FEW_TOKENS; q += WG) cnt[q / FEW_TOKENS][q % FEW_TOKENS] = 0;
   const int i0 = 64 * steps * w + lane;   // (of the workgroup's rows; a run of 64 `steps` a wavefront)
   I tok[LOCAL_STEPS];
+  int row[LOCAL_STEPS];
 #pragma unroll
   for (int u = 0; u < LOCAL_STEPS; ++u)
-    if (u < steps) tok[u] = tokens[min(row0 + i0 + 64 * u, (int64_t)n - 1)];
+    if (u < steps) {
+      const int p = (int)min(row0 + i0 + 64 * u, stop - 1);
+      row[u] = BUCKETS ? order[p] : p;
+    }
+#pragma unroll
+  for (int u = 0; u < LOCAL_STEPS; ++u)
+    if (u < steps) {
+      tok[u] = tokens[row[u]];
+      if (BUCKETS) rowid[i0 + 64 * u] = row[u];
+    }
   __syncthreads();
   int key[LOCAL_STEPS], rank[LOCAL_STEPS];
 #pragma unroll
   for (int u = 0; u < LOCAL_STEPS; ++u) {
-    const bool in = u < steps && row0 + i0 + 64 * u < n && tok[u] >= 0 && tok[u] < (I)vocab;
-    key[u] = in ? (int)tok[u] : -1;
+    const bool in = u < steps && row0 + i0 + 64 * u < stop && tok[u] >= 0 && tok[u] < (I)vocab;
+    key[u] = in ? (int)tok[u] - base : -1;   // (0 .. 127)
     if (u >= steps) continue;   // (all lanes alike)
     unsigned long long m = __ballot(in);
 #pragma unroll
-    for (int b = 0; (1 << b) < FEW_TOKENS; ++b) {
+    for (int b = 0; b < BUCKET_BITS; ++b) {
       const bool one = (key[u] >> b) & 1;
       const unsigned long long v = __ballot(one);
       m &= one ? v : ~v;
@@ -318,7 +376,7 @@ __global__ __launch_bounds__(WG) void k_embed_grad_local(const T* __restrict__ g
   if (t < FEW_TOKENS) {
     int at = inc - sum + (w == 1 ? wsum[0] : 0);
     if (t == FEW_TOKENS - 1) kept = at + sum;
-    if (t < vocab && blockIdx.y == 0) seen[(int64_t)blockIdx.x * vocab + t] = sum;
+    if (t < width && blockIdx.y == 0) seen[(int64_t)blockIdx.x * width + t] = sum;
     for (int k = 0; k < WAVES; ++k) {
       const int c = cnt[k][t];
       cnt[k][t] = at;
@@ -332,7 +390,7 @@ __global__ __launch_bounds__(WG) void k_embed_grad_local(const T* __restrict__ g
   __syncthreads();
   const int count = kept;
   if (count == 0) return;
-  const LocalRows<T, V> src{list, row0, count, vocab, channels, part};
+  const LocalRows<T, V, BUCKETS> src{list, rowid, row0, count, width, channels, part};
   const int groups = WG / lanes;
   sums.run(src, g, channels / V, lanes, 0, count, (count + groups - 1) / groups);
 }
@@ -379,29 +437,34 @@ __global__ __launch_bounds__(WG) void k_embed_grad_join(const I* __restrict__ to
   }
 }
 
-// grad of k_embed_grad_local's sums: 16 columns of a token a workgroup
-template <typename T>
-__global__ __launch_bounds__(WG) void k_embed_grad_total(const int* __restrict__ seen, int workgroups, int vocab,
-                                                         int channels, row_sum_t<T> scale,
+// grad of k_embed_grad_local's sums: COLS columns of a token for each WG / TOKENS
+// threads.  Without buckets there are few tokens and many sums of each; with
+// them (first) many tokens, most of few sums.
+template <typename T, int COLS, int TOKENS>
+__global__ __launch_bounds__(WG) void k_embed_grad_total(const int* __restrict__ seen, const int* __restrict__ first,
+                                                         int workgroups, int vocab, int channels, row_sum_t<T> scale,
                                                          const row_sum_t<T>* __restrict__ part, T* __restrict__ grad) {
   typedef row_sum_t<T> S;
-  __shared__ S red[JOIN_ROWS][JOIN_COLS];
-  const int t = (int)threadIdx.x, x = t % JOIN_COLS, y = t / JOIN_COLS, v = (int)blockIdx.x;
-  const int c = (int)blockIdx.y * JOIN_COLS + x;
+  constexpr int ROWS = WG / COLS / TOKENS;
+  __shared__ S red[TOKENS * ROWS][COLS];
+  const int t = (int)threadIdx.x, x = t % COLS, yy = t / COLS, y = yy % ROWS;
+  const int v = (int)blockIdx.x * TOKENS + yy / ROWS, c = (int)blockIdx.y * COLS + x;
+  const int bucket = v >> BUCKET_BITS, width = first ? FEW_TOKENS : vocab, at = first ? v % FEW_TOKENS : v;
   S sum = 0;
-  if (c < channels) {
+  if (c < channels && v < vocab) {
+    const int q0 = first ? first[bucket] : 0, q1 = first ? first[bucket + 1] : workgroups;
 #pragma unroll 8
-    for (int q = y; q < workgroups; q += JOIN_ROWS) {
-      const int64_t at = (int64_t)q * vocab + v;
-      const S p = part[at * channels + c];   // (holds nothing where the token was not seen)
-      sum += seen[at] ? p : (S)0;
+    for (int q = q0 + y; q < q1; q += ROWS) {
+      const int64_t i = (int64_t)q * width + at;
+      const S p = part[i * channels + c];   // (holds nothing where the token was not seen)
+      sum += seen[i] ? p : (S)0;
     }
   }
-  red[y][x] = sum;
+  red[yy][x] = sum;
   __syncthreads();
-  if (y == 0 && c < channels) {
+  if (y == 0 && c < channels && v < vocab) {
 #pragma unroll
-    for (int k = 1; k < JOIN_ROWS; ++k) sum += red[k][x];
+    for (int k = 1; k < ROWS; ++k) sum += red[yy + k][x];
     grad[(int64_t)v * channels + c] = (T)(sum * scale);
   }
 }
@@ -479,25 +542,6 @@ int64_t embed_wgs(int64_t n, int lanes) {
   return (n + span - 1) / span;
 }
 
-// Which form the gradient takes without a grouping of the tokens: looking
-// through all of them, sorting them workgroup by workgroup, or none (it needs
-// one).  us, this form | grouping and sums: SCANS 1,024 rows of 4 tokens 4.7 |
-// 11.8, 4,096 of 1,000 tokens 7.5 | 21.8; SORTS 5,000 of 89 13 | 18, 101,306 of 2
-// 18 | 30, 1 M of 89 71 | 76, 1 M of 128 tokens (512 MB) 125 | 115.
-enum { SCANS = 1, SORTS = 2, GROUPED = 0 };
-int embed_form(int64_t n, int64_t vocab) {
-  return n <= SCAN_N && vocab <= 1024 ? SCANS : vocab <= FEW_TOKENS ? SORTS : GROUPED;
-}
-
-// SORTS: rows a workgroup (256 .. 1,024: about 256 workgroups), their number,
-// and the threads a row: 16 where that leaves the GPU few workgroups
-int local_rows(int64_t n) {
-  const int64_t steps = (n + 256 * WG - 1) / (256 * WG);
-  return WG * (int)std::min<int64_t>(std::max<int64_t>(steps, 1), LOCAL_STEPS);
-}
-int64_t local_wgs(int64_t n) { return (n + local_rows(n) - 1) / local_rows(n); }
-int64_t local_seen(int64_t n, int64_t vocab) { return (local_wgs(n) * vocab * 4 + 15) / 16 * 16; }   // bytes
-
 // --------------------------------------------------------------- routing ----
 // A row's chunks in blocks that lie apart: block b of R rows starts at R *
 // start[b] chunks and holds start[b + 1] - start[b] of each row.
@@ -532,11 +576,15 @@ __global__ __launch_bounds__(WG) void k_route_place(const int* __restrict__ orde
 // 24,576 of 8 8 | 17, 200,000 of 255 15 | 24, 1 M of 89 22 | 31.
 constexpr int FEW_WG = 1024, FEW_STEPS = 8, FEW_KEYS = 256, FEW_WGS = 128;
 
-template <typename I>
-__device__ __forceinline__ int few_key(I e, int n_keys) { return e >= 0 && e < (I)n_keys ? (int)e : n_keys; }
+// keys are the values below `limit`, shifted
+struct FewKeys {
+  int limit, shift, count;
+  template <typename I>
+  __device__ __forceinline__ int of(I e) const { return e >= 0 && e < (I)limit ? (int)e >> shift : count; }
+};
 
 template <typename I>
-__global__ __launch_bounds__(FEW_WG) void k_few_count(const I* __restrict__ keys, int64_t stride, int n, int n_keys,
+__global__ __launch_bounds__(FEW_WG) void k_few_count(const I* __restrict__ keys, int64_t stride, int n, FewKeys fk,
                                                       int steps, int* __restrict__ hist) {
   __shared__ int cnt[FEW_KEYS];
   const int t = (int)threadIdx.x;
@@ -549,19 +597,19 @@ __global__ __launch_bounds__(FEW_WG) void k_few_count(const I* __restrict__ keys
     if (u < steps) e[u] = keys[min(i0 + FEW_WG * u, (int64_t)n - 1) * stride];
 #pragma unroll
   for (int u = 0; u < FEW_STEPS; ++u)
-    if (u < steps && i0 + FEW_WG * u < n) atomicAdd(cnt + few_key(e[u], n_keys), 1);
+    if (u < steps && i0 + FEW_WG * u < n) atomicAdd(cnt + fk.of(e[u]), 1);
   __syncthreads();
-  if (t <= n_keys) hist[(int64_t)blockIdx.x * (n_keys + 1) + t] = cnt[t];
+  if (t <= fk.count) hist[(int64_t)blockIdx.x * (fk.count + 1) + t] = cnt[t];
 }
 
 template <typename I>
-__global__ __launch_bounds__(FEW_WG) void k_few_place(const I* __restrict__ keys, int64_t stride, int n, int n_keys,
+__global__ __launch_bounds__(FEW_WG) void k_few_place(const I* __restrict__ keys, int64_t stride, int n, FewKeys fk,
                                                       int steps, int bits, const int* __restrict__ hist,
                                                       int* __restrict__ rowptr, int* __restrict__ order,
                                                       int* __restrict__ place) {
   constexpr int WAVES = FEW_WG / 64;
   __shared__ int cnt[WAVES][FEW_KEYS], red[FEW_WG], before[FEW_KEYS], total[FEW_KEYS], wsum[4];
-  const int t = (int)threadIdx.x, lane = t & 63, w = t >> 6, nwg = (int)gridDim.x, K = n_keys + 1;
+  const int t = (int)threadIdx.x, lane = t & 63, w = t >> 6, nwg = (int)gridDim.x, K = fk.count + 1;
   for (int q = t; q < WAVES * FEW_KEYS; q += FEW_WG) cnt[q / FEW_KEYS][q % FEW_KEYS] = 0;
   const int64_t i0 = ((int64_t)blockIdx.x * WAVES + w) * 64 * steps + lane;
   I e[FEW_STEPS];
@@ -599,7 +647,7 @@ __global__ __launch_bounds__(FEW_WG) void k_few_place(const I* __restrict__ keys
 #pragma unroll
   for (int u = 0; u < FEW_STEPS; ++u) {
     const bool in = u < steps && i0 + 64 * u < n;
-    key[u] = in ? few_key(e[u], n_keys) : -1;
+    key[u] = in ? fk.of(e[u]) : -1;
     if (u >= steps) continue;   // (all lanes alike)
     const int k = key[u];
     // this lane's place among its wavefront's equal keys so far
@@ -632,7 +680,7 @@ __global__ __launch_bounds__(FEW_WG) void k_few_place(const I* __restrict__ keys
   if (t < FEW_KEYS) {
     int at = inc - sum;
     for (int k = 0; k < w; ++k) at += wsum[k];
-    if (t < K && blockIdx.x == 0) rowptr[t] = at;   // (key n_keys: the end of the others)
+    if (t < K && blockIdx.x == 0) rowptr[t] = at;   // (the last: the end of the others)
     if (nwg > 1 && t < K) at += before[t];
     for (int k = 0; k < WAVES; ++k) {
       const int c = cnt[k][t];
@@ -653,21 +701,74 @@ __global__ __launch_bounds__(FEW_WG) void k_few_place(const I* __restrict__ keys
 // whether few_group takes it, and its workgroups and steps
 bool few_fits(int64_t n, int64_t n_keys, int* wgs, int* steps) {
   const int64_t most = n <= FEW_WG * FEW_STEPS ? 1 : FEW_WGS;
-  *steps = (int)std::min<int64_t>((n + FEW_WG * most - 1) / (FEW_WG * most), FEW_STEPS + 1);
-  *wgs = *steps ? (int)((n + FEW_WG * *steps - 1) / (FEW_WG * *steps)) : 0;
-  return n >= 1 && n_keys < FEW_KEYS && *steps <= FEW_STEPS;
+  *steps = (int)std::min<int64_t>((n + FEW_WG * most - 1) / (FEW_WG * most), FEW_STEPS);
+  const int64_t count = n < 1 ? 0 : (n + FEW_WG * *steps - 1) / (FEW_WG * *steps);
+  *wgs = (int)std::min<int64_t>(count, 1 << 20);
+  return n >= 1 && n_keys < FEW_KEYS && count <= 4 * FEW_WGS;
 }
 
 template <typename I>
-void few_group(const I* keys, int64_t stride, int n, int n_keys, int wgs, int steps, int32_t* rowptr, int32_t* order,
-               int32_t* place, int32_t* work, hipStream_t s) {
+void few_group(const I* keys, int64_t stride, int n, const FewKeys& fk, int wgs, int steps, int32_t* rowptr,
+               int32_t* order, int32_t* place, int32_t* work, hipStream_t s) {
   int bits = 1;
-  while ((1 << bits) < n_keys + 1) ++bits;
+  while ((1 << bits) < fk.count + 1) ++bits;
   if (wgs > 1)
-    hipLaunchKernelGGL((k_few_count<I>), dim3((unsigned)wgs), dim3(FEW_WG), 0, s, keys, stride, n, n_keys, steps, work);
-  hipLaunchKernelGGL((k_few_place<I>), dim3((unsigned)wgs), dim3(FEW_WG), 0, s, keys, stride, n, n_keys, steps, bits,
-                     work, rowptr, order, place);
+    hipLaunchKernelGGL((k_few_count<I>), dim3((unsigned)wgs), dim3(FEW_WG), 0, s, keys, stride, n, fk, steps, work);
+  hipLaunchKernelGGL((k_few_place<I>), dim3((unsigned)wgs), dim3(FEW_WG), 0, s, keys, stride, n, fk, steps, bits, work,
+                     rowptr, order, place);
 }
+
+// ------------------------------------------- the embedding gradient's form ----
+// Which form it takes without a grouping of the tokens: looking through all of
+// them, sorting them workgroup by workgroup, that in buckets of 128 tokens, or
+// none (it needs a grouping).  us, this form | grouping and sums: SCANS 1,024
+// rows of 4 tokens 4.9 | 11.9, 4,096 of 1,000 tokens 7.5 | 21.5; SORTS 5,000 of 89
+// 14 | 19, 101,306 of 2 19 | 29, 1 M of 89 64 | 77, 1 M of 128 tokens (512 MB) 119
+// | 116; BUCKETS 9,000 rows of 1,000 tokens 23 | 41, 50,000 of 8,000 30 | 47, 1.06 M
+// of 7,921 102 | 119, 300,000 of 3,000 99 | 99, 1 M of 300 100 | 98.
+enum { SCANS = 1, SORTS = 2, BUCKETS = 3, GROUPED = 0 };
+
+// rows a workgroup (256 .. 2,048: about 256 workgroups) and workgroups, one more
+// a bucket where they are not full
+int local_rows(int64_t n) {
+  const int64_t steps = (n + 256 * WG - 1) / (256 * WG);
+  return WG * (int)std::min<int64_t>(std::max<int64_t>(steps, 1), LOCAL_STEPS);
+}
+int64_t buckets_of(int64_t vocab) { return (vocab + FEW_TOKENS - 1) / FEW_TOKENS; }
+
+int embed_form(int64_t n, int64_t vocab) {
+  if (n <= SCAN_N && vocab <= 1024) return SCANS;
+  if (vocab <= FEW_TOKENS) return SORTS;
+  int wgs, steps;
+  const int64_t buckets = buckets_of(vocab);
+  // (its sums are at most about as many as the rows)
+  return n > 8192 && buckets <= MAX_BUCKETS && buckets * FEW_TOKENS <= n && few_fits(n, buckets, &wgs, &steps)
+             ? BUCKETS : GROUPED;
+}
+
+// parts of the workspace of SORTS and BUCKETS, in bytes
+struct LocalWork {
+  int64_t wgs, hist, bptr, order, first, seen, part, bytes;
+  LocalWork(int64_t n, int64_t vocab, int64_t row_bytes) {
+    const bool many = vocab > FEW_TOKENS;
+    const int64_t buckets = many ? buckets_of(vocab) : 0, width = many ? FEW_TOKENS : vocab;
+    wgs = (n + local_rows(n) - 1) / local_rows(n) + buckets;
+    int few = 0, steps = 0;
+    if (many) few_fits(n, buckets, &few, &steps);
+    bytes = 0;
+    auto take = [&](int64_t b) {
+      const int64_t at = bytes;
+      bytes += (b + 15) / 16 * 16;
+      return at;
+    };
+    hist = take(4 * few * (buckets + 1));
+    bptr = take(many ? 4 * (buckets + 1) : 0);
+    order = take(many ? 4 * n : 0);
+    first = take(many ? 4 * (buckets + 1) : 0);
+    seen = take(4 * wgs * width);
+    part = take(wgs * width * row_bytes);
+  }
+};
 
 // STREAM: stores that do not stay in the caches
 template <bool STREAM, typename Vec>
@@ -868,7 +969,10 @@ extern "C" int tace_embed_grad_grouped(int64_t n, int64_t vocab) { return embed_
 extern "C" int64_t tace_embed_grad_work(int type, int64_t n, int64_t vocab, int32_t channels, int grouped) {
   if (n < 1 || vocab < 1 || channels < 1 || channels > MAX_ROW) return 16;
   const int64_t row = (int64_t)channels * (type == TACE_ROW_F64 ? 8 : 4);
-  if (!grouped) return embed_form(n, vocab) == SORTS ? local_seen(n, vocab) + local_wgs(n) * vocab * row : 16;
+  if (!grouped) {
+    const int form = embed_form(n, vocab);
+    return form == SORTS || form == BUCKETS ? LocalWork(n, vocab, row).bytes : 16;
+  }
   // (rows may be moved by 16 bytes, 8, or one element: the largest count of workgroups)
   const int bytes = type == TACE_ROW_F64 ? 8 : type == TACE_ROW_F32 ? 4 : 2;
   int64_t wgs = 0;
@@ -915,16 +1019,34 @@ extern "C" int tace_embed_grad(int type, int index_bytes, const void* g, const v
               return;
             }
             const int columns = (channels + JOIN_COLS - 1) / JOIN_COLS;
-            if (form == SORTS) {
-              const int64_t locals = local_wgs(n);
-              const int ln = locals < 512 && cw > 16 ? 16 : lanes;
-              int* seen = (int*)work;
-              S* sums = (S*)((char*)work + local_seen(n, vocab));
-              hipLaunchKernelGGL((k_embed_grad_local<T, V, I>), dim3((unsigned)locals, (unsigned)((cw + ln - 1) / ln)),
-                                 dim3(WG), 0, s, (const T*)g, (const I*)tokens, (int)n, (int)vocab, channels,
-                                 local_rows(n), ln, seen, sums);
-              hipLaunchKernelGGL((k_embed_grad_total<T>), dim3((unsigned)vocab, (unsigned)columns), dim3(WG), 0, s,
-                                 seen, (int)locals, (int)vocab, channels, (S)scale, sums, (T*)grad);
+            if (form == SORTS || form == BUCKETS) {
+              const LocalWork lw(n, vocab, channels * (int64_t)sizeof(S));
+              char* at = (char*)work;
+              int *bptr = (int*)(at + lw.bptr), *by = (int*)(at + lw.order), *first = (int*)(at + lw.first);
+              int* seen = (int*)(at + lw.seen);
+              S* sums = (S*)(at + lw.part);
+              // (16 threads a row where that leaves the GPU few workgroups)
+              const int ln = lw.wgs < 512 && cw > 16 ? 16 : lanes, rows = local_rows(n);
+              const dim3 grid((unsigned)lw.wgs, (unsigned)((cw + ln - 1) / ln));
+              if (form == SORTS) {
+                hipLaunchKernelGGL((k_embed_grad_local<T, V, I, false>), grid, dim3(WG), 0, s, (const T*)g,
+                                   (const I*)tokens, nullptr, nullptr, 0, (int)n, (int)vocab, channels, rows, ln,
+                                   nullptr, seen, sums);
+                hipLaunchKernelGGL((k_embed_grad_total<T, 16, 1>), dim3((unsigned)vocab, (unsigned)columns), dim3(WG),
+                                   0, s, seen, nullptr, (int)lw.wgs, (int)vocab, channels, (S)scale, sums, (T*)grad);
+                return;
+              }
+              const int buckets = (int)buckets_of(vocab);
+              int few, steps;
+              few_fits(n, buckets, &few, &steps);
+              few_group((const I*)tokens, 1, (int)n, FewKeys{(int)vocab, BUCKET_BITS, buckets}, few, steps, bptr, by,
+                        nullptr, (int32_t*)(at + lw.hist), s);
+              hipLaunchKernelGGL((k_embed_grad_local<T, V, I, true>), grid, dim3(WG), 0, s, (const T*)g,
+                                 (const I*)tokens, by, bptr, buckets, (int)n, (int)vocab, channels, rows, ln, first,
+                                 seen, sums);
+              hipLaunchKernelGGL((k_embed_grad_total<T, 32, 2>),
+                                 dim3((unsigned)((vocab + 1) / 2), (unsigned)((channels + 31) / 32)), dim3(WG), 0, s,
+                                 seen, first, 0, (int)vocab, channels, (S)scale, sums, (T*)grad);
               return;
             }
             hipLaunchKernelGGL((k_embed_grad_part<T, V, I>), dim3((unsigned)wgs, (unsigned)tiles), dim3(WG), 0, s,
@@ -960,10 +1082,11 @@ extern "C" int tace_route_group(int index_bytes, const void* keys, int64_t strid
   hipStream_t s = (hipStream_t)stream;
   int wgs, steps;
   if (few_fits(n, n_keys, &wgs, &steps)) {
+    const FewKeys fk{(int)n_keys, 0, (int)n_keys};
     if (index_bytes == 4)
-      few_group((const int32_t*)keys, stride, (int)n, (int)n_keys, wgs, steps, rowptr, order, place, work, s);
+      few_group((const int32_t*)keys, stride, (int)n, fk, wgs, steps, rowptr, order, place, work, s);
     else
-      few_group((const int64_t*)keys, stride, (int)n, (int)n_keys, wgs, steps, rowptr, order, place, work, s);
+      few_group((const int64_t*)keys, stride, (int)n, fk, wgs, steps, rowptr, order, place, work, s);
     return tace_check_launch("tace_route_group");
   }
   int32_t* k32 = work + tace_group_keys_work(n, n_keys);

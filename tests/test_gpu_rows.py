@@ -68,7 +68,8 @@ def _check_embedding(cuda, table, tokens, scale, g, index=torch.int64, groups=Fa
 @pytest.mark.parametrize("kind", ["even", "one", "hub", "sorted", "outside", "none"])
 @pytest.mark.parametrize("n,V,C", [(1, 1, 1), (7, 3, 4), (63, 89, 128), (4096, 1024, 8), (4097, 5, 64), (4096, 1025, 16),
                                    (5000, 89, 100), (20001, 2, 128), (9000, 7921, 64),
-                                   (70000, 128, 40), (70000, 129, 40), (262145, 7, 12)])
+                                   (70000, 128, 40), (70000, 129, 40), (262145, 7, 12),
+                                   (40000, 32640, 8), (40000, 32641, 8), (8193, 300, 68), (30000, 3000, 4)])
 def test_embedding(cuda, kind, n, V, C):
     _check_embedding(cuda, _rand((V, C), torch.float32, 1), _tokens(kind, n, V, n + V), 0.37,
                      _rand((n, C), torch.float32, 2))
@@ -80,6 +81,13 @@ def test_embedding(cuda, kind, n, V, C):
 def test_embedding_types_and_widths(cuda, dt, index, n, V, C):
     _check_embedding(cuda, _rand((V, C), dt, 3), _tokens("outside", n, V, C), 1.7, _rand((n, C), dt, 4), index,
                      groups=n > 4096)
+
+
+@pytest.mark.parametrize("kind", ["even", "hub", "outside", "none"])
+@pytest.mark.parametrize("n,V,C", [(4000, 7, 12), (70000, 2, 128), (70000, 3000, 20), (270000, 300, 8)])
+def test_embedding_with_a_grouping(cuda, kind, n, V, C):
+    _check_embedding(cuda, _rand((V, C), torch.float32, 1), _tokens(kind, n, V, n + V), 0.37,
+                     _rand((n, C), torch.float32, 2), groups=True)
 
 
 def test_embedding_long_sums(cuda):

@@ -102,8 +102,10 @@ def test_workspace_covers_every_workgroup():
                 # ungrouped: a sum for each of 128 tokens and at least 256 rows
                 nbytes = L.tace_embed_grad_work(ty, n, 128, C, 0)
                 assert nbytes <= 16 + (n / 256 + 1) * 128 * (C * size + 4)
-    assert [L.tace_embed_grad_grouped(*a) for a in ((4096, 1024), (4097, 128), (4097, 129), (4096, 1025), (0, 9))] == [
-        0, 0, 1, 1, 0]
+    assert [L.tace_embed_grad_grouped(*a) for a in ((4096, 1024), (4097, 128), (4097, 129), (4096, 1025), (0, 9),
+                                                         (8193, 8192), (8193, 8193), (40000, 32640), (40000, 32641),
+                                                         (2 ** 22, 999), (2 ** 22 + 1, 999))] == [
+        0, 0, 1, 1, 0, 0, 1, 0, 1, 0, 1]
     _refused(L.tace_embed_grad(0, 8, 4096, 4096, 4096, 4096, 0, 4, 4, 1.0, 4096, 4096, 16, None), b"no rows")
 
 
