@@ -742,7 +742,7 @@ int embed_form(int64_t n, int64_t vocab) {
   int wgs, steps;
   const int64_t buckets = buckets_of(vocab);
   // (its sums are at most about as many as the rows)
-  return n > 8192 && buckets <= MAX_BUCKETS && buckets * FEW_TOKENS <= n && few_fits(n, buckets, &wgs, &steps)
+  return n > SCAN_N && buckets <= MAX_BUCKETS && buckets * FEW_TOKENS <= n && few_fits(n, buckets, &wgs, &steps)
              ? BUCKETS : GROUPED;
 }
 

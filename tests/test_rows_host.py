@@ -58,7 +58,7 @@ def test_entries_refuse_bad_arguments():
     _refused(L.tace_embed_fwd(0, 8, p, p, 4, 2 ** 31, 4, 1.0, p, None), b"bad sizes")
     _refused(L.tace_embed_fwd(0, 8, None, p, 4, 4, 4, 1.0, p, None), b"null")
     assert L.tace_embed_fwd(0, 8, None, None, 0, 4, 4, 1.0, None, None) == 0
-    _refused(L.tace_embed_grad(0, 8, p, p, None, None, 5000, 400, 4, 1.0, p, None, 0, None), b"without a grouping")
+    _refused(L.tace_embed_grad(0, 8, p, p, None, None, 4096, 5000, 4, 1.0, p, None, 0, None), b"without a grouping")
     _refused(L.tace_embed_grad(0, 8, p, p, None, None, 5000, 4, 4, 1.0, p, None, 0, None), b"workspace")
     _refused(L.tace_embed_grad(0, 8, p, p, p, p, 5000, 4, 4, 1.0, p, p, 16, None), b"workspace")
     need = L.tace_embed_grad_work(0, 5000, 4, 4, 1)
@@ -105,7 +105,7 @@ def test_workspace_covers_every_workgroup():
     assert [L.tace_embed_grad_grouped(*a) for a in ((4096, 1024), (4097, 128), (4097, 129), (4096, 1025), (0, 9),
                                                          (8193, 8192), (8193, 8193), (40000, 32640), (40000, 32641),
                                                          (2 ** 22, 999), (2 ** 22 + 1, 999))] == [
-        0, 0, 1, 1, 0, 0, 1, 0, 1, 0, 1]
+        0, 0, 0, 1, 0, 0, 1, 0, 1, 0, 1]
     _refused(L.tace_embed_grad(0, 8, 4096, 4096, 4096, 4096, 0, 4, 4, 1.0, 4096, 4096, 16, None), b"no rows")
 
 
