@@ -50,7 +50,9 @@ struct Parts {
 // each component) in the order of memory: of its q-th V each, a lane takes the
 // ones that lane q 8 V + lane V / 8 drew for.  Needs channels % V == 0, or one
 // block of one component (flat: the last V elements may be fewer).  Bound by
-// HBM: the ten rounds are 160 integer operations for 8 elements.  us (TB/s): 25 M
+// HBM: the ten rounds are 20 wide multiplications and 34 exclusive ors for 8
+// elements, and twice that, for draws of 32 bits, took the same time (81 us for
+// 117 M bfloat16): 16 bits are enough for a probability.  us (TB/s): 25 M
 // float32 in degrees 0 .. 3 37 (5.4), with a residual 56 (5.4); 117 M bfloat16 in
 // degrees 0 .. 2 80 (5.9).  With lanes that kept their own 8 elements (two moves
 // of every other 16 bytes, one component after the other) 51, 74 and 89; with
