@@ -64,25 +64,38 @@ def _compile(src: str, force: bool) -> str:
 ROWS_LIB = os.path.join(LIBDIR, "_rows.so")
 
 
-def _build_rows(force: bool) -> None:
-    """The row operators' torch binding (host code only), linked to the library beside it."""
+ROWS_SRC = os.path.join(CSRC, "rows_torch.cpp")
+
+
+def _compile_rows(force: bool) -> str:
+    """The object of the row operators' torch binding (host code only)."""
     import sysconfig
 
     import torch
 
-    src = os.path.join(CSRC, "rows_torch.cpp")
-    deps = [src] + [os.path.join(ROOT, "include", h) for h in ("tace_hip.h", "tace_rows.h")]
-    if not force and os.path.exists(ROWS_LIB) and os.path.getmtime(ROWS_LIB) >= max(os.path.getmtime(d) for d in deps):
-        return
-    top = os.path.dirname(torch.__file__)
-    inc = [os.path.join(top, "include"), os.path.join(top, "include", "torch", "csrc", "api", "include"),
-           sysconfig.get_paths()["include"], os.path.join(os.path.dirname(os.path.dirname(HIPCC)), "include")]
+    obj = os.path.join(OBJ, "rows_torch.o")
+    deps = [ROWS_SRC] + [os.path.join(ROOT, "include", h) for h in ("tace_hip.h", "tace_rows.h")]
+    if not force and os.path.exists(obj) and os.path.getmtime(obj) >= max(os.path.getmtime(d) for d in deps):
+        return obj
+    top = os.path.join(os.path.dirname(torch.__file__), "include")
+    inc = [top, os.path.join(top, "torch", "csrc", "api", "include"), sysconfig.get_paths()["include"],
+           os.path.join(os.path.dirname(os.path.dirname(HIPCC)), "include")]
+    tmp = obj + ".tmp.o"
+    subprocess.run([os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-D__HIP_PLATFORM_AMD__",
+                    f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *("-I" + d for d in inc), "-c",
+                    ROWS_SRC, "-o", tmp], check=True, stdout=subprocess.PIPE, stderr=subprocess.STDOUT)
+    os.replace(tmp, obj)
+    return obj
+
+
+def _link_rows(obj: str) -> None:
+    """``_rows.so`` beside the library it calls."""
+    import torch
+
     tmp = ROWS_LIB + ".tmp"
-    subprocess.run([os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-D__HIP_PLATFORM_AMD__",
-                    f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *("-I" + d for d in inc), src,
-                    "-o", tmp, "-L" + LIBDIR, "-ltace_hip", "-L" + os.path.join(top, "lib"), "-lc10", "-lc10_hip",
-                    "-ltorch_cpu", "-ltorch_python", "-Wl,-rpath,$ORIGIN"], check=True, stdout=subprocess.PIPE,
-                   stderr=subprocess.STDOUT)
+    subprocess.check_call([os.environ.get("CXX", "g++"), "-shared", obj, "-o", tmp, "-L" + LIBDIR, "-ltace_hip",
+                           "-L" + os.path.join(os.path.dirname(torch.__file__), "lib"), "-lc10", "-lc10_hip",
+                           "-ltorch_cpu", "-ltorch_python", "-Wl,-rpath,$ORIGIN"])
     os.replace(tmp, ROWS_LIB)
 
 
@@ -98,11 +111,15 @@ def build(verbose: bool = True, force: bool = True, jobs: int = 0) -> str:
     if verbose:
         print(f"[tace_amd.build] {len(srcs)} translation units, {jobs} jobs: {HIPCC} {' '.join(HIP_FLAGS)}", flush=True)
     with cf.ThreadPoolExecutor(jobs) as ex:
-        futs = {ex.submit(_compile, s, force): s for s in srcs}
+        futs = {ex.submit(_compile_rows, force): ROWS_SRC}
+        futs.update({ex.submit(_compile, s, force): s for s in srcs})
         objs = []
         for f in cf.as_completed(futs):
             try:
-                objs.append(f.result())
+                if futs[f] == ROWS_SRC:
+                    rows_obj = f.result()
+                else:
+                    objs.append(f.result())
             except subprocess.CalledProcessError as e:
                 sys.stderr.write(e.stdout.decode(errors="replace"))
                 raise
@@ -110,11 +127,7 @@ def build(verbose: bool = True, force: bool = True, jobs: int = 0) -> str:
     tmp = LIB + ".tmp"
     subprocess.check_call([HIPCC, "--offload-arch=gfx950", "-shared", "-fPIC", *objs, "-o", tmp])
     os.replace(tmp, LIB)
-    try:
-        _build_rows(force)
-    except subprocess.CalledProcessError as e:
-        sys.stderr.write(e.stdout.decode(errors="replace"))
-        raise
+    _link_rows(rows_obj)
     if verbose:
         print(f"[tace_amd.build] {LIB} in {time.time() - t0:.1f}s", flush=True)
     return LIB

@@ -88,7 +88,8 @@ def gpu_graph(structs: List[Dict], atomic_numbers: Sequence[int], cutoff: float,
     g["_species_counts"] = attrs_h.sum(0).to(torch.int64).tolist()
     attrs = up(attrs_h)
     # these rows (as they are now) are one-hot: what reads them may look up instead of multiplying
-    g["_one_hot"] = (attrs, attrs._version)
+    if not attrs.is_inference():   # (those have no version)
+        g["_one_hot"] = (attrs, attrs._version)
     return dict(positions=p64.to(dtype), node_attrs=attrs, lattice=lat, batch=batch, ptr=up(ptr), **g)
 
 

@@ -4,6 +4,8 @@ Bounds count roundings: a sum of m terms in the sums' type is off by at most (m 
 terms' magnitudes (m - 1 additions, a product and a scale), and one more rounding gives the output's type.
 """
 
+import threading
+
 import pytest
 import torch
 
@@ -283,6 +285,116 @@ def test_routing_strided_rows_and_weights(cuda):
     (gw,) = torch.autograd.grad(out, wg, g.to(cuda))
     rows = y[ref.place].view(40, 2, 33).sum(1)
     assert torch.allclose(gw.cpu(), (rows * g).sum(1, keepdim=True), rtol=1e-13, atol=1e-13)
+
+
+def test_gradients_of_one_input_only(cuda):
+    e = _experts(50, 2, 4, 0.2, 5)
+    plan = ops.route_plan(e.to(cuda), 4)
+    x, y = _rand((50, 12), torch.float64, 1).to(cuda), _rand((100, 12), torch.float64, 2).to(cuda)
+    w, g = _rand((50, 2), torch.float64, 3).to(cuda), _rand((50, 12), torch.float64, 4).to(cuda)
+    leaf = lambda t: t.clone().requires_grad_(True)
+    both = [leaf(y), leaf(w)]
+    want = torch.autograd.grad(ops.expert_combine(both[0], plan, both[1]), both, g)
+    a, b = leaf(y), leaf(w)
+    assert torch.equal(torch.autograd.grad(ops.expert_combine(a, plan, w), a, g)[0], want[0])
+    assert torch.equal(torch.autograd.grad(ops.expert_combine(y, plan, b), b, g)[0], want[1])
+    both = [leaf(x), leaf(w)]
+    want = torch.autograd.grad(ops.expert_dispatch(both[0], plan, both[1]), both, y)
+    a, b = leaf(x), leaf(w)
+    assert torch.equal(torch.autograd.grad(ops.expert_dispatch(a, plan, w), a, y)[0], want[0])
+    assert torch.equal(torch.autograd.grad(ops.expert_dispatch(x, plan, b), b, y)[0], want[1])
+    r = leaf(g)
+    out = ops.dropout(x, 0.3, (1, 2), residual=r)
+    assert torch.equal(torch.autograd.grad(out, r, g)[0], g)
+    both = leaf(x)   # the same tensor dropped and added
+    assert torch.equal(torch.autograd.grad(ops.dropout(both, 0.3, (1, 2), residual=both), both, g)[0],
+                       ops.dropout(g, 0.3, (1, 2)) + g)
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16], ids=ids)
+@pytest.mark.parametrize("shift", [1, 2, 4])
+def test_unaligned_rows(cuda, dt, shift):
+    """Contiguous rows that start inside 16 bytes give what aligned ones give."""
+    T, k, D = 40, 2, 24
+    e = _experts(T, k, 4, 0.2, 5)
+    plan = ops.route_plan(e.to(cuda), 4)
+    off = lambda t: torch.cat([t.new_zeros(shift), t.reshape(-1)])[shift:].view(t.shape)
+    x, y, g = (_rand((r, D), dt, i).to(cuda) for i, r in enumerate((T, T * k, T)))
+    w = _rand((T, k), torch.float32, 5).to(cuda)
+
+    def run(move):
+        a, b, c = (move(t).detach().requires_grad_(True) for t in (x, y, w))
+        xs, out = ops.expert_dispatch(a, plan, widths=(8, 16)), ops.expert_combine(b, plan, c, widths=(8, 16))
+        t = torch.arange(T, device=cuda) % 7
+        rows = ops.embedding(a[:7], t)
+        return [xs, out, rows, *torch.autograd.grad(out, (b, c), move(g)), *torch.autograd.grad(xs, a, move(y)),
+                torch.autograd.grad(rows, a, move(g))[0]]
+    for p, q in zip(run(off), run(lambda t: t)):
+        # (the dot products are summed in another order: D terms a slot)
+        assert torch.equal(p, q) or (p - q).abs().max().item() <= 2 * D * 2.0 ** -24 * D * 16
+
+
+def test_rows_past_32_bit_offsets(cuda):
+    """2.3 G elements: 70,000 rows of 32,768 bfloat16."""
+    n, C = 70000, 32768
+    table = torch.randn(3, C, device=cuda).bfloat16()
+    t = torch.arange(n, device=cuda) % 3
+    rows = ops.embedding(table, t)
+    for i in (0, 65535, 65536, n - 1):
+        assert torch.equal(rows[i], table[i % 3])
+    leaf = table.clone().requires_grad_(True)
+    (grad,) = torch.autograd.grad(ops.embedding(leaf, t), leaf, torch.ones((), device=cuda).bfloat16().expand(n, C))
+    counts = torch.bincount(t, minlength=3).bfloat16()
+    assert torch.equal(grad, counts.view(3, 1).expand(3, C))
+    plan = ops.route_plan(t.flip(0), 3)
+    xs = ops.expert_dispatch(rows, plan)
+    tok = plan.order.long()
+    for i in (0, 65535, 65536, n - 1):
+        assert torch.equal(xs[i], rows[tok[i]])
+    del rows
+    back = ops.expert_combine(xs, plan, torch.full((n,), 2.0, device=cuda))
+    for i in (0, 65535, 65536, n - 1):
+        assert torch.equal(back[i], 2 * table[i % 3])
+    del back
+    dropped = ops.dropout(xs, 0.5, (1, 2))
+    at = 2 ** 31 + 12345   # (of the flat order)
+    want = R.draws(16, 1, 2, 0)
+    assert torch.equal((dropped.view(-1)[:16] != 0).cpu(), (want >= 32768) & (xs.view(-1)[:16] != 0).cpu())
+    block = [w for b in (at // 8, at // 8 + 1) for v in R.philox((b, 0, 2, 0), (1, 0)) for w in (v & 0xFFFF, v >> 16)]
+    first = at // 8 * 8
+    assert torch.equal((dropped.view(-1)[first:first + 16] != 0).cpu(),
+                       (torch.tensor(block) >= 32768) & (xs.view(-1)[first:first + 16] != 0).cpu())
+
+
+def test_without_autograd(cuda):
+    x = _rand((6, 8), torch.float32, 1).to(cuda)
+    with torch.inference_mode():
+        plan = ops.route_plan(torch.tensor([0, 1, 0, 1, 2, 2], device=cuda), 3)
+        y = ops.expert_dispatch(ops.dropout(ops.embedding(x, plan.order), 0.5, (1, 2)), plan)
+        z = ops.expert_combine(y, plan)
+    plan = ops.route_plan(torch.tensor([0, 1, 0, 1, 2, 2], device=cuda), 3)
+    leaf = x.clone().requires_grad_(True)
+    with torch.no_grad():
+        a = ops.expert_dispatch(ops.dropout(ops.embedding(leaf, plan.order), 0.5, (1, 2)), plan)
+    assert torch.equal(a, y) and not a.requires_grad
+    assert torch.equal(ops.expert_combine(y.clone(), plan), z)
+
+
+def test_passes_from_two_threads(cuda):
+    states = [_pass_inputs(cuda, 5000, s) for s in (1, 30)]
+    want = [_training_pass(s) for s in states]
+    torch.cuda.synchronize()
+    got = [[], []]
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(10):
+                got[i].append(_training_pass(states[i]))
+            torch.cuda.current_stream().synchronize()
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    [t.start() for t in threads], [t.join() for t in threads]
+    for i in range(2):
+        assert len(got[i]) == 10 and all(torch.equal(p, q) for r in got[i] for p, q in zip(r, want[i]))
 
 
 def test_routing_differentiates_again(cuda):
