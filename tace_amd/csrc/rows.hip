@@ -253,7 +253,7 @@ __global__ __launch_bounds__(WG) void k_embed_grad_part(const T* __restrict__ g,
 // bptr [buckets + 1]; few keys, two launches) and a workgroup has rows of one
 // bucket.  first [buckets + 1]: each bucket's first workgroup.  1.06 M rows of 64
 // float32 of 7,921 tokens: 20 us to group them, 77 here, 14 for the total.
-constexpr int FEW_TOKENS = 128, BUCKET_BITS = 7, LOCAL_STEPS = 8, LOCAL_ROWS = WG * LOCAL_STEPS, MAX_BUCKETS = 255;
+constexpr int FEW_TOKENS = 128, BUCKET_BITS = 7, LOCAL_STEPS = 10, LOCAL_ROWS = WG * LOCAL_STEPS, MAX_BUCKETS = 255;
 template <typename T, int V, bool BUCKETS>
 struct LocalRows {
   const int* list;    // token << 16 | row in the workgroup, sorted
@@ -728,7 +728,7 @@ void few_group(const I* keys, int64_t stride, int n, const FewKeys& fk, int wgs,
 // of 7,921 102 | 119, 300,000 of 3,000 99 | 99, 1 M of 300 100 | 98.
 enum { SCANS = 1, SORTS = 2, BUCKETS = 3, GROUPED = 0 };
 
-// rows a workgroup (256 .. 2,048: about 256 workgroups) and workgroups, one more
+// rows a workgroup (256 .. 2,560: about 256 workgroups) and workgroups, one more
 // a bucket where they are not full
 int local_rows(int64_t n) {
   const int64_t steps = (n + 256 * WG - 1) / (256 * WG);
