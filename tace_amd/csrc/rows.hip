@@ -252,7 +252,7 @@ __global__ __launch_bounds__(WG) void k_embed_grad_part(const T* __restrict__ g,
 // More tokens in buckets of 128: the rows are grouped by bucket first (order,
 // bptr [buckets + 1]; few keys, two launches) and a workgroup has rows of one
 // bucket.  first [buckets + 1]: each bucket's first workgroup.  1.06 M rows of 64
-// float32 of 7,921 tokens: 20 us to group them, 77 here, 14 for the total.
+// float32 of 7,921 tokens: 20 us to group them, 70 here, 11 for the total.
 constexpr int FEW_TOKENS = 128, BUCKET_BITS = 7, LOCAL_STEPS = 10, LOCAL_ROWS = WG * LOCAL_STEPS, MAX_BUCKETS = 255;
 template <typename T, int V, bool BUCKETS>
 struct LocalRows {
@@ -725,7 +725,7 @@ void few_group(const I* keys, int64_t stride, int n, const FewKeys& fk, int wgs,
 // rows of 4 tokens 4.9 | 11.9, 4,096 of 1,000 tokens 7.5 | 21.5; SORTS 5,000 of 89
 // 14 | 19, 101,306 of 2 19 | 29, 1 M of 89 64 | 77, 1 M of 128 tokens (512 MB) 119
 // | 116; BUCKETS 9,000 rows of 1,000 tokens 23 | 41, 50,000 of 8,000 30 | 47, 1.06 M
-// of 7,921 102 | 119, 300,000 of 3,000 99 | 99, 1 M of 300 100 | 98.
+// of 7,921 100 | 119, 300,000 of 3,000 103 | 101, 1 M of 300 102 | 96.
 enum { SCANS = 1, SORTS = 2, BUCKETS = 3, GROUPED = 0 };
 
 // rows a workgroup (256 .. 2,560: about 256 workgroups) and workgroups, one more
