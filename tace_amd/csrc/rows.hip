@@ -70,9 +70,9 @@ __global__ __launch_bounds__(WG) void k_embed_fwd(const T* __restrict__ table, c
 //       ends inside the workgroup, and of one that goes on (slot 0: began before it)
 // Bound by rows read in no order, past the caches, eight in flight a thread while
 // the next eight positions are looked up: 1.06 M rows of 64 float32 of 7,921
-// tokens 61 us, 4.5 TB/s (70 through the caches; 166 with sixteen in flight, which
-// leave a SIMD too few wavefronts).  Joining all groups' runs by one group, not by
-// teams, made 1 M rows of 16 float32 47 us instead of 37: 128 sums in sequence.
+// tokens 61 us, 4.5 TB/s (70 through the caches; four or sixteen in flight are
+// within 3%).  Joining all groups' runs by one group, not by teams, made 1 M rows
+// of 16 float32 47 us instead of 37: 128 sums in sequence.
 constexpr int TEAM = 8;   // groups whose open runs one of them joins
 template <typename T, int V>
 struct RunSums {

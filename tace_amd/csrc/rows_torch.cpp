@@ -337,7 +337,7 @@ std::tuple<Tensor, Tensor, Tensor, int64_t, int64_t> route_plan(const Tensor& ex
   TORCH_CHECK_VALUE(experts.dim() == 1 || (experts.dim() == 2 && experts.size(1) >= 1), "experts has shape ",
                     experts.sizes(), ", expected [T] or [T, k]");
   const int64_t T = experts.size(0), k = experts.dim() == 1 ? 1 : experts.size(1);
-  TORCH_CHECK_VALUE(n_experts >= 0 && n_experts <= MAX_INDEX && T * k <= MAX_INDEX,
+  TORCH_CHECK_VALUE(n_experts >= 0 && n_experts <= MAX_INDEX && k <= MAX_INDEX && T * k <= MAX_INDEX,
                     "route_plan: slots or experts exceed 32-bit indices");
   const Groups g = group(experts.reshape({-1}), n_experts, true, timed);
   return {g.rowptr, g.order, g.place, T, k};
@@ -353,6 +353,7 @@ Tensor route(bool combine, const Tensor& x, const Tensor& place, const Tensor& r
   want_device(x, place, name);
   want_int32(place, tokens * k, x, "plan.place");
   want_int32(rowptr, rowptr.numel(), x, "plan.rowptr");
+  TORCH_CHECK_VALUE(rowptr.numel() >= 1, "plan.rowptr is empty");
   Routed r{place, rowptr, tokens, (int)k, widths ? *widths : std::vector<int64_t>{x.size(1)}, timed};
   int64_t total = 0;
   bool positive = true;
