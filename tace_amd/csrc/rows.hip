@@ -728,10 +728,13 @@ void few_group(const I* keys, int64_t stride, int n, const FewKeys& fk, int wgs,
 // of 7,921 100 | 119, 300,000 of 3,000 103 | 101, 1 M of 300 102 | 96.
 enum { SCANS = 1, SORTS = 2, BUCKETS = 3, GROUPED = 0 };
 
-// rows a workgroup (256 .. 2,560: about 256 workgroups) and workgroups, one more
-// a bucket where they are not full
-int local_rows(int64_t n) {
-  const int64_t steps = (n + 256 * WG - 1) / (256 * WG);
+// Rows a workgroup (256 .. 2,560) and workgroups, one more a bucket where they
+// are not full: about 256 of them, fewer of wide rows, whose columns are dealt to
+// several (us of 256, 128, 64: 100,000 rows of 1,000 float32 of 89 tokens 153, 138,
+// 116; 300,000 of 256 of 3,000 tokens 104, 109, 109; 101,306 of 128 28, 30, 37).
+int local_rows(int64_t n, int32_t channels) {
+  const int64_t target = std::min(std::max(65536 / channels, 64), 256);
+  const int64_t steps = (n + target * WG - 1) / (target * WG);
   return WG * (int)std::min<int64_t>(std::max<int64_t>(steps, 1), LOCAL_STEPS);
 }
 int64_t buckets_of(int64_t vocab) { return (vocab + FEW_TOKENS - 1) / FEW_TOKENS; }
@@ -749,10 +752,11 @@ int embed_form(int64_t n, int64_t vocab) {
 // parts of the workspace of SORTS and BUCKETS, in bytes
 struct LocalWork {
   int64_t wgs, hist, bptr, order, first, seen, part, bytes;
-  LocalWork(int64_t n, int64_t vocab, int64_t row_bytes) {
+  LocalWork(int64_t n, int64_t vocab, int32_t channels, int64_t row_bytes) {
     const bool many = vocab > FEW_TOKENS;
     const int64_t buckets = many ? buckets_of(vocab) : 0, width = many ? FEW_TOKENS : vocab;
-    wgs = (n + local_rows(n) - 1) / local_rows(n) + buckets;
+    const int64_t rows = local_rows(n, channels);
+    wgs = (n + rows - 1) / rows + buckets;
     int few = 0, steps = 0;
     if (many) few_fits(n, buckets, &few, &steps);
     bytes = 0;
@@ -971,7 +975,7 @@ extern "C" int64_t tace_embed_grad_work(int type, int64_t n, int64_t vocab, int3
   const int64_t row = (int64_t)channels * (type == TACE_ROW_F64 ? 8 : 4);
   if (!grouped) {
     const int form = embed_form(n, vocab);
-    return form == SORTS || form == BUCKETS ? LocalWork(n, vocab, row).bytes : 16;
+    return form == SORTS || form == BUCKETS ? LocalWork(n, vocab, channels, row).bytes : 16;
   }
   // (rows may be moved by 16 bytes, 8, or one element: the largest count of workgroups)
   const int bytes = type == TACE_ROW_F64 ? 8 : type == TACE_ROW_F32 ? 4 : 2;
@@ -1020,13 +1024,13 @@ extern "C" int tace_embed_grad(int type, int index_bytes, const void* g, const v
             }
             const int columns = (channels + JOIN_COLS - 1) / JOIN_COLS;
             if (form == SORTS || form == BUCKETS) {
-              const LocalWork lw(n, vocab, channels * (int64_t)sizeof(S));
+              const LocalWork lw(n, vocab, channels, channels * (int64_t)sizeof(S));
               char* at = (char*)work;
               int *bptr = (int*)(at + lw.bptr), *by = (int*)(at + lw.order), *first = (int*)(at + lw.first);
               int* seen = (int*)(at + lw.seen);
               S* sums = (S*)(at + lw.part);
               // (16 threads a row where that leaves the GPU few workgroups)
-              const int ln = lw.wgs < 512 && cw > 16 ? 16 : lanes, rows = local_rows(n);
+              const int ln = lw.wgs < 512 && cw > 16 ? 16 : lanes, rows = local_rows(n, channels);
               const dim3 grid((unsigned)lw.wgs, (unsigned)((cw + ln - 1) / ln));
               if (form == SORTS) {
                 hipLaunchKernelGGL((k_embed_grad_local<T, V, I, false>), grid, dim3(WG), 0, s, (const T*)g,
