@@ -36,7 +36,7 @@ int tace_embed_fwd(int type, int index_bytes, const void* table, const void* tok
  * on the sizes alone.  order [n] and rowptr [vocab + 1] are tace_route_group's
  * of the tokens; NULL where tace_embed_grad_grouped is 0 (few rows or tokens,
  * always for n = 0).  work: tace_embed_grad_work bytes (16-byte aligned) of the
- * same choice, grouped or not. */
+ * same choice, grouped or not; NULL where that is 0. */
 int tace_embed_grad_grouped(int64_t n, int64_t vocab);
 int64_t tace_embed_grad_work(int type, int64_t n, int64_t vocab, int32_t channels, int grouped);
 int tace_embed_grad(int type, int index_bytes, const void* g, const void* tokens, const int32_t* order,

@@ -971,11 +971,11 @@ extern "C" int tace_embed_fwd(int type, int index_bytes, const void* table, cons
 extern "C" int tace_embed_grad_grouped(int64_t n, int64_t vocab) { return embed_form(n, vocab) == GROUPED; }
 
 extern "C" int64_t tace_embed_grad_work(int type, int64_t n, int64_t vocab, int32_t channels, int grouped) {
-  if (n < 1 || vocab < 1 || channels < 1 || channels > MAX_ROW) return 16;
+  if (n < 1 || vocab < 1 || channels < 1 || channels > MAX_ROW) return 0;
   const int64_t row = (int64_t)channels * (type == TACE_ROW_F64 ? 8 : 4);
   if (!grouped) {
     const int form = embed_form(n, vocab);
-    return form == SORTS || form == BUCKETS ? LocalWork(n, vocab, channels, row).bytes : 16;
+    return form == SORTS || form == BUCKETS ? LocalWork(n, vocab, channels, row).bytes : 0;
   }
   // (rows may be moved by 16 bytes, 8, or one element: the largest count of workgroups)
   const int bytes = type == TACE_ROW_F64 ? 8 : type == TACE_ROW_F32 ? 4 : 2;
