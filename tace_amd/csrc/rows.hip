@@ -526,6 +526,12 @@ __global__ __launch_bounds__(WG) void k_embed_grad_scan(const T* __restrict__ g,
   }
 }
 
+// no rows
+template <typename T>
+__global__ __launch_bounds__(WG) void k_embed_grad_none(int64_t total, T* __restrict__ grad) {
+  for (int64_t i = (int64_t)blockIdx.x * WG + threadIdx.x; i < total; i += (int64_t)gridDim.x * WG) grad[i] = (T)0;
+}
+
 int embed_lanes(int cw) { return cw < WG ? cw : WG; }
 
 // Positions a group: 512 workgroups, at least 8.  (us of 256, 512, 1,024
@@ -740,7 +746,7 @@ int local_rows(int64_t n, int32_t channels) {
 int64_t buckets_of(int64_t vocab) { return (vocab + FEW_TOKENS - 1) / FEW_TOKENS; }
 
 int embed_form(int64_t n, int64_t vocab) {
-  if (n <= SCAN_N && vocab <= 1024) return SCANS;
+  if (n < 1 || (n <= SCAN_N && vocab <= 1024)) return SCANS;   // (no rows: zeros)
   if (vocab <= FEW_TOKENS) return SORTS;
   int wgs, steps;
   const int64_t buckets = buckets_of(vocab);
@@ -1006,6 +1012,12 @@ extern "C" int tace_embed_grad(int type, int index_bytes, const void* g, const v
   row_dispatch(type, [&](auto z) {
     typedef decltype(z) T;
     typedef row_sum_t<T> S;
+    if (n == 0) {
+      const int64_t total = vocab * channels, grid = std::min<int64_t>((total + WG - 1) / WG, 4096);
+      hipLaunchKernelGGL((k_embed_grad_none<T>), dim3((unsigned)grid), dim3(WG), 0, (hipStream_t)stream, total,
+                         (T*)grad);
+      return;
+    }
     row_moves<T>(
         [&](int v, int bytes) { return channels % v == 0 && ((uintptr_t)g | (uintptr_t)grad) % bytes == 0; },
         [&](auto vc) {

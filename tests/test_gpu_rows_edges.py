@@ -4,6 +4,7 @@ type and order of a sum holds exactly)."""
 import pytest
 import torch
 
+from tace_amd import _native as N
 from tace_amd import ops
 
 import _rows as R
@@ -11,6 +12,7 @@ import _rows as R
 pytestmark = pytest.mark.gpu
 
 ids = lambda v: str(v).replace("torch.", "")
+CODES = {torch.float32: 0, torch.float64: 1, torch.bfloat16: 2, torch.float16: 3}   # TACE_ROW_*
 
 
 @pytest.mark.parametrize("dt", R.TYPES, ids=ids)
@@ -34,3 +36,19 @@ def test_gradient_of_narrow_tables(cuda, dt, groups, n, V, C):
     assert torch.equal(grad.detach().cpu(), sums.to(dt))
     (again,) = torch.autograd.grad(grad, gl, table.to(cuda))   # the rows of table again
     assert torch.equal(again.cpu(), want)
+
+
+@pytest.mark.parametrize("dt", R.TYPES, ids=ids)
+@pytest.mark.parametrize("V,C", [(1, 1), (9, 5), (1025, 3), (5000, 64), (32641, 7), (300001, 33)])
+def test_gradient_of_no_rows_is_zeros(cuda, dt, V, C):
+    """Through the C entry, without a grouping, and through autograd; nothing behind the gradient is written."""
+    grad = torch.full((V * C + 64,), float("nan"), dtype=dt, device=cuda)
+    for index in (4, 8):
+        grad.fill_(float("nan"))
+        rc = N.lib().tace_embed_grad(CODES[dt], index, None, None, None, None, 0, V, C, 0.5, grad.data_ptr(), None,
+                                     0, torch.cuda.current_stream().cuda_stream)
+        assert rc == 0, N.lib().tace_last_error()
+        assert not bool(grad[:V * C].any()) and bool(grad[V * C:].isnan().all())
+    leaf = torch.ones(V, C, dtype=dt, device=cuda, requires_grad=True)
+    out = ops.embedding(leaf, torch.zeros(0, dtype=torch.int64, device=cuda))
+    assert torch.equal(torch.autograd.grad(out.sum(), leaf)[0], torch.zeros_like(leaf))

@@ -16,3 +16,13 @@ def test_workspace_is_asked_for_wherever_one_is_needed(ty):
                 none = n <= 4096 and V <= 1024
                 if none or not L.tace_embed_grad_grouped(n, V):
                     assert (L.tace_embed_grad_work(ty, n, V, C, 0) == 0) == none
+
+
+def test_no_rows_need_no_grouping():
+    """A gradient of no rows takes neither a grouping nor a workspace, whatever the table's size."""
+    L = N.lib()
+    for V in (0, 1, 9, 128, 129, 1024, 1025, 32640, 32641, 2 ** 31 - 8193):
+        assert L.tace_embed_grad_grouped(0, V) == 0, V
+        assert L.tace_embed_grad_work(0, 0, V, 4, 0) == 0
+    assert L.tace_embed_grad(0, 8, None, None, None, None, 0, 5000, 4, 1.0, None, None, 0, None) < 0
+    assert b"null" in L.tace_last_error()   # (the gradient itself is what is missing)
