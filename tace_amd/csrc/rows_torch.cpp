@@ -202,6 +202,7 @@ Tensor embedding(const Tensor& table, const Tensor& tokens, double scale, const 
   const int64_t n = tokens.numel(), V = table.size(0);
   TORCH_CHECK_VALUE(n <= MAX_INDEX && V <= MAX_INDEX, "embedding: tokens or table rows exceed 32-bit indices");
   Lookup a{V, scale, {}, {}, timed};
+  TORCH_CHECK_VALUE(rowptr.has_value() == order.has_value(), "groups: one of (rowptr, order) is None");
   if (order) {
     want_int32(*rowptr, V + 1, table, "groups[0] (rowptr)");
     want_int32(*order, n, table, "groups[1] (order)");

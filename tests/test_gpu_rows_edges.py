@@ -52,3 +52,11 @@ def test_gradient_of_no_rows_is_zeros(cuda, dt, V, C):
     leaf = torch.ones(V, C, dtype=dt, device=cuda, requires_grad=True)
     out = ops.embedding(leaf, torch.zeros(0, dtype=torch.int64, device=cuda))
     assert torch.equal(torch.autograd.grad(out.sum(), leaf)[0], torch.zeros_like(leaf))
+
+
+def test_half_a_grouping_is_refused(cuda):
+    x, t = torch.zeros(6, 8, device=cuda), torch.zeros(6, dtype=torch.int64, device=cuda)
+    rowptr, order = ops.group_by_key(t, 6)
+    for groups in ((None, order), (rowptr, None)):
+        with pytest.raises(ValueError, match="one of"):
+            ops.embedding(x, t, 1.0, groups)
