@@ -50,7 +50,7 @@ int tace_embed_grad(int type, int index_bytes, const void* g, const void* tokens
  *
  * Tokens sorted by expert: slot s = t k + j is choice j of token t, its key the
  * expert; n = tokens k.  rows_end points to rowptr[experts]: rows from there on
- * belong to dropped slots.  Rows are `blocks` blocks of widths[b] elements (host
+ * belong to dropped slots.  A place outside [0, n) is taken for n - 1.  Rows are `blocks` blocks of widths[b] elements (host
  * array); a batch of R rows holds block after block, each [R, widths[b]]
  * (blocks = 1: ordinary rows). */
 int64_t tace_route_group_work(int64_t n, int64_t n_keys);

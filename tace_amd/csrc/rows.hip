@@ -787,6 +787,12 @@ __device__ __forceinline__ void put(Vec* p, const Vec& v) {
   else *p = v;
 }
 
+// The sorted row of slot s of n: places that are none (of a plan not made by
+// tace_route_group) stay inside the rows.
+__device__ __forceinline__ int place_of(const int* __restrict__ place, int64_t s, int64_t n) {
+  return (int)min((unsigned)place[s], (unsigned)n - 1u);
+}
+
 // A row is read once and stored k times: 12,288 x 2 rows of 2,048 float32 53 us
 // (5.7 TB/s), 101,306 x 2 of 1,152 bfloat16 119 (5.9).
 template <typename T, int V, bool STREAM>
@@ -803,7 +809,7 @@ __global__ __launch_bounds__(WG) void k_route_dispatch(const T* __restrict__ x, 
 #pragma unroll 2
     for (int j = 0; j < k; ++j) {
       const int64_t s = t * k + j;
-      const int p = place[s];
+      const int p = place_of(place, s, n);
       Vec o = v;
       if (p >= end || w) {
         S a[V];
@@ -840,7 +846,7 @@ __global__ __launch_bounds__(WG) void k_route_combine(const T* __restrict__ y, c
 #pragma unroll
       for (int q = 0; q < K; ++q) {
         const int64_t s = t * k + min(j + q, k - 1);
-        p[q] = place[s];
+        p[q] = place_of(place, s, n);
         f[q] = w ? w[s] : (S)1;
       }
 #pragma unroll
@@ -875,7 +881,7 @@ __global__ __launch_bounds__(WG) void k_route_dots(const T* __restrict__ x, cons
   if (s >= n) return;   // (whole groups of lanes; the shuffles stay inside one)
   const unsigned lane = threadIdx.x % lanes;
   const int64_t t = (uint64_t)s / (unsigned)k;
-  const int p = place[s];
+  const int p = place_of(place, s, n);
   const bool kept = p < *rows_end;
   const S f = w ? w[s] : (S)1;
   S dot = 0;

@@ -60,3 +60,38 @@ def test_half_a_grouping_is_refused(cuda):
     for groups in ((None, order), (rowptr, None)):
         with pytest.raises(ValueError, match="one of"):
             ops.embedding(x, t, 1.0, groups)
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16], ids=ids)
+@pytest.mark.parametrize("k", [1, 2, 3])
+@pytest.mark.parametrize("D", [5, 64])
+def test_places_outside_the_rows_stay_inside(cuda, dt, k, D):
+    """A plan whose places are not ``route_plan``'s: what lies outside the rows is taken for the last one."""
+    T = 40
+    n = T * k
+    plan = ops.route_plan(torch.arange(n, device=cuda).view(T, k) % 5, 5)
+    bad = plan.place.clone()
+    # (the last row's own slot among them, so that the rows stay distinct but for it)
+    slots = torch.cat([torch.tensor([0, n // 2, n - 2], device=cuda), (plan.place == n - 1).nonzero().view(-1)]).unique()
+    values = torch.tensor([n, -1, 2 ** 31 - 1, -2 ** 31], device=cuda, dtype=torch.int32)[:len(slots)]
+    bad[slots] = values
+    mine = ops.RoutePlan(plan.rowptr, plan.order, bad, T, k)
+    near = torch.where((bad < 0) | (bad >= n), n - 1, bad).long().cpu()
+    gen = torch.Generator().manual_seed(k)
+    x, y, g = (torch.randint(-4, 5, (r, D), generator=gen).to(dt) for r in (T, n, T))
+    w = torch.randint(1, 4, (T, k), generator=gen).float()
+    xs = ops.expert_dispatch(x.to(cuda), mine).cpu()
+    rows = x.repeat_interleave(k, 0)
+    sure = torch.ones(n, dtype=torch.bool)
+    sure[slots.cpu()] = False
+    assert torch.equal(xs[near[sure]], rows[sure])
+    # every element of the last row is one of those that were sent there
+    assert bool((xs[n - 1] == rows[slots.cpu()]).any(0).all())
+    yc, wc = y.to(cuda).requires_grad_(True), w.to(cuda).requires_grad_(True)
+    out = ops.expert_combine(yc, mine, wc)
+    picked = y.double()[near].view(T, k, D)
+    assert torch.equal(out.detach().cpu(), (picked * w.double().unsqueeze(2)).sum(1).to(dt))   # (small whole numbers)
+    gy, gw = torch.autograd.grad(out, (yc, wc), g.to(cuda))
+    assert torch.equal(gw.cpu(), (picked * g.double().unsqueeze(1)).sum(2).float())
+    sent = (g.double().unsqueeze(1) * w.double().unsqueeze(2)).view(n, D).to(dt)
+    assert torch.equal(gy.cpu()[near[sure]], sent[sure])
