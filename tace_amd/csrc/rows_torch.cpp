@@ -75,6 +75,12 @@ struct Launch {
       token = py::reinterpret_borrow<py::object>(start)(name);
     }
   }
+  ~Launch() {
+    if (token) {   // (left by an error)
+      py::gil_scoped_acquire gil;
+      token = py::object();
+    }
+  }
   void done(int rc, std::initializer_list<int64_t> sizes) {
     if (token) {
       py::gil_scoped_acquire gil;
@@ -110,6 +116,22 @@ const T& held(AutogradContext* ctx) {
   return static_cast<Held<T>*>(ctx->saved_data["args"].toCapsule().get())->v;
 }
 
+// A grouping's or plan's tensor beside the saved variables (which would refuse
+// one made in inference mode, where there are no versions): a backward that
+// finds it written to since raises, as for a saved variable.
+struct Pinned {
+  Tensor t;
+  uint32_t version = 0;
+
+  Pinned() = default;
+  Pinned(const Tensor& x) : t(x), version(x.is_inference() ? 0 : x._version()) {}
+  const Tensor& get(const char* name) const {
+    TORCH_CHECK(t.is_inference() || t._version() == version, "one of the variables needed for gradient computation has "
+                "been modified by an inplace operation: ", name, " is at version ", t._version(), ", expected ", version);
+    return t;
+  }
+};
+
 // positions grouped by key: rowptr [n_keys + 1], order [n] and, where wanted, place [n]
 struct Groups {
   Tensor rowptr, order, place;
@@ -129,7 +151,7 @@ Groups group(const Tensor& keys, int64_t n_keys, bool want_place, bool timed) {
 struct Lookup {
   int64_t vocab;
   double scale;
-  Tensor rowptr, order;   // the tokens' grouping, where the caller gave it
+  Pinned rowptr, order;   // the tokens' grouping, where the caller gave it
   bool timed;
 };
 
@@ -147,9 +169,9 @@ Tensor embed_grad(const Tensor& g, const Tensor& tokens, const Lookup& a) {
   if (n == 0) return at::zeros({a.vocab, C}, g.options());
   const int code = type_code(g.scalar_type());
   Tensor grad = at::empty({a.vocab, C}, g.options()), rowptr, order, work;
-  if (a.order.defined()) {
-    rowptr = a.rowptr;
-    order = a.order;
+  if (a.order.t.defined()) {
+    rowptr = a.rowptr.get("groups[0]");
+    order = a.order.get("groups[1]");
   } else if (tace_embed_grad_grouped(n, a.vocab)) {
     const Groups by = group(tokens, a.vocab, false, a.timed);
     rowptr = by.rowptr;
@@ -219,19 +241,20 @@ Tensor embedding(const Tensor& table, const Tensor& tokens, double scale, const 
 
 // ------------------------------------------------------------------- routing ----
 struct Routed {
-  Tensor place, rowptr;
+  Pinned place, rowptr;
   int64_t tokens;
   int k;
   std::vector<int64_t> widths;
   bool timed;
 
-  const int32_t* end() const { return rowptr.data_ptr<int>() + (rowptr.numel() - 1); }
+  const int32_t* places() const { return place.get("plan.place").data_ptr<int>(); }
+  const int32_t* end() const { return rowptr.get("plan.rowptr").data_ptr<int>() + (rowptr.t.numel() - 1); }
 };
 
 Tensor dispatch_rows(const Tensor& x, const Tensor& w, const Routed& r) {
   Tensor out = at::empty({r.tokens * r.k, x.size(1)}, x.options());
   Launch l(x, "route_dispatch", r.timed);
-  l.done(tace_route_dispatch(type_code(x.scalar_type()), ptr(x), ptr(w), ints(r.place), r.end(), r.tokens, r.k,
+  l.done(tace_route_dispatch(type_code(x.scalar_type()), ptr(x), ptr(w), r.places(), r.end(), r.tokens, r.k,
                              (int)r.widths.size(), r.widths.data(), ptr(out), l.stream), {r.tokens, r.k, x.size(1)});
   return out;
 }
@@ -239,7 +262,7 @@ Tensor dispatch_rows(const Tensor& x, const Tensor& w, const Routed& r) {
 Tensor combine_rows(const Tensor& y, const Tensor& w, const Routed& r) {
   Tensor out = at::empty({r.tokens, y.size(1)}, y.options());
   Launch l(y, "route_combine", r.timed);
-  l.done(tace_route_combine(type_code(y.scalar_type()), ptr(y), ptr(w), ints(r.place), r.end(), r.tokens, r.k,
+  l.done(tace_route_combine(type_code(y.scalar_type()), ptr(y), ptr(w), r.places(), r.end(), r.tokens, r.k,
                             (int)r.widths.size(), r.widths.data(), ptr(out), l.stream), {r.tokens, r.k, y.size(1)});
   return out;
 }
@@ -249,7 +272,7 @@ std::pair<Tensor, Tensor> dots_of(const Tensor& x, const Tensor& y, const Tensor
   Tensor gy = want ? at::empty_like(y) : Tensor();
   Tensor dots = at::empty({r.tokens, r.k}, x.options().dtype(sum_type(x)));
   Launch l(x, "route_dots", r.timed);
-  l.done(tace_route_dots(type_code(x.scalar_type()), ptr(x), ptr(y), ptr(w), ints(r.place), r.end(), r.tokens, r.k,
+  l.done(tace_route_dots(type_code(x.scalar_type()), ptr(x), ptr(y), ptr(w), r.places(), r.end(), r.tokens, r.k,
                          (int)r.widths.size(), r.widths.data(), ptr(gy), ptr(dots), l.stream),
          {r.tokens, r.k, x.size(1)});
   return {gy, dots};

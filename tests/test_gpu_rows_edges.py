@@ -95,3 +95,70 @@ def test_places_outside_the_rows_stay_inside(cuda, dt, k, D):
     assert torch.equal(gw.cpu(), (picked * g.double().unsqueeze(1)).sum(2).float())
     sent = (g.double().unsqueeze(1) * w.double().unsqueeze(2)).view(n, D).to(dt)
     assert torch.equal(gy.cpu()[near[sure]], sent[sure])
+
+
+def test_buffers_written_before_the_backward_are_noticed(cuda):
+    """The grouping's and the plan's tensors, first and second order; what a backward does not read may be written to."""
+    t = torch.arange(50, device=cuda) % 7
+    table = torch.ones(7, 8, device=cuda, requires_grad=True)
+    written = pytest.raises(RuntimeError, match="modified by an inplace operation")
+    for i in (0, 1):
+        groups = ops.group_by_key(t, 7)
+        out = ops.embedding(table, t, 1.0, groups)
+        groups[i].add_(0)
+        with written:
+            torch.autograd.grad(out.sum(), table)
+    groups = ops.group_by_key(t, 7)
+    g = torch.ones(50, 8, device=cuda, requires_grad=True)
+    (grad,) = torch.autograd.grad(ops.embedding(table, t, 1.0, groups), table, g, create_graph=True)
+    groups[1].add_(0)
+    assert torch.equal(torch.autograd.grad(grad, g, torch.ones_like(grad))[0], torch.ones_like(g))   # (a lookup again)
+
+    e = torch.tensor([[0, 1], [1, 2], [2, 0], [0, -1]], device=cuda)
+    x, y = torch.ones(4, 8, device=cuda, requires_grad=True), torch.ones(8, 8, device=cuda, requires_grad=True)
+    w = torch.ones(4, 2, device=cuda, requires_grad=True)
+    for f, leaf in ((lambda p: ops.expert_dispatch(x, p), x), (lambda p: ops.expert_combine(y, p), y),
+                    (lambda p: ops.expert_dispatch(x, p, w), w), (lambda p: ops.expert_combine(y, p, w), w)):
+        for name in ("place", "rowptr"):
+            plan = ops.route_plan(e, 3)
+            out = f(plan)
+            getattr(plan, name).add_(0)
+            with written:
+                torch.autograd.grad(out.sum(), leaf)
+            plan = ops.route_plan(e, 3)
+            (first,) = torch.autograd.grad((f(plan) ** 2).sum(), leaf, create_graph=True)
+            getattr(plan, name).add_(0)
+            with written:
+                torch.autograd.grad(first.sum(), leaf)
+        plan = ops.route_plan(e, 3)
+        out = f(plan)
+        plan.order.add_(0)   # (no pass reads it)
+        torch.autograd.grad(out.sum(), leaf)
+
+
+def test_plans_of_inference_mode_train(cuda):
+    e = torch.tensor([[0, 1], [1, 2], [2, 0], [0, -1]], device=cuda)
+    t = torch.arange(50, device=cuda) % 7
+    with torch.inference_mode():
+        plan, groups = ops.route_plan(e, 3), ops.group_by_key(t, 7)
+    x, table = torch.ones(4, 8, device=cuda, requires_grad=True), torch.ones(7, 8, device=cuda, requires_grad=True)
+    out = ops.expert_combine(ops.expert_dispatch(x, plan), plan)
+    want = torch.tensor([2.0, 2, 2, 1], device=cuda).view(4, 1).expand(4, 8)
+    assert torch.equal(out, want) and torch.equal(torch.autograd.grad(out.sum(), x)[0], want)
+    out = ops.embedding(table, t, 1.0, groups)
+    assert torch.equal(torch.autograd.grad(out.sum(), table)[0], torch.bincount(t).float().view(7, 1).expand(7, 8))
+
+
+def test_written_buffers_are_noticed_while_timed(cuda):
+    """The error leaves autograd's thread while a timed launch is open."""
+    x = torch.ones(4, 8, device=cuda, requires_grad=True)
+    ops.TIMER = ops.KernelTimer()
+    try:
+        plan = ops.route_plan(torch.tensor([0, 1, 2, 0], device=cuda), 3)
+        out = ops.expert_dispatch(x, plan)
+        plan.place.add_(0)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            torch.autograd.grad(out.sum(), x)
+        assert "route_dispatch" in ops.TIMER.summary()
+    finally:
+        ops.TIMER = None
