@@ -332,6 +332,16 @@ def _gm_route(route, x: Tensor, gm, plan: ops.RoutePlan) -> Tensor:
     return torch.cat(out).view(Z, -1)
 
 
+def _species_ranges(plan: ops.RoutePlan):
+    """``plan.ranges`` (waits for the GPU); a species without weights is an
+    error here, not a dropped choice."""
+    rowptr, ranges = plan._read()
+    if rowptr[-1] != plan.n_rows:
+        raise ValueError(f"element_linear: {plan.n_rows - rowptr[-1]} of {plan.n_rows} species are outside "
+                         f"0 .. {plan.n_experts - 1}")
+    return ranges
+
+
 @torch.library.custom_op("tace_amd::element_linear", mutates_args=(), device_types="cuda")
 def element_linear(x: Tensor, weight: Tensor, bias: Optional[Tensor], species: Tensor, irreps_in: str,
                    irreps_out: str, alpha: float) -> Tensor:
@@ -340,7 +350,7 @@ def element_linear(x: Tensor, weight: Tensor, bias: Optional[Tensor], species: T
     with torch.no_grad():
         plan = ops.route_plan(species, weight.shape[0])
         xs = _gm_route(ops.expert_dispatch, x, lay.gin, plan)
-        ys = _LinearFn.apply(xs, weight, bias, lay, plan.ranges, alpha)
+        ys = _LinearFn.apply(xs, weight, bias, lay, _species_ranges(plan), alpha)
         return _gm_route(ops.expert_combine, ys, lay.gout, plan)
 
 
@@ -360,7 +370,7 @@ def element_linear_backward(x: Tensor, weight: Tensor, species: Tensor, grad_out
         gs = _gm_route(ops.expert_dispatch, grad_out.contiguous(), lay.gout, plan)
     with torch.enable_grad():
         xs = xs.detach().requires_grad_(True)
-        ys = _LinearFn.apply(xs, weight.detach(), None, lay, plan.ranges, alpha)
+        ys = _LinearFn.apply(xs, weight.detach(), None, lay, _species_ranges(plan), alpha)
         (gx,) = torch.autograd.grad(ys, xs, gs)
     with torch.no_grad():
         return _gm_route(ops.expert_combine, gx, lay.gin, plan)

@@ -1527,11 +1527,11 @@ class RoutePlan:
     expert, the dropped ones last; ``place`` (int32 [n]) the sorted row of each
     slot; ``rowptr`` (int32 [n_experts + 1]) each expert's range of rows."""
 
-    __slots__ = ("rowptr", "order", "place", "n_tokens", "k", "_ranges")
+    __slots__ = ("rowptr", "order", "place", "n_tokens", "k", "_host")
 
     def __init__(self, rowptr, order, place, n_tokens: int, k: int):
         self.rowptr, self.order, self.place, self.n_tokens, self.k = rowptr, order, place, n_tokens, k
-        self._ranges = None
+        self._host = None   # rowptr's values and the ranges, once read back
 
     @property
     def n_experts(self) -> int:
@@ -1550,14 +1550,18 @@ class RoutePlan:
         the dropped slots' go with the last (they are zeros, and
         ``expert_combine`` neither reads nor gives a gradient to what an expert
         makes of them)."""
-        if self._ranges is None:
+        return self._read()[1]
+
+    def _read(self):
+        """rowptr's values and ``ranges``, on the host."""
+        if self._host is None:
             rp = self.rowptr.tolist()
             r = [(e, a, b) for e, (a, b) in enumerate(zip(rp, rp[1:])) if b > a]
             if rp[-1] < self.n_rows and self.n_experts:
                 e, a, _ = r.pop() if r else (0, 0, 0)
                 r.append((e, a, self.n_rows))
-            self._ranges = r
-        return self._ranges
+            self._host = rp, r
+        return self._host
 
 
 def route_plan(experts: torch.Tensor, n_experts: int) -> RoutePlan:

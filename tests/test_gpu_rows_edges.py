@@ -5,6 +5,8 @@ import pytest
 import torch
 
 from tace_amd import _native as N
+from tace_amd import library
+from tace_amd import model as pm
 from tace_amd import ops
 
 import _rows as R
@@ -162,3 +164,21 @@ def test_written_buffers_are_noticed_while_timed(cuda):
         assert "route_dispatch" in ops.TIMER.summary()
     finally:
         ops.TIMER = None
+
+
+@pytest.mark.parametrize("index", [torch.int32, torch.int64], ids=ids)
+def test_species_without_weights_are_refused(cuda, index):
+    """The per-species linear of exported programs, forward and backward; all species known, or no atoms, pass."""
+    lin = pm.e3nnElementLinear("4x0e+4x1o", "4x0e+4x1o", 3).to(cuda)
+    args = "4x0e+4x1o", "4x0e+4x1o", 1.0
+    x = torch.ones(5, 16, device=cuda)
+    for bad in ([0, 1, 2, 3, 0], [0, 1, -1, 2, 0], [9, 9, 9, 9, 9], [0, 0, 0, 0, 2 ** 31 - 1]):
+        species = torch.tensor(bad, device=cuda, dtype=index)
+        with pytest.raises(ValueError, match="species are outside 0 .. 2"):
+            library.element_linear(x, lin.weight, lin.bias, species, *args)
+        with pytest.raises(ValueError, match="species are outside 0 .. 2"):
+            library.element_linear_backward(x, lin.weight, species, x, *args)
+    species = torch.tensor([2, 0, 2, 0, 0], device=cuda, dtype=index)   # (one species without atoms)
+    assert library.element_linear(x, lin.weight, lin.bias, species, *args).shape == (5, 16)
+    assert library.element_linear(x[:0], lin.weight, lin.bias, species[:0], *args).shape == (0, 16)
+    assert library.element_linear_backward(x[:0], lin.weight, species[:0], x[:0], *args).shape == (0, 16)
