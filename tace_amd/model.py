@@ -545,6 +545,11 @@ class e3nnElementLinear(torch.nn.Module):
                      if bias and self.lay.bias_numel else None)
 
     def forward(self, x: torch.Tensor, sp: SpeciesPlan, alpha: float = 1.0) -> torch.Tensor:
+        if isinstance(sp, ops.RoutePlan):   # (rows of ``ops.expert_dispatch``)
+            if x.shape[0] != sp.n_rows:
+                raise ValueError(f"x has {x.shape[0]} rows, its plan {sp.n_rows} rows")
+            if sp.n_rows and not sp.n_experts:
+                raise ValueError("a plan of no experts has no weights for its rows")
         if ops.MODE.export:
             from . import library
             return library.element_linear(x.contiguous(), self.weight, self.bias, sp.species, str(self.irreps_in),

@@ -1556,6 +1556,8 @@ class RoutePlan:
         """rowptr's values and ``ranges``, on the host."""
         if self._host is None:
             rp = self.rowptr.tolist()
+            if rp[0] != 0 or rp[-1] > self.n_rows or any(b < a for a, b in zip(rp, rp[1:])):
+                raise ValueError(f"plan.rowptr does not divide {self.n_rows} rows among experts")
             r = [(e, a, b) for e, (a, b) in enumerate(zip(rp, rp[1:])) if b > a]
             if rp[-1] < self.n_rows and self.n_experts:
                 e, a, _ = r.pop() if r else (0, 0, 0)

@@ -1,8 +1,11 @@
 """The row operators at the ends of their arguments (CPU)."""
 
 import pytest
+import torch
 
 from tace_amd import _native as N
+from tace_amd import model as pm
+from tace_amd import ops
 
 
 @pytest.mark.parametrize("ty", range(4))
@@ -26,3 +29,31 @@ def test_no_rows_need_no_grouping():
         assert L.tace_embed_grad_work(0, 0, V, 4, 0) == 0
     assert L.tace_embed_grad(0, 8, None, None, None, None, 0, 5000, 4, 1.0, None, None, 0, None) < 0
     assert b"null" in L.tace_last_error()   # (the gradient itself is what is missing)
+
+
+def _plan(rowptr, tokens, k=1):
+    return ops.RoutePlan(torch.tensor(rowptr, dtype=torch.int32), None, None, tokens, k)
+
+
+def test_ranges_of_a_plan_that_is_none_are_refused():
+    """Ranges reach the linears as row numbers."""
+    assert _plan([0, 2, 2, 5], 5).ranges == [(0, 0, 2), (2, 2, 5)]
+    assert _plan([0, 2, 2, 3], 3, 2).ranges == [(0, 0, 2), (2, 2, 6)]
+    for rowptr in ([0, 5, 3, 6], [0, 2, 9], [1, 2, 6], [-1, 3, 6], [0, -4, 6]):
+        with pytest.raises(ValueError, match="rowptr"):
+            _plan(rowptr, 6).ranges
+
+
+@pytest.mark.parametrize("double", [False, True])
+def test_experts_take_the_rows_of_their_plan(double):
+    """Rows that the plan does not have, or too few of them, are refused; so is a plan without experts."""
+    lin = pm.e3nnElementLinear("4x0e+4x1o", "4x0e+4x1o", 3)
+    with ops.differentiable_twice(double), torch.no_grad():
+        if double:   # (the kernels' path takes GPU tensors)
+            assert lin(torch.ones(6, 16), _plan([0, 2, 2, 5], 3, 2)).shape == (6, 16)
+            assert lin(torch.ones(0, 16), _plan([0, 0, 0, 0], 0)).shape == (0, 16)
+        for rows in (3, 5, 7, 12):
+            with pytest.raises(ValueError, match="6 rows"):
+                lin(torch.ones(rows, 16), _plan([0, 2, 2, 5], 3, 2))
+        with pytest.raises(ValueError, match="no experts"):
+            lin(torch.ones(6, 16), _plan([0], 6))
