@@ -51,10 +51,13 @@ void want_device(const Tensor& t, const Tensor& like, const char* name) {
 }
 
 void want_int32(const Tensor& t, int64_t n, const Tensor& like, const char* name) {
-  TORCH_CHECK_VALUE(t.scalar_type() == at::kInt && t.is_contiguous() && t.dim() == 1 && t.size(0) == n, name,
+  TORCH_CHECK_VALUE(t.scalar_type() == at::kInt && t.is_contiguous() && !t.is_neg() && t.dim() == 1 && t.size(0) == n, name,
                     " must be a contiguous int32 tensor of ", n);
   want_device(t, like, name);
 }
+
+// what a kernel reads: rows one after the other, their signs in memory
+Tensor dense(const Tensor& t) { return t.resolve_neg().contiguous(); }
 
 void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 int* ints(const Tensor& t) { return t.defined() ? t.data_ptr<int>() : nullptr; }
@@ -202,14 +205,14 @@ struct EmbeddingGrad : torch::autograd::Function<EmbeddingGrad> {
     return embed_grad(g, tokens, a);
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    const Tensor g = grads[0].contiguous(), tokens = ctx->get_saved_variables()[0];
+    const Tensor g = dense(grads[0]), tokens = ctx->get_saved_variables()[0];
     const Lookup& a = held<Lookup>(ctx);
     return {tracked(g) ? Embedding::apply(g, tokens, a) : embed_rows(g, tokens, a), Tensor(), Tensor()};
   }
 };
 
 variable_list Embedding::backward(AutogradContext* ctx, variable_list grads) {
-  const Tensor g = grads[0].contiguous(), tokens = ctx->get_saved_variables()[0];
+  const Tensor g = dense(grads[0]), tokens = ctx->get_saved_variables()[0];
   const Lookup& a = held<Lookup>(ctx);
   return {tracked(g) ? EmbeddingGrad::apply(g, tokens, a) : embed_grad(g, tokens, a), Tensor(), Tensor()};
 }
@@ -231,7 +234,7 @@ Tensor embedding(const Tensor& table, const Tensor& tokens, double scale, const 
     a.rowptr = *rowptr;
     a.order = *order;
   }
-  const Tensor tab = table.contiguous(), flat = tokens.reshape({-1}).contiguous();
+  const Tensor tab = dense(table), flat = dense(tokens.reshape({-1}));
   const Tensor out = tracked(tab) ? Embedding::apply(tab, flat, a) : embed_rows(tab, flat, a);
   if (tokens.dim() == 1) return out;
   auto shape = tokens.sizes().vec();
@@ -296,7 +299,7 @@ struct Dispatch : torch::autograd::Function<Dispatch> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const auto saved = ctx->get_saved_variables();
     const Routed& r = held<Routed>(ctx);
-    const Tensor g = grads[0].contiguous(), &x = saved[0], &w = saved[1];
+    const Tensor g = dense(grads[0]), &x = saved[0], &w = saved[1];
     variable_list out(3);
     if (ctx->needs_input_grad(0)) out[0] = combine_op(g, w, r);
     if (w.defined() && ctx->needs_input_grad(1)) out[1] = dots_op(x, g, r);
@@ -313,7 +316,7 @@ struct Combine : torch::autograd::Function<Combine> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const auto saved = ctx->get_saved_variables();
     const Routed& r = held<Routed>(ctx);
-    const Tensor g = grads[0].contiguous(), &y = saved[0], &w = saved[1];
+    const Tensor g = dense(grads[0]), &y = saved[0], &w = saved[1];
     const bool need_y = ctx->needs_input_grad(0), need_w = w.defined() && ctx->needs_input_grad(1);
     variable_list out(3);
     if (need_w && !tracked(g) && !tracked(y) && !tracked(w)) {   // both in one pass
@@ -335,7 +338,7 @@ struct RowDots : torch::autograd::Function<RowDots> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const auto saved = ctx->get_saved_variables();
     const Routed& r = held<Routed>(ctx);
-    const Tensor g = grads[0].contiguous(), &x = saved[0], &y = saved[1];
+    const Tensor g = dense(grads[0]), &x = saved[0], &y = saved[1];
     variable_list out(3);
     if (ctx->needs_input_grad(0)) out[0] = combine_op(y, g, r);
     if (ctx->needs_input_grad(1)) out[1] = dispatch_op(x, g, r);
@@ -363,7 +366,7 @@ std::tuple<Tensor, Tensor, Tensor, int64_t, int64_t> route_plan(const Tensor& ex
   const int64_t T = experts.size(0), k = experts.dim() == 1 ? 1 : experts.size(1);
   TORCH_CHECK_VALUE(n_experts >= 0 && n_experts <= MAX_INDEX && k <= MAX_INDEX && T * k <= MAX_INDEX,
                     "route_plan: slots or experts exceed 32-bit indices");
-  const Groups g = group(experts.reshape({-1}), n_experts, true, timed);
+  const Groups g = group(experts.resolve_neg().reshape({-1}), n_experts, true, timed);
   return {g.rowptr, g.order, g.place, T, k};
 }
 
@@ -394,9 +397,9 @@ Tensor route(bool combine, const Tensor& x, const Tensor& place, const Tensor& r
                                                 (w.dim() == 1 && k == 1 && w.size(0) == tokens)),
                       "weights must be floating point [", tokens, ", ", k, "], got ", w.scalar_type(), " ", w.sizes());
     want_device(w, x, "weights");
-    w = w.reshape({tokens, k}).to(sum_type(x)).contiguous();
+    w = dense(w.reshape({tokens, k}).to(sum_type(x)));
   }
-  return combine ? combine_op(x.contiguous(), w, r) : dispatch_op(x.contiguous(), w, r);
+  return combine ? combine_op(dense(x), w, r) : dispatch_op(dense(x), w, r);
 }
 
 // ------------------------------------------------------------------- dropout ----
@@ -431,7 +434,7 @@ struct Dropout : torch::autograd::Function<Dropout> {
     if (m.residual && ctx->needs_input_grad(1)) out[1] = grads[0];
     m.residual = false;
     if (ctx->needs_input_grad(0)) {
-      const Tensor g = grads[0].contiguous();
+      const Tensor g = dense(grads[0]);
       out[0] = tracked(g) ? Dropout::apply(g, std::nullopt, maybe(state), m) : masked(g, Tensor(), state, m);
     }
     return out;
@@ -462,7 +465,7 @@ Tensor dropout(const Tensor& x, double p, const optional<Tensor>& state, int64_t
   TORCH_CHECK_VALUE(x.numel() / m.total * (int64_t)m.comps.size() <= (int64_t)1 << 34, "dropout: over 2^34 draws");
   if (state) {
     TORCH_CHECK_VALUE(state->scalar_type() == at::kLong && state->dim() == 1 && state->size(0) == 2 &&
-                      state->is_contiguous(), "rng must be a contiguous int64 tensor [2] or two integers");
+                      state->is_contiguous() && !state->is_neg(), "rng must be a contiguous int64 tensor [2] or two integers");
     want_device(*state, x, "rng");
   }
   Tensor res;
@@ -470,9 +473,9 @@ Tensor dropout(const Tensor& x, double p, const optional<Tensor>& state, int64_t
     TORCH_CHECK_VALUE(residual->sizes() == x.sizes() && residual->scalar_type() == x.scalar_type(), "residual is ",
                       residual->scalar_type(), " ", residual->sizes(), ", expected ", x.scalar_type(), " ", x.sizes());
     want_device(*residual, x, "residual");
-    res = residual->contiguous();
+    res = dense(*residual);
   }
-  const Tensor in = x.contiguous();
+  const Tensor in = dense(x);
   if (tracked(in) || tracked(res)) return Dropout::apply(in, maybe(res), state, m);
   return masked(in, res, state.value_or(Tensor()), m);
 }

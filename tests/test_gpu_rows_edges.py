@@ -182,3 +182,36 @@ def test_species_without_weights_are_refused(cuda, index):
     assert library.element_linear(x, lin.weight, lin.bias, species, *args).shape == (5, 16)
     assert library.element_linear(x[:0], lin.weight, lin.bias, species[:0], *args).shape == (0, 16)
     assert library.element_linear_backward(x[:0], lin.weight, species[:0], x[:0], *args).shape == (0, 16)
+
+
+def test_signs_of_negated_views(cuda):
+    """Parts of conjugates are views whose sign is not in memory: one by one, as inputs and as gradients."""
+    gen = torch.Generator().manual_seed(1)
+    z = lambda *shape: torch.view_as_complex(torch.randint(-4, 5, (*shape, 2), generator=gen).float()).to(cuda)
+    minus = lambda t: torch._neg_view(-t)   # t, by a view of -t
+    e = torch.tensor([[0], [1], [0], [2]], device=cuda)
+    plan, t = ops.route_plan(e, 3), torch.tensor([0, 3, 1, 1], device=cuda)
+    x, w = z(4, 8).real.contiguous(), z(4, 1).imag.contiguous()
+    fs = (lambda x, w: ops.embedding(x, t), lambda x, w: ops.expert_dispatch(x, plan, w), lambda x, w: ops.dropout(x, 0.5, (1, 2)),
+          lambda x, w: ops.expert_combine(x, plan, w), lambda x, w: ops.dropout(w.expand(4, 8).contiguous(), 0.5, (1, 2), residual=x))
+    for f in fs:
+        want = f(x, w)
+        for v in (minus(x), torch.complex(x, -x).conj().imag):
+            assert v.is_neg() and torch.equal(v, x)
+            assert torch.equal(f(v, w), want)
+        assert torch.equal(f(x, minus(w)), want)
+        leaf = x.clone().requires_grad_(True)
+        out = f(leaf, w)
+        g = torch.randint(-4, 5, out.shape, generator=gen).float().to(cuda)
+        (want,) = torch.autograd.grad(out, leaf, g, retain_graph=True)
+        assert torch.equal(torch.autograd.grad(out, leaf, minus(g))[0], want)
+    assert torch.equal(ops.embedding(x, minus(t)), x[t])
+    other = ops.route_plan(minus(e), 3)
+    assert torch.equal(other.order, plan.order) and torch.equal(other.rowptr, plan.rowptr)
+    one = z(1, 1)
+    assert ops.dropout(one.conj().imag, 0.0, (1, 2)).item() == -one.imag.item()
+    with pytest.raises(ValueError, match="rng"):
+        ops.dropout(x, 0.5, minus(torch.tensor([1, 2], device=cuda)))
+    rowptr, order = ops.group_by_key(t, 4)
+    with pytest.raises(ValueError, match="groups"):
+        ops.embedding(x, t, 1.0, (rowptr, minus(order)))
