@@ -35,19 +35,27 @@ int type_code(at::ScalarType t) {
 
 at::ScalarType sum_type(const Tensor& t) { return t.scalar_type() == at::kDouble ? at::kDouble : at::kFloat; }
 
+// (a transform's wrapper, without storage, is refused by autograd or where its address is asked for)
+void want_memory(const Tensor& t, const char* name) {
+  TORCH_CHECK_VALUE(!t.has_storage() || t.numel() == 0 || t.const_data_ptr(), name, " holds no memory (a fake tensor)");
+}
+
 void want_rows(const Tensor& t, const char* name) {
   TORCH_CHECK_VALUE(t.is_cuda(), name, " must be a GPU tensor (got ", t.device(), ")");
   TORCH_CHECK_VALUE(type_code(t.scalar_type()) >= 0, name, " has dtype ", t.scalar_type(),
                     ", expected float32, float64, bfloat16 or float16");
+  want_memory(t, name);
 }
 
 void want_indices(const Tensor& t, const char* name) {
   TORCH_CHECK_VALUE(t.scalar_type() == at::kInt || t.scalar_type() == at::kLong, name, " has dtype ", t.scalar_type(),
                     ", expected int32 or int64");
+  want_memory(t, name);
 }
 
 void want_device(const Tensor& t, const Tensor& like, const char* name) {
   TORCH_CHECK_VALUE(t.device() == like.device(), name, " is on ", t.device(), ", expected ", like.device());
+  want_memory(t, name);
 }
 
 void want_int32(const Tensor& t, int64_t n, const Tensor& like, const char* name) {

@@ -3,6 +3,8 @@ type and order of a sum holds exactly)."""
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fwd
+from torch._subclasses.fake_tensor import FakeTensorMode
 
 from tace_amd import _native as N
 from tace_amd import library
@@ -215,3 +217,44 @@ def test_signs_of_negated_views(cuda):
     rowptr, order = ops.group_by_key(t, 4)
     with pytest.raises(ValueError, match="groups"):
         ops.embedding(x, t, 1.0, (rowptr, minus(order)))
+
+
+def _operators(cuda):
+    """name -> (function of its float tensors, the tensors)"""
+    t = torch.tensor([0, 3, 1, 1], device=cuda)
+    plan = ops.route_plan(t, 4)
+    x, w = torch.ones(4, 8, device=cuda), torch.full((4, 1), 0.5, device=cuda)
+    return dict(
+        embedding=(lambda x: ops.embedding(x, t), [x]),
+        dispatch=(lambda x, w: ops.expert_dispatch(x, plan, w), [x, w]),
+        combine=(lambda x, w: ops.expert_combine(x, plan, w), [x, w]),
+        dropout=(lambda x, r: ops.dropout(x, 0.5, (1, 2), residual=r), [x, x]))
+
+
+@pytest.mark.parametrize("name", ["embedding", "dispatch", "combine", "dropout"])
+def test_forward_mode_and_transforms_are_refused(cuda, name):
+    """There is no forward-mode derivative and no batching rule: an error for every input, never a wrong value."""
+    f, inputs = _operators(cuda)[name]
+    for i in range(len(inputs)):
+        one = lambda v: f(*inputs[:i], v, *inputs[i + 1:])
+        with fwd.dual_level(), pytest.raises(RuntimeError, match="jvp is not implemented"):
+            one(fwd.make_dual(inputs[i], torch.ones_like(inputs[i])))
+        with pytest.raises(RuntimeError, match="functorch"):
+            torch.func.grad(lambda v: one(v).sum())(inputs[i])
+        with pytest.raises((RuntimeError, ValueError)):
+            torch.vmap(one)(torch.stack([inputs[i]] * 2))
+
+
+@pytest.mark.parametrize("name", ["embedding", "dispatch", "combine", "dropout"])
+def test_fake_tensors_are_refused(cuda, name):
+    f, inputs = _operators(cuda)[name]
+    mode = FakeTensorMode(allow_non_fake_inputs=True)
+    for i in range(len(inputs)):
+        with pytest.raises(ValueError, match="holds no memory"):
+            f(*inputs[:i], mode.from_tensor(inputs[i]), *inputs[i + 1:])
+    t = mode.from_tensor(torch.zeros(4, dtype=torch.int64, device=cuda))
+    state = mode.from_tensor(torch.zeros(2, dtype=torch.int64, device=cuda))
+    for call in (lambda: ops.embedding(inputs[0], t), lambda: ops.route_plan(t, 3),
+                 lambda: ops.dropout(inputs[0], 0.5, state)):
+        with pytest.raises(ValueError, match="holds no memory"):
+            call()
