@@ -1464,6 +1464,11 @@ class Dropout:
         self.features, self.attention, self.seed, self.step = float(features), float(attention), int(seed), 0
 
     def step_masks(self) -> "_Masks":
+        # (seed and counter go with the launches as numbers: every replay would draw this forward's masks)
+        if torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("a training forward with dropout cannot be recorded into a graph: its replays would all "
+                               "have the same masks; set_dropout(model) switches it off, ops.dropout takes its counter "
+                               "as a tensor")
         self.step += 1
         return _Masks(self, (self.seed, self.step))
 
@@ -1498,7 +1503,10 @@ def set_dropout(model: torch.nn.Module, features: float = 0.0, attention: float 
     stress of one forward are derivatives of the same masked energy.  The masks
     are functions of (seed, forward, layer, index), ``ops.dropout``; give every
     rank of a data-parallel run a seed of its own.  Zeros switch it off;
-    evaluation never drops.  Returns the number of interactions it applies to."""
+    evaluation never drops, and a forward that would be recorded into a graph
+    raises.  Every forward draws anew: one that is run a second time for its
+    backward (activation checkpointing around the model) needs ``dropout.step``
+    set back first.  Returns the number of interactions it applies to."""
     for name, p in (("features", features), ("attention", attention)):
         if not (p == 0.0 or 2.0 ** -17 < p < 1.0 - 2.0 ** -17):
             raise ValueError(f"dropout of {name}: {p} is not 0 or a probability inside (0, 1) of the mask's 2^-16")

@@ -258,3 +258,18 @@ def test_fake_tensors_are_refused(cuda, name):
                  lambda: ops.dropout(inputs[0], 0.5, state)):
         with pytest.raises(ValueError, match="holds no memory"):
             call()
+
+
+def test_recording_notices_dropout_of_a_model(cuda):
+    drop = pm.Dropout(0.2, 0.0, seed=1)
+    drop.step_masks()
+    x = torch.ones(4, device=cuda)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = x + 1
+        with pytest.raises(RuntimeError, match="recorded into a graph"):
+            drop.step_masks()
+    x.fill_(2)
+    graph.replay()
+    assert y.tolist() == [3.0] * 4 and drop.step == 1

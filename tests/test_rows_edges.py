@@ -57,3 +57,15 @@ def test_experts_take_the_rows_of_their_plan(double):
                 lin(torch.ones(rows, 16), _plan([0, 2, 2, 5], 3, 2))
         with pytest.raises(ValueError, match="no experts"):
             lin(torch.ones(6, 16), _plan([0], 6))
+
+
+def test_masks_of_a_recorded_forward_are_refused(monkeypatch):
+    drop = pm.Dropout(0.2, 0.0, seed=1)
+    assert drop.step_masks().rng == (1, 1)
+    monkeypatch.setattr(torch.cuda, "is_initialized", lambda: True)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with pytest.raises(RuntimeError, match="recorded into a graph"):
+        drop.step_masks()
+    assert drop.step == 1   # (no forward was drawn for)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    assert drop.step_masks().rng == (1, 2)
