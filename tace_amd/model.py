@@ -1458,10 +1458,16 @@ def set_tece_channel_mixing(model: torch.nn.Module, dtype: Optional[torch.dtype]
 class Dropout:
     """Dropout of the training mode (``set_dropout``): probabilities, seed, and
     the number of forwards drawn for, which is the mask's counter.  ``step`` may
-    be set to repeat or resume a run's masks."""
+    be set to repeat or resume a run's masks.  ``member``: which of the networks
+    of one ``set_dropout`` this is (each draws at sites of its own)."""
 
-    def __init__(self, features: float, attention: float, seed: int):
+    def __init__(self, features: float, attention: float, seed: int, member: int = 0):
         self.features, self.attention, self.seed, self.step = float(features), float(attention), int(seed), 0
+        self.member = member
+
+    def site(self, layer: int, kind: int) -> int:
+        """Where layer's features (kind 0) or attention weights (1) draw."""
+        return (self.member << 16) + 2 * layer + kind
 
     def step_masks(self) -> "_Masks":
         # (seed and counter go with the launches as numbers: every replay would draw this forward's masks)
@@ -1485,13 +1491,14 @@ class _Masks:
         if self.drop.features == 0.0:
             return x
         assert len({m for m, _ in irreps}) == 1, irreps
-        return ops.dropout(x, self.drop.features, self.rng, site=2 * layer, components=[ir.dim for _, ir in irreps])
+        return ops.dropout(x, self.drop.features, self.rng, site=self.drop.site(layer, 0),
+                           components=[ir.dim for _, ir in irreps])
 
     def attention(self, alpha: torch.Tensor, layer: int) -> torch.Tensor:
         """Attention weights [E, H] of a TECE layer."""
         if self.drop.attention == 0.0:
             return alpha
-        return ops.dropout(alpha, self.drop.attention, self.rng, site=2 * layer + 1)
+        return ops.dropout(alpha, self.drop.attention, self.rng, site=self.drop.site(layer, 1))
 
 
 def set_dropout(model: torch.nn.Module, features: float = 0.0, attention: float = 0.0, seed: int = 0) -> int:
@@ -1502,7 +1509,8 @@ def set_dropout(model: torch.nn.Module, features: float = 0.0, attention: float 
     an (edge, head) attention weight of the TECE layers.  Energies, forces and
     stress of one forward are derivatives of the same masked energy.  The masks
     are functions of (seed, forward, layer, index), ``ops.dropout``; give every
-    rank of a data-parallel run a seed of its own.  Zeros switch it off;
+    rank of a data-parallel run a seed of its own.  Of several TACE inside
+    ``model`` (an ensemble) each draws its own masks.  Zeros switch it off;
     evaluation never drops, and a forward that would be recorded into a graph
     raises.  Every forward draws anew: one that is run a second time for its
     backward (activation checkpointing around the model) needs ``dropout.step``
@@ -1514,9 +1522,9 @@ def set_dropout(model: torch.nn.Module, features: float = 0.0, attention: float 
     if not top:
         raise ValueError("set_dropout needs a TensorModel or TACE")
     n = 0
-    for m in top:
-        m.dropout = Dropout(features, attention, seed) if features or attention else None
-        n += sum(bool(features or (attention and isinstance(i, TeceInteraction))) for i in m.representation.interactions)
+    for i, m in enumerate(top):
+        m.dropout = Dropout(features, attention, seed, i) if features or attention else None
+        n += sum(bool(features or (attention and isinstance(j, TeceInteraction))) for j in m.representation.interactions)
     return n
 
 

@@ -10,6 +10,7 @@ from tace_amd import _native as N
 from tace_amd import library
 from tace_amd import model as pm
 from tace_amd import ops
+from tace_amd.so3 import Irreps
 
 import _rows as R
 
@@ -273,3 +274,12 @@ def test_recording_notices_dropout_of_a_model(cuda):
     x.fill_(2)
     graph.replay()
     assert y.tolist() == [3.0] * 4 and drop.step == 1
+
+
+def test_masks_differ_between_members(cuda):
+    x, irreps = torch.ones(500, 32, device=cuda), Irreps("8x0e+8x1o")
+    masks = [pm.Dropout(0.5, 0.5, 3, member).step_masks() for member in (0, 1)]
+    for draw in (lambda m: m.features(x, irreps, 1), lambda m: m.attention(x, 1)):
+        a, b = (draw(m) != 0 for m in masks)
+        # 8,000 draws at least, by block: a share of 0.5 agrees by chance, its standard deviation below 0.007
+        assert 0.45 < (a == b).float().mean().item() < 0.55

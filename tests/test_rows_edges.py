@@ -4,6 +4,7 @@ import pytest
 import torch
 
 from tace_amd import _native as N
+from tace_amd import configs
 from tace_amd import model as pm
 from tace_amd import ops
 
@@ -69,3 +70,15 @@ def test_masks_of_a_recorded_forward_are_refused(monkeypatch):
     assert drop.step == 1   # (no forward was drawn for)
     monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
     assert drop.step_masks().rng == (1, 2)
+
+
+def test_members_of_an_ensemble_draw_their_own_masks():
+    make = lambda: pm.create_model(configs.model_cfg("tece", [26], 58.0, num_channel=16, num_head=2, edge_ace_hidden=8))
+    both = torch.nn.ModuleList([make(), make()])
+    assert pm.set_dropout(both, features=0.1, attention=0.1, seed=5) == 4
+    drops = [m.readout_fn.dropout for m in both]
+    sites = [d.site(layer, kind) for d in drops for layer in range(64) for kind in (0, 1)]
+    assert len(set(sites)) == len(sites) and all(0 <= s < 2 ** 32 for s in sites)
+    # a single network draws where it always did
+    pm.set_dropout(both[1], features=0.1)
+    assert [both[1].readout_fn.dropout.site(layer, kind) for layer in (0, 3) for kind in (0, 1)] == [0, 1, 6, 7]
