@@ -179,24 +179,30 @@ def lib() -> ctypes.CDLL:
 _rows_mod = None
 
 
+def _load_rows(path: str):
+    import importlib.machinery
+    import importlib.util
+
+    import torch  # noqa: F401  (its libraries first)
+
+    loader = importlib.machinery.ExtensionFileLoader("_rows", path)
+    mod = importlib.util.module_from_spec(importlib.util.spec_from_loader("_rows", loader))
+    loader.exec_module(mod)
+    return mod
+
+
 def rows():
     """The row operators on torch tensors (``_lib/_rows.so``), loaded once."""
     global _rows_mod
     if _rows_mod is None:
-        lib()   # (checks the versions)
-        import importlib.machinery
-        import importlib.util
-
-        import torch  # noqa: F401  (its libraries first)
-
+        lib()   # (checks the library's versions)
         path = os.path.join(_HERE, "_lib", "_rows.so")
         if not os.path.exists(path):
             raise NativeError(f"_rows.so not found at {path}; build it with `python -m tace_amd.build`")
-        loader = importlib.machinery.ExtensionFileLoader("_rows", path)
-        mod = importlib.util.module_from_spec(importlib.util.spec_from_loader("_rows", loader))
-        loader.exec_module(mod)
-        if mod.abi_version() != ROWS_ABI_VERSION:
-            raise NativeError(f"{path} has row operators of version {mod.abi_version()}, these bindings are for "
+        mod = _load_rows(path)
+        built = getattr(mod, "BUILT_FOR", None)
+        if built != ROWS_ABI_VERSION:
+            raise NativeError(f"{path} was built for row operators of version {built}, these bindings are for "
                               f"{ROWS_ABI_VERSION}; build it again with `python -m tace_amd.build`")
         with _lock:
             if _rows_mod is None:

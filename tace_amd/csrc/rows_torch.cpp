@@ -491,7 +491,7 @@ Tensor dropout(const Tensor& x, double p, const optional<Tensor>& state, int64_t
 }  // namespace
 
 PYBIND11_MODULE(_rows, mod) {
-  mod.def("abi_version", &tace_rows_abi_version);
+  mod.attr("BUILT_FOR") = TACE_ROWS_ABI_VERSION;   // (the library's own may differ)
   mod.def("timer", [](py::object start, py::object stop) {
     Launch::start = start.release().ptr();
     Launch::stop = stop.release().ptr();

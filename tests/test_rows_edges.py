@@ -82,3 +82,14 @@ def test_members_of_an_ensemble_draw_their_own_masks():
     # a single network draws where it always did
     pm.set_dropout(both[1], features=0.1)
     assert [both[1].readout_fn.dropout.site(layer, kind) for layer in (0, 3) for kind in (0, 1)] == [0, 1, 6, 7]
+
+
+def test_a_binding_of_another_version_is_refused(monkeypatch):
+    """The torch binding has the version of the header it was compiled with, beside the library's own."""
+    mod = N.rows()
+    assert mod.BUILT_FOR == N.ROWS_ABI_VERSION == N.lib().tace_rows_abi_version()
+    monkeypatch.setattr(N, "_rows_mod", None)
+    monkeypatch.setattr(mod, "BUILT_FOR", N.ROWS_ABI_VERSION - 1)
+    monkeypatch.setattr(N, "_load_rows", lambda path: mod)
+    with pytest.raises(N.NativeError, match="built for row operators of version"):
+        N.rows()
