@@ -283,3 +283,34 @@ def test_masks_differ_between_members(cuda):
         a, b = (draw(m) != 0 for m in masks)
         # 8,000 draws at least, by block: a share of 0.5 agrees by chance, its standard deviation below 0.007
         assert 0.45 < (a == b).float().mean().item() < 0.55
+
+
+@pytest.mark.parametrize("dt", R.TYPES, ids=ids)
+@pytest.mark.parametrize("shift", [1, 2, 4])
+def test_unaligned_rows_hold_the_same_bits(cuda, dt, shift):
+    """What is not a sum over a row's elements does not depend on where the rows start.  (float16: a product of an element
+    and a float32 may be rounded once, or to float32 first, as the compiler has it for each width of a move.  Both lie
+    within half a step, eps / 2, of float32 values that differ by at most four half steps, 2^-24 each, of terms of
+    together less than 32: within a step of each other and 4 * 32 * 2^-24 = 2^-17.)"""
+    T, k, D = 40, 2, 24
+    gen = torch.Generator().manual_seed(shift)
+    e = torch.randint(-1, 4, (T, k), generator=gen).to(cuda)
+    plan, t = ops.route_plan(e, 4), (torch.arange(T, device=cuda) * 3) % 8 - 1
+    off = lambda v: torch.cat([v.new_zeros(shift), v.reshape(-1)])[shift:].view(v.shape)
+    x, y, g = (torch.randn(r, D, generator=gen, dtype=torch.float64).to(dt).to(cuda) for r in (T, T * k, T))
+    w = torch.rand(T, k, generator=gen, dtype=torch.float64).to(cuda).requires_grad_(True)
+
+    def run(move):
+        a, b = (move(v).detach().requires_grad_(True) for v in (x, y))
+        kw = dict(widths=(8, 16))
+        xs, xw, out = ops.expert_dispatch(a, plan, **kw), ops.expert_dispatch(a, plan, w, **kw), ops.expert_combine(b, plan, w, **kw)
+        rows, kept = ops.embedding(a, t, 0.7), ops.dropout(a, 0.4, (1, 2), components=(1, 2), residual=move(g))
+        return [xs, xw, out, rows, kept, torch.autograd.grad(out, b, move(g), retain_graph=True)[0],
+                torch.autograd.grad(out, (b, w), move(g))[0], torch.autograd.grad(xs, a, move(y))[0],
+                torch.autograd.grad(xw, a, move(y))[0], torch.autograd.grad(kept, a, move(g))[0]]
+    for i, (p, q) in enumerate(zip(run(off), run(lambda v: v))):
+        if dt == torch.float16:
+            p, q = p.double(), q.double()
+            assert bool(((p - q).abs() <= torch.finfo(dt).eps * torch.maximum(p.abs(), q.abs()) + 2.0 ** -17).all()), i
+        else:
+            assert torch.equal(p, q), i
