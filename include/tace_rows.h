@@ -7,7 +7,12 @@
  * Row types: TACE_ROW_F32, _F64, _BF16, _F16.  Sums, weights and scales are
  * double for TACE_ROW_F64 and float otherwise ("the type's sums").  Indices
  * (`index_bytes` 4 or 8) outside their range are no error: their rows are
- * zero and take no gradient. */
+ * zero and take no gradient.  Calls that need 2^32 threads or more (one for
+ * each move of up to 16 bytes) are refused.
+ *
+ * The same inputs at the same alignment give the same bits on every run.  The
+ * order of a sum depends on the tokens or places as well as on the sizes, and
+ * on the width of a move, which the channels and the rows' alignment set. */
 #ifndef TACE_ROWS_H
 #define TACE_ROWS_H
 
@@ -32,11 +37,11 @@ int tace_embed_fwd(int type, int index_bytes, const void* table, const void* tok
                    int32_t channels, double scale, void* out, void* stream);
 
 /* grad [vocab, channels]: row v is scale * the sum of g's rows (g [n,
- * channels]) whose token is v, zeros without any; the order of the sum depends
- * on the sizes alone.  order [n] and rowptr [vocab + 1] are tace_route_group's
- * of the tokens; NULL where tace_embed_grad_grouped is 0 (few rows or tokens,
- * always for n = 0).  work: tace_embed_grad_work bytes (16-byte aligned) of the
- * same choice, grouped or not; NULL where that is 0. */
+ * channels]) whose token is v, zeros without any.  order [n] and rowptr
+ * [vocab + 1] are tace_route_group's of the tokens; NULL where
+ * tace_embed_grad_grouped is 0 (few rows or tokens, always for n = 0).  work:
+ * tace_embed_grad_work bytes (16-byte aligned) of the same choice, grouped or
+ * not; NULL where that is 0. */
 int tace_embed_grad_grouped(int64_t n, int64_t vocab);
 int64_t tace_embed_grad_work(int type, int64_t n, int64_t vocab, int32_t channels, int grouped);
 int tace_embed_grad(int type, int index_bytes, const void* g, const void* tokens, const int32_t* order,
@@ -50,9 +55,9 @@ int tace_embed_grad(int type, int index_bytes, const void* g, const void* tokens
  *
  * Tokens sorted by expert: slot s = t k + j is choice j of token t, its key the
  * expert; n = tokens k.  rows_end points to rowptr[experts]: rows from there on
- * belong to dropped slots.  A place outside [0, n) is taken for n - 1.  Rows are `blocks` blocks of widths[b] elements (host
- * array); a batch of R rows holds block after block, each [R, widths[b]]
- * (blocks = 1: ordinary rows). */
+ * belong to dropped slots.  A place outside [0, n) is taken for n - 1.  Rows
+ * are `blocks` blocks of widths[b] elements (host array); a batch of R rows
+ * holds block after block, each [R, widths[b]] (blocks = 1: ordinary rows). */
 int64_t tace_route_group_work(int64_t n, int64_t n_keys);
 int tace_route_group(int index_bytes, const void* keys, int64_t stride, int64_t n, int64_t n_keys, int32_t* rowptr,
                      int32_t* order, int32_t* place, int32_t* work, void* stream);

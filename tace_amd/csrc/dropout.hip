@@ -53,8 +53,8 @@ struct Parts {
 // HBM: the ten rounds are 20 wide multiplications and 34 exclusive ors for 8
 // elements, and twice that, for draws of 32 bits, took the same time (81 us for
 // 117 M bfloat16): 16 bits are enough for a probability.  us (TB/s): 25 M
-// float32 in degrees 0 .. 3 37 (5.4), with a residual 56 (5.4); 117 M bfloat16 in
-// degrees 0 .. 2 80 (5.9).  With lanes that kept their own 8 elements (two moves
+// float32 in degrees 0 .. 3 38 (5.3), with a residual 57 (5.3); 117 M bfloat16 in
+// degrees 0 .. 2 81 (5.7).  With lanes that kept their own 8 elements (two moves
 // of every other 16 bytes, one component after the other) 51, 74 and 89; with
 // stores that stay in the caches 40, 59 and 83.
 template <typename T, int V>
@@ -119,7 +119,10 @@ __global__ __launch_bounds__(WG) void k_dropout_vec(const T* __restrict__ x, con
   }
 }
 
-// any channels and alignment, 8 draws a thread
+// any channels and alignment, 8 draws a thread.  Bound by its loads and stores of
+// single elements: a thread's 8 draws are neighbours, so a wavefront's addresses
+// lie 8 elements apart.  12,288 rows of 99 channels of float32 in degrees 0 .. 3
+// 222 us, of 100 (the kernel above) 33.
 template <typename T>
 __global__ __launch_bounds__(WG) void k_dropout_any(const T* __restrict__ x, const T* __restrict__ res, Draws dr,
                                                     int64_t total, int64_t rows, int channels, Parts pt,

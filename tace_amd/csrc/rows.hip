@@ -31,7 +31,7 @@ struct RowChunks {
 
 // out[i] = scale table[tokens[i]], zeros outside the table.  The table stays in
 // L2; bound by the stores, which go past the caches: 1.06 M rows of 64 float32
-// (272 MB) 43 us, 6.3 TB/s (57 with four chunks a thread and stores that stay
+// (272 MB) 44 us, 6.3 TB/s (57 with four chunks a thread and stores that stay
 // in the caches, 47 with two and stores past them).
 template <typename T, int V, typename I>
 __global__ __launch_bounds__(WG) void k_embed_fwd(const T* __restrict__ table, const I* __restrict__ tokens,
@@ -246,13 +246,13 @@ __global__ __launch_bounds__(WG) void k_embed_grad_part(const T* __restrict__ g,
 // LDS, so no grouping of all of them is needed; each token's sum goes to part
 // [workgroup][token][channels] and its presence to seen [workgroup][token], for
 // k_embed_grad_total.  Two launches instead of four; bound by the chain of loads
-// of a workgroup: 101,306 rows of 128 bfloat16 of two tokens 13.4 us and 3.8 for
+// of a workgroup: 101,306 rows of 128 bfloat16 of two tokens 13.9 us and 3.9 for
 // the total.
 //
 // More tokens in buckets of 128: the rows are grouped by bucket first (order,
 // bptr [buckets + 1]; few keys, two launches) and a workgroup has rows of one
 // bucket.  first [buckets + 1]: each bucket's first workgroup.  1.06 M rows of 64
-// float32 of 7,921 tokens: 20 us to group them, 70 here, 11 for the total.
+// float32 of 7,921 tokens: 19 us to group them, 71 here, 11 for the total.
 constexpr int FEW_TOKENS = 128, BUCKET_BITS = 7, LOCAL_STEPS = 10, LOCAL_ROWS = WG * LOCAL_STEPS, MAX_BUCKETS = 255;
 template <typename T, int V, bool BUCKETS>
 struct LocalRows {
@@ -471,7 +471,7 @@ __global__ __launch_bounds__(WG) void k_embed_grad_total(const int* __restrict__
 
 // Few rows: a workgroup per token (and tile of columns) lists the token's rows
 // in LDS and sums them; no grouping, one launch.  Bound by latency: 1,024 rows of
-// 128 float32 of 4 tokens 4.7 us.
+// 128 float32 of 4 tokens 5.5 us.
 constexpr int SCAN_N = 4096;
 template <typename T, int V, typename I>
 __global__ __launch_bounds__(WG) void k_embed_grad_scan(const T* __restrict__ g, const I* __restrict__ tokens, int n,
@@ -579,7 +579,9 @@ __global__ __launch_bounds__(WG) void k_route_place(const int* __restrict__ orde
 // ballots and writes their places.  One workgroup (n <= 8,192) counts for
 // itself.  Bound by latency; us, with places | general grouping (tace_group_keys:
 // any keys, four launches or more), without: 8,192 slots of 8 experts 9 | 11,
-// 24,576 of 8 8 | 17, 200,000 of 255 15 | 24, 1 M of 89 22 | 31.
+// 24,576 of 8 8 | 17, 200,000 of 255 15 | 24, 1 M of 89 22 | 30.  (256 and more, by
+// the general grouping and a launch for the places: 8,192 of 256 19, 200,000 of
+// 1,000 37, 1 M of 1,000 57.)
 constexpr int FEW_WG = 1024, FEW_STEPS = 8, FEW_KEYS = 256, FEW_WGS = 128;
 
 // keys are the values below `limit`, shifted
@@ -727,11 +729,15 @@ void few_group(const I* keys, int64_t stride, int n, const FewKeys& fk, int wgs,
 // ------------------------------------------- the embedding gradient's form ----
 // Which form it takes without a grouping of the tokens: looking through all of
 // them, sorting them workgroup by workgroup, that in buckets of 128 tokens, or
-// none (it needs a grouping).  us, this form | grouping and sums: SCANS 1,024
-// rows of 4 tokens 4.9 | 11.9, 4,096 of 1,000 tokens 7.5 | 21.5; SORTS 5,000 of 89
-// 14 | 19, 101,306 of 2 19 | 29, 1 M of 89 64 | 77, 1 M of 128 tokens (512 MB) 119
-// | 116; BUCKETS 9,000 rows of 1,000 tokens 23 | 41, 50,000 of 8,000 30 | 47, 1.06 M
-// of 7,921 100 | 119, 300,000 of 3,000 103 | 101, 1 M of 300 102 | 96.
+// none (it needs a grouping).  us, this form | grouping and sums, float32: SCANS
+// 1,024 rows of 128 of 4 tokens 4.7 | 12, 4,096 of 128 of 1,000 tokens 7.5 | 22;
+// SORTS 5,000 of 128 of 89 14 | 17, 12,801 of 256 of 89 19 | 20, 101,306 of 128 of 2
+// 19 | 30, 1 M of 64 of 89 62 | 77; BUCKETS 9,000 of 64 of 1,000 tokens 23 | 41,
+// 50,000 of 64 of 8,000 30 | 47, 1.06 M of 64 of 7,921 95 | 119.  The rule knows
+// neither channels nor how full the buckets are, and loses where rows are many
+// and wide or buckets few: 1 M of 128 of 128 tokens 124 | 116, 300,000 of 256 of
+// 3,000 99 | 98, 1 M of 64 of 300 98 | 98, 300,000 of 64 of 300 55 | 51, 1 M of 128
+// of 300 155 | 133.
 enum { SCANS = 1, SORTS = 2, BUCKETS = 3, GROUPED = 0 };
 
 // Rows a workgroup (256 .. 2,560) and workgroups, one more a bucket where they
@@ -788,13 +794,15 @@ __device__ __forceinline__ void put(Vec* p, const Vec& v) {
 }
 
 // The sorted row of slot s of n: places that are none (of a plan not made by
-// tace_route_group) stay inside the rows.
+// tace_route_group) stay inside the rows.  (101,306 x 2 rows of 1,152 bfloat16, both
+// directions with gradients, 568 us without and 578 with the bound; 12,288 x 2 of
+// 2,048 float32 249 either way.)
 __device__ __forceinline__ int place_of(const int* __restrict__ place, int64_t s, int64_t n) {
   return (int)min((unsigned)place[s], (unsigned)n - 1u);
 }
 
-// A row is read once and stored k times: 12,288 x 2 rows of 2,048 float32 53 us
-// (5.7 TB/s), 101,306 x 2 of 1,152 bfloat16 119 (5.9).
+// A row is read once and stored k times: 12,288 x 2 rows of 2,048 float32 56 us
+// (5.4 TB/s), 101,306 x 2 of 1,152 bfloat16 120 (5.9).
 template <typename T, int V, bool STREAM>
 __global__ __launch_bounds__(WG) void k_route_dispatch(const T* __restrict__ x, const row_sum_t<T>* __restrict__ w,
                                                        const int* __restrict__ place, const int* __restrict__ rows_end,
@@ -825,7 +833,7 @@ __global__ __launch_bounds__(WG) void k_route_dispatch(const T* __restrict__ x, 
 
 // K slots' rows are loaded before the first is added (the dropped ones too:
 // they have a row, which is not added): 12,288 x 2 rows of 2,048 float32 53 us (5.7
-// TB/s; 60 one after the other), 101,306 x 2 of 1,152 bfloat16 112 (6.2; 131).
+// TB/s; 60 one after the other), 101,306 x 2 of 1,152 bfloat16 112 (6.1; 131).
 template <typename T, int V, int K>
 __global__ __launch_bounds__(WG) void k_route_combine(const T* __restrict__ y, const row_sum_t<T>* __restrict__ w,
                                                       const int* __restrict__ place, const int* __restrict__ rows_end,
@@ -868,7 +876,7 @@ __global__ __launch_bounds__(WG) void k_route_combine(const T* __restrict__ y, c
 // by side: its row of x comes from memory once.  U chunks of both rows are
 // loaded before the first is multiplied.  12,288 x 2 rows of 2,048 float32 79 us
 // (6.4 TB/s; 103 with lanes that take a token's slots one after the other), 1,024
-// x 2 of them 9.3 (15), 101,306 x 2 of 1,152 bfloat16 214 (5.5).
+// x 2 of them 10.5 (15), 101,306 x 2 of 1,152 bfloat16 227 (5.2).
 template <typename T, int V, int U>
 __global__ __launch_bounds__(WG) void k_route_dots(const T* __restrict__ x, const T* __restrict__ y,
                                                    const row_sum_t<T>* __restrict__ w, const int* __restrict__ place,
@@ -1122,9 +1130,9 @@ extern "C" int tace_route_group(int index_bytes, const void* keys, int64_t strid
 namespace {
 
 // Rows that go to scattered places are stored past the caches where they are
-// whole 128-byte lines (12,288 x 2 rows of 2,048 float32 50 us instead of 58),
-// not where two rows meet in a line (20,000 x 4 rows of 400 float16 27 instead
-// of 16).
+// whole 128-byte lines (12,288 x 2 rows of 2,048 float32 take 1.16 times as long
+// through them), not where two rows meet in a line (20,000 x 4 rows of 400 float16
+// take 1.7 times as long past them).
 bool whole_lines(int32_t blocks, const int64_t* widths, int size) {
   for (int b = 0; b < blocks; ++b)
     if (widths[b] * size % 128) return false;

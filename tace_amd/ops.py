@@ -1503,7 +1503,8 @@ def sender_csr(rows_src: torch.Tensor, n_rows: int) -> Tuple[torch.Tensor, torch
 # Lookups, routed rows and dropout (csrc/rows_torch.cpp): float64, float32,
 # bfloat16 and float16 rows, sums in float64 for float64 rows and in float32
 # for the others.  Every backward is made of the same operators, so each can be
-# differentiated any number of times.
+# differentiated any number of times.  Forward-mode derivatives and functional
+# transforms (torch.func) are refused.
 ROW_MAX = 32768   # elements a row
 ROW_BLOCKS = 8    # blocks a row
 
@@ -1513,10 +1514,11 @@ def embedding(table: torch.Tensor, tokens: torch.Tensor, scale: float = 1.0,
     """``scale * table[tokens]``: rows of ``table`` [V, C] for integer
     ``tokens`` of any shape, C up to ``ROW_MAX``.  A token outside [0, V) (padding) gives a row of
     zeros and takes no gradient.  The table's gradient sums each token's rows in
-    an order that depends on the sizes alone (the same bits on every run) and
-    rounds once.  ``groups``: ``group_by_key(tokens.reshape(-1), V)`` where the
+    a fixed order (the same bits on every run with the same inputs at the same
+    alignment; other tokens, padding and alignment move the order) and rounds
+    once.  ``groups``: ``group_by_key(tokens.reshape(-1), V)`` where the
     caller has it already (several lookups of the same tokens); made when needed
-    otherwise.  Differentiable any number of times."""
+    otherwise.  Differentiable any number of times (in reverse mode)."""
     rowptr, order = (None, None) if groups is None else groups
     return N.rows().embedding(table, tokens, scale, rowptr, order, TIMER is not None)
 
@@ -1525,7 +1527,8 @@ class RoutePlan:
     """Rows sorted by expert (``route_plan``): slot s = t k + j is choice j of
     token t.  ``order`` (int32 [n]) the slots by expert, in slot order within an
     expert, the dropped ones last; ``place`` (int32 [n]) the sorted row of each
-    slot; ``rowptr`` (int32 [n_experts + 1]) each expert's range of rows."""
+    slot; ``rowptr`` (int32 [n_experts + 1]) each expert's range of rows.  A
+    backward raises if place or rowptr was written to since its forward."""
 
     __slots__ = ("rowptr", "order", "place", "n_tokens", "k", "_host")
 
@@ -1548,7 +1551,7 @@ class RoutePlan:
         per-species linears take them (``e3nnElementLinear(..)(xs, plan)``; read
         back from the GPU once).  They cover all rows, as those linears need:
         the dropped slots' go with the last (they are zeros, and
-        ``expert_combine`` neither reads nor gives a gradient to what an expert
+        ``expert_combine`` neither uses nor gives a gradient to what an expert
         makes of them)."""
         return self._read()[1]
 
