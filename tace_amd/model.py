@@ -1183,7 +1183,8 @@ class LinearNodeEmbedding(torch.nn.Module):
         lin = self.elem_emb1
         if species is not None and type(lin) is e3nnLinear and "forward" not in vars(lin) and not _hooked(lin):
             S, C = lin.lay.dim_in, lin.lay.dim_out
-            if C <= ops.ROW_MAX and lin.weight.dtype in (torch.float32, torch.float64):
+            # (other columns than the weight's are the linear's to refuse)
+            if attrs.shape[1] == S and C <= ops.ROW_MAX and lin.weight.dtype in (torch.float32, torch.float64):
                 return ops.embedding(lin.weight.view(S, C), species, lin.lay.ins[0][5])
         return lin(attrs)
 

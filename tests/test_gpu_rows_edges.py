@@ -7,6 +7,7 @@ import torch.autograd.forward_ad as fwd
 from torch._subclasses.fake_tensor import FakeTensorMode
 
 from tace_amd import _native as N
+from tace_amd import configs, data, structures
 from tace_amd import library
 from tace_amd import model as pm
 from tace_amd import ops
@@ -314,3 +315,18 @@ def test_unaligned_rows_hold_the_same_bits(cuda, dt, shift):
             assert bool(((p - q).abs() <= torch.finfo(dt).eps * torch.maximum(p.abs(), q.abs()) + 2.0 ** -17).all()), i
         else:
             assert torch.equal(p, q), i
+
+
+@pytest.mark.parametrize("model_zs,batch_zs", [([24, 26, 27, 28], [26]), ([26], [24, 26, 27, 28]), ([24, 26, 27, 28], [26, 27])])
+def test_batches_of_other_elements_are_refused(cuda, model_zs, batch_zs):
+    """A batch made for another list of elements than the model's has other columns: an error in training (where the
+    species are looked up) as in evaluation."""
+    s = structures.bcc_fe(reps=(2, 2, 2), seed=4)
+    cfg = configs.model_cfg("tece", model_zs, 58.0, num_channel=16, num_head=2, edge_ace_hidden=8)
+    m = pm.create_model(cfg).to(cuda)
+    m.reset_target_property(["energy", "forces"])
+    d = data.gpu_graph([s], batch_zs, 5.0, torch.float32, cuda)
+    for mode in (True, False):
+        with pytest.raises((RuntimeError, ValueError, IndexError)):
+            m.train(mode)(d)
+    m.train()(data.gpu_graph([s], model_zs, 5.0, torch.float32, cuda))
