@@ -65,7 +65,8 @@ void want_int32(const Tensor& t, int64_t n, const Tensor& like, const char* name
 }
 
 // what a kernel reads: rows one after the other, their signs in memory
-Tensor dense(const Tensor& t) { return t.resolve_neg().contiguous(); }
+Tensor signed_values(const Tensor& t) { return t.is_neg() ? t.resolve_neg() : t; }
+Tensor dense(const Tensor& t) { return signed_values(t).contiguous(); }
 
 void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 int* ints(const Tensor& t) { return t.defined() ? t.data_ptr<int>() : nullptr; }
@@ -374,7 +375,7 @@ std::tuple<Tensor, Tensor, Tensor, int64_t, int64_t> route_plan(const Tensor& ex
   const int64_t T = experts.size(0), k = experts.dim() == 1 ? 1 : experts.size(1);
   TORCH_CHECK_VALUE(n_experts >= 0 && n_experts <= MAX_INDEX && k <= MAX_INDEX && T * k <= MAX_INDEX,
                     "route_plan: slots or experts exceed 32-bit indices");
-  const Groups g = group(experts.resolve_neg().reshape({-1}), n_experts, true, timed);
+  const Groups g = group(signed_values(experts).reshape({-1}), n_experts, true, timed);
   return {g.rowptr, g.order, g.place, T, k};
 }
 
