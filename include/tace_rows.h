@@ -1,6 +1,7 @@
 /* C ABI of libtace_hip.so, second part: operators on rows of atoms -- table
  * lookup by token and its gradient, rows sorted by expert and back, dropout
- * from a counter-based generator.  Conventions are tace_hip.h's (device
+ * from a counter-based generator, root-mean-square norm, the experts' products
+ * -- and the step that trains them (AdamW over many tensors).  Conventions are tace_hip.h's (device
  * pointers of the caller, asynchronous on `stream`, 0 or a negative code and
  * tace_last_error()); this part has a version of its own.
  *
@@ -22,7 +23,7 @@
 extern "C" {
 #endif
 
-#define TACE_ROWS_ABI_VERSION 3
+#define TACE_ROWS_ABI_VERSION 4
 #define TACE_ROW_F32 0
 #define TACE_ROW_F64 1
 #define TACE_ROW_BF16 2
@@ -83,6 +84,59 @@ int tace_route_dots(int type, const void* x, const void* y, const void* weights,
 int tace_dropout(int type, const void* x, const void* residual, const int64_t* state, int64_t seed, int64_t offset,
                  uint32_t site, int32_t threshold, int64_t rows, int32_t channels, int32_t blocks,
                  const int32_t* comps, void* out, void* stream);
+
+/* Root-mean-square norm.  x: `blocks` blocks [rows, comps[b], channels], one
+ * after the other (plain rows: one block of one component, channels = the
+ * row).  For each (row, block), n = comps[b] channels elements:
+ * h = x + residual (rounded; without a residual h is x and must be NULL),
+ * q = 1 / sqrt(sum h^2 / n + eps), y = h q weight[b][channel].  weight [blocks,
+ * channels] has the rows' type, or its sums' where weight_wide.  inv [rows,
+ * blocks] (the type's sums, may be NULL) receives q.  scales (float [rows,
+ * blocks], NULL: y has the rows' type): y receives e4m3 codes, y = code *
+ * scale, scale = max |y| / 448; a row with a NaN has scale NaN, one below 2^-100
+ * is zeros under scale 0.
+ *
+ * Backward: dh = the gradient of h (and so of x and of residual) given gy and gh
+ * (NULL: none); dw [blocks, channels] (NULL: not wanted) has weight's type.
+ * work: tace_rms_norm_bwd_work bytes, 16-byte aligned (may be NULL without dw). */
+int tace_rms_norm_fwd(int type, const void* x, const void* residual, const void* weight, int weight_wide, int64_t rows,
+                      int32_t channels, int32_t blocks, const int32_t* comps, double eps, void* h, void* y,
+                      float* scales, void* inv, void* stream);
+int64_t tace_rms_norm_bwd_work(int type, int64_t rows, int32_t channels, int32_t blocks, const int32_t* comps);
+int tace_rms_norm_bwd(int type, const void* gy, const void* gh, const void* h, const void* weight, int weight_wide,
+                      const void* inv, int64_t rows, int32_t channels, int32_t blocks, const int32_t* comps, void* dh,
+                      void* dw, void* work, int64_t work_bytes, void* stream);
+
+/* AdamW.  tensors: host array; p, g [n] of the row type, m, s [n] the states:
+ * averages of g and g^2 in the type's sums, or (`eight`) of g and the root of the
+ * average of g^2 as e4m3 codes with scales float [ceil(n / 256), 2]; master
+ * (weights of 16 bits; may be NULL) [n] float, which p is rounded from.
+ * counter: device int64 [2], the steps done and zero; the step counts itself.
+ * lr_at (may be NULL): device learning rate, float or (lr_wide) double, used
+ * instead of lr.  norm (may be NULL): tace_grad_norm's of all gradients, which are
+ * multiplied by min(1, max_norm / norm); where it is infinite or NaN nothing
+ * changes.  Draws of the codes: a function of (seed; position / 4, index in
+ * `tensors`, step).
+ *
+ * tace_grad_norm: norm (double for TACE_ROW_F64, else float) = the 2-norm of all
+ * g.  ticket: a device int64 that is zero before and after (counter + 1 will
+ * do).  work: tace_grad_norm_work bytes, 8-byte aligned. */
+#define TACE_ADAM_BLOCK 256
+typedef struct {
+  void* p;
+  const void* g;
+  void* m;
+  void* s;
+  void* master;
+  void* scales;
+  int64_t n;
+} tace_adam_tensor;
+int64_t tace_grad_norm_work(const tace_adam_tensor* tensors, int64_t count);
+int tace_grad_norm(int type, const tace_adam_tensor* tensors, int64_t count, int64_t* ticket, void* norm, void* work,
+                   int64_t work_bytes, void* stream);
+int tace_adamw(int type, int eight, const tace_adam_tensor* tensors, int64_t count, int64_t* counter, double lr,
+               const void* lr_at, int lr_wide, double beta1, double beta2, double eps, double decay, const void* norm,
+               double max_norm, uint64_t seed, void* stream);
 
 #ifdef __cplusplus
 }

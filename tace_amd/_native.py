@@ -126,7 +126,7 @@ _SIGS = {
 EXPORTED = tuple(_SIGS)
 
 # the row operators (include/tace_rows.h), with a version of their own
-ROWS_ABI_VERSION = 3
+ROWS_ABI_VERSION = 4
 _ROW_SIGS = {
     "tace_rows_abi_version": (_c_int, []),
     "tace_embed_fwd": (_c_int, [_c_int, _c_int, _vp, _vp, _c_i64, _c_i64, _c_i32, _c_dbl, _vp, _vp]),
@@ -141,6 +141,15 @@ _ROW_SIGS = {
     "tace_route_dots": (_c_int, [_c_int, _vp, _vp, _vp, _vp, _vp, _c_i64, _c_i32, _c_i32, _vp, _vp, _vp, _vp]),
     "tace_dropout": (_c_int, [_c_int, _vp, _vp, _vp, _c_i64, _c_i64, ctypes.c_uint32, _c_i32, _c_i64, _c_i32, _c_i32,
                               _vp, _vp, _vp]),
+    "tace_rms_norm_fwd": (_c_int, [_c_int, _vp, _vp, _vp, _c_int, _c_i64, _c_i32, _c_i32, _vp, _c_dbl, _vp, _vp, _vp,
+                                   _vp, _vp]),
+    "tace_rms_norm_bwd_work": (_c_i64, [_c_int, _c_i64, _c_i32, _c_i32, _vp]),
+    "tace_rms_norm_bwd": (_c_int, [_c_int, _vp, _vp, _vp, _vp, _c_int, _vp, _c_i64, _c_i32, _c_i32, _vp, _vp, _vp, _vp,
+                                   _c_i64, _vp]),
+    "tace_grad_norm_work": (_c_i64, [_vp, _c_i64]),
+    "tace_grad_norm": (_c_int, [_c_int, _vp, _c_i64, _vp, _vp, _vp, _c_i64, _vp]),
+    "tace_adamw": (_c_int, [_c_int, _c_int, _vp, _c_i64, _vp, _c_dbl, _vp, _c_int, _c_dbl, _c_dbl, _c_dbl, _c_dbl, _vp,
+                            _c_dbl, ctypes.c_uint64, _vp]),
 }
 ROWS_EXPORTED = tuple(_ROW_SIGS)
 

@@ -34,7 +34,7 @@ HIP_FLAGS = [
 ]
 
 # the row operators (include/tace_rows.h)
-ROW_SRCS = ("rows.hip", "dropout.hip")
+ROW_SRCS = ("rows.hip", "dropout.hip", "norm.hip", "adamw.hip")
 
 
 def generate():
@@ -51,7 +51,8 @@ def _compile(src: str, force: bool) -> str:
             os.path.join(ROOT, "include", "tace_hip.h")]
     deps += glob.glob(os.path.join(GEN, "*.inc"))
     if os.path.basename(src) in ROW_SRCS:
-        deps += [os.path.join(CSRC, "row_types.h"), os.path.join(ROOT, "include", "tace_rows.h")]
+        deps += [os.path.join(CSRC, "row_types.h"), os.path.join(CSRC, "philox.h"),
+                 os.path.join(ROOT, "include", "tace_rows.h")]
     if not force and os.path.exists(obj) and os.path.getmtime(obj) >= max(os.path.getmtime(d) for d in deps):
         return obj
     tmp = obj + ".tmp.o"
@@ -64,17 +65,18 @@ def _compile(src: str, force: bool) -> str:
 ROWS_LIB = os.path.join(LIBDIR, "_rows.so")
 
 
-ROWS_SRC = os.path.join(CSRC, "rows_torch.cpp")
+ROWS_TORCH = tuple(os.path.join(CSRC, n) for n in ("rows_torch.cpp", "layer_torch.cpp"))
 
 
-def _compile_rows(force: bool) -> str:
-    """The object of the row operators' torch binding (host code only)."""
+def _compile_rows(src: str, force: bool) -> str:
+    """An object of the row operators' torch binding (host code only)."""
     import sysconfig
 
     import torch
 
-    obj = os.path.join(OBJ, "rows_torch.o")
-    deps = [ROWS_SRC] + [os.path.join(ROOT, "include", h) for h in ("tace_hip.h", "tace_rows.h")]
+    obj = os.path.join(OBJ, os.path.splitext(os.path.basename(src))[0] + ".o")
+    deps = [src, os.path.join(CSRC, "rows_torch.h")]
+    deps += [os.path.join(ROOT, "include", h) for h in ("tace_hip.h", "tace_rows.h")]
     if not force and os.path.exists(obj) and os.path.getmtime(obj) >= max(os.path.getmtime(d) for d in deps):
         return obj
     top = os.path.join(os.path.dirname(torch.__file__), "include")
@@ -83,17 +85,17 @@ def _compile_rows(force: bool) -> str:
     tmp = obj + ".tmp.o"
     subprocess.run([os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-D__HIP_PLATFORM_AMD__",
                     f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *("-I" + d for d in inc), "-c",
-                    ROWS_SRC, "-o", tmp], check=True, stdout=subprocess.PIPE, stderr=subprocess.STDOUT)
+                    src, "-o", tmp], check=True, stdout=subprocess.PIPE, stderr=subprocess.STDOUT)
     os.replace(tmp, obj)
     return obj
 
 
-def _link_rows(obj: str) -> None:
+def _link_rows(objs) -> None:
     """``_rows.so`` beside the library it calls."""
     import torch
 
     tmp = ROWS_LIB + ".tmp"
-    subprocess.check_call([os.environ.get("CXX", "g++"), "-shared", obj, "-o", tmp, "-L" + LIBDIR, "-ltace_hip",
+    subprocess.check_call([os.environ.get("CXX", "g++"), "-shared", *objs, "-o", tmp, "-L" + LIBDIR, "-ltace_hip",
                            "-L" + os.path.join(os.path.dirname(torch.__file__), "lib"), "-lc10", "-lc10_hip",
                            "-ltorch_cpu", "-ltorch_python", "-Wl,-rpath,$ORIGIN"])
     os.replace(tmp, ROWS_LIB)
@@ -111,15 +113,12 @@ def build(verbose: bool = True, force: bool = True, jobs: int = 0) -> str:
     if verbose:
         print(f"[tace_amd.build] {len(srcs)} translation units, {jobs} jobs: {HIPCC} {' '.join(HIP_FLAGS)}", flush=True)
     with cf.ThreadPoolExecutor(jobs) as ex:
-        futs = {ex.submit(_compile_rows, force): ROWS_SRC}
+        futs = {ex.submit(_compile_rows, s, force): s for s in ROWS_TORCH}
         futs.update({ex.submit(_compile, s, force): s for s in srcs})
-        objs = []
+        objs, rows_objs = [], []
         for f in cf.as_completed(futs):
             try:
-                if futs[f] == ROWS_SRC:
-                    rows_obj = f.result()
-                else:
-                    objs.append(f.result())
+                (rows_objs if futs[f] in ROWS_TORCH else objs).append(f.result())
             except subprocess.CalledProcessError as e:
                 sys.stderr.write(e.stdout.decode(errors="replace"))
                 raise
@@ -127,7 +126,7 @@ def build(verbose: bool = True, force: bool = True, jobs: int = 0) -> str:
     tmp = LIB + ".tmp"
     subprocess.check_call([HIPCC, "--offload-arch=gfx950", "-shared", "-fPIC", *objs, "-o", tmp])
     os.replace(tmp, LIB)
-    _link_rows(rows_obj)
+    _link_rows(sorted(rows_objs))
     if verbose:
         print(f"[tace_amd.build] {LIB} in {time.time() - t0:.1f}s", flush=True)
     return LIB

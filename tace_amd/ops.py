@@ -1626,6 +1626,80 @@ def dropout(x: torch.Tensor, p: float, rng, site: int = 0, components: Sequence[
     return N.rows().dropout(x, p, state, seed, offset, site, components, residual, TIMER is not None)
 
 
+# ------------------------------------------------------- routed layers ----
+def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residual: Optional[torch.Tensor] = None,
+             components: Sequence[int] = (1,)):
+    """Root-mean-square norm: y = h ``weight`` / sqrt(mean(h^2) + eps) over the
+    last axis of ``x`` [..., D], with h = x.  With ``residual`` (x's shape and
+    type) h = x + residual, rounded to x's type, and (y, h) is returned.
+
+    ``components``: x is group-major [rows, sum(components) C] (blocks [rows,
+    components[b], C], at most ``ROW_BLOCKS``), each (row, block) has its own
+    mean square over components and channels, and ``weight`` is [blocks, C]: one
+    factor for all components of a channel, so degree-l blocks stay
+    equivariant.  (1,): plain rows and ``weight`` [D].  ``weight`` has x's type
+    or its sums' (float32; float64 for float64), and its gradient has weight's.
+    A normed row has at most ``ROW_MAX`` elements; squares are summed in
+    the sums' type.  Differentiable any number of times: the first gradient is a
+    kernel's, gradients of it are torch's."""
+    out = N.rows().rms_norm(x, weight, eps, residual, components, TIMER is not None)
+    return out[0] if residual is None else tuple(out)
+
+
+def rms_norm_e4m3(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residual: Optional[torch.Tensor] = None,
+                  components: Sequence[int] = (1,)):
+    """``rms_norm`` with y in 8 bits: (codes, scales) or (codes, scales, h), y =
+    codes * scales.  ``codes`` is float8_e4m3fn of x's shape, ``scales`` float32
+    [rows, blocks] (rows: all axes but the last) with max |y| / 448 of each
+    (row, block).  A row that holds a NaN has scale NaN; one whose largest |y| is
+    below 2^-100 is zeros under scale 0.  x is float32, bfloat16 or float16.
+    No gradient."""
+    return tuple(N.rows().rms_norm_e4m3(x, weight, eps, residual, components, TIMER is not None))
+
+
+def grad_norm(grads: Sequence[torch.Tensor]) -> torch.Tensor:
+    """The 2-norm of all ``grads`` together (GPU tensors of one row type), a
+    tensor of no axes in the type's sums.  Summed in a fixed order."""
+    return N.rows().grad_norm(list(grads), TIMER is not None)
+
+
+ADAM_BLOCK = 256   # TACE_ADAM_BLOCK, elements to a scale of 8-bit states
+
+
+def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], exp_avgs: Sequence[torch.Tensor],
+               exp_avg_sqs: Sequence[torch.Tensor], counter: torch.Tensor, *, lr, betas: Tuple[float, float] = (0.9, 0.999),
+               eps: float = 1e-8, weight_decay: float = 0.01, scales: Optional[Sequence[torch.Tensor]] = None,
+               masters: Optional[Sequence[torch.Tensor]] = None, max_norm: Optional[float] = None,
+               norm: Optional[torch.Tensor] = None, seed: int = 0) -> Optional[torch.Tensor]:
+    """One step of AdamW, in place, over all ``params`` (contiguous, one row type)
+    in one launch for each 56 of them; ``tace_amd.optim.AdamW`` is the optimiser
+    around it.
+
+    ``exp_avgs``, ``exp_avg_sqs``: the averages of g and g^2, of the parameters'
+    shapes in the type's sums.  With ``scales`` (float32 [ceil(numel / ADAM_BLOCK),
+    2] each) they are float8_e4m3fn codes of the average of g and of the ROOT of
+    the average of g^2, ``ADAM_BLOCK`` elements to a scale, rounded at random (a
+    function of ``seed``, the step, the parameter's place in the list and the
+    element).  ``masters`` (parameters of 16 bits): float32 weights that are
+    stepped, the parameters are rounded from them.  ``counter``: int64 [2] on the
+    device, the steps done and 0; it counts the step when the kernel runs, so a
+    recorded graph goes on counting.  ``lr``: a number, or a tensor of one
+    element on the device that is read when the kernel runs.  ``max_norm``:
+    gradients are scaled to this norm where theirs (all of ``grads``, or
+    ``norm``, ``grad_norm``'s of more) is larger; where it is infinite or NaN the
+    step leaves everything as it was.  Returns the norm, None without
+    ``max_norm``."""
+    lr_at = None
+    if isinstance(lr, torch.Tensor) and lr.is_cuda:
+        lr, lr_at = 0.0, lr
+    seed = int(seed)
+    if not -2 ** 63 <= seed < 2 ** 64:
+        raise ValueError("adamw_step: seed has 64 bits")
+    return N.rows().adamw_step(params, grads, exp_avgs, exp_avg_sqs, counter, float(lr), lr_at, betas[0], betas[1], eps,
+                               weight_decay, scales, masters, max_norm, norm, seed - 2 ** 64 if seed >= 2 ** 63 else seed,
+                               TIMER is not None)
+
+
 def _pad4(lst):
     return [N.ptr(t) for t in lst] + [None] * (4 - len(lst))
 

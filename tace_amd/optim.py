@@ -1,0 +1,154 @@
+"""AdamW for models in training mode: one pass over the parameters a step.
+
+``AdamW`` is a ``torch.optim.Optimizer`` (parameter groups, ``state_dict``,
+schedulers, hooks) whose step is ``ops.adamw_step``: the parameters of a type in
+one launch for each 56 of them, the clipping norm in one more, states in 32 bits
+or in 8."""
+
+from __future__ import annotations
+
+from typing import Dict, List, Optional
+
+import torch
+
+from . import ops
+
+
+class AdamW(torch.optim.Optimizer):
+    """AdamW (decoupled weight decay) on GPU parameters of float64, float32,
+    bfloat16 or float16.
+
+    ``bits``: 32, states in float32 (float64 for float64 parameters), or 8, e4m3
+    codes with a float32 scale for each 256 (``exp_avg_sq`` then holds the codes of
+    the root).  Parameters of 16 bits are stepped as float32 masters kept with
+    the states, unless ``masters`` is False.  ``max_norm``: the gradients of all
+    groups together are scaled to this norm where it is exceeded, and a step whose
+    norm is infinite or NaN changes nothing; ``norm`` is the last step's.
+    ``seed``: of the 8-bit states' rounding.  ``lr`` of a group may be a tensor of
+    one element on the GPU.
+
+    A step can be recorded into a graph (its gradients' addresses are part of
+    it) once the states are made, by a first step or ``init_states()``."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 0.01,
+                 bits: int = 32, max_norm: Optional[float] = None, masters: bool = True, seed: int = 0):
+        if bits not in (8, 32):
+            raise ValueError(f"AdamW: states of {bits} bits, expected 8 or 32")
+        if not (0 <= betas[0] < 1 and 0 <= betas[1] < 1):
+            raise ValueError(f"AdamW: betas {betas} are not in [0, 1)")
+        if not (eps >= 0 and weight_decay >= 0 and (isinstance(lr, torch.Tensor) or lr >= 0)):
+            raise ValueError("AdamW: lr, eps and weight_decay are not negative")
+        if max_norm is not None and not max_norm > 0:
+            raise ValueError(f"AdamW: max_norm {max_norm} is not positive")
+        super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay))
+        self.bits, self.max_norm, self.masters, self.seed = bits, max_norm, masters, int(seed)
+        self.norm: Optional[torch.Tensor] = None
+
+    # ------------------------------------------------------------ states ----
+    def _init(self, p: torch.Tensor, counter: torch.Tensor) -> Dict[str, torch.Tensor]:
+        wide = torch.float64 if p.dtype == torch.float64 else torch.float32
+        if self.bits == 8 and p.dtype == torch.float64:
+            raise ValueError("AdamW: float64 parameters have no states of 8 bits")
+        held = torch.float8_e4m3fn if self.bits == 8 else wide
+        like = dict(dtype=held, device=p.device)
+        s = {"step": counter, "exp_avg": torch.zeros(p.shape, **like), "exp_avg_sq": torch.zeros(p.shape, **like)}
+        if self.bits == 8:
+            s["scales"] = torch.zeros(-(-p.numel() // ops.ADAM_BLOCK), 2, dtype=torch.float32, device=p.device)
+        if self.masters and p.dtype in (torch.bfloat16, torch.float16):
+            s["master"] = p.detach().to(torch.float32, copy=True)
+        return s
+
+    def _init_of(self, params: List[torch.Tensor]) -> None:
+        """States of those that have none; one counter for each type and device."""
+        counters: Dict[tuple, torch.Tensor] = {}
+        for p in params:
+            if not self.state.get(p):
+                key = (p.device, p.dtype)
+                if key not in counters:
+                    counters[key] = torch.zeros(2, dtype=torch.int64, device=p.device)
+                self.state[p] = self._init(p, counters[key])
+
+    def init_states(self) -> None:
+        """Makes the states of all parameters that require a gradient now."""
+        for group in self.param_groups:
+            self._init_of([p for p in group["params"] if p.requires_grad])
+
+    def _launches(self, group) -> List[List[torch.Tensor]]:
+        """Parameters with gradients that take one launch: those of one counter
+        (and so of one type).  A counter counts the steps of all that share it, so
+        parameters without a gradient this time leave with a copy."""
+        with_grad = [p for p in group["params"] if p.grad is not None]
+        self._init_of(with_grad)
+        sets: Dict[int, List[torch.Tensor]] = {}
+        for p in with_grad:
+            sets.setdefault(id(self.state[p]["step"]), []).append(p)
+        if len(with_grad) < len(group["params"]):
+            copies: Dict[int, torch.Tensor] = {}
+            for p in group["params"]:
+                s = self.state.get(p) if p.grad is None else None
+                if s and id(s["step"]) in sets:
+                    shared = s["step"]
+                    if id(shared) not in copies:
+                        copies[id(shared)] = shared.clone()
+                    s["step"] = copies[id(shared)]
+        return list(sets.values())
+
+    # -------------------------------------------------------------- step ----
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        launches = [(group, ps) for group in self.param_groups for ps in self._launches(group)]
+        self.norm = None
+        if self.max_norm is not None and launches:
+            by_type: Dict[torch.dtype, List[torch.Tensor]] = {}
+            for _, ps in launches:
+                by_type.setdefault(ps[0].dtype, []).extend(p.grad for p in ps)
+            if len(launches) > 1:
+                norms = [ops.grad_norm(g) for g in by_type.values()]
+                self.norm = norms[0] if len(norms) == 1 else torch.stack([n.double() for n in norms]).square().sum().sqrt()
+        for group, ps in launches:
+            states = [self.state[p] for p in ps]
+            norm = self.norm
+            if norm is not None:
+                norm = norm.to(torch.float64 if ps[0].dtype == torch.float64 else torch.float32)
+            place = next(i for i, p in enumerate(group["params"]) if p is ps[0])
+            got = ops.adamw_step(
+                ps, [p.grad for p in ps], [s["exp_avg"] for s in states], [s["exp_avg_sq"] for s in states],
+                states[0]["step"], lr=group["lr"], betas=group["betas"], eps=group["eps"],
+                weight_decay=group["weight_decay"], scales=[s["scales"] for s in states] if self.bits == 8 else None,
+                masters=[s["master"] for s in states] if "master" in states[0] else None, max_norm=self.max_norm,
+                norm=norm, seed=(self.seed * 1000003 + self.param_groups.index(group) * 8191 + place) % 2 ** 64)
+            if self.norm is None:
+                self.norm = got
+        return loss
+
+    # ------------------------------------------------------------- state ----
+    def load_state_dict(self, state_dict) -> None:
+        """As ``Optimizer.load_state_dict``, but states keep their types (masters
+        and codes are not cast to the parameters' type) and parameters whose steps
+        are equal share a counter again."""
+        given = state_dict["state"]
+        super().load_state_dict(state_dict)
+        order = [i for g in state_dict["param_groups"] for i in g["params"]]
+        params = [p for g in self.param_groups for p in g["params"]]
+        counters: Dict[tuple, torch.Tensor] = {}
+        group_of = [k for k, g in enumerate(self.param_groups) for _ in g["params"]]
+        for i, p, k in zip(order, params, group_of):
+            if i not in given:
+                continue
+            s = {}
+            want = self._init(p, torch.zeros(2, dtype=torch.int64, device=p.device))
+            for name, zero in want.items():
+                if name not in given[i]:
+                    raise ValueError(f"AdamW: the state of parameter {i} has no {name}; its states have other bits")
+                v = given[i][name]
+                if v.dtype != zero.dtype or v.shape != zero.shape:
+                    raise ValueError(f"AdamW: {name} of parameter {i} is {v.dtype} {tuple(v.shape)}, expected "
+                                     f"{zero.dtype} {tuple(zero.shape)}")
+                s[name] = v.detach().to(p.device, copy=True)
+            key = (k, p.dtype, p.device, int(s["step"][0]))
+            s["step"] = counters.setdefault(key, s["step"])
+            self.state[p] = s

@@ -1,0 +1,115 @@
+"""The routed layer's operators: boundary and refusals (CPU)."""
+
+import ctypes
+
+import pytest
+import torch
+
+from tace_amd import _native as N
+from tace_amd import ops, optim
+
+P = 4096   # an address that is never read
+
+
+def _refused(rc, text):
+    assert rc < 0 and text in N.lib().tace_last_error(), N.lib().tace_last_error()
+
+
+def _ints(*v):
+    return (ctypes.c_int32 * len(v))(*v)
+
+
+def test_norm_entries_refuse_bad_arguments():
+    L = N.lib()
+    fwd = lambda ty=0, x=P, r=None, w=P, rows=4, C=8, blocks=1, comps=_ints(1), h=None, y=P, s=None: L.tace_rms_norm_fwd(
+        ty, x, r, w, 0, rows, C, blocks, comps, 1e-6, h, y, s, None, None)
+    _refused(fwd(ty=4), b"row type")
+    _refused(fwd(rows=-1), b"bad sizes")
+    _refused(fwd(C=0), b"bad sizes")
+    _refused(fwd(blocks=9, comps=_ints(*[1] * 9)), b"bad sizes")
+    _refused(fwd(comps=_ints(0)), b"components")
+    _refused(fwd(C=32769), b"32768")
+    _refused(fwd(C=16385, comps=_ints(2)), b"32768")
+    _refused(fwd(rows=2 ** 31 - 1), b"bad sizes")
+    _refused(fwd(x=None), b"null")
+    _refused(fwd(r=P), b"null")          # a residual without a place for the sum
+    _refused(fwd(h=P), b"null")
+    _refused(fwd(ty=1, s=P), b"8 bits")
+    assert fwd(rows=0, x=None, y=None) == 0
+    bwd = lambda ty=0, gy=P, rows=4, dw=None, work=None, nbytes=0: L.tace_rms_norm_bwd(
+        ty, gy, None, P, P, 0, P, rows, 8, 1, _ints(1), P, dw, work, nbytes, None)
+    _refused(bwd(gy=None), b"null")
+    _refused(bwd(rows=0), b"no rows")
+    _refused(bwd(dw=P), b"workspace")
+    need = L.tace_rms_norm_bwd_work(0, 4, 8, 1, _ints(1))
+    _refused(bwd(dw=P, work=P, nbytes=need - 1), b"workspace")
+    _refused(bwd(dw=P, work=P + 8, nbytes=need), b"workspace")
+    _refused(L.tace_rms_norm_bwd_work(7, 4, 8, 1, _ints(1)), b"row type")
+
+
+def test_norm_workspace_is_bounded():
+    """A row of sums for each of about 1,024 workgroups (or one a row, if they are fewer)."""
+    L = N.lib()
+    for ty, size in ((0, 4), (1, 8), (2, 4), (3, 4)):
+        for rows in (1, 7, 1000, 10 ** 6):
+            for C, comps in ((1, (1,)), (63, (1, 3)), (128, (1, 3, 5, 7)), (4096, (1,)), (32768, (1,)), (32767, (1,))):
+                nbytes = L.tace_rms_norm_bwd_work(ty, rows, C, len(comps), _ints(*comps))
+                assert C * len(comps) * size <= nbytes <= min(1024 + 8, rows * len(comps)) * C * max(comps) * size
+
+
+class Row(ctypes.Structure):
+    _fields_ = [(k, ctypes.c_void_p) for k in ("p", "g", "m", "s", "master", "scales")] + [("n", ctypes.c_int64)]
+
+
+def test_adamw_entries_refuse_bad_arguments():
+    L = N.lib()
+    row = lambda **over: Row(**{**dict(p=P, g=P, m=P, s=P, n=5), **over})
+
+    def step(ty=0, eight=0, rows=(row(),), counter=P, b1=0.9, b2=0.99, eps=1e-8):
+        t = (Row * max(1, len(rows)))(*rows)
+        return L.tace_adamw(ty, eight, t, len(rows), counter, 1e-3, None, 0, b1, b2, eps, 0.0, None, 0.0, 0, None)
+
+    _refused(step(ty=9), b"row type")
+    _refused(step(counter=None), b"null")
+    _refused(step(rows=(row(), row(m=None))), b"null")
+    _refused(step(rows=(row(g=None),)), b"null")
+    _refused(step(eight=1), b"null")                                 # no scales
+    _refused(step(ty=1, eight=1, rows=(row(scales=P),)), b"float64")
+    _refused(step(rows=(row(master=P),)), b"masters")
+    _refused(step(rows=(row(n=-1),)), b"2^34")
+    _refused(step(rows=(row(n=2 ** 34 + 1),)), b"2^34")
+    for bad in (dict(b1=1.0), dict(b2=-0.1), dict(b1=float("nan")), dict(eps=-1.0)):
+        _refused(step(**bad), b"betas")
+    assert step(rows=()) == 0 and step(rows=(Row(n=0),)) == 0
+    t = (Row * 2)(row(n=10 ** 9), row())
+    need = L.tace_grad_norm_work(t, 2)
+    assert need == 8 * 1024
+    norm = lambda count=2, ticket=P, out=P, work=P, nbytes=need: L.tace_grad_norm(0, t, count, ticket, out, work, nbytes, None)
+    _refused(norm(count=0), b"no gradients")
+    for bad in (dict(ticket=None), dict(out=None), dict(work=None), dict(work=P + 4), dict(nbytes=need - 1)):
+        _refused(norm(**bad), b"workspace")
+
+
+def test_operators_take_no_cpu_tensors():
+    x, w = torch.ones(4, 8), torch.ones(8)
+    for call in (lambda: ops.rms_norm(x, w), lambda: ops.rms_norm_e4m3(x, w), lambda: ops.grad_norm([x]),
+                 lambda: ops.adamw_step([x], [x], [x], [x], torch.zeros(2, dtype=torch.int64), lr=0.1)):
+        with pytest.raises(ValueError, match="GPU tensor"):
+            call()
+    with pytest.raises(ValueError, match="no gradients"):
+        ops.grad_norm([])
+    with pytest.raises(ValueError, match="64 bits"):
+        ops.adamw_step([x], [x], [x], [x], x, lr=0.1, seed=2 ** 64)
+
+
+def test_optimiser_arguments():
+    p = [torch.ones(3, requires_grad=True)]
+    for bad, text in ((dict(bits=16), "bits"), (dict(betas=(1.0, 0.9)), "betas"), (dict(eps=-1.0), "negative"),
+                      (dict(lr=-1.0), "negative"), (dict(weight_decay=-0.1), "negative"), (dict(max_norm=0.0), "max_norm")):
+        with pytest.raises(ValueError, match=text):
+            optim.AdamW(p, **bad)
+    o = optim.AdamW(p, max_norm=1.0)
+    o.step()                                  # nothing has a gradient
+    assert o.norm is None and not o.state[p[0]]
+    o.init_states()
+    assert o.state[p[0]]["step"].tolist() == [0, 0] and o.state[p[0]]["exp_avg"].dtype == torch.float32
