@@ -107,6 +107,33 @@ int tace_rms_norm_bwd(int type, const void* gy, const void* gh, const void* h, c
                       const void* inv, int64_t rows, int32_t channels, int32_t blocks, const int32_t* comps, void* dh,
                       void* dw, void* work, int64_t work_bytes, void* stream);
 
+/* The experts' products.  Rows sorted by expert as tace_route_group's (rowptr
+ * [experts + 1]; rows from rowptr[experts] on are dropped) in `blocks` blocks of
+ * comps[b] components: a batch is block after block, each [rows, comps[b], K].
+ * weight [experts, blocks, K, N].
+ * tace_expert_linear: out [.., N] = scale x weight[expert][block], or (transposed;
+ * x [.., N]) out [.., K] = scale x weight^T; zeros for dropped rows.
+ * tace_expert_linear_grad: dw = scale x^T g of each expert's rows, zeros without
+ * any; work: tace_expert_linear_grad_work bytes, 16-byte aligned, NULL where 0.
+ * Products are summed in float (double for TACE_ROW_F64), float32's as six
+ * products of three bfloat16 terms each.
+ * tace_expert_linear_e4m3: out [rows, N] (TACE_ROW_F32, _BF16 or _F16) = x_scale
+ * w_scale[expert] (x codes, w codes), x codes [.., K], weight codes [experts, N,
+ * K] (both 16-byte aligned, K a multiple of 16), w_scale [experts, N].  order
+ * (tace_route_group's): sorted row r is x's row order[r] / choices, x [rows /
+ * choices, K]; NULL: x [rows, K] is sorted. */
+int tace_expert_linear(int type, int transposed, const void* x, const void* weight, const int32_t* rowptr, int64_t rows,
+                       int32_t experts, int32_t blocks, const int32_t* comps, int32_t K, int32_t N, double scale,
+                       void* out, void* stream);
+int64_t tace_expert_linear_grad_work(int type, int64_t rows, int32_t experts, int32_t blocks, const int32_t* comps,
+                                     int32_t K, int32_t N);
+int tace_expert_linear_grad(int type, const void* x, const void* g, const int32_t* rowptr, int64_t rows, int32_t experts,
+                            int32_t blocks, const int32_t* comps, int32_t K, int32_t N, double scale, void* dw, void* work,
+                            int64_t work_bytes, void* stream);
+int tace_expert_linear_e4m3(int out_type, const void* x, const float* x_scale, const int32_t* order, int32_t choices,
+                            const void* weight, const float* w_scale, const int32_t* rowptr, int64_t rows,
+                            int32_t experts, int32_t K, int32_t N, void* out, void* stream);
+
 /* AdamW.  tensors: host array; p, g [n] of the row type, m, s [n] the states:
  * averages of g and g^2 in the type's sums, or (`eight`) of g and the root of the
  * average of g^2 as e4m3 codes with scales float [ceil(n / 256), 2]; master

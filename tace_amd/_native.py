@@ -146,6 +146,13 @@ _ROW_SIGS = {
     "tace_rms_norm_bwd_work": (_c_i64, [_c_int, _c_i64, _c_i32, _c_i32, _vp]),
     "tace_rms_norm_bwd": (_c_int, [_c_int, _vp, _vp, _vp, _vp, _c_int, _vp, _c_i64, _c_i32, _c_i32, _vp, _vp, _vp, _vp,
                                    _c_i64, _vp]),
+    "tace_expert_linear": (_c_int, [_c_int, _c_int, _vp, _vp, _vp, _c_i64, _c_i32, _c_i32, _vp, _c_i32, _c_i32, _c_dbl,
+                                    _vp, _vp]),
+    "tace_expert_linear_grad_work": (_c_i64, [_c_int, _c_i64, _c_i32, _c_i32, _vp, _c_i32, _c_i32]),
+    "tace_expert_linear_grad": (_c_int, [_c_int, _vp, _vp, _vp, _c_i64, _c_i32, _c_i32, _vp, _c_i32, _c_i32, _c_dbl, _vp,
+                                         _vp, _c_i64, _vp]),
+    "tace_expert_linear_e4m3": (_c_int, [_c_int, _vp, _vp, _vp, _c_i32, _vp, _vp, _vp, _c_i64, _c_i32, _c_i32, _c_i32,
+                                         _vp, _vp]),
     "tace_grad_norm_work": (_c_i64, [_vp, _c_i64]),
     "tace_grad_norm": (_c_int, [_c_int, _vp, _c_i64, _vp, _vp, _vp, _c_i64, _vp]),
     "tace_adamw": (_c_int, [_c_int, _c_int, _vp, _c_i64, _vp, _c_dbl, _vp, _c_int, _c_dbl, _c_dbl, _c_dbl, _c_dbl, _vp,

@@ -34,7 +34,7 @@ HIP_FLAGS = [
 ]
 
 # the row operators (include/tace_rows.h)
-ROW_SRCS = ("rows.hip", "dropout.hip", "norm.hip", "adamw.hip")
+ROW_SRCS = ("rows.hip", "dropout.hip", "norm.hip", "adamw.hip", "experts.hip")
 
 
 def generate():

@@ -165,6 +165,165 @@ std::vector<Tensor> rms_norm_e4m3(Tensor x, Tensor weight, double eps, optional<
   return a.residual ? std::vector<Tensor>{q, scales, h} : std::vector<Tensor>{q, scales};
 }
 
+// ------------------------------------------------------------------- experts ----
+struct Experts {
+  Pinned rowptr;
+  int64_t rows, experts;
+  std::vector<int32_t> comps;
+  int64_t total;   // components
+  int64_t K, N;
+  double scale;
+  bool timed, flat;   // flat: weights [E, K, N]
+
+  int blocks() const { return (int)comps.size(); }
+  const int32_t* starts() const { return rowptr.get("plan.rowptr").data_ptr<int>(); }
+};
+
+Tensor expert_rows(bool transposed, const Tensor& x, const Tensor& w, const Experts& a) {
+  Tensor out = at::empty({a.rows, a.total * (transposed ? a.K : a.N)}, x.options());
+  Launch l(x, "expert_linear", a.timed);
+  l.done(tace_expert_linear(type_code(x.scalar_type()), transposed, ptr(x), ptr(w), a.starts(), a.rows, (int)a.experts,
+                            a.blocks(), a.comps.data(), (int)a.K, (int)a.N, a.scale, ptr(out), l.stream),
+         {a.rows, a.total, a.K, a.N});
+  return out;
+}
+
+Tensor expert_weights(const Tensor& x, const Tensor& g, const Experts& a) {
+  Tensor dw = a.flat ? at::empty({a.experts, a.K, a.N}, x.options())
+                     : at::empty({a.experts, a.blocks(), a.K, a.N}, x.options()), work;
+  const int code = type_code(x.scalar_type());
+  const int64_t bytes = tace_expert_linear_grad_work(code, a.rows, (int)a.experts, a.blocks(), a.comps.data(), (int)a.K,
+                                                     (int)a.N);
+  if (bytes > 0) work = at::empty({bytes}, x.options().dtype(at::kByte));
+  Launch l(x, "expert_linear_grad", a.timed);
+  l.done(tace_expert_linear_grad(code, ptr(x), ptr(g), a.starts(), a.rows, (int)a.experts, a.blocks(), a.comps.data(),
+                                 (int)a.K, (int)a.N, a.scale, ptr(dw), ptr(work), bytes, l.stream),
+         {a.rows, a.total, a.K, a.N});
+  return dw;
+}
+
+// L(x, w) = s x w, T(g, w) = s g w^T and G(x, g) = s x^T g by expert are bilinear and each other's derivatives
+Tensor rows_op(bool transposed, const Tensor& x, const Tensor& w, const Experts& a);
+Tensor weights_op(const Tensor& x, const Tensor& g, const Experts& a);
+
+template <bool TRANSPOSED>
+struct ExpertRows : torch::autograd::Function<ExpertRows<TRANSPOSED>> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const Experts& a) {
+    ctx->save_for_backward({x, w});
+    hold(ctx, a);
+    return expert_rows(TRANSPOSED, x, w, a);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const Experts& a = held<Experts>(ctx);
+    const Tensor c = dense(grads[0]);
+    variable_list out(3);
+    if (ctx->needs_input_grad(0)) out[0] = rows_op(!TRANSPOSED, c, saved[1], a);
+    if (ctx->needs_input_grad(1)) out[1] = TRANSPOSED ? weights_op(c, saved[0], a) : weights_op(saved[0], c, a);
+    return out;
+  }
+};
+
+struct ExpertWeights : torch::autograd::Function<ExpertWeights> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& g, const Experts& a) {
+    ctx->save_for_backward({x, g});
+    hold(ctx, a);
+    return expert_weights(x, g, a);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const Experts& a = held<Experts>(ctx);
+    const Tensor v = dense(grads[0]);
+    variable_list out(3);
+    if (ctx->needs_input_grad(0)) out[0] = rows_op(true, saved[1], v, a);
+    if (ctx->needs_input_grad(1)) out[1] = rows_op(false, saved[0], v, a);
+    return out;
+  }
+};
+
+Tensor rows_op(bool transposed, const Tensor& x, const Tensor& w, const Experts& a) {
+  if (!tracked(x) && !tracked(w)) return expert_rows(transposed, x, w, a);
+  return transposed ? ExpertRows<true>::apply(x, w, a) : ExpertRows<false>::apply(x, w, a);
+}
+Tensor weights_op(const Tensor& x, const Tensor& g, const Experts& a) {
+  return tracked(x) || tracked(g) ? ExpertWeights::apply(x, g, a) : expert_weights(x, g, a);
+}
+
+void want_rowptr(const Tensor& rowptr, const Tensor& like, int64_t rows) {
+  TORCH_CHECK_VALUE(rowptr.dim() == 1 && rowptr.numel() >= 1, "plan.rowptr is empty");
+  want_int32(rowptr, rowptr.numel(), like, "plan.rowptr");
+  TORCH_CHECK_VALUE(rows >= 0 && rows <= MAX_INDEX, "expert_linear: rows exceed 32-bit indices");
+}
+
+Tensor expert_linear(const Tensor& x, const Tensor& weight, const Tensor& rowptr, int64_t rows, double scale,
+                     const std::vector<int64_t>& components, bool timed) {
+  want_rows(x, "x");
+  want_rowptr(rowptr, x, rows);
+  Experts a{rowptr, rows, rowptr.numel() - 1, {}, 0, 0, 0, scale, timed, weight.dim() == 3};
+  bool ok = !components.empty() && components.size() <= TACE_ROW_MAX_BLOCKS;
+  for (int64_t c : components) {
+    ok = ok && c >= 1 && c <= 1024;
+    a.comps.push_back((int32_t)c);
+    a.total += c;
+  }
+  TORCH_CHECK_VALUE(ok, "expert_linear: components ", components, " are not 1 to ", TACE_ROW_MAX_BLOCKS,
+                    " blocks of 1 to 1024");
+  const int64_t B = a.blocks();
+  TORCH_CHECK_VALUE(weight.scalar_type() == x.scalar_type() && weight.size(0) == a.experts &&
+                    ((B == 1 && weight.dim() == 3) || (weight.dim() == 4 && weight.size(1) == B)),
+                    "weight is ", weight.scalar_type(), " ", weight.sizes(), ", expected ", x.scalar_type(), " [",
+                    a.experts, ", ", B, ", K, N]", B == 1 ? " or [E, K, N]" : "");
+  want_device(weight, x, "weight");
+  a.K = weight.size(-2);
+  a.N = weight.size(-1);
+  TORCH_CHECK_VALUE(a.K >= 1 && a.K <= 65536 && a.N >= 1 && a.N <= 65536, "weight has shape ", weight.sizes(),
+                    ", expected K and N of 1 to 65536");
+  TORCH_CHECK_VALUE(x.dim() == 2 && x.size(0) == rows && x.size(1) == a.total * a.K, "x has shape ", x.sizes(),
+                    ", expected [", rows, ", ", a.total * a.K, "]");
+  return rows_op(false, dense(x), dense(weight), a);
+}
+
+Tensor expert_linear_e4m3(const Tensor& q, const Tensor& q_scale, const Tensor& w, const Tensor& w_scale,
+                          const Tensor& rowptr, const Tensor& order, int64_t tokens, int64_t k, bool gather,
+                          at::ScalarType out_type, bool timed) {
+  const int64_t rows = tokens * k, from = gather ? tokens : rows, E = rowptr.numel() - 1;
+  TORCH_CHECK_VALUE(q.is_cuda(), "q must be a GPU tensor (got ", q.device(), ")");
+  want_memory(q, "q");
+  want_rowptr(rowptr, q, rows);
+  if (gather) want_int32(order, rows, q, "plan.order");
+  TORCH_CHECK_VALUE(out_type == at::kFloat || out_type == at::kBFloat16 || out_type == at::kHalf,
+                    "expert_linear_e4m3: out_dtype ", out_type, ", expected float32, bfloat16 or float16");
+  TORCH_CHECK_VALUE(w.scalar_type() == at::kFloat8_e4m3fn && w.dim() == 3 && w.size(0) == E && w.size(1) >= 1 &&
+                    w.size(1) <= 65536 && w.size(2) >= 16 && w.size(2) <= 65536 && w.size(2) % 16 == 0, "weight is ",
+                    w.scalar_type(), " ", w.sizes(), ", expected float8_e4m3fn [", E, ", N, K], K a multiple of 16");
+  const int64_t N = w.size(1), K = w.size(2);
+  TORCH_CHECK_VALUE(q.scalar_type() == at::kFloat8_e4m3fn && q.dim() == 2 && q.size(0) == from && q.size(1) == K, "q is ",
+                    q.scalar_type(), " ", q.sizes(), ", expected float8_e4m3fn [", from, ", ", K, "]");
+  TORCH_CHECK_VALUE(q_scale.scalar_type() == at::kFloat && q_scale.numel() == from && q_scale.size(0) == from,
+                    "q_scale is ", q_scale.scalar_type(), " ", q_scale.sizes(), ", expected float32 [", from, "]");
+  TORCH_CHECK_VALUE(w_scale.scalar_type() == at::kFloat && w_scale.dim() == 2 && w_scale.size(0) == E &&
+                    w_scale.size(1) == N, "w_scale is ", w_scale.scalar_type(), " ", w_scale.sizes(),
+                    ", expected float32 [", E, ", ", N, "]");
+  want_device(w, q, "weight");
+  want_device(q_scale, q, "q_scale");
+  want_device(w_scale, q, "w_scale");
+  TORCH_CHECK_VALUE(!tracked(q_scale) && !tracked(w_scale), "expert_linear_e4m3 has no gradient: call it under "
+                    "torch.no_grad()");
+  // (a view of codes may begin anywhere: 16-byte loads need a copy)
+  auto codes = [](const Tensor& t) {
+    const Tensor c = t.contiguous();
+    return c.numel() && (uintptr_t)c.const_data_ptr() % 16 ? c.clone() : c;
+  };
+  const Tensor x = codes(q), wt = codes(w), xs = dense(q_scale), ws = dense(w_scale);
+  Tensor out = at::empty({rows, N}, q_scale.options().dtype(out_type).requires_grad(false));
+  Launch l(q, "expert_linear_e4m3", timed);
+  l.done(tace_expert_linear_e4m3(type_code(out_type), x.const_data_ptr(), xs.const_data_ptr<float>(),
+                                 gather ? order.const_data_ptr<int>() : nullptr, (int)k, wt.const_data_ptr(),
+                                 ws.const_data_ptr<float>(), rowptr.const_data_ptr<int>(), rows, (int)E, (int)K, (int)N,
+                                 out.data_ptr(), l.stream), {rows, K, N});
+  return out;
+}
+
 // --------------------------------------------------------------------- AdamW ----
 typedef std::vector<Tensor> Tensors;
 
@@ -312,6 +471,8 @@ optional<Tensor> adamw_step(const Tensors& params, const Tensors& grads, const T
 void bind_layer(py::module_& mod) {
   mod.def("rms_norm", torch::wrap_pybind_function(rms_norm));
   mod.def("rms_norm_e4m3", torch::wrap_pybind_function(rms_norm_e4m3));
+  mod.def("expert_linear", torch::wrap_pybind_function(expert_linear));
+  mod.def("expert_linear_e4m3", torch::wrap_pybind_function(expert_linear_e4m3));
   mod.def("grad_norm", torch::wrap_pybind_function(grad_norm));
   mod.def("adamw_step", torch::wrap_pybind_function(adamw_step));
 }

@@ -1657,6 +1657,46 @@ def rms_norm_e4m3(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, resi
     return tuple(N.rows().rms_norm_e4m3(x, weight, eps, residual, components, TIMER is not None))
 
 
+def expert_linear(x: torch.Tensor, weight: torch.Tensor, plan: RoutePlan, scale: float = 1.0,
+                  components: Sequence[int] = (1,)) -> torch.Tensor:
+    """The experts' products on sorted rows (``expert_dispatch``): row r of
+    ``x`` [plan.n_rows, K], one of expert e's, times ``scale weight[e]``,
+    ``weight`` [E, K, N]; zeros for rows behind the last expert's (dropped
+    slots).  ``components``: x is group-major (blocks [rows, components[b], K], at
+    most ``ROW_BLOCKS``) and ``weight`` [E, blocks, K, N]: every component of a
+    block by the same matrix, so degree-l blocks stay equivariant; the output is
+    group-major with N channels.  The experts' sizes stay on the GPU: no host
+    synchronisation.  x and weight have one type; float32 products are six of three
+    bfloat16 terms (float32's accuracy), sums float32 (float64 for float64).
+    Differentiable any number of times in x and weight, in a fixed order of
+    sums."""
+    return N.rows().expert_linear(x, weight, plan.rowptr, plan.n_rows, scale, components, TIMER is not None)
+
+
+def expert_weights_e4m3(weight: torch.Tensor, scale: float = 1.0) -> Tuple[torch.Tensor, torch.Tensor]:
+    """``scale weight`` [E, K, N] as ``expert_linear_e4m3`` reads it, laid out
+    once: codes float8_e4m3fn [E, N, K] and their scales float32 [E, N]
+    (largest magnitude of a column / 448)."""
+    w = weight.detach().float().transpose(1, 2) * scale
+    top = w.abs().amax(2)
+    codes = (w * torch.where(top > 0, 448 / top, torch.zeros_like(top)).unsqueeze(2)).to(torch.float8_e4m3fn)
+    return codes.contiguous(), top / 448
+
+
+def expert_linear_e4m3(q: torch.Tensor, q_scale: torch.Tensor, weight: torch.Tensor, w_scale: torch.Tensor,
+                       plan: RoutePlan, gather: bool = False, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """``expert_linear`` on rows and weights of 8 bits, for serving: out
+    [plan.n_rows, N] = ``q_scale`` ``w_scale[e]`` (q . ``weight[e]``), sums in
+    float32, in ``out_dtype`` (bfloat16, float16, float32).  ``q`` float8_e4m3fn
+    [rows, K] and ``q_scale`` float32 [rows] or [rows, 1] as ``rms_norm_e4m3``
+    gives them, K a multiple of 16; ``weight``, ``w_scale``:
+    ``expert_weights_e4m3``.  ``gather``: q holds the tokens' rows [plan.n_tokens,
+    K], read through the plan (no ``expert_dispatch`` before); else sorted rows
+    [plan.n_rows, K].  Zeros behind the last expert's rows.  No gradient."""
+    return N.rows().expert_linear_e4m3(q, q_scale, weight, w_scale, plan.rowptr, plan.order, plan.n_tokens, plan.k,
+                                       gather, out_dtype, TIMER is not None)
+
+
 def grad_norm(grads: Sequence[torch.Tensor]) -> torch.Tensor:
     """The 2-norm of all ``grads`` together (GPU tensors of one row type), a
     tensor of no axes in the type's sums.  Summed in a fixed order."""

@@ -113,3 +113,63 @@ def test_optimiser_arguments():
     assert o.norm is None and not o.state[p[0]]
     o.init_states()
     assert o.state[p[0]]["step"].tolist() == [0, 0] and o.state[p[0]]["exp_avg"].dtype == torch.float32
+
+
+def test_expert_entries_refuse_bad_arguments():
+    L = N.lib()
+    one = _ints(1)
+
+    def rows(ty=0, x=P, w=P, ptr=P, n=4, E=2, blocks=1, comps=one, K=8, M=8, out=P):
+        return L.tace_expert_linear(ty, 0, x, w, ptr, n, E, blocks, comps, K, M, 1.0, out, None)
+
+    _refused(rows(ty=5), b"row type")
+    for bad in (dict(n=-1), dict(n=2 ** 31 - 1), dict(E=-1), dict(E=2 ** 21), dict(blocks=0), dict(blocks=9), dict(K=0),
+                dict(M=0), dict(K=65537), dict(M=65537), dict(comps=None)):
+        _refused(rows(**bad), b"bad sizes")
+    _refused(rows(comps=_ints(0)), b"components")
+    for bad in (dict(x=None), dict(w=None), dict(ptr=None), dict(out=None)):
+        _refused(rows(**bad), b"null")
+    assert rows(n=0, x=None, w=None, out=None) == 0
+
+    def grad(ty=0, x=P, g=P, ptr=P, n=100000, E=2, dw=P, work=P, nbytes=1 << 40):
+        return L.tace_expert_linear_grad(ty, x, g, ptr, n, E, 1, one, 64, 64, 1.0, dw, work, nbytes, None)
+
+    need = L.tace_expert_linear_grad_work(0, 100000, 2, 1, one, 64, 64)
+    assert need > 0 and L.tace_expert_linear_grad_work(0, 100, 2, 1, one, 64, 64) == 0
+    for bad in (dict(work=None), dict(work=P + 8), dict(nbytes=need - 1)):
+        _refused(grad(**bad), b"workspace")
+    for bad in (dict(x=None), dict(g=None), dict(dw=None), dict(ptr=None)):
+        _refused(grad(**bad), b"null")
+    _refused(grad(ty=4), b"row type")
+    _refused(grad(E=70000), b"bad sizes")
+    assert grad(E=0, dw=None) == 0
+
+    def codes(out=2, x=P, xs=P, order=None, k=1, w=P, ws=P, ptr=P, n=4, K=32, o=P):
+        return L.tace_expert_linear_e4m3(out, x, xs, order, k, w, ws, ptr, n, 2, K, 8, o, None)
+
+    _refused(codes(out=1), b"float32, bfloat16 or float16")
+    _refused(codes(K=24), b"multiple of 16")
+    _refused(codes(k=0), b"bad sizes")
+    _refused(codes(order=P, k=3), b"bad sizes")
+    for bad in (dict(x=None), dict(xs=None), dict(w=None), dict(ws=None), dict(ptr=None), dict(o=None)):
+        _refused(codes(**bad), b"null")
+    _refused(codes(x=P + 8), b"aligned")
+    _refused(codes(w=P + 1), b"aligned")
+    assert codes(n=0, x=None, o=None) == 0
+
+
+def test_expert_workspace_covers_every_part():
+    """Parts of 2^shift rows: a slot for each of them and one for each group, whatever the rows' distribution."""
+    L = N.lib()
+    for ty, size in ((0, 4), (1, 8), (2, 4)):
+        for rows in (1, 257, 5000, 300000):
+            for E in (1, 7, 90):
+                for comps in ((1,), (1, 3, 5, 7)):
+                    for K, M in ((16, 8), (128, 128), (1024, 2048)):
+                        nbytes = L.tace_expert_linear_grad_work(ty, rows, E, len(comps), _ints(*comps), K, M)
+                        slots, rest = divmod(nbytes, K * M * size)
+                        assert rest == 0
+                        if nbytes:      # at least 256 rows a part
+                            assert len(comps) * (E + 1) <= slots <= rows * sum(comps) // 256 + len(comps) * (E + 1)
+                        else:
+                            assert rows * max(comps) <= 2 ** 22
