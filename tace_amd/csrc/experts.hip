@@ -8,10 +8,9 @@
 // are one kernel over output tiles: A [M, n] B [n, N] with either operand stored
 // along the summed index or across it.
 //
-// Tiles without a table: group g of the sorted groups takes tile slots
-// start(g) / TM + g and up, at least ceil(length / TM) of them since
-// floor(end / TM) - floor(start / TM) + 1 >= ceil((end - start) / TM); so slot ->
-// group is one ballot over the starts, and rows / TM + groups slots cover all.
+// Tiles without a table: every workgroup sums the groups' tiles up to each over its
+// lanes and looks its own up there, so the host launches for a bound (rows /
+// height + groups) and the tiles that exist are shared out evenly.
 //
 // Tiles pass through LDS, the next step's loads in registers meanwhile.  An
 // operand stored along the summed index is read from LDS as 16-byte fragments,
@@ -59,40 +58,129 @@ struct Groups {
 
 struct Place {
   int64_t first;    // row of the stacked blocks
-  int64_t count;    // rows from there on
-  int64_t group0;   // the group's first row
+  int64_t count;    // rows of the group from there on
   int64_t part;     // slots of the group before this one
   int expert, block;
 };
 
-// The group of a slot of 2^shift rows, its rows from the slot's on (count <= 0:
-// none).  Groups of a block: the experts, and the dropped rows as one more.
-__device__ __forceinline__ Place place_of(const Groups& gr, int slot, int shift) {
-  const int lane = (int)threadIdx.x & 63, per = gr.experts + 1, n = per * gr.blocks;
-  int found = 0;
-  for (int g0 = 0; g0 < n; g0 += 64) {
-    const int g = g0 + lane;
-    bool ok = false;
+// Numbers the slots of 2^shift rows of all groups without gaps and finds a slot's
+// group, a slot a lane: 64 groups at a time are in the lanes, with the sum of their
+// slots up to each.  Groups of a block: the experts and, with DROPPED, the
+// dropped rows as one more; EMPTY: a group without rows has a slot all the same.
+template <bool DROPPED, bool EMPTY>
+struct Places {
+  const Groups& gr;
+  int shift, n, base;   // base: the first group in the lanes
+  int64_t from, to;     // this lane's group's rows
+  int upto;             // slots of the lanes' groups up to this one
+
+  __device__ __forceinline__ Places(const Groups& gr, int shift)
+      : gr(gr), shift(shift), n((gr.experts + (DROPPED ? 1 : 0)) * gr.blocks) {
+    take(0);
+  }
+  __device__ __forceinline__ void take(int at) {
+    const int lane = (int)threadIdx.x & 63, per = gr.experts + (DROPPED ? 1 : 0), g = at + lane;
+    base = at;
+    from = to = 0;
+    int slots = 0;
     if (g < n) {
       const int b = g / per, e = g - b * per;
-      const int64_t start = gr.rows * gr.before[b] + gr.comps[b] * gr.end_of(e);
-      ok = (start >> shift) + g <= slot;
+      const int64_t block0 = gr.rows * gr.before[b];
+      from = block0 + gr.comps[b] * gr.end_of(e);
+      to = block0 + gr.comps[b] * gr.end_of(e + 1);
+      slots = to > from ? (int)((to - from + ((int64_t)1 << shift) - 1) >> shift) : EMPTY ? 1 : 0;
     }
-    const int here = __popcll(__ballot(ok));
-    found += here;
-    if (here < 64) break;
+    upto = slots;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int v = __shfl_up(upto, o, 64);
+      if (lane >= o) upto += v;
+    }
   }
-  const int g = __builtin_amdgcn_readfirstlane(found > 0 ? found - 1 : 0);
-  Place p;
-  p.block = g / per;
-  p.expert = g - p.block * per;
-  const int64_t base = gr.rows * gr.before[p.block];
-  p.group0 = base + gr.comps[p.block] * gr.end_of(p.expert);
-  const int64_t end = base + gr.comps[p.block] * gr.end_of(p.expert + 1);
-  p.part = (int64_t)slot - g - (p.group0 >> shift);
-  p.first = p.group0 + (p.part << shift);
-  p.count = end - p.first;
-  return p;
+  __device__ __forceinline__ int last() const { return __builtin_amdgcn_readlane(upto, 63); }
+  // all slots
+  __device__ __forceinline__ int total() {
+    if (n <= 64) return last();
+    int sum = 0;
+    for (int at = 0; at < n; at += 64) {
+      take(at);
+      sum += last();
+    }
+    return sum;
+  }
+  // (every lane of the wavefront calls it; slots behind the last give a place without rows)
+  __device__ __forceinline__ Place find(int slot) {
+    Place p{0, 0, 0, gr.experts, 0};
+    int before = 0;
+    for (int at = 0; at < n; at += 64) {
+      if (n > 64) take(at);
+      int lane = 0;   // the first of the 64 groups whose slots reach past this one
+#pragma unroll
+      for (int o = 32; o > 0; o >>= 1)
+        if (__shfl(upto, lane + o - 1, 64) <= slot - before) lane += o;
+      const int64_t f = __shfl((long long)from, lane, 64), t = __shfl((long long)to, lane, 64);
+      const int prior = __shfl(upto, max(lane - 1, 0), 64);
+      if (slot >= before && slot - before < last()) {
+        const int per = gr.experts + (DROPPED ? 1 : 0), g = at + lane;
+        p.block = g / per;
+        p.expert = g - p.block * per;
+        p.part = slot - before - (lane ? prior : 0);
+        p.first = f + (p.part << shift);
+        p.count = t - p.first;
+      }
+      before += last();
+    }
+    return p;
+  }
+};
+
+// What a tile is, by elements from its operands' and outputs' first ones; a lane
+// holds one, a wavefront takes them one after the other.
+struct Job {
+  int64_t a, b, out;
+  int sum;          // the summed index
+  int m, n;         // rows and columns, up to the tile's
+  int kind, whole;
+
+  __device__ __forceinline__ static int of(int v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
+  __device__ __forceinline__ static int64_t of(int64_t v, int lane) {
+    const unsigned lo = (unsigned)__builtin_amdgcn_readlane((int)v, lane);
+    return (int64_t)((unsigned long long)(unsigned)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32 | lo);
+  }
+  __device__ __forceinline__ Job lane(int l) const {
+    return Job{of(a, l), of(b, l), of(out, l), of(sum, l), of(m, l), of(n, l), of(kind, l), of(whole, l)};
+  }
+};
+enum { NO_TILE, ZERO_TILE, PRODUCT };
+
+// Tiles of an XCD (every eighth workgroup) are contiguous, its workgroups take them
+// in turn: what runs together shares rows and columns in the XCD's L2.
+struct Share {
+  int first, end, step;
+};
+__device__ __forceinline__ Share share_of(int tiles, bool apart) {
+  const int x = (int)(blockIdx.x & 7);
+  if (apart) {
+    const int n = (int)gridDim.x, i = x * (n >> 3) + (int)(blockIdx.x >> 3);
+    return {(int)((int64_t)tiles * i / n), (int)((int64_t)tiles * (i + 1) / n), 1};
+  }
+  return {(int)((int64_t)tiles * x / 8) + (int)(blockIdx.x >> 3), (int)((int64_t)tiles * (x + 1) / 8), (int)(gridDim.x >> 3)};
+}
+
+// The (row, column) of tile t of rows x cols in blocks of eight rows, down the
+// columns of a block: 64 tiles beside each other then have 8 rows and 8 columns
+// of operands, where 64 along the rows had one to four rows and all columns.
+__device__ __forceinline__ void blocked(int t, int rows, int cols, int* row, int* col) {
+  const int block = t / (8 * cols), r = t - block * 8 * cols, high = min(rows - 8 * block, 8);
+  *row = 8 * block + r % high;
+  *col = r / high;
+}
+
+// one slot for the workgroup
+template <bool DROPPED, bool EMPTY>
+__device__ __forceinline__ Place place_of(const Groups& gr, int slot, int shift) {
+  const Place p = Places<DROPPED, EMPTY>(gr, shift).find(slot);
+  return Place{Job::of(p.first, 0), Job::of(p.count, 0), Job::of(p.part, 0), Job::of(p.expert, 0), Job::of(p.block, 0)};
 }
 
 // workgroups of an XCD (every eighth) take a contiguous range of tiles
@@ -251,6 +339,57 @@ struct Tile {
   }
 };
 
+// The same for 32 x 32 products of 16 of the summed index (a lane: eight of output
+// lane % 32, from 8 (lane / 32) on); 16-bit elements, steps of 64.  (Their sums
+// of 16 registers are updated in place, by the instruction's form; with those
+// of four the compiler moved them about, 32 moves for 64 products.)
+template <typename T, int TM, bool ACROSS>
+struct WideTile {
+  static constexpr int BK = 64, ELEMS = TM * BK;
+  static_assert(sizeof(T) == 2 && TM % 32 == 0, "16-bit tiles of 32");
+
+  __device__ __forceinline__ static int lds_at(int line, int piece) {
+    if constexpr (ACROSS) {
+      // (16 lanes read 32 bytes of four lines; lines 8 apart, and the 32 bytes
+      // beside, are read by the other lanes)
+      const int f = (TM >= 128 ? (line & 3) << 1 : TM == 64 ? line & 2 : 0) | ((line >> 3) & 1);
+      return line * TM + (((piece >> 1) ^ f) << 4) + ((piece & 1) << 3);
+    } else {
+      return line * BK + ((piece ^ ((line >> 1) & 7)) << 3);
+    }
+  }
+  // of outputs 32 j .., 16 s .. of the summed index
+  __device__ __forceinline__ static s8 fragment(const unsigned short* l, int j, int s, int lane) {
+    if constexpr (ACROSS) {
+      union {
+        s4 h[2];
+        s8 v;
+      } o;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int line = 16 * s + 8 * (lane >> 5) + 4 * h + ((lane >> 2) & 3);
+        o.h[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            (__attribute__((address_space(3))) s4*)(l + lds_at(line, 4 * j + ((lane >> 3) & 2) + ((lane >> 1) & 1)) +
+                                                    ((lane & 1) << 2)));
+      }
+      return o.v;
+    } else {
+      return *(const s8*)(l + lds_at(32 * j + (lane & 31), 2 * s + (lane >> 5)));
+    }
+  }
+};
+
+typedef float f16v __attribute__((ext_vector_type(16)));
+template <typename T>
+__device__ __forceinline__ f16v mfma32(s8 a, s8 b, f16v c) {
+  typedef __bf16 b8 __attribute__((ext_vector_type(8)));
+  typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+  if constexpr (std::is_same<T, _Float16>::value)
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
+}
+
 template <typename T>
 __device__ __forceinline__ f4 mfma(s8 a, s8 b, f4 c) {
   typedef __bf16 b8 __attribute__((ext_vector_type(8)));
@@ -350,10 +489,11 @@ __device__ float sum_again(const Work<T>& w, int i, int j) {
 }
 
 template <typename T, bool AT, bool BT, int WM, int WN, int FM, int FN, bool FAST, typename Store>
-__device__ __forceinline__ void product(const Work<T>& w, unsigned short* lds, Store&& put) {
+__device__ __forceinline__ void product(const Work<T>& w, Store&& put) {
   constexpr int TM = 16 * WM * FM, TN = 16 * WN * FN, BK = Plane<T>::BK;
   typedef Tile<T, TM, AT> TA;
   typedef Tile<T, TN, BT> TB;
+  __shared__ __attribute__((aligned(16))) unsigned short lds[TA::ELEMS + TB::ELEMS];
   static_assert(WM * WN * 64 == WG, "four wavefronts");
   const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6, fr = lane & 15, fg = lane >> 4;
   const int i0 = wave / WN * FM, j0 = wave % WN * FN;
@@ -414,22 +554,227 @@ __device__ __forceinline__ void product(const Work<T>& w, unsigned short* lds, S
   }
 }
 
+// ------------------------------------------------- loads straight into LDS ----
+// One operand's steps by loads that write LDS themselves (16 bytes a lane, a
+// wavefront's 1,024 in a row): the permutation of LDS rows is made by the lanes'
+// addresses, which repeat after a few loads but for whole lines.  Offsets past
+// the descriptor's range read zeros: lines behind the tile's rows or the summed
+// index's end cost no branch.
+template <typename T, int TM, bool ACROSS, int WAVES>
+struct Stream {
+  typedef WideTile<T, TM, ACROSS> L;
+  static constexpr int BK = L::BK, LINE = (ACROSS ? TM : BK) * 2, LOADS = TM * BK * 2 / 1024;
+  static constexpr int COUNT = (LOADS + WAVES - 1) / WAVES;   // a wavefront's
+  static constexpr int LINES = 1024 / LINE;                   // a load's
+  static constexpr bool EVEN = LOADS % WAVES == 0;
+  static constexpr unsigned NONE = 0x80000000u;
+  // lines that differ by a multiple of 16 are permuted alike
+  static constexpr int KINDS = COUNT < 16 / LINES ? COUNT : 16 / LINES;
+  static_assert(sizeof(T) == 2 && TM * BK * 2 % 1024 == 0 && LINES >= 1 && LINES <= 16, "whole loads");
+
+  const T* p;
+  unsigned ld, range;    // bytes of a line, and up to the end of the last one with values
+  int first;             // this wavefront's first load
+  unsigned at[KINDS];    // this lane's offsets, in bytes,
+  int k[KINDS];          // and places on the summed index (not ACROSS)
+
+  __device__ __forceinline__ Stream() : first(__builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6) * COUNT) {}
+  __device__ __forceinline__ void set(const T* from0, int64_t elems, int outs) {
+    p = from0;
+    ld = (unsigned)elems * 2;
+    range = (unsigned)outs * ld;
+#pragma unroll
+    for (int j = 0; j < KINDS; ++j) {
+      int line, from;
+      place(j, (int)threadIdx.x & 63, &line, &from);
+      k[j] = from;
+      at[j] = !ACROSS || from < outs ? (unsigned)line * ld + (unsigned)from * 2 : NONE;
+    }
+  }
+
+  // the line and the first of the eight elements that this lane's j-th load brings
+  __device__ __forceinline__ void place(int j, int lane, int* line, int* from) const {
+    const int pos = (first + j) * 1024 + lane * 16;
+    *line = pos / LINE;
+    *from = L::lds_at(*line, pos % LINE / 16) - *line * (LINE / 2);   // (the permutation is its own inverse)
+  }
+
+  // the step at p, of which n of the summed index are left, into lds; then the next
+  __device__ __forceinline__ void issue(unsigned short* lds, int n) {
+    const unsigned most = ACROSS ? (n <= 0 ? 0u : min((unsigned)n, (unsigned)BK) * ld) : range;
+    // (the same in every lane, which the compiler loses sight of)
+    const uintptr_t u = (uintptr_t)p;
+    const uintptr_t q = (uintptr_t)(unsigned)__builtin_amdgcn_readfirstlane((int)(u >> 32)) << 32 |
+                        (unsigned)__builtin_amdgcn_readfirstlane((int)u);
+    const auto rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)q, (short)0, __builtin_amdgcn_readfirstlane((int)most),
+                                                        0x00027000);
+    const unsigned line_bytes = (unsigned)__builtin_amdgcn_readfirstlane((int)ld);
+    auto load = [&](int j, unsigned o) {
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(
+          rsrc, (__attribute__((address_space(3))) void*)(lds + (first + j) * 512), 16, (int)o, 0, 0, 0);
+    };
+#pragma unroll
+    for (int j = 0; j < COUNT; ++j) {
+      if (!EVEN && first + j >= LOADS) break;
+      const unsigned o = at[j % KINDS] + (unsigned)(j / KINDS * KINDS * LINES) * line_bytes;
+      load(j, ACROSS || k[j % KINDS] < n ? o : NONE);   // (n may be negative: a step of zeros)
+    }
+    p += ACROSS ? (int64_t)(ld / 2) * BK : BK;
+    if (!ACROSS) range -= min(range, (unsigned)(BK * 2));
+  }
+};
+
+// waits until at most LOADS of this wavefront's loads are in flight and (READS)
+// none of its LDS reads, then for the other wavefronts.  (The builtin's counts
+// are the compiler's too: it adds no waits of its own.)
+template <int LOADS, bool READS>
+__device__ __forceinline__ void arrive() {
+  __builtin_amdgcn_s_waitcnt((LOADS & 15) | (LOADS >> 4) << 14 | (READS ? 0x0070 : 0x0f70));
+  asm volatile("s_barrier" ::: "memory");
+}
+
+// the fragments of 32 of the summed index, of a wavefront's FM x FN blocks of 32
+template <typename TA, typename TB, int FM, int FN>
+struct Fragments {
+  s8 a[2][FM], b[2][FN];
+  __device__ __forceinline__ void read(const unsigned short* l, int half, int i0, int j0, int lane) {
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+#pragma unroll
+      for (int i = 0; i < FM; ++i) a[s][i] = TA::fragment(l, i0 + i, 2 * half + s, lane);
+#pragma unroll
+      for (int j = 0; j < FN; ++j) b[s][j] = TB::fragment(l + TA::ELEMS, j0 + j, 2 * half + s, lane);
+    }
+    __builtin_amdgcn_sched_barrier(0);   // (these go out before what follows)
+  }
+  template <typename T>
+  __device__ __forceinline__ void multiply(f16v (&acc)[FM][FN]) const {
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int i = 0; i < FM; ++i)
+#pragma unroll
+        for (int j = 0; j < FN; ++j) acc[i][j] = mfma32<T>(b[s][j], a[s][i], acc[i][j]);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+};
+
+// Products of 16-bit elements, sizes multiples of eight and rows aligned: a
+// wavefront's list of tiles (the lanes in `mask`) as one stream of steps, so a
+// tile's first loads fly while the one before is multiplied and stored.
+//
+// Two buffers of 64 of the summed index.  Either half's fragments are read while
+// the other half is multiplied; the barrier is between the halves of a step, when
+// its second half is in registers: the buffer then takes the step after the
+// next, whose loads fly for a whole step.  Tiles take an even number of steps
+// (the last may be zeros that no load brings), so a step's buffer is known to
+// the compiler, as it must be for it to wait for no load in flight.
+template <typename T, bool AT, bool BT, int WM, int WN, int FM, int FN, typename Store>
+__device__ __forceinline__ void stream_products(const T* __restrict__ a_base, const T* __restrict__ b_base, int64_t lda,
+                                                int64_t ldb, const Job& jobs, unsigned long long mask, Store& store) {
+  constexpr int TM = 32 * WM * FM, TN = 32 * WN * FN, BK = 64;
+  typedef WideTile<T, TM, AT> TA;
+  typedef WideTile<T, TN, BT> TB;
+  typedef Stream<T, TM, AT, WM * WN> SA;
+  typedef Stream<T, TN, BT, WM * WN> SB;
+  constexpr int NEXT = SA::EVEN && SB::EVEN ? SA::COUNT + SB::COUNT : 0;   // a step's loads of every wavefront
+  // (arrays of their own: the compiler then knows which loads a read waits for)
+  __shared__ __attribute__((aligned(16))) unsigned short even[TA::ELEMS + TB::ELEMS], odd[TA::ELEMS + TB::ELEMS];
+  const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
+  const int i0 = wave / WN * FM, j0 = wave % WN * FN;
+
+  unsigned long long ahead = mask;   // tiles whose steps are not loaded yet
+  int left = 0;                      // of the summed index of the one that is, from the next step on
+  SA a;
+  SB b;
+  auto turn = [&]() {
+    const int l = __ffsll((long long)ahead) - 1;
+    ahead &= ahead - 1;
+    a.set(a_base + Job::of(jobs.a, l), lda, Job::of(jobs.m, l));
+    b.set(b_base + Job::of(jobs.b, l), ldb, Job::of(jobs.n, l));
+    left = Job::of(jobs.sum, l);
+  };
+  auto load = [&](unsigned short* to) {
+    a.issue(to, left);
+    b.issue(to + TA::ELEMS, left);
+    left -= BK;
+  };
+  turn();
+  load(even);
+  load(odd);
+  arrive<NEXT, false>();
+  Fragments<TA, TB, FM, FN> f, g;
+  f.read(even, 0, i0, j0, lane);
+  g.read(even, 1, i0, j0, lane);
+  bool more = true;
+  f16v acc[FM][FN];
+  auto clear = [&]() {
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+      for (int j = 0; j < FN; ++j) acc[i][j] = f16v{};
+  };
+  clear();
+  int l = __ffsll((long long)mask) - 1;
+  f.template multiply<T>(acc);
+  // Loops begin where all loads have to be there, in the middle of an even step (at
+  // a loop's head the compiler no longer knows which are for the other buffer).
+  auto pair = [&](auto stores) {
+    arrive<0, true>();
+    if (left <= 0) {
+      more = ahead != 0;
+      if (more) turn();
+    }
+    if (more) load(even);
+    if constexpr (decltype(stores)::value) store.later(0);
+    f.read(odd, 0, i0, j0, lane);
+    g.template multiply<T>(acc);
+    g.read(odd, 1, i0, j0, lane);
+    f.template multiply<T>(acc);
+    arrive<0, true>();
+    if (more) load(odd);
+    if constexpr (decltype(stores)::value) store.later(1);
+    f.read(even, 0, i0, j0, lane);   // (the next tile's, if there is one)
+    g.template multiply<T>(acc);
+  };
+  for (;;) {
+    pair(std::true_type());
+    for (int n = Job::of(jobs.sum, l) - 2 * BK; n > 0; n -= 2 * BK) {
+      g.read(even, 1, i0, j0, lane);
+      f.template multiply<T>(acc);
+      pair(std::false_type());
+    }
+    store.tile(jobs.lane(l), acc, lane, i0, j0);
+    mask &= mask - 1;
+    if (mask == 0) break;
+    l = __ffsll((long long)mask) - 1;
+    clear();
+    g.read(even, 1, i0, j0, lane);
+    f.template multiply<T>(acc);
+  }
+  store.later(0);
+  store.later(1);
+}
+
 // stores of a tile's four consecutive columns
 template <typename O>
 struct Put {
   O* out;   // the tile's first element
   int64_t ldo;
   int m, n;
-  float scale;
+  row_sum_t<O> scale;
   bool fours;   // rows of a multiple of four, aligned
   const float *row_scale, *col_scale;   // of the tile's rows (by `rows` where given) and columns, or null
   const int* rows;
   __device__ __forceinline__ void one(int i, int j, float v) const {
     out[i * ldo + j] = (O)(v * scale);
   }
+  __device__ __forceinline__ void operator()(int i, int j, double v) const {
+    if (i < m && j < n) out[i * ldo + j] = (O)(v * scale);
+  }
   __device__ __forceinline__ void operator()(int i, int j, f4 v) const {
     if (i >= m || j >= n) return;
-    float s = scale;
+    float s = (float)scale;
     if (row_scale) s *= row_scale[rows ? rows[i] : i];
     O* p = out + i * ldo + j;
     if (fours) {
@@ -446,121 +791,113 @@ struct Put {
   }
 };
 
+// the output, or float32 sums
+template <typename T>
+struct PutPart {
+  Put<T> out;
+  Put<row_sum_t<T>> part;
+  bool whole;
+  __device__ __forceinline__ void one(int i, int j, float v) const {
+    if (whole) out.one(i, j, v);
+    else part.one(i, j, v);
+  }
+  template <typename V>
+  __device__ __forceinline__ void operator()(int i, int j, V v) const {
+    if (whole) out(i, j, v);
+    else part(i, j, v);
+  }
+};
+
+// A tile's results rounded and kept, and stored half by half beside the next
+// tile's loads: a step waits for both together (vmcnt counts stores too), where
+// stores at a tile's end were waited for by themselves.  A wavefront's blocks pass
+// through 2 or 4 KB of its own in LDS before, so that a store writes whole rows of
+// its blocks (128 bytes) and not 16 bytes of each of 32 rows.  (A lane holds row
+// lane % 32 and columns 8 q + 4 (lane / 32) .. + 3 of a block of 32.)
+template <typename T, int WAVES, int FM, int FN, typename Make>
+struct Results {
+  // pieces (PutPart) have too many registers in use for that, and long sums between them
+  static constexpr bool LATE = std::is_same<std::decay_t<std::invoke_result_t<Make, const Job&>>, Put<T>>::value;
+  static constexpr int SLOTS = 8 * FN, READS = SLOTS / 4;   // 8-byte slots of a row; 16-byte reads a lane for 32 rows
+  typedef T t4 __attribute__((ext_vector_type(4)));
+  typedef unsigned u2 __attribute__((ext_vector_type(2)));
+  Make make;
+  u4 lined[FM][READS];
+  T* at;            // this lane's first element
+  int64_t ld;
+  int rows, cols;   // that are there, from it on
+  bool any = false;
+
+  __device__ __forceinline__ explicit Results(Make make) : make(make) {}
+  __device__ __forceinline__ void tile(const Job& j, const f16v (&acc)[FM][FN], int lane, int i0, int j0) {
+    const auto to = make(j);
+    if constexpr (LATE) {
+      rows_of(to, acc, lane, i0, j0);
+    } else if (to.whole) {
+      rows_of(to.out, acc, lane, i0, j0);
+      half(0);
+      half(1);
+    } else {
+#pragma unroll
+      for (int i = 0; i < FM; ++i)
+#pragma unroll
+        for (int k = 0; k < FN; ++k)
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            to.part(32 * (i0 + i) + (lane & 31), 32 * (j0 + k) + 8 * q + 4 * (lane >> 5),
+                    f4{acc[i][k][4 * q], acc[i][k][4 * q + 1], acc[i][k][4 * q + 2], acc[i][k][4 * q + 3]});
+    }
+  }
+  __device__ __forceinline__ void rows_of(const Put<T>& put, const f16v (&acc)[FM][FN], int lane, int i0, int j0) {
+    __shared__ __attribute__((aligned(16))) u2 stage[WAVES][32 * SLOTS];
+    u2* w = stage[(int)threadIdx.x >> 6];
+#pragma unroll
+    for (int i = 0; i < FM; ++i) {
+      // slots of a row in another order by row: two lanes to a bank in writing, one in reading
+      const int row = lane & 31;
+#pragma unroll
+      for (int k = 0; k < FN; ++k)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          t4 v;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) v[r] = (T)(acc[i][k][4 * q + r] * put.scale);
+          w[row * SLOTS + ((8 * k + 2 * q + (lane >> 5)) ^ (row & (SLOTS - 1)))] = __builtin_bit_cast(u2, v);
+        }
+#pragma unroll
+      for (int n = 0; n < READS; ++n) {
+        const int u = lane + 64 * n, r = u / (SLOTS / 2), c = (u % (SLOTS / 2)) ^ ((r & (SLOTS - 1)) >> 1);
+        const u4 v = *(const u4*)(w + r * SLOTS + 2 * c);
+        lined[i][n] = r & 1 ? u4{v[2], v[3], v[0], v[1]} : v;
+      }
+    }
+    const int row = 32 * i0 + lane / (SLOTS / 2), col = 32 * j0 + lane % (SLOTS / 2) * 8;
+    at = put.out + row * put.ldo + col;
+    ld = put.ldo;
+    rows = put.m - row;
+    cols = put.n - col;
+    any = true;
+  }
+  __device__ __forceinline__ void later(int which) {
+    if (!LATE || !any) return;
+    half(which);
+    if (which) any = false;
+  }
+  __device__ __forceinline__ void half(int which) {
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+      for (int n = 0; n < READS; ++n) {
+        if ((i * READS + n) / ((FM * READS + 1) / 2) != which) continue;
+        const int row = 32 * i + n * (128 / SLOTS);
+        if (row < rows && cols > 0) *(u4*)(at + row * ld) = lined[i][n];   // (eight columns are all there or none)
+      }
+  }
+};
+
 template <typename O>
 __device__ __forceinline__ void zero_rows(O* out, int64_t ldo, int m, int n) {
-  for (int u = (int)threadIdx.x; u < m * n; u += WG) out[(u / n) * ldo + u % n] = (O)0.0f;
-}
-
-// Y = s X W (BT) or dX = s G W^T: a group's rows by all columns
-template <typename T, bool BT, int WM, int WN, int FM, int FN, bool FAST>
-__global__ __launch_bounds__(WG) void k_expert_rows(const T* __restrict__ x, const T* __restrict__ weight, Groups gr,
-                                                    int64_t wsize, int sum, int n, float scale, T* __restrict__ out,
-                                                    int tiles, int cols) {
-  constexpr int TM = 16 * WM * FM, TN = 16 * WN * FN;
-  __shared__ __attribute__((aligned(16))) unsigned short lds[Tile<T, TM, false>::ELEMS + Tile<T, TN, BT>::ELEMS];
-  const int t = tile_of(tiles);
-  if (t < 0) return;
-  const Place p = place_of(gr, t / cols, __builtin_ctz(TM));
-  if (p.count <= 0) return;
-  const int c0 = t % cols * TN, m = (int)min(p.count, (int64_t)TM), nn = n - c0;
-  T* o = out + p.first * n + c0;
-  if (p.expert >= gr.experts) {
-    zero_rows(o, n, m, min(nn, TN));
-    return;
-  }
-  const T* wt = weight + ((int64_t)p.expert * gr.blocks + p.block) * wsize;
-  const Work<T> w{x + p.first * sum, wt + (BT ? (int64_t)c0 : (int64_t)c0 * sum), sum, BT ? n : sum, sum, m, nn, nullptr};
-  product<T, false, BT, WM, WN, FM, FN, FAST>(w, lds, Put<T>{o, n, m, nn, scale, FAST, nullptr, nullptr, nullptr});
-}
-
-// dW: up to 2^shift rows of a group, by tiles of [K, N].  A group of one such
-// part goes to dw itself, others as float32 sums to part [slots, K N].
-template <typename T, int WM, int WN, int FM, int FN, bool FAST>
-__global__ __launch_bounds__(WG) void k_expert_weights(const T* __restrict__ x, const T* __restrict__ g, Groups gr,
-                                                       int shift, int K, int N, float scale, T* __restrict__ dw,
-                                                       float* __restrict__ part, int tiles, int per, int cols) {
-  constexpr int TM = 16 * WM * FM, TN = 16 * WN * FN;
-  __shared__ __attribute__((aligned(16))) unsigned short lds[Tile<T, TM, true>::ELEMS + Tile<T, TN, true>::ELEMS];
-  const int t = tile_of(tiles);
-  if (t < 0) return;
-  const int slot = t / per, tile = t - slot * per, r0 = tile / cols * TM, c0 = tile % cols * TN;
-  const Place p = place_of(gr, slot, shift);
-  if (p.expert >= gr.experts || (p.part > 0 && p.count <= 0)) return;
-  const int64_t n = min(max(p.count, (int64_t)0), (int64_t)1 << shift);
-  const Work<T> w{x + p.first * K + r0, g + p.first * N + c0, K, N, n, K - r0, N - c0, nullptr};
-  const int64_t at = (int64_t)r0 * N + c0, size = (int64_t)K * N;
-  if (p.part == 0 && p.count <= n) {
-    T* o = dw + ((int64_t)p.expert * gr.blocks + p.block) * size + at;
-    product<T, true, true, WM, WN, FM, FN, FAST>(w, lds, Put<T>{o, N, K - r0, N - c0, scale, FAST, nullptr, nullptr, nullptr});
-  } else {
-    product<T, true, true, WM, WN, FM, FN, FAST>(
-        w, lds, Put<float>{part + slot * size + at, N, K - r0, N - c0, 1.0f, FAST, nullptr, nullptr, nullptr});
-  }
-}
-
-// dW of the groups of several parts: their sums in order
-template <typename T>
-__global__ __launch_bounds__(WG) void k_expert_join(const float* __restrict__ part, Groups gr, int shift, int64_t size,
-                                                    float scale, T* __restrict__ dw) {
-  const int b = (int)blockIdx.y / gr.experts, e = (int)blockIdx.y - b * gr.experts;
-  const int64_t base = gr.rows * gr.before[b], first = base + gr.comps[b] * gr.end_of(e);
-  const int64_t n = base + gr.comps[b] * gr.end_of(e + 1) - first;
-  const int parts = (int)((n + ((int64_t)1 << shift) - 1) >> shift);
-  if (parts <= 1) return;
-  const int64_t slot = (first >> shift) + b * (gr.experts + 1) + e;
-  const float* p = part + slot * size;
-  T* o = dw + ((int64_t)e * gr.blocks + b) * size;
-  if ((size & 3) == 0 && ((uintptr_t)dw & 15) == 0) {
-    const int64_t i = 4 * ((int64_t)blockIdx.x * WG + threadIdx.x);
-    if (i >= size) return;
-    f4 sum = *(const f4*)(p + i);
-    for (int q = 1; q < parts; ++q) sum += *(const f4*)(p + q * size + i);
-    typedef T o4 __attribute__((ext_vector_type(4)));
-    o4 v;
-#pragma unroll
-    for (int r = 0; r < 4; ++r) v[r] = (T)(sum[r] * scale);
-    *(o4*)(o + i) = v;
-  } else {
-    for (int64_t i = 4 * ((int64_t)blockIdx.x * WG) + threadIdx.x; i < min(size, 4 * ((int64_t)blockIdx.x + 1) * WG); i += WG) {
-      float sum = p[i];
-      for (int q = 1; q < parts; ++q) sum += p[q * size + i];
-      o[i] = (T)(sum * scale);
-    }
-  }
-}
-
-// Y = s_row s_col (codes of X) (codes of W [E, N, K])^T, rows gathered where order is given
-template <typename O, int WM, int WN, int FM, int FN>
-__global__ __launch_bounds__(WG) void k_expert_codes(const E4m3* __restrict__ x, const float* __restrict__ xs,
-                                                     const int* __restrict__ order, unsigned choices, int tokens,
-                                                     const E4m3* __restrict__ weight, const float* __restrict__ ws,
-                                                     Groups gr, int pairs, int n, O* __restrict__ out, int tiles, int cols) {
-  constexpr int TM = 16 * WM * FM, TN = 16 * WN * FN;
-  __shared__ __attribute__((aligned(16))) unsigned short lds[Tile<E4m3, TM, false>::ELEMS + Tile<E4m3, TN, false>::ELEMS];
-  __shared__ int rows[TM];
-  const int t = tile_of(tiles);
-  if (t < 0) return;
-  const Place p = place_of(gr, t / cols, __builtin_ctz(TM));
-  if (p.count <= 0) return;
-  const int c0 = t % cols * TN, m = (int)min(p.count, (int64_t)TM), nn = n - c0;
-  O* o = out + p.first * n + c0;
-  if (p.expert >= gr.experts) {
-    zero_rows(o, n, m, min(nn, TN));
-    return;
-  }
-  if (order) {   // (a slot outside the tokens is taken for the last)
-    for (int i = (int)threadIdx.x; i < TM; i += WG) {
-      const unsigned slot = (unsigned)order[p.first + min(i, m - 1)];
-      rows[i] = (int)min(min(slot, (unsigned)gr.rows - 1) / choices, (unsigned)tokens - 1);
-    }
-    __syncthreads();
-  }
-  const E4m3* wt = weight + (int64_t)p.expert * n * pairs;
-  const Work<E4m3> w{order ? x : x + p.first * pairs, wt + (int64_t)c0 * pairs, pairs, pairs, pairs, m, nn,
-                     order ? rows : nullptr};
-  product<E4m3, false, false, WM, WN, FM, FN, true>(
-      w, lds, Put<O>{o, n, m, nn, 1.0f, (n & 3) == 0 && ((uintptr_t)out & 15) == 0, order ? xs : xs + p.first,
-                     ws + (int64_t)p.expert * n + c0, order ? rows : nullptr});
+  for (int u = (int)threadIdx.x; u < m * n; u += (int)blockDim.x) out[(u / n) * ldo + u % n] = (O)0.0f;
 }
 
 // ----------------------------------------------------------------- float64 ----
@@ -598,7 +935,8 @@ struct TileD {
 };
 
 template <bool AT, bool BT, typename Store>
-__device__ __forceinline__ void product_f64(const Work<double>& w, double* lds, Store&& put) {
+__device__ __forceinline__ void product_f64(const Work<double>& w, Store&& put) {
+  __shared__ double lds[2 * DK * DS];
   const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6, fr = lane & 15, fg = lane >> 4;
   const int i0 = (wave >> 1) * 32, j0 = (wave & 1) * 32;
   double *la = lds, *lb = lds + DK * DS;
@@ -644,63 +982,267 @@ __device__ __forceinline__ void product_f64(const Work<double>& w, double* lds, 
       for (int r = 0; r < 4; ++r) put(i0 + 16 * i + fr, j0 + 16 * j + fg + 4 * r, acc[i][j][r]);
 }
 
-template <bool BT>
-__global__ __launch_bounds__(WG) void k_expert_rows_f64(const double* __restrict__ x, const double* __restrict__ weight,
-                                                        Groups gr, int64_t wsize, int sum, int n, double scale,
-                                                        double* __restrict__ out, int tiles, int cols) {
-  __shared__ double lds[2 * DK * DS];
+template <typename T, bool FAST>
+constexpr bool STREAMS = FAST && sizeof(T) == 2;
+
+// waves a SIMD for a wavefront's tile of that many fragments
+constexpr int waves_for(int fragments) { return fragments > 32 ? 1 : fragments > 4 ? 2 : 4; }
+
+// Walks over a workgroup's tiles: make(t) gives each lane's, zero(job) fills one,
+// put(job) stores a tile's results.
+template <typename T, bool AT, bool BT, int WM, int WN, int FM, int FN, bool FAST, typename Make, typename Zero, typename Store>
+__device__ __forceinline__ void walk(const T* __restrict__ a, const T* __restrict__ b, int64_t lda, int64_t ldb, Share sh,
+                                     Make&& make, Zero&& zero, Store&& put) {
+  for (int t0 = sh.first; t0 < sh.end; t0 += 64 * sh.step) {
+    asm volatile("" : : : "memory");   // (what make() reads is read again)
+    const int t = t0 + ((int)threadIdx.x & 63) * sh.step;
+    Job jobs = make(min(t, sh.end - 1));
+    if (t >= sh.end) jobs.kind = NO_TILE;
+    for (unsigned long long z = __ballot(jobs.kind == ZERO_TILE); z; z &= z - 1) zero(jobs.lane(__ffsll((long long)z) - 1));
+    unsigned long long mask = __ballot(jobs.kind == PRODUCT);
+    if (mask == 0) continue;
+    if constexpr (STREAMS<T, FAST>) {
+      Results<T, WM * WN, FM / 2, FN / 2, std::decay_t<Store>> store{put};
+      stream_products<T, AT, BT, WM, WN, FM / 2, FN / 2>(a, b, lda, ldb, jobs, mask, store);
+      if (t0 + 64 * sh.step < sh.end) __syncthreads();
+    } else {
+      for (; mask; mask &= mask - 1) {
+        const Job j = jobs.lane(__ffsll((long long)mask) - 1);
+        const Work<T> w{a + j.a, b + j.b, lda, ldb, j.sum, j.m, j.n, nullptr};
+        if constexpr (std::is_same<T, double>::value) product_f64<AT, BT>(w, put(j));
+        else product<T, AT, BT, WM, WN, FM, FN, FAST>(w, put(j));
+      }
+    }
+  }
+}
+
+// Y = s X W (BT) or dX = s G W^T: tiles of TM rows by TN columns
+template <typename T, bool BT, int WM, int WN, int FM, int FN, bool FAST>
+__global__ __launch_bounds__(64 * WM * WN, waves_for(FM * FN)) void k_expert_rows(
+    const T* __restrict__ x, const T* __restrict__ weight, Groups gr, int64_t wsize, int sum, int n, row_sum_t<T> scale,
+    T* __restrict__ out, int cols, bool apart) {
+  constexpr int TM = 16 * WM * FM, TN = 16 * WN * FN;
+  const int slots = Places<true, false>(gr, __builtin_ctz(TM)).total();
+  walk<T, false, BT, WM, WN, FM, FN, FAST>(
+      x, weight, sum, BT ? n : sum, share_of(slots * cols, apart),
+      [&](int t) {   // (asked for again for every 64 tiles: nothing of it stays in registers)
+        int slot, col;
+        if (apart) slot = t / cols, col = t % cols;
+        else blocked(t, slots, cols, &slot, &col);
+        const Place p = Places<true, false>(gr, __builtin_ctz(TM)).find(slot);
+        const int c0 = col * TN;
+        return Job{p.first * sum,
+                   ((int64_t)p.expert * gr.blocks + p.block) * wsize + (BT ? (int64_t)c0 : (int64_t)c0 * sum),
+                   p.first * n + c0, sum, (int)min(p.count, (int64_t)TM), min(n - c0, TN),
+                   p.count <= 0 ? NO_TILE : p.expert < gr.experts ? PRODUCT : ZERO_TILE, 1};
+      },
+      [&](const Job& j) { zero_rows(out + j.out, n, j.m, j.n); },
+      [&](const Job& j) { return Put<T>{out + j.out, n, j.m, j.n, scale, FAST, nullptr, nullptr, nullptr}; });
+}
+
+// dW: the groups' rows as one line of units of 128 (a group without rows is one
+// unit, of zeros), cut into `cuts` equal stretches.  A stretch's groups' tiles of
+// [K, N] are shared by `team` workgroups, which then read the same rows at the same
+// time and have equal work, however the rows are spread over the groups.  (Equal
+// lengths of a line of all tiles' units cost up to a third more: workgroups side
+// by side were at different rows, and the L2 held none of them twice.)  A group
+// within one stretch goes to dw itself; pieces of others go as float32 sums to
+// part [2 cuts, tiles], first groups of a stretch before last ones, and are added
+// up in order.
+struct Units {
+  const Groups& gr;
+  int n;               // groups
+  int64_t from, to;    // this lane's group's rows
+  int64_t upto;        // units of the lanes' groups up to this one
+
+  __device__ __forceinline__ explicit Units(const Groups& gr) : gr(gr), n(gr.experts * gr.blocks) { take(0); }
+  __device__ __forceinline__ static int64_t units(int64_t rows) { return rows > 0 ? (rows + 127) >> 7 : 1; }
+  __device__ __forceinline__ void take(int at) {
+    const int lane = (int)threadIdx.x & 63, g = at + lane;
+    from = to = upto = 0;
+    if (g < n) {
+      const int b = g / gr.experts, e = g - b * gr.experts;
+      from = gr.rows * gr.before[b] + gr.comps[b] * gr.end_of(e);
+      to = gr.rows * gr.before[b] + gr.comps[b] * gr.end_of(e + 1);
+      upto = units(to - from);
+    }
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int64_t v = __shfl_up((long long)upto, o, 64);
+      if (lane >= o) upto += v;
+    }
+  }
+  __device__ __forceinline__ int64_t last() const { return Job::of(upto, 63); }
+  __device__ __forceinline__ int64_t total() {
+    if (n <= 64) return last();
+    int64_t sum = 0;
+    for (int at = 0; at < n; at += 64) {
+      take(at);
+      sum += last();
+    }
+    return sum;
+  }
+  // the group of a unit below the total, the same in all lanes
+  __device__ __forceinline__ int group_of(int64_t unit) {
+    int64_t before = 0;
+    for (int at = 0; at < n; at += 64) {
+      if (n > 64) take(at);
+      if (unit < before + last()) return at + __popcll(__ballot(before + upto <= unit));
+      before += last();
+    }
+    return n - 1;
+  }
+  // each lane's own group (every lane of the wavefront calls it)
+  struct Span {
+    int64_t first, count;   // units
+    int64_t row, rows;
+  };
+  __device__ __forceinline__ Span span(int g) {
+    Span s{0, 1, 0, 0};
+    int64_t before = 0;
+    for (int at = 0; at < n; at += 64) {
+      if (n > 64) take(at);
+      const int l = min(max(g - at, 0), 63);
+      const int64_t f = __shfl((long long)from, l, 64), t = __shfl((long long)to, l, 64);
+      const int64_t prior = __shfl((long long)upto, max(l - 1, 0), 64);
+      if (g >= at && g - at < 64) s = Span{before + (l ? prior : 0), units(t - f), f, t > f ? t - f : 0};
+      before += last();
+    }
+    return s;
+  }
+};
+
+// (a unit at least in each)
+__device__ __forceinline__ int stretches(int64_t units, int cuts) { return (int)min(units, (int64_t)cuts); }
+// the first unit of stretch i of n
+__device__ __forceinline__ int64_t cut_of(int64_t units, int i, int n) { return units / n * i + units % n * i / n; }
+
+template <typename T, int WM, int WN, int FM, int FN, bool FAST>
+__global__ __launch_bounds__(64 * WM * WN, waves_for(FM * FN)) void k_expert_weights(
+    const T* __restrict__ x, const T* __restrict__ g, Groups gr, int K, int N, row_sum_t<T> scale, T* __restrict__ dw,
+    row_sum_t<T>* __restrict__ part, int per, int cols, int cuts, int team) {
+  constexpr int TM = 16 * WM * FM, TN = 16 * WN * FN;
+  const int64_t size = (int64_t)K * N;
+  // (an XCD's workgroups beside each other)
+  const int line = (int)(blockIdx.x & 7) * (int)(gridDim.x >> 3) + (int)(blockIdx.x >> 3);
+  const int cut = line / team, mate = line - cut * team, rounds = (per - mate + team - 1) / team;
+  if (rounds <= 0) return;
+  int64_t u0, u1;
+  int g0, groups;
+  {
+    Units units(gr);
+    const int64_t total = units.total();
+    const int n = stretches(total, cuts);
+    if (cut >= n) return;
+    u0 = cut_of(total, cut, n);
+    u1 = cut_of(total, cut + 1, n);
+    g0 = units.group_of(u0);
+    groups = units.group_of(u1 - 1) - g0 + 1;
+  }
+  walk<T, true, true, WM, WN, FM, FN, FAST>(
+      x, g, K, N, Share{0, groups * rounds, 1},
+      [&](int t) {
+        const int of = t / rounds, tile = mate + (t - of * rounds) * team, grp = g0 + of;
+        const Units::Span s = Units(gr).span(grp);
+        int row, col;
+        blocked(tile, per / cols, cols, &row, &col);
+        const int r0 = row * TM, c0 = col * TN, b = grp / gr.experts, e = grp - b * gr.experts;
+        const int64_t a = max(u0 - s.first, (int64_t)0), z = min(u1 - s.first, s.count);   // of the group's units
+        const int64_t first = s.row + (a << 7), rows = min(z << 7, s.rows) - (a << 7);
+        const bool whole = a == 0 && z == s.count;
+        return Job{first * K + r0, first * N + c0,
+                   whole ? ((int64_t)e * gr.blocks + b) * size + (int64_t)r0 * N + c0
+                         : ((int64_t)(2 * cut + (of ? 1 : 0)) * per + tile) * TM * TN,
+                   (int)rows, min(K - r0, TM), min(N - c0, TN), rows > 0 ? PRODUCT : ZERO_TILE, whole};
+      },
+      [&](const Job& j) { zero_rows(dw + j.out, N, j.m, j.n); },
+      [&](const Job& j) {
+        return PutPart<T>{{dw + j.out, N, j.m, j.n, scale, FAST, nullptr, nullptr, nullptr},
+                          {part + j.out, TN, j.m, j.n, 1, true, nullptr, nullptr, nullptr}, j.whole != 0};
+      });
+}
+
+// dW of the groups of several stretches: their pieces' sums in order
+template <typename T, int TM, int TN>
+__global__ __launch_bounds__(WG) void k_expert_join(const row_sum_t<T>* __restrict__ part, Groups gr, int K, int N,
+                                                    row_sum_t<T> scale, T* __restrict__ dw, int per, int cols, int cuts) {
+  typedef row_sum_t<T> s4v __attribute__((ext_vector_type(4)));
+  const int64_t tile = blockIdx.x >> 3;
+  const int grp = (int)(tile / per), place = (int)(tile - (int64_t)grp * per);
+  Units units(gr);
+  const int64_t total = units.total();
+  const Units::Span s = units.span(grp);
+  cuts = stretches(total, cuts);
+  // the stretch of a unit
+  auto cut_with = [&](int64_t unit) {
+    int i = (int)((float)unit / (float)total * cuts);
+    i = min(max(i, 0), cuts - 1);
+    while (i > 0 && cut_of(total, i, cuts) > unit) --i;
+    while (i + 1 < cuts && cut_of(total, i + 1, cuts) <= unit) ++i;
+    return i;
+  };
+  const int i0 = cut_with(s.first), i1 = cut_with(s.first + s.count - 1);
+  if (i0 == i1) return;
+  int row, col;
+  blocked(place, per / cols, cols, &row, &col);
+  const int r0 = row * TM, c0 = col * TN, b = grp / gr.experts, e = grp - b * gr.experts;
+  T* o = dw + ((int64_t)e * gr.blocks + b) * K * N + (int64_t)r0 * N + c0;
+  const int64_t step = (int64_t)2 * per * TM * TN;
+  // (the first stretch's piece is of its last group, if it has more)
+  const int64_t lead = cut_of(total, i0, cuts) < s.first ? step / 2 : 0;
+  constexpr int SHARE = TM * TN / 8;
+  for (int q = 4 * (int)threadIdx.x; q < SHARE; q += 4 * WG) {
+    const int at = (int)(blockIdx.x & 7) * SHARE + q, i = at / TN, j = at % TN;
+    if (r0 + i >= K || c0 + j >= N) continue;
+    const row_sum_t<T>* p = part + (int64_t)place * TM * TN + at + i0 * step;
+    s4v sum = *(const s4v*)(p + lead);
+    int k = 1;
+    const int count = i1 - i0 + 1;
+    for (; k + 8 <= count; k += 8) {   // (their loads go out together)
+      s4v v[8];
+#pragma unroll
+      for (int m = 0; m < 8; ++m) v[m] = *(const s4v*)(p + (k + m) * step);
+#pragma unroll
+      for (int m = 0; m < 8; ++m) sum += v[m];
+    }
+    for (; k < count; ++k) sum += *(const s4v*)(p + k * step);
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if (c0 + j + r < N) o[(int64_t)i * N + j + r] = (T)(sum[r] * scale);
+  }
+}
+
+// Y = s_row s_col (codes of X) (codes of W [E, N, K])^T, rows gathered where order is given
+template <typename O, int WM, int WN, int FM, int FN>
+__global__ __launch_bounds__(WG) void k_expert_codes(const E4m3* __restrict__ x, const float* __restrict__ xs,
+                                                     const int* __restrict__ order, unsigned choices, int tokens,
+                                                     const E4m3* __restrict__ weight, const float* __restrict__ ws,
+                                                     Groups gr, int pairs, int n, O* __restrict__ out, int tiles, int cols) {
+  constexpr int TM = 16 * WM * FM, TN = 16 * WN * FN;
+  __shared__ int rows[TM];
   const int t = tile_of(tiles);
   if (t < 0) return;
-  const Place p = place_of(gr, t / cols, __builtin_ctz(DT));
+  const Place p = place_of<true, false>(gr, t / cols, __builtin_ctz(TM));
   if (p.count <= 0) return;
-  const int c0 = t % cols * DT, m = (int)min(p.count, (int64_t)DT), nn = n - c0;
-  double* o = out + p.first * n + c0;
+  const int c0 = t % cols * TN, m = (int)min(p.count, (int64_t)TM), nn = n - c0;
+  O* o = out + p.first * n + c0;
   if (p.expert >= gr.experts) {
-    zero_rows(o, n, m, min(nn, DT));
+    zero_rows(o, n, m, min(nn, TN));
     return;
   }
-  const double* wt = weight + ((int64_t)p.expert * gr.blocks + p.block) * wsize;
-  const Work<double> w{x + p.first * sum, wt + (BT ? (int64_t)c0 : (int64_t)c0 * sum), sum, BT ? n : sum, sum, m, nn, nullptr};
-  product_f64<false, BT>(w, lds, [&](int i, int j, double v) {
-    if (i < m && j < nn) o[(int64_t)i * n + j] = v * scale;
-  });
-}
-
-__global__ __launch_bounds__(WG) void k_expert_weights_f64(const double* __restrict__ x, const double* __restrict__ g,
-                                                           Groups gr, int shift, int K, int N, double scale,
-                                                           double* __restrict__ dw, double* __restrict__ part, int tiles,
-                                                           int per, int cols) {
-  __shared__ double lds[2 * DK * DS];
-  const int t = tile_of(tiles);
-  if (t < 0) return;
-  const int slot = t / per, tile = t - slot * per, r0 = tile / cols * DT, c0 = tile % cols * DT;
-  const Place p = place_of(gr, slot, shift);
-  if (p.expert >= gr.experts || (p.part > 0 && p.count <= 0)) return;
-  const int64_t n = min(max(p.count, (int64_t)0), (int64_t)1 << shift);
-  const Work<double> w{x + p.first * K + r0, g + p.first * N + c0, K, N, n, K - r0, N - c0, nullptr};
-  const int64_t at = (int64_t)r0 * N + c0, size = (int64_t)K * N;
-  const bool whole = p.part == 0 && p.count <= n;
-  double* o = whole ? dw + ((int64_t)p.expert * gr.blocks + p.block) * size + at : part + slot * size + at;
-  const double s = whole ? scale : 1.0;
-  product_f64<true, true>(w, lds, [&](int i, int j, double v) {
-    if (i < K - r0 && j < N - c0) o[(int64_t)i * N + j] = v * s;
-  });
-}
-
-__global__ __launch_bounds__(WG) void k_expert_join_f64(const double* __restrict__ part, Groups gr, int shift,
-                                                        int64_t size, double scale, double* __restrict__ dw) {
-  const int b = (int)blockIdx.y / gr.experts, e = (int)blockIdx.y - b * gr.experts;
-  const int64_t base = gr.rows * gr.before[b], first = base + gr.comps[b] * gr.end_of(e);
-  const int64_t n = base + gr.comps[b] * gr.end_of(e + 1) - first;
-  const int parts = (int)((n + ((int64_t)1 << shift) - 1) >> shift);
-  if (parts <= 1) return;
-  const double* p = part + ((first >> shift) + b * (gr.experts + 1) + e) * size;
-  double* o = dw + ((int64_t)e * gr.blocks + b) * size;
-  for (int64_t i = 4 * ((int64_t)blockIdx.x * WG) + threadIdx.x; i < min(size, 4 * ((int64_t)blockIdx.x + 1) * WG); i += WG) {
-    double sum = p[i];
-    for (int q = 1; q < parts; ++q) sum += p[q * size + i];
-    o[i] = sum * scale;
+  if (order) {   // (a slot outside the tokens is taken for the last)
+    for (int i = (int)threadIdx.x; i < TM; i += WG) {
+      const unsigned slot = (unsigned)order[p.first + min(i, m - 1)];
+      rows[i] = (int)min(min(slot, (unsigned)gr.rows - 1) / choices, (unsigned)tokens - 1);
+    }
+    __syncthreads();
   }
+  const E4m3* wt = weight + (int64_t)p.expert * n * pairs;
+  const Work<E4m3> w{order ? x : x + p.first * pairs, wt + (int64_t)c0 * pairs, pairs, pairs, pairs, m, nn,
+                     order ? rows : nullptr};
+  product<E4m3, false, false, WM, WN, FM, FN, true>(
+      w, Put<O>{o, n, m, nn, 1.0f, (n & 3) == 0 && ((uintptr_t)out & 15) == 0, order ? xs : xs + p.first,
+                     ws + (int64_t)p.expert * n + c0, order ? rows : nullptr});
 }
 
 // -------------------------------------------------------------------- host ----
@@ -732,15 +1274,30 @@ int total_comps(const Groups& gr) { return gr.before[gr.blocks - 1] + gr.comps[g
 int64_t slots_of(const Groups& gr, int shift) {
   return ((gr.rows * total_comps(gr)) >> shift) + (int64_t)gr.blocks * (gr.experts + 1);
 }
+// the tiles that there are kernels for
+template <typename T, bool FAST>
+constexpr bool has_tile(int tm, int tn) {
+  if (std::is_same<T, double>::value) return !FAST && tm == 64;
+  return STREAMS<T, FAST> ? tm >= 32 : tm == 128 || tm == 64 || tm == 16;
+}
+
+template <typename F>
+void choose(bool a, bool b, F&& f) {
+  auto one = [&](auto x) { b ? f(x, std::true_type()) : f(x, std::false_type()); };
+  a ? one(std::true_type()) : one(std::false_type());
+}
+
 unsigned grid_of(int64_t tiles) { return (unsigned)((tiles + 7) / 8 * 8); }
+// workgroups that walk over tiles: as many as run at once
+unsigned walkers(int64_t tiles, int most) { return grid_of(tiles < most ? tiles : most); }
 
 // Tiles of 128 x 128 where they fill the card, 64 x 64 below, 16 x 128 for
 // experts of a few rows each (a product then reads its weights once and little
 // else; higher tiles would be mostly empty).
-enum { T128, T64, T16 };
-int rows_tile(const Groups& gr, int n) {
+enum { T128, T64, T32, T16 };
+int rows_tile(const Groups& gr, int n, bool streams) {
   const int64_t rows = gr.rows * total_comps(gr), groups = (int64_t)gr.blocks * (gr.experts > 0 ? gr.experts : 1);
-  if (rows <= 24 * groups) return T16;
+  if (rows <= 24 * groups) return streams ? T32 : T16;
   return slots_of(gr, 7) * ((n + 127) / 128) >= 512 ? T128 : T64;
 }
 
@@ -752,26 +1309,42 @@ void with_tile(int tile, F&& f) {
   typedef integral_constant<int, 4> I4;
   if (tile == T128) f(I2(), I2(), I4(), I4());
   else if (tile == T64) f(I2(), I2(), I2(), I2());
+  else if (tile == T32) f(I1(), I4(), I2(), I2());
   else f(I1(), I4(), I1(), I2());
 }
 
-// A weight gradient's rows go in parts of 2^shift: about 1,024 workgroups, at
-// least 256 rows each.
-int weight_shift(const Groups& gr, int64_t per) {
-  const int64_t rows = gr.rows * total_comps(gr);
-  int shift = 8;
-  while (((int64_t)1 << shift) < rows && (rows >> shift) * per > 1024) ++shift;
-  return shift;
+// The weight gradient's tiles, and the workgroups that share its units.
+int weight_tile(int type, int K, int N) {
+  return type == TACE_ROW_F64 || K <= 64 || N <= 64 ? T64 : T128;
 }
-bool weight_small(int K, int N) { return K <= 64 || N <= 64; }
-int64_t weight_tiles(int type, int K, int N) {
-  const int64_t t = type == TACE_ROW_F64 || weight_small(K, N) ? 64 : 128;
+int64_t tiles_of(int tile, int K, int N) {
+  const int64_t t = tile == T64 ? 64 : 128;
   return ((K + t - 1) / t) * ((N + t - 1) / t);
 }
-bool in_parts(const Groups& gr, int shift) {
-  int most = 1;
-  for (int b = 0; b < gr.blocks; ++b) most = gr.comps[b] > most ? gr.comps[b] : most;
-  return gr.rows * most > (int64_t)1 << shift;
+// whether a group may have more than a unit
+bool may_be_cut(const Groups& gr) {
+  for (int b = 0; b < gr.blocks; ++b)
+    if (gr.rows * gr.comps[b] > 128) return true;
+  return false;
+}
+// As many workgroups as run at once, in teams whose members have one to four of the
+// tiles each, whichever leaves the fewest idle.
+struct Teams {
+  int cuts, team;
+};
+Teams teams_of(int tile, const Groups& gr, int64_t per) {
+  const int64_t most = tile == T64 ? 1024 : 512;
+  const int64_t units = ((gr.rows * total_comps(gr)) >> 7) + (int64_t)gr.blocks * gr.experts;   // (there are no more)
+  Teams best{1, (int)(per < most ? per : most)};
+  double used = -1;
+  for (int64_t r = 1; r <= 4; ++r) {
+    const int64_t team = (per + r - 1) / r;
+    if (team > most) continue;
+    const int64_t cuts = std::min(most / team, units);
+    const double u = (double)(cuts * per) / (double)(r * most) - 0.02 * (double)r;
+    if (u > used) used = u, best = {(int)cuts, (int)team};
+  }
+  return best;
 }
 
 }  // namespace
@@ -786,36 +1359,25 @@ extern "C" int tace_expert_linear(int type, int transposed, const void* x, const
   if (!x || (!weight && experts) || !out) return tace_fail_msg("expert_linear: null argument");
   const int sum = transposed ? N : K, n = transposed ? K : N;
   const int64_t wsize = (int64_t)K * N;
-  if (type == TACE_ROW_F64) {
-    const int64_t cols = (n + DT - 1) / DT, tiles = slots_of(gr, 6) * cols;
-    if (tiles > MOST_WGS) return tace_fail_msg("expert_linear: bad sizes");
-    if (transposed)
-      hipLaunchKernelGGL((k_expert_rows_f64<false>), dim3(grid_of(tiles)), dim3(WG), 0, (hipStream_t)stream, (const double*)x,
-                         (const double*)weight, gr, wsize, sum, n, scale, (double*)out, (int)tiles, (int)cols);
-    else
-      hipLaunchKernelGGL((k_expert_rows_f64<true>), dim3(grid_of(tiles)), dim3(WG), 0, (hipStream_t)stream, (const double*)x,
-                         (const double*)weight, gr, wsize, sum, n, scale, (double*)out, (int)tiles, (int)cols);
-    return tace_check_launch("expert_linear");
-  }
-  const bool fast = sum % 8 == 0 && n % 8 == 0 && row_aligned(x) && row_aligned(weight) && row_aligned(out);
+  const bool fast = type != TACE_ROW_F64 && sum % 8 == 0 && n % 8 == 0 && row_aligned(x) && row_aligned(weight) && row_aligned(out);
   bool fits = true;
   row_dispatch(type, [&](auto zero) {
     typedef decltype(zero) T;
-    if constexpr (!std::is_same<T, double>::value) {
-      with_tile(rows_tile(gr, n), [&](auto wm, auto wn, auto fm, auto fn) {
-        constexpr int WM = decltype(wm)::value, WN = decltype(wn)::value, FM = decltype(fm)::value, FN = decltype(fn)::value;
-        constexpr int TM = 16 * WM * FM, TN = 16 * WN * FN;
-        const int64_t cols = (n + TN - 1) / TN, tiles = slots_of(gr, __builtin_ctz(TM)) * cols;
-        if (!(fits = tiles <= MOST_WGS)) return;
-        auto launch = [&](auto bt, auto quick) {
-          hipLaunchKernelGGL((k_expert_rows<T, decltype(bt)::value, WM, WN, FM, FN, decltype(quick)::value>),
-                             dim3(grid_of(tiles)), dim3(WG), 0, (hipStream_t)stream, (const T*)x, (const T*)weight, gr,
-                             wsize, sum, n, (float)scale, (T*)out, (int)tiles, (int)cols);
-        };
-        if (transposed) fast ? launch(std::false_type(), std::true_type()) : launch(std::false_type(), std::false_type());
-        else fast ? launch(std::true_type(), std::true_type()) : launch(std::true_type(), std::false_type());
+    typedef row_sum_t<T> S;
+    with_tile(std::is_same<T, double>::value ? T64 : rows_tile(gr, n, fast && sizeof(T) == 2), [&](auto wm, auto wn, auto fm, auto fn) {
+      constexpr int WM = decltype(wm)::value, WN = decltype(wn)::value, FM = decltype(fm)::value, FN = decltype(fn)::value;
+      constexpr int TM = 16 * WM * FM, TN = 16 * WN * FN;
+      const int64_t cols = (n + TN - 1) / TN, tiles = slots_of(gr, __builtin_ctz(TM)) * cols;
+      if (!(fits = tiles <= MOST_WGS)) return;
+      choose(transposed == 0, fast, [&](auto bt, auto quick) {
+        constexpr bool BT = decltype(bt)::value, FAST = decltype(quick)::value;
+        if constexpr (has_tile<T, FAST>(TM, TN))
+          hipLaunchKernelGGL((k_expert_rows<T, BT, WM, WN, FM, FN, FAST>),
+                             dim3(STREAMS<T, FAST> ? walkers(tiles, TM == 128 ? 512 : 1024) : grid_of(tiles)),
+                             dim3(64 * WM * WN), 0, (hipStream_t)stream, (const T*)x, (const T*)weight, gr, wsize, sum, n,
+                             (S)scale, (T*)out, (int)cols, sum <= 256);
       });
-    }
+    });
   });
   if (!fits) return tace_fail_msg("expert_linear: bad sizes");
   return tace_check_launch("expert_linear");
@@ -827,9 +1389,11 @@ extern "C" int64_t tace_expert_linear_grad_work(int type, int64_t rows, int32_t 
   static const int32_t none = 0;
   if (check_groups(rows, experts, blocks, comps, K, N, &none, &gr)) return -1;
   if (type < 0 || type > TACE_ROW_F16) return tace_fail_msg("expert_linear: unknown row type"), -1;
-  const int shift = weight_shift(gr, weight_tiles(type, K, N));
-  if (!in_parts(gr, shift)) return 0;
-  return slots_of(gr, shift) * K * N * (type == TACE_ROW_F64 ? 8 : 4);
+  if (experts == 0 || rows == 0) return 0;
+  const int tile = weight_tile(type, K, N);
+  const int64_t per = tiles_of(tile, K, N), side = tile == T64 ? 64 : 128;
+  const Teams teams = teams_of(tile, gr, per);
+  return teams.cuts > 1 && may_be_cut(gr) ? 2 * per * teams.cuts * side * side * (type == TACE_ROW_F64 ? 8 : 4) : 0;
 }
 
 extern "C" int tace_expert_linear_grad(int type, const void* x, const void* g, const int32_t* rowptr, int64_t rows,
@@ -840,42 +1404,34 @@ extern "C" int tace_expert_linear_grad(int type, const void* x, const void* g, c
   if (type < 0 || type > TACE_ROW_F16) return tace_fail_msg("expert_linear: unknown row type");
   if (experts == 0) return 0;
   if ((rows && (!x || !g)) || !dw) return tace_fail_msg("expert_linear: null argument");
-  const int64_t per = weight_tiles(type, K, N), size = (int64_t)K * N;
-  const int shift = weight_shift(gr, per);
-  const bool parts = in_parts(gr, shift);
-  const int64_t tiles = slots_of(gr, shift) * per;
-  if (tiles > MOST_WGS || (int64_t)blocks * experts > 65535) return tace_fail_msg("expert_linear: bad sizes");
-  if (parts && (!work || !row_aligned(work) ||
+  const int tile = weight_tile(type, K, N);
+  const int64_t per = tiles_of(tile, K, N);
+  if ((int64_t)blocks * experts * per > MOST_WGS / 8) return tace_fail_msg("expert_linear: bad sizes");
+  const Teams teams = teams_of(tile, gr, per);
+  const bool joins = teams.cuts > 1 && may_be_cut(gr);
+  if (joins && (!work || !row_aligned(work) ||
                 work_bytes < tace_expert_linear_grad_work(type, rows, experts, blocks, comps, K, N)))
     return tace_fail_msg("expert_linear: the workspace is too small or not 16-byte aligned");
-  const dim3 grid(grid_of(tiles)), join((unsigned)((size + 4 * WG - 1) / (4 * WG)), (unsigned)(blocks * experts));
+  const unsigned n = grid_of((int64_t)teams.cuts * teams.team);
   const hipStream_t st = (hipStream_t)stream;
-  if (type == TACE_ROW_F64) {
-    hipLaunchKernelGGL(k_expert_weights_f64, grid, dim3(WG), 0, st, (const double*)x, (const double*)g, gr, shift, K, N,
-                       scale, (double*)dw, (double*)work, (int)tiles, (int)per, (N + DT - 1) / DT);
-    if (parts)
-      hipLaunchKernelGGL(k_expert_join_f64, join, dim3(WG), 0, st, (const double*)work, gr, shift, size, scale, (double*)dw);
-    return tace_check_launch("expert_linear_grad");
-  }
-  const bool fast = K % 8 == 0 && N % 8 == 0 && row_aligned(x) && row_aligned(g) && row_aligned(dw);
+  const bool fast = type != TACE_ROW_F64 && K % 8 == 0 && N % 8 == 0 && row_aligned(x) && row_aligned(g) && row_aligned(dw);
   row_dispatch(type, [&](auto zero) {
     typedef decltype(zero) T;
-    if constexpr (!std::is_same<T, double>::value) {
-      with_tile(weight_small(K, N) ? T64 : T128, [&](auto wm, auto wn, auto fm, auto fn) {
-        constexpr int WM = decltype(wm)::value, WN = decltype(wn)::value, FM = decltype(fm)::value, FN = decltype(fn)::value;
-        if constexpr (WM == 2) {
-          auto launch = [&](auto quick) {
-            hipLaunchKernelGGL((k_expert_weights<T, WM, WN, FM, FN, decltype(quick)::value>), grid, dim3(WG), 0, st,
-                               (const T*)x, (const T*)g, gr, shift, K, N, (float)scale, (T*)dw, (float*)work, (int)tiles,
-                               (int)per, (N + 16 * WN * FN - 1) / (16 * WN * FN));
-          };
-          fast ? launch(std::true_type()) : launch(std::false_type());
-        }
-      });
-      if (parts)
-        hipLaunchKernelGGL((k_expert_join<T>), join, dim3(WG), 0, st, (const float*)work, gr, shift, size, (float)scale,
-                           (T*)dw);
-    }
+    typedef row_sum_t<T> S;
+    with_tile(tile, [&](auto wm, auto wn, auto fm, auto fn) {
+      constexpr int WM = decltype(wm)::value, WN = decltype(wn)::value, FM = decltype(fm)::value, FN = decltype(fn)::value;
+      constexpr int TM = 16 * WM * FM, TN = 16 * WN * FN;
+      if constexpr (TM == TN && (TM == 64 || (TM == 128 && !std::is_same<T, double>::value))) {
+        const int cols = (N + TN - 1) / TN;
+        choose(fast, true, [&](auto quick, auto) {
+          hipLaunchKernelGGL((k_expert_weights<T, WM, WN, FM, FN, decltype(quick)::value>), dim3(n), dim3(64 * WM * WN), 0,
+                             st, (const T*)x, (const T*)g, gr, K, N, (S)scale, (T*)dw, (S*)work, (int)per, cols, teams.cuts, teams.team);
+        });
+        if (joins)
+          hipLaunchKernelGGL((k_expert_join<T, TM, TN>), dim3((unsigned)(8 * blocks * experts * per)), dim3(WG), 0, st,
+                             (const S*)work, gr, K, N, (S)scale, (T*)dw, (int)per, cols, teams.cuts);
+      }
+    });
   });
   return tace_check_launch("expert_linear_grad");
 }
@@ -898,14 +1454,16 @@ extern "C" int tace_expert_linear_e4m3(int out_type, const void* x, const float*
   row_dispatch(out_type, [&](auto zero) {
     typedef decltype(zero) O;
     if constexpr (!std::is_same<O, double>::value) {
-      with_tile(rows_tile(gr, N), [&](auto wm, auto wn, auto fm, auto fn) {
+      with_tile(rows_tile(gr, N, false), [&](auto wm, auto wn, auto fm, auto fn) {
         constexpr int WM = decltype(wm)::value, WN = decltype(wn)::value, FM = decltype(fm)::value, FN = decltype(fn)::value;
         constexpr int TM = 16 * WM * FM, TN = 16 * WN * FN;
+        if constexpr (TM != 32) {
         const int64_t cols = (N + TN - 1) / TN, tiles = slots_of(gr, __builtin_ctz(TM)) * cols;
         if (!(fits = tiles <= MOST_WGS)) return;
         hipLaunchKernelGGL((k_expert_codes<O, WM, WN, FM, FN>), dim3(grid_of(tiles)), dim3(WG), 0, (hipStream_t)stream,
                            (const E4m3*)x, x_scale, order, (unsigned)choices, (int)(rows / choices),
                            (const E4m3*)weight, w_scale, gr, K / 2, N, (O*)out, (int)tiles, (int)cols);
+        }
       });
     }
   });

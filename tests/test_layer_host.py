@@ -131,8 +131,8 @@ def test_expert_entries_refuse_bad_arguments():
         _refused(rows(**bad), b"null")
     assert rows(n=0, x=None, w=None, out=None) == 0
 
-    def grad(ty=0, x=P, g=P, ptr=P, n=100000, E=2, dw=P, work=P, nbytes=1 << 40):
-        return L.tace_expert_linear_grad(ty, x, g, ptr, n, E, 1, one, 64, 64, 1.0, dw, work, nbytes, None)
+    def grad(ty=0, x=P, g=P, ptr=P, n=100000, E=2, dw=P, work=P, nbytes=1 << 40, M=64):
+        return L.tace_expert_linear_grad(ty, x, g, ptr, n, E, 1, one, M, M, 1.0, dw, work, nbytes, None)
 
     need = L.tace_expert_linear_grad_work(0, 100000, 2, 1, one, 64, 64)
     assert need > 0 and L.tace_expert_linear_grad_work(0, 100, 2, 1, one, 64, 64) == 0
@@ -141,7 +141,7 @@ def test_expert_entries_refuse_bad_arguments():
     for bad in (dict(x=None), dict(g=None), dict(dw=None), dict(ptr=None)):
         _refused(grad(**bad), b"null")
     _refused(grad(ty=4), b"row type")
-    _refused(grad(E=70000), b"bad sizes")
+    _refused(grad(E=70000, M=1024), b"bad sizes")
     assert grad(E=0, dw=None) == 0
 
     def codes(out=2, x=P, xs=P, order=None, k=1, w=P, ws=P, ptr=P, n=4, K=32, o=P):
@@ -159,17 +159,21 @@ def test_expert_entries_refuse_bad_arguments():
 
 
 def test_expert_workspace_covers_every_part():
-    """Parts of 2^shift rows: a slot for each of them and one for each group, whatever the rows' distribution."""
+    """Two pieces of every tile of [K, M] for each stretch of rows; stretches are no more than units of 128 rows and empty
+    groups, and a stretch's workgroups, with one to four tiles each, all run at once."""
     L = N.lib()
     for ty, size in ((0, 4), (1, 8), (2, 4)):
         for rows in (1, 257, 5000, 300000):
             for E in (1, 7, 90):
                 for comps in ((1,), (1, 3, 5, 7)):
-                    for K, M in ((16, 8), (128, 128), (1024, 2048)):
+                    for K, M in ((16, 8), (128, 128), (1024, 2048), (8192, 8192)):
                         nbytes = L.tace_expert_linear_grad_work(ty, rows, E, len(comps), _ints(*comps), K, M)
-                        slots, rest = divmod(nbytes, K * M * size)
+                        side = 64 if ty == 1 or min(K, M) <= 64 else 128
+                        tiles = -(-K // side) * -(-M // side)
+                        cuts, rest = divmod(nbytes, 2 * tiles * side * side * size)
                         assert rest == 0
-                        if nbytes:      # at least 256 rows a part
-                            assert len(comps) * (E + 1) <= slots <= rows * sum(comps) // 256 + len(comps) * (E + 1)
+                        if cuts:
+                            assert 2 <= cuts <= rows * sum(comps) // 128 + len(comps) * E
+                            assert cuts * -(-tiles // 4) <= (1024 if side == 64 else 512)
                         else:
-                            assert rows * max(comps) <= 2 ** 22
+                            assert rows * max(comps) <= 128 or tiles > 512 or rows * sum(comps) // 128 + E * len(comps) < 2
