@@ -132,9 +132,13 @@ struct Now {
   S clip, keep, rate, root;   // gradients' factor, 1 - lr decay, lr / (1 - b1^t), 1 / sqrt(1 - b2^t)
 };
 
-// p, m and v (or r) after the step
+// p, m and v (or r) after the step.  Each product and sum is rounded by itself, as
+// in a program of one operation after the other: codes' draws then fall alike in
+// both (a largest element a last place higher or lower, rounded the other way,
+// would move its block's next scale by 7 %).  The step waits for memory anyway.
 template <typename S>
 __device__ __forceinline__ void adam(const Step<S>& st, const Now<S>& c, S g, S& p, S& m, S& v, S& r) {
+#pragma clang fp contract(off)
   g *= c.clip;
   m = m * st.b1 + g * st.rest1;
   v = v * st.b2 + g * g * st.rest2;
@@ -164,8 +168,8 @@ __device__ __forceinline__ int drawn_codes(const float* x, const unsigned* words
   for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
   if (__ballot(bad)) top = __builtin_nanf("");
   if (top < 0x1p-100f) top = 0.0f;   // (448 / top overflows below 2^-118)
-  const float up = top == 0.0f ? 0.0f : 448.0f / top;
-  *scale = top / 448.0f;
+  const float up = top == 0.0f ? 0.0f : 1.0f / top * 448.0f;   // (as tensors' quotients with numbers are made)
+  *scale = top * (1.0f / 448.0f);
   float q[4];
 #pragma unroll
   for (int e = 0; e < 4; ++e) {

@@ -208,6 +208,27 @@ def test_codes_are_the_drawn_ones(cuda):
             assert bool(ok.all()) and float((near | edge).double().mean()) < 0.01
 
 
+@pytest.mark.parametrize("dt,masters", [(torch.float32, False), (torch.bfloat16, True)], ids=ids)
+def test_scales_are_those_of_single_operations(cuda, dt, masters):
+    """Every product and sum rounded by itself: a largest element a last place off could draw another code."""
+    c = Case(cuda, dt, [(BLOCK * 500 + 77,), (4096,)], 8, masters=masters)
+    b1, b2 = (torch.tensor(b, dtype=torch.float64) for b in HYPER["betas"])
+    want = []
+    for g, m, s, sc in zip(c.g, c.m, c.s, c.scales):
+        g, m, s, sc = g.cpu().float(), m.cpu().float(), s.cpu().float(), sc.cpu()
+        sm, sr = (sc[:, k].repeat_interleave(BLOCK)[:g.numel()] for k in (0, 1))
+        m, r = m * sm, s * sr
+        m = m * b1.float() + g * (1 - b1).float()
+        v = (r * r) * b2.float() + (g * g) * (1 - b2).float()
+        flat = torch.zeros(2, sc.shape[0] * BLOCK)
+        # (a root in 64 bits, rounded once: the host's float32 root is not always the nearest)
+        flat[0, :g.numel()], flat[1, :g.numel()] = m.abs(), v.double().sqrt().float()
+        want.append(flat.view(2, -1, BLOCK).amax(2).mul(torch.tensor(1 / 448)).t())
+    c.step()
+    for w, sc in zip(want, c.scales):
+        assert torch.equal(w, sc.cpu())
+
+
 def test_a_slow_average_moves_in_the_mean(cuda):
     """0.1 % of the way a step: codes to nearest would never move."""
     n, steps = 1 << 16, 60
