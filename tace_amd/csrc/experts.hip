@@ -63,6 +63,39 @@ struct Place {
   int expert, block;
 };
 
+// What a tile is, by elements from its operands' and outputs' first ones; a lane
+// holds one, a wavefront takes them one after the other.
+struct Job {
+  int64_t a, b, out;
+  int sum;          // the summed index
+  int m, n;         // rows and columns, up to the tile's
+  int kind, whole;
+
+  __device__ __forceinline__ static int of(int v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
+  __device__ __forceinline__ static int64_t of(int64_t v, int lane) {
+    const unsigned lo = (unsigned)__builtin_amdgcn_readlane((int)v, lane);
+    return (int64_t)((unsigned long long)(unsigned)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32 | lo);
+  }
+  __device__ __forceinline__ Job lane(int l) const {
+    return Job{of(a, l), of(b, l), of(out, l), of(sum, l), of(m, l), of(n, l), of(kind, l), of(whole, l)};
+  }
+};
+enum { NO_TILE, ZERO_TILE, PRODUCT };
+
+// The sum over the lanes up to each (within rows of 16, then from row to row).
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int plus_dpp(int v) {
+  return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false);
+}
+__device__ __forceinline__ int up_to_lane(int v) {
+  v = plus_dpp<0x111, 0xf>(v);
+  v = plus_dpp<0x112, 0xf>(v);
+  v = plus_dpp<0x114, 0xf>(v);
+  v = plus_dpp<0x118, 0xf>(v);
+  v = plus_dpp<0x142, 0xa>(v);
+  return plus_dpp<0x143, 0xc>(v);
+}
+
 // Numbers the slots of 2^shift rows of all groups without gaps and finds a slot's
 // group, a slot a lane: 64 groups at a time are in the lanes, with the sum of their
 // slots up to each.  Groups of a block: the experts and, with DROPPED, the
@@ -90,12 +123,7 @@ struct Places {
       to = block0 + gr.comps[b] * gr.end_of(e + 1);
       slots = to > from ? (int)((to - from + ((int64_t)1 << shift) - 1) >> shift) : EMPTY ? 1 : 0;
     }
-    upto = slots;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int v = __shfl_up(upto, o, 64);
-      if (lane >= o) upto += v;
-    }
+    upto = up_to_lane(slots);
   }
   __device__ __forceinline__ int last() const { return __builtin_amdgcn_readlane(upto, 63); }
   // all slots
@@ -108,7 +136,24 @@ struct Places {
     }
     return sum;
   }
-  // (every lane of the wavefront calls it; slots behind the last give a place without rows)
+  __device__ __forceinline__ Place place(int g, int64_t part, int64_t f, int64_t t) const {
+    const int per = gr.experts + (DROPPED ? 1 : 0), b = g / per;
+    return Place{f + (part << shift), t - f - (part << shift), part, g - b * per, b};
+  }
+  // a slot that is the same in all lanes
+  __device__ __forceinline__ Place find_one(int slot) {
+    int before = 0;
+    for (int at = 0; at < n; at += 64) {
+      if (n > 64) take(at);
+      if (slot - before < last()) {
+        const int l = __popcll(__ballot(before + upto <= slot));   // groups that end before
+        return place(at + l, slot - before - (l ? Job::of(upto, max(l - 1, 0)) : 0), Job::of(from, l), Job::of(to, l));
+      }
+      before += last();
+    }
+    return Place{0, 0, 0, gr.experts, 0};
+  }
+  // each lane's own (every lane of the wavefront calls it); slots behind the last give a place without rows
   __device__ __forceinline__ Place find(int slot) {
     Place p{0, 0, 0, gr.experts, 0};
     int before = 0;
@@ -120,38 +165,12 @@ struct Places {
         if (__shfl(upto, lane + o - 1, 64) <= slot - before) lane += o;
       const int64_t f = __shfl((long long)from, lane, 64), t = __shfl((long long)to, lane, 64);
       const int prior = __shfl(upto, max(lane - 1, 0), 64);
-      if (slot >= before && slot - before < last()) {
-        const int per = gr.experts + (DROPPED ? 1 : 0), g = at + lane;
-        p.block = g / per;
-        p.expert = g - p.block * per;
-        p.part = slot - before - (lane ? prior : 0);
-        p.first = f + (p.part << shift);
-        p.count = t - p.first;
-      }
+      if (slot >= before && slot - before < last()) p = place(at + lane, slot - before - (lane ? prior : 0), f, t);
       before += last();
     }
     return p;
   }
 };
-
-// What a tile is, by elements from its operands' and outputs' first ones; a lane
-// holds one, a wavefront takes them one after the other.
-struct Job {
-  int64_t a, b, out;
-  int sum;          // the summed index
-  int m, n;         // rows and columns, up to the tile's
-  int kind, whole;
-
-  __device__ __forceinline__ static int of(int v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
-  __device__ __forceinline__ static int64_t of(int64_t v, int lane) {
-    const unsigned lo = (unsigned)__builtin_amdgcn_readlane((int)v, lane);
-    return (int64_t)((unsigned long long)(unsigned)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32 | lo);
-  }
-  __device__ __forceinline__ Job lane(int l) const {
-    return Job{of(a, l), of(b, l), of(out, l), of(sum, l), of(m, l), of(n, l), of(kind, l), of(whole, l)};
-  }
-};
-enum { NO_TILE, ZERO_TILE, PRODUCT };
 
 // Tiles of an XCD (every eighth workgroup) are contiguous, its workgroups take them
 // in turn: what runs together shares rows and columns in the XCD's L2.
@@ -174,13 +193,6 @@ __device__ __forceinline__ void blocked(int t, int rows, int cols, int* row, int
   const int block = t / (8 * cols), r = t - block * 8 * cols, high = min(rows - 8 * block, 8);
   *row = 8 * block + r % high;
   *col = r / high;
-}
-
-// one slot for the workgroup
-template <bool DROPPED, bool EMPTY>
-__device__ __forceinline__ Place place_of(const Groups& gr, int slot, int shift) {
-  const Place p = Places<DROPPED, EMPTY>(gr, shift).find(slot);
-  return Place{Job::of(p.first, 0), Job::of(p.count, 0), Job::of(p.part, 0), Job::of(p.expert, 0), Job::of(p.block, 0)};
 }
 
 // workgroups of an XCD (every eighth) take a contiguous range of tiles
@@ -1053,7 +1065,7 @@ struct Units {
   const Groups& gr;
   int n;               // groups
   int64_t from, to;    // this lane's group's rows
-  int64_t upto;        // units of the lanes' groups up to this one
+  int upto;            // units of the lanes' groups up to this one
 
   __device__ __forceinline__ explicit Units(const Groups& gr) : gr(gr), n(gr.experts * gr.blocks) { take(0); }
   __device__ __forceinline__ static int64_t units(int64_t rows) { return rows > 0 ? (rows + 127) >> 7 : 1; }
@@ -1064,15 +1076,11 @@ struct Units {
       const int b = g / gr.experts, e = g - b * gr.experts;
       from = gr.rows * gr.before[b] + gr.comps[b] * gr.end_of(e);
       to = gr.rows * gr.before[b] + gr.comps[b] * gr.end_of(e + 1);
-      upto = units(to - from);
+      upto = (int)units(to - from);
     }
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int64_t v = __shfl_up((long long)upto, o, 64);
-      if (lane >= o) upto += v;
-    }
+    upto = up_to_lane(upto);
   }
-  __device__ __forceinline__ int64_t last() const { return Job::of(upto, 63); }
+  __device__ __forceinline__ int last() const { return Job::of(upto, 63); }
   __device__ __forceinline__ int64_t total() {
     if (n <= 64) return last();
     int64_t sum = 0;
@@ -1104,7 +1112,7 @@ struct Units {
       if (n > 64) take(at);
       const int l = min(max(g - at, 0), 63);
       const int64_t f = __shfl((long long)from, l, 64), t = __shfl((long long)to, l, 64);
-      const int64_t prior = __shfl((long long)upto, max(l - 1, 0), 64);
+      const int prior = __shfl(upto, max(l - 1, 0), 64);
       if (g >= at && g - at < 64) s = Span{before + (l ? prior : 0), units(t - f), f, t > f ? t - f : 0};
       before += last();
     }
@@ -1222,7 +1230,7 @@ __global__ __launch_bounds__(WG) void k_expert_codes(const E4m3* __restrict__ x,
   __shared__ int rows[TM];
   const int t = tile_of(tiles);
   if (t < 0) return;
-  const Place p = place_of<true, false>(gr, t / cols, __builtin_ctz(TM));
+  const Place p = Places<true, false>(gr, __builtin_ctz(TM)).find_one(t / cols);
   if (p.count <= 0) return;
   const int c0 = t % cols * TN, m = (int)min(p.count, (int64_t)TM), nn = n - c0;
   O* o = out + p.first * n + c0;
