@@ -370,23 +370,40 @@ struct WideTile {
       return line * BK + ((piece ^ ((line >> 1) & 7)) << 3);
     }
   }
-  // of outputs 32 j .., 16 s .. of the summed index
-  __device__ __forceinline__ static s8 fragment(const unsigned short* l, int j, int s, int lane) {
+  // A lane's first elements, of which all its fragments are at constant distances:
+  // one for each of F blocks (ACROSS), or for each 16 of the summed index.  (The
+  // compiler is kept from seeing how they come about: of longer sums it loses which
+  // array they are in, and waits for the loads into the other one.)
+  template <int F>
+  struct At {
+    int v[ACROSS ? F : BK / 16];
+    __device__ __forceinline__ At(int block0, int lane) {
+#pragma unroll
+      for (int k = 0; k < (ACROSS ? F : BK / 16); ++k) {
+        if constexpr (ACROSS)
+          v[k] = lds_at(8 * (lane >> 5) + ((lane >> 2) & 3), 4 * (block0 + k) + ((lane >> 3) & 2) + ((lane >> 1) & 1)) +
+                 ((lane & 1) << 2);
+        else
+          v[k] = lds_at(32 * block0 + (lane & 31), 2 * k + (lane >> 5));
+        asm volatile("" : "+v"(v[k]));
+      }
+    }
+  };
+  // of block j's 16 s .. of the summed index
+  template <int F>
+  __device__ __forceinline__ static s8 fragment(const unsigned short* l, const At<F>& at, int j, int s) {
     if constexpr (ACROSS) {
       union {
         s4 h[2];
         s8 v;
       } o;
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int line = 16 * s + 8 * (lane >> 5) + 4 * h + ((lane >> 2) & 3);
+      for (int h = 0; h < 2; ++h)
         o.h[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-            (__attribute__((address_space(3))) s4*)(l + lds_at(line, 4 * j + ((lane >> 3) & 2) + ((lane >> 1) & 1)) +
-                                                    ((lane & 1) << 2)));
-      }
+            (__attribute__((address_space(3))) s4*)(l + (16 * s + 4 * h) * TM + at.v[j]));
       return o.v;
     } else {
-      return *(const s8*)(l + lds_at(32 * j + (lane & 31), 2 * s + (lane >> 5)));
+      return *(const s8*)(l + 32 * j * BK + at.v[s]);
     }
   }
 };
@@ -648,14 +665,16 @@ __device__ __forceinline__ void arrive() {
 // the fragments of 32 of the summed index, of a wavefront's FM x FN blocks of 32
 template <typename TA, typename TB, int FM, int FN>
 struct Fragments {
+  typedef typename TA::template At<FM> AtA;
+  typedef typename TB::template At<FN> AtB;
   s8 a[2][FM], b[2][FN];
-  __device__ __forceinline__ void read(const unsigned short* l, int half, int i0, int j0, int lane) {
+  __device__ __forceinline__ void read(const unsigned short* l, int half, const AtA& at_a, const AtB& at_b) {
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
 #pragma unroll
-      for (int i = 0; i < FM; ++i) a[s][i] = TA::fragment(l, i0 + i, 2 * half + s, lane);
+      for (int i = 0; i < FM; ++i) a[s][i] = TA::fragment(l, at_a, i, 2 * half + s);
 #pragma unroll
-      for (int j = 0; j < FN; ++j) b[s][j] = TB::fragment(l + TA::ELEMS, j0 + j, 2 * half + s, lane);
+      for (int j = 0; j < FN; ++j) b[s][j] = TB::fragment(l + TA::ELEMS, at_b, j, 2 * half + s);
     }
     __builtin_amdgcn_sched_barrier(0);   // (these go out before what follows)
   }
@@ -715,9 +734,11 @@ __device__ __forceinline__ void stream_products(const T* __restrict__ a_base, co
   load(even);
   load(odd);
   arrive<NEXT, false>();
+  const typename TA::template At<FM> at_a(i0, lane);
+  const typename TB::template At<FN> at_b(j0, lane);
   Fragments<TA, TB, FM, FN> f, g;
-  f.read(even, 0, i0, j0, lane);
-  g.read(even, 1, i0, j0, lane);
+  f.read(even, 0, at_a, at_b);
+  g.read(even, 1, at_a, at_b);
   bool more = true;
   f16v acc[FM][FN];
   auto clear = [&]() {
@@ -726,46 +747,35 @@ __device__ __forceinline__ void stream_products(const T* __restrict__ a_base, co
 #pragma unroll
       for (int j = 0; j < FN; ++j) acc[i][j] = f16v{};
   };
-  clear();
-  int l = __ffsll((long long)mask) - 1;
-  f.template multiply<T>(acc);
-  // Loops begin where all loads have to be there, in the middle of an even step (at
-  // a loop's head the compiler no longer knows which are for the other buffer).
+  // Loops begin with nothing to read until all loads are there (at a loop's head
+  // the compiler no longer knows which are for the other buffer, and waits).
   auto pair = [&](auto stores) {
+    f.template multiply<T>(acc);
     arrive<0, true>();
     if (left <= 0) {
       more = ahead != 0;
       if (more) turn();
     }
     if (more) load(even);
-    if constexpr (decltype(stores)::value) store.later(0);
-    f.read(odd, 0, i0, j0, lane);
+    if constexpr (decltype(stores)::value) store.later();
+    f.read(odd, 0, at_a, at_b);
     g.template multiply<T>(acc);
-    g.read(odd, 1, i0, j0, lane);
+    g.read(odd, 1, at_a, at_b);
     f.template multiply<T>(acc);
-    arrive<0, true>();
+    arrive<decltype(stores)::value ? Store::STORES : 0, true>();   // (the stores after the loads stay in flight)
     if (more) load(odd);
-    if constexpr (decltype(stores)::value) store.later(1);
-    f.read(even, 0, i0, j0, lane);   // (the next tile's, if there is one)
+    f.read(even, 0, at_a, at_b);   // (the next tile's, if there is one)
     g.template multiply<T>(acc);
+    g.read(even, 1, at_a, at_b);
   };
-  for (;;) {
-    pair(std::true_type());
-    for (int n = Job::of(jobs.sum, l) - 2 * BK; n > 0; n -= 2 * BK) {
-      g.read(even, 1, i0, j0, lane);
-      f.template multiply<T>(acc);
-      pair(std::false_type());
-    }
-    store.tile(jobs.lane(l), acc, lane, i0, j0);
-    mask &= mask - 1;
-    if (mask == 0) break;
-    l = __ffsll((long long)mask) - 1;
+  for (; mask; mask &= mask - 1) {
+    const int l = __ffsll((long long)mask) - 1;
     clear();
-    g.read(even, 1, i0, j0, lane);
-    f.template multiply<T>(acc);
+    pair(std::true_type());
+    for (int n = Job::of(jobs.sum, l) - 2 * BK; n > 0; n -= 2 * BK) pair(std::false_type());
+    store.tile(jobs.lane(l), acc, lane, i0, j0);
   }
-  store.later(0);
-  store.later(1);
+  store.later();
 }
 
 // stores of a tile's four consecutive columns
@@ -820,8 +830,8 @@ struct PutPart {
   }
 };
 
-// A tile's results rounded and kept, and stored half by half beside the next
-// tile's loads: a step waits for both together (vmcnt counts stores too), where
+// A tile's results rounded and kept, and stored behind the next tile's first loads:
+// the step after waits for the loads alone (vmcnt counts both, in order), where
 // stores at a tile's end were waited for by themselves.  A wavefront's blocks pass
 // through 2 or 4 KB of its own in LDS before, so that a store writes whole rows of
 // its blocks (128 bytes) and not 16 bytes of each of 32 rows.  (A lane holds row
@@ -834,21 +844,25 @@ struct Results {
   typedef T t4 __attribute__((ext_vector_type(4)));
   typedef unsigned u2 __attribute__((ext_vector_type(2)));
   Make make;
+  static constexpr int STORES = LATE ? FM * READS : 0;
+  static constexpr unsigned NONE = 0x80000000u;
   u4 lined[FM][READS];
-  T* at;            // this lane's first element
-  int64_t ld;
-  int rows, cols;   // that are there, from it on
-  bool any = false;
+  T* base;                  // the tile's first element,
+  unsigned range, ld, at;   // and bytes of its rows, of a row, and before this lane's first
 
-  __device__ __forceinline__ explicit Results(Make make) : make(make) {}
+  __device__ __forceinline__ explicit Results(Make make) : make(make), base(nullptr), range(0), ld(0), at(NONE) {
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+      for (int n = 0; n < READS; ++n) lined[i][n] = u4{0u, 0u, 0u, 0u};
+  }
   __device__ __forceinline__ void tile(const Job& j, const f16v (&acc)[FM][FN], int lane, int i0, int j0) {
     const auto to = make(j);
     if constexpr (LATE) {
       rows_of(to, acc, lane, i0, j0);
     } else if (to.whole) {
       rows_of(to.out, acc, lane, i0, j0);
-      half(0);
-      half(1);
+      flush();
     } else {
 #pragma unroll
       for (int i = 0; i < FM; ++i)
@@ -883,27 +897,31 @@ struct Results {
         lined[i][n] = r & 1 ? u4{v[2], v[3], v[0], v[1]} : v;
       }
     }
-    const int row = 32 * i0 + lane / (SLOTS / 2), col = 32 * j0 + lane % (SLOTS / 2) * 8;
-    at = put.out + row * put.ldo + col;
-    ld = put.ldo;
-    rows = put.m - row;
-    cols = put.n - col;
-    any = true;
+    const int col = 32 * j0 + lane % (SLOTS / 2) * 8;   // (eight columns are all there or none)
+    base = put.out;
+    ld = (unsigned)put.ldo * 2;
+    range = (unsigned)put.m * ld;
+    at = col < put.n ? (unsigned)(32 * i0 + lane / (SLOTS / 2)) * ld + (unsigned)col * 2 : NONE;
   }
-  __device__ __forceinline__ void later(int which) {
-    if (!LATE || !any) return;
-    half(which);
-    if (which) any = false;
+  // (STORES instructions whatever there is to store: the next step counts them)
+  __device__ __forceinline__ void later() {
+    __builtin_amdgcn_sched_barrier(0);
+    if constexpr (LATE) flush();
+    __builtin_amdgcn_sched_barrier(0);
   }
-  __device__ __forceinline__ void half(int which) {
+  __device__ __forceinline__ void flush() {
+    const uintptr_t u = (uintptr_t)base;
+    const uintptr_t q = (uintptr_t)(unsigned)__builtin_amdgcn_readfirstlane((int)(u >> 32)) << 32 |
+                        (unsigned)__builtin_amdgcn_readfirstlane((int)u);
+    const auto rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)q, (short)0, __builtin_amdgcn_readfirstlane((int)range),
+                                                        0x00027000);
+    const unsigned line = (unsigned)__builtin_amdgcn_readfirstlane((int)ld);
 #pragma unroll
     for (int i = 0; i < FM; ++i)
 #pragma unroll
-      for (int n = 0; n < READS; ++n) {
-        if ((i * READS + n) / ((FM * READS + 1) / 2) != which) continue;
-        const int row = 32 * i + n * (128 / SLOTS);
-        if (row < rows && cols > 0) *(u4*)(at + row * ld) = lined[i][n];   // (eight columns are all there or none)
-      }
+      for (int n = 0; n < READS; ++n)
+        __builtin_amdgcn_raw_buffer_store_b128(lined[i][n], rsrc, (int)(at + (unsigned)(32 * i + n * (128 / SLOTS)) * line), 0, 0);
+    range = 0;
   }
 };
 
