@@ -893,7 +893,9 @@ struct Results {
 #pragma unroll
       for (int n = 0; n < READS; ++n) {
         const int u = lane + 64 * n, r = u / (SLOTS / 2), c = (u % (SLOTS / 2)) ^ ((r & (SLOTS - 1)) >> 1);
-        const u4 v = *(const u4*)(w + r * SLOTS + 2 * c);
+        int place = r * SLOTS + 2 * c;
+        asm volatile("" : "+v"(place));   // (as At's)
+        const u4 v = *(const u4*)(w + place);
         lined[i][n] = r & 1 ? u4{v[2], v[3], v[0], v[1]} : v;
       }
     }
