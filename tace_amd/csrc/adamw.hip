@@ -7,10 +7,10 @@
 //   p = p (1 - lr decay) - lr / (1 - b1^t) m / (sqrt(v / (1 - b2^t)) + eps)
 //
 // Bound by HBM: each operand is read once and written once (a gradient twice
-// where it is clipped).  The tensors' addresses travel with the launch, up to 56
-// in its 4 KB of arguments, so a step over new gradients copies nothing ahead
-// of it and a recorded one replays; a workgroup finds its tensor by one ballot
-// over the tensors' first units.
+// where it is clipped).  The tensors' addresses travel with the launch, as many as
+// its 4 KB of arguments hold (56; 84 without masters and scales, 160 for norms), so
+// a step over new gradients copies nothing ahead of it and a recorded one replays;
+// a workgroup finds its tensor by ballots over the tensors' first units.
 //
 // States of 8 bits: m and r = sqrt(v) as e4m3 codes, 256 elements to a float32
 // scale (the block's largest magnitude / 448): r has half the range of v, and
@@ -25,21 +25,58 @@
 
 #include <math.h>
 
+#include <algorithm>
+
 namespace {
 
-constexpr int WG = 256, UNIT = 4096, MOST = 56, BLOCK = TACE_ADAM_BLOCK;
+constexpr int WG = 256, UNIT = 4096, BLOCK = TACE_ADAM_BLOCK;
 
+// a tensor as a launch has it: for the norm, without masters and scales, with them
+struct Gradient {
+  static constexpr int MOST = 160;
+  const void* g;
+  int64_t n;
+  Gradient() = default;
+  explicit Gradient(const tace_adam_tensor& t) : g(t.g), n(t.n) {}
+};
+struct Plain {
+  static constexpr int MOST = 84;
+  void* p;
+  const void* g;
+  void *m, *s;
+  int64_t n;
+  Plain() = default;
+  explicit Plain(const tace_adam_tensor& t) : p(t.p), g(t.g), m(t.m), s(t.s), n(t.n) {}
+  __device__ __forceinline__ void* the_master() const { return nullptr; }
+  __device__ __forceinline__ float* the_scales() const { return nullptr; }
+};
+struct Full : Plain {
+  static constexpr int MOST = 56;
+  void* master;
+  float* scales;
+  Full() = default;
+  explicit Full(const tace_adam_tensor& t) : Plain(t), master(t.master), scales((float*)t.scales) {}
+  __device__ __forceinline__ void* the_master() const { return master; }
+  __device__ __forceinline__ float* the_scales() const { return scales; }
+};
+
+template <typename E>
 struct Tensors {
-  tace_adam_tensor t[MOST];
-  int first[MOST + 1];   // units of the tensors before
+  E t[E::MOST];
+  int first[E::MOST + 1];   // units of the tensors before
   int count;
 };
 
 // the tensor of a unit (uniform over the workgroup)
-__device__ __forceinline__ int tensor_of(const Tensors& ts, int unit) {
-  const int lane = (int)threadIdx.x & 63;
-  const bool before = lane < ts.count && ts.first[lane < MOST ? lane : 0] <= unit;
-  return __builtin_amdgcn_readfirstlane(__popcll(__ballot(before)) - 1);
+template <typename E>
+__device__ __forceinline__ int tensor_of(const Tensors<E>& ts, int unit) {
+  int before = 0;
+#pragma unroll
+  for (int at = 0; at < E::MOST; at += 64) {
+    const int k = at + ((int)threadIdx.x & 63);
+    before += __popcll(__ballot(k < ts.count && ts.first[k < E::MOST ? k : 0] <= unit));
+  }
+  return __builtin_amdgcn_readfirstlane(before - 1);
 }
 
 // ------------------------------------------------------------------- norm ----
@@ -57,7 +94,7 @@ __device__ __forceinline__ double over_wg(S v, double* lds) {
 }
 
 template <typename T>
-__global__ __launch_bounds__(WG) void k_grad_norm(Tensors ts, double* __restrict__ part, int slot0, int slots,
+__global__ __launch_bounds__(WG) void k_grad_norm(Tensors<Gradient> ts, double* __restrict__ part, int slot0, int slots,
                                                   bool last, unsigned long long* ticket, bool wide,
                                                   void* __restrict__ norm) {
   typedef row_sum_t<T> S;
@@ -209,15 +246,15 @@ __device__ __forceinline__ void store4(T* p, int n, const row_sum_t<T>* a) {
 // A unit of up to 4,096 elements; V = 4: whole, its addresses multiples of four
 // elements (a lane's four go as one move each).  EIGHT: a wavefront's 256
 // elements are a block.
-template <typename T, bool EIGHT, int V>
-__device__ __forceinline__ void run_unit(const Step<row_sum_t<T>>& st, const tace_adam_tensor& t, int tensor,
+template <typename T, bool EIGHT, int V, typename E>
+__device__ __forceinline__ void run_unit(const Step<row_sum_t<T>>& st, const E& t, int tensor,
                                          int64_t i0, int n, long long steps) {
   typedef row_sum_t<T> S;
   constexpr int U = sizeof(T) == 8 ? 2 : 4;   // passes whose loads go out together
-  const bool master = t.master != nullptr;
+  const bool master = t.the_master() != nullptr;
   T* p = (T*)t.p + i0;
   const T* g = (const T*)t.g + i0;
-  S* w = master ? (S*)t.master + i0 : nullptr;
+  S* w = master ? (S*)t.the_master() + i0 : nullptr;
   const int lane = (int)threadIdx.x & 63;
 #pragma unroll
   for (int r = 0; r < UNIT / (4 * WG); r += U) {
@@ -244,7 +281,7 @@ __device__ __forceinline__ void run_unit(const Step<row_sum_t<T>>& st, const tac
             }
           }
         }
-        const float2 sc = ((const float2*)t.scales)[(i0 + i - 4 * lane) / BLOCK];
+        const float2 sc = ((const float2*)t.the_scales())[(i0 + i - 4 * lane) / BLOCK];
         sm[u] = sc.x;
         sr[u] = sc.y;
         mv[u][0] = __builtin_amdgcn_cvt_f32_fp8(cm, 0), mv[u][1] = __builtin_amdgcn_cvt_f32_fp8(cm, 1);
@@ -298,7 +335,7 @@ __device__ __forceinline__ void run_unit(const Step<row_sum_t<T>>& st, const tac
             }
           }
         }
-        if (lane == 0) ((float2*)t.scales)[at / BLOCK] = sc;
+        if (lane == 0) ((float2*)t.the_scales())[at / BLOCK] = sc;
       } else {
         store4<V>((S*)t.m + i0 + i, left, mv[u]);
         store4<V>((S*)t.s + i0 + i, left, sv[u]);
@@ -308,19 +345,19 @@ __device__ __forceinline__ void run_unit(const Step<row_sum_t<T>>& st, const tac
 }
 
 // whether a unit's operands can be moved four elements at a time
-template <typename T, bool EIGHT>
-__device__ __forceinline__ bool fours(const tace_adam_tensor& t, int64_t i0) {
+template <typename T, bool EIGHT, typename E>
+__device__ __forceinline__ bool fours(const E& t, int64_t i0) {
   const uintptr_t a4 = (uintptr_t)((T*)t.p + i0) | (uintptr_t)((const T*)t.g + i0);
   uintptr_t s4 = EIGHT ? ((uintptr_t)t.m | (uintptr_t)t.s) * sizeof(row_sum_t<T>) : (uintptr_t)t.m | (uintptr_t)t.s;
-  if (t.master) s4 |= (uintptr_t)t.master;
+  s4 |= (uintptr_t)t.the_master();
   return a4 % (4 * sizeof(T)) == 0 && s4 % (4 * sizeof(row_sum_t<T>)) == 0;
 }
 
-template <typename T, bool EIGHT>
-__global__ __launch_bounds__(WG) void k_adamw(Tensors ts, Step<row_sum_t<T>> st) {
+template <typename T, bool EIGHT, typename E>
+__global__ __launch_bounds__(WG) void k_adamw(Tensors<E> ts, Step<row_sum_t<T>> st) {
   typedef row_sum_t<T> S;
   const int unit = (int)blockIdx.x, k = tensor_of(ts, unit);
-  const tace_adam_tensor& t = ts.t[k];
+  const E& t = ts.t[k];
   const int64_t i0 = (int64_t)(unit - ts.first[k]) * UNIT, left = t.n - i0;
   const int n = (int)(left < UNIT ? left : UNIT);
   long long steps = st.counter[0] + 1;
@@ -363,23 +400,25 @@ int check_tensors(int type, const tace_adam_tensor* t, int64_t count, bool state
   return 0;
 }
 
-// calls f(tensors, index of the first, whether they are the last) for launches of up to 56 tensors
-template <typename F>
+// calls f(tensors, index of the first, whether they are the last) for launches of as
+// many tensors as fit.  (60 of 1 to 131,072 elements: a step takes 27 us in one
+// launch, 32 in two.)
+template <typename E, typename F>
 bool chunks(const tace_adam_tensor* t, int64_t count, F&& f) {
   int64_t end = count;
   while (end > 0 && t[end - 1].n == 0) --end;
-  Tensors ts;
+  Tensors<E> ts;
   ts.count = 0;
   ts.first[0] = 0;
   int64_t from = 0;
   for (int64_t i = 0; i < end; ++i) {
     const int64_t units = (t[i].n + UNIT - 1) / UNIT;
-    if (ts.count && ((int64_t)ts.first[ts.count] + units > (1 << 23) || ts.count == MOST)) {
-      f(ts, from, false);
+    if (ts.count && ((int64_t)ts.first[ts.count] + units > (1 << 23) || ts.count == E::MOST)) {
+      if (ts.first[ts.count]) f(ts, from, false);   // (not where all are empty)
       ts.count = 0;
       from = i;
     }
-    ts.t[ts.count] = t[i];
+    ts.t[ts.count] = E(t[i]);
     ts.first[ts.count + 1] = ts.first[ts.count] + (int)units;
     ++ts.count;
   }
@@ -387,14 +426,16 @@ bool chunks(const tace_adam_tensor* t, int64_t count, F&& f) {
   return ts.count > 0;
 }
 
-constexpr int NORM_WGS = 1024;
-int norm_wgs(const Tensors& ts) {
+// Workgroups of a norm: four units each, 256 to 1,024.  The last one's ticket is one
+// address for all, about 10 ns each: 968 units take 12.2 us with 256, 14.7 with
+// 512, 20.0 with 968 workgroups; 35,000 units 283, 235 and (1,024) 219 us.
+int norm_wgs(const Tensors<Gradient>& ts) {
   const int units = ts.first[ts.count];
-  return units < NORM_WGS ? units : NORM_WGS;
+  return std::min(units, std::min(std::max(units / 4, 256), 1024));
 }
 int64_t norm_slots(const tace_adam_tensor* t, int64_t count) {
   int64_t slots = 0;
-  chunks(t, count, [&](const Tensors& ts, int64_t, bool) { slots += norm_wgs(ts); });
+  chunks<Gradient>(t, count, [&](const Tensors<Gradient>& ts, int64_t, bool) { slots += norm_wgs(ts); });
   return slots;
 }
 
@@ -415,7 +456,7 @@ extern "C" int tace_grad_norm(int type, const tace_adam_tensor* tensors, int64_t
   row_dispatch(type, [&](auto zero) {
     typedef decltype(zero) T;
     int64_t slot0 = 0;
-    chunks(tensors, count, [&](const Tensors& ts, int64_t, bool last) {
+    chunks<Gradient>(tensors, count, [&](const Tensors<Gradient>& ts, int64_t, bool last) {
       hipLaunchKernelGGL((k_grad_norm<T>), dim3((unsigned)norm_wgs(ts)), dim3(WG), 0, (hipStream_t)stream, ts,
                          (double*)work, (int)slot0, (int)slots, last, (unsigned long long*)ticket,
                          type == TACE_ROW_F64, norm);
@@ -445,18 +486,26 @@ extern "C" int tace_adamw(int type, int eight, const tace_adam_tensor* tensors, 
     st.log_b1 = (S)::log(beta1), st.log_b2 = (S)::log(beta2);
     st.lr_at = lr_at, st.lr_wide = lr_wide, st.norm = norm, st.counter = (long long*)counter;
     st.seed_lo = (unsigned)seed, st.seed_hi = (unsigned)(seed >> 32);
-    chunks(tensors, count, [&](const Tensors& ts, int64_t from, bool last) {
-      st.tensor0 = (unsigned)from;
-      st.ticks = last;
-      const dim3 grid((unsigned)ts.first[ts.count]);
-      if constexpr (!std::is_same<T, double>::value) {
-        if (eight) {
-          hipLaunchKernelGGL((k_adamw<T, true>), grid, dim3(WG), 0, (hipStream_t)stream, ts, st);
-          return;
-        }
-      }
-      hipLaunchKernelGGL((k_adamw<T, false>), grid, dim3(WG), 0, (hipStream_t)stream, ts, st);
-    });
+    auto launch = [&](auto eight_type, auto entry) {
+      typedef decltype(entry) E;
+      constexpr bool EIGHT = decltype(eight_type)::value;
+      static_assert(sizeof(Tensors<E>) + sizeof(Step<S>) <= 4096, "a launch's arguments");
+      chunks<E>(tensors, count, [&](const Tensors<E>& ts, int64_t from, bool last) {
+        st.tensor0 = (unsigned)from;
+        st.ticks = last;
+        hipLaunchKernelGGL((k_adamw<T, EIGHT, E>), dim3((unsigned)ts.first[ts.count]), dim3(WG), 0, (hipStream_t)stream, ts,
+                           st);
+      });
+    };
+    if constexpr (!std::is_same<T, double>::value) {
+      if (eight) return launch(std::true_type(), Full());
+    }
+    bool masters = false;
+    for (int64_t i = 0; i < count; ++i) masters |= tensors[i].master != nullptr;
+    if constexpr (!std::is_same<T, S>::value) {
+      if (masters) return launch(std::false_type(), Full());
+    }
+    launch(std::false_type(), Plain());
   });
   return tace_check_launch("adamw");
 }

@@ -1712,7 +1712,7 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
                masters: Optional[Sequence[torch.Tensor]] = None, max_norm: Optional[float] = None,
                norm: Optional[torch.Tensor] = None, seed: int = 0) -> Optional[torch.Tensor]:
     """One step of AdamW, in place, over all ``params`` (contiguous, one row type)
-    in one launch for each 56 of them; ``tace_amd.optim.AdamW`` is the optimiser
+    in few launches (56 to 84 tensors each); ``tace_amd.optim.AdamW`` is the optimiser
     around it.
 
     ``exp_avgs``, ``exp_avg_sqs``: the averages of g and g^2, of the parameters'

@@ -2,8 +2,8 @@
 
 ``AdamW`` is a ``torch.optim.Optimizer`` (parameter groups, ``state_dict``,
 schedulers, hooks) whose step is ``ops.adamw_step``: the parameters of a type in
-one launch for each 56 of them, the clipping norm in one more, states in 32 bits
-or in 8."""
+few launches (56 to 84 of them each), the clipping norm in one for each 160,
+states in 32 bits or in 8."""
 
 from __future__ import annotations
 

@@ -166,6 +166,15 @@ def test_many_tensors_and_large_ones(cuda):
     _run(Case(cuda, torch.bfloat16, [(2_000_001,), (7,), (1 << 20,)], 8, True), 0.3)
 
 
+@pytest.mark.parametrize("before", [56, 84, 160, 330])
+def test_empty_tensors_before_others(cuda, before):
+    """(a launch's worth of tensors without an element)"""
+    for dt, bits, masters in ((torch.float32, 32, False), (torch.bfloat16, 32, True), (torch.float32, 8, False)):
+        _run(Case(cuda, dt, [(0,)] * before + [(5,), (0,), (300,)], bits, masters), 0.3)
+    g = [torch.zeros(0, device=cuda)] * before + [torch.full((4,), 3.0, device=cuda)]
+    assert float(ops.grad_norm(g)) == 6.0
+
+
 def test_elements_past_32_bits(cuda):
     """A parameter of 2^31 + 4097 elements: those at its end are stepped as those of a small one."""
     n = 2 ** 31 + 4097
