@@ -177,12 +177,8 @@ struct Places {
 struct Share {
   int first, end, step;
 };
-__device__ __forceinline__ Share share_of(int tiles, bool apart) {
+__device__ __forceinline__ Share share_of(int tiles) {
   const int x = (int)(blockIdx.x & 7);
-  if (apart) {
-    const int n = (int)gridDim.x, i = x * (n >> 3) + (int)(blockIdx.x >> 3);
-    return {(int)((int64_t)tiles * i / n), (int)((int64_t)tiles * (i + 1) / n), 1};
-  }
   return {(int)((int64_t)tiles * x / 8) + (int)(blockIdx.x >> 3), (int)((int64_t)tiles * (x + 1) / 8), (int)(gridDim.x >> 3)};
 }
 
@@ -1052,15 +1048,14 @@ __device__ __forceinline__ void walk(const T* __restrict__ a, const T* __restric
 template <typename T, bool BT, int WM, int WN, int FM, int FN, bool FAST>
 __global__ __launch_bounds__(64 * WM * WN, waves_for(FM * FN)) void k_expert_rows(
     const T* __restrict__ x, const T* __restrict__ weight, Groups gr, int64_t wsize, int sum, int n, row_sum_t<T> scale,
-    T* __restrict__ out, int cols, bool apart) {
+    T* __restrict__ out, int cols) {
   constexpr int TM = 16 * WM * FM, TN = 16 * WN * FN;
   const int slots = Places<true, false>(gr, __builtin_ctz(TM)).total();
   walk<T, false, BT, WM, WN, FM, FN, FAST>(
-      x, weight, sum, BT ? n : sum, share_of(slots * cols, apart),
+      x, weight, sum, BT ? n : sum, share_of(slots * cols),
       [&](int t) {   // (asked for again for every 64 tiles: nothing of it stays in registers)
         int slot, col;
-        if (apart) slot = t / cols, col = t % cols;
-        else blocked(t, slots, cols, &slot, &col);
+        blocked(t, slots, cols, &slot, &col);
         const Place p = Places<true, false>(gr, __builtin_ctz(TM)).find(slot);
         const int c0 = col * TN;
         return Job{p.first * sum,
@@ -1193,9 +1188,9 @@ __global__ __launch_bounds__(64 * WM * WN, waves_for(FM * FN)) void k_expert_wei
 // dW of the groups of several stretches: their pieces' sums in order
 template <typename T, int TM, int TN>
 __global__ __launch_bounds__(WG) void k_expert_join(const row_sum_t<T>* __restrict__ part, Groups gr, int K, int N,
-                                                    row_sum_t<T> scale, T* __restrict__ dw, int per, int cols, int cuts) {
+                                                    row_sum_t<T> scale, T* __restrict__ dw, int per, int cols, int cuts, int parts) {
   typedef row_sum_t<T> s4v __attribute__((ext_vector_type(4)));
-  const int64_t tile = blockIdx.x >> 3;
+  const int64_t tile = blockIdx.x / parts;
   const int grp = (int)(tile / per), place = (int)(tile - (int64_t)grp * per);
   Units units(gr);
   const int64_t total = units.total();
@@ -1218,9 +1213,9 @@ __global__ __launch_bounds__(WG) void k_expert_join(const row_sum_t<T>* __restri
   const int64_t step = (int64_t)2 * per * TM * TN;
   // (the first stretch's piece is of its last group, if it has more)
   const int64_t lead = cut_of(total, i0, cuts) < s.first ? step / 2 : 0;
-  constexpr int SHARE = TM * TN / 8;
-  for (int q = 4 * (int)threadIdx.x; q < SHARE; q += 4 * WG) {
-    const int at = (int)(blockIdx.x & 7) * SHARE + q, i = at / TN, j = at % TN;
+  const int share = TM * TN / parts;
+  for (int q = 4 * (int)threadIdx.x; q < share; q += 4 * WG) {
+    const int at = (int)(blockIdx.x % parts) * share + q, i = at / TN, j = at % TN;
     if (r0 + i >= K || c0 + j >= N) continue;
     const row_sum_t<T>* p = part + (int64_t)place * TM * TN + at + i0 * step;
     s4v sum = *(const s4v*)(p + lead);
@@ -1306,7 +1301,7 @@ int64_t slots_of(const Groups& gr, int shift) {
 template <typename T, bool FAST>
 constexpr bool has_tile(int tm, int tn) {
   if (std::is_same<T, double>::value) return !FAST && tm == 64;
-  return STREAMS<T, FAST> ? tm >= 32 : tm == 128 || tm == 64 || tm == 16;
+  return tm >= (STREAMS<T, FAST> ? 64 : 16);
 }
 
 template <typename F>
@@ -1319,14 +1314,19 @@ unsigned grid_of(int64_t tiles) { return (unsigned)((tiles + 7) / 8 * 8); }
 // workgroups that walk over tiles: as many as run at once
 unsigned walkers(int64_t tiles, int most) { return grid_of(tiles < most ? tiles : most); }
 
-// Tiles of 128 x 128 where they fill the card, 64 x 64 below, 16 x 128 for
-// experts of a few rows each (a product then reads its weights once and little
-// else; higher tiles would be mostly empty).
-enum { T128, T64, T32, T16 };
+// Tiles of 128 x 128 where there are 512 full ones, as many as run at once, 64 x 64
+// below: 32,768 rows of 256 x 512 in bfloat16 take 18.5 us with the one and 21.3
+// with the other, 8,192 rows 9.9 and 9.6, 2,048 rows of 128 x 128 in float32 12.8
+// and 7.4, 768 rows of 1024 x 4096 for 16 experts 98.9 and 74.6.  16 x 128 for
+// experts of up to 24 rows each in what does not stream (a product reads its
+// weights once and little else): 48 rows there 53 us and, with 64 x 64, 67; 384
+// rows 63 and 68, 768 rows 106 and 75.
+enum { T128, T64, T16 };
+bool fills(int64_t rows, int64_t cols) { return (rows >> 7) * ((cols + 127) / 128) >= 512; }
 int rows_tile(const Groups& gr, int n, bool streams) {
   const int64_t rows = gr.rows * total_comps(gr), groups = (int64_t)gr.blocks * (gr.experts > 0 ? gr.experts : 1);
-  if (rows <= 24 * groups) return streams ? T32 : T16;
-  return slots_of(gr, 7) * ((n + 127) / 128) >= 512 ? T128 : T64;
+  if (!streams && rows <= 24 * groups) return T16;
+  return fills(rows, n) ? T128 : T64;
 }
 
 template <typename F>
@@ -1337,17 +1337,19 @@ void with_tile(int tile, F&& f) {
   typedef integral_constant<int, 4> I4;
   if (tile == T128) f(I2(), I2(), I4(), I4());
   else if (tile == T64) f(I2(), I2(), I2(), I2());
-  else if (tile == T32) f(I1(), I4(), I2(), I2());
   else f(I1(), I4(), I1(), I2());
 }
 
-// The weight gradient's tiles, and the workgroups that share its units.
-int weight_tile(int type, int K, int N) {
-  return type == TACE_ROW_F64 || K <= 64 || N <= 64 ? T64 : T128;
-}
+// The weight gradient's tiles, by the same rule: 2,048 rows of 128 x 128 in float32
+// take 22 us with 128 x 128 and 16 with 64 x 64, 196,608 rows 72 and 74; 202,752
+// rows of 256 x 512 in bfloat16 96 and 149.
 int64_t tiles_of(int tile, int K, int N) {
   const int64_t t = tile == T64 ? 64 : 128;
   return ((K + t - 1) / t) * ((N + t - 1) / t);
+}
+int weight_tile(int type, const Groups& gr, int K, int N) {
+  const bool wide = type != TACE_ROW_F64 && K > 64 && N > 64;
+  return wide && fills(gr.rows * total_comps(gr), 128 * tiles_of(T128, K, N)) ? T128 : T64;
 }
 // whether a group may have more than a unit
 bool may_be_cut(const Groups& gr) {
@@ -1403,7 +1405,7 @@ extern "C" int tace_expert_linear(int type, int transposed, const void* x, const
           hipLaunchKernelGGL((k_expert_rows<T, BT, WM, WN, FM, FN, FAST>),
                              dim3(STREAMS<T, FAST> ? walkers(tiles, TM == 128 ? 512 : 1024) : grid_of(tiles)),
                              dim3(64 * WM * WN), 0, (hipStream_t)stream, (const T*)x, (const T*)weight, gr, wsize, sum, n,
-                             (S)scale, (T*)out, (int)cols, sum <= 256);
+                             (S)scale, (T*)out, (int)cols);
       });
     });
   });
@@ -1418,7 +1420,7 @@ extern "C" int64_t tace_expert_linear_grad_work(int type, int64_t rows, int32_t 
   if (check_groups(rows, experts, blocks, comps, K, N, &none, &gr)) return -1;
   if (type < 0 || type > TACE_ROW_F16) return tace_fail_msg("expert_linear: unknown row type"), -1;
   if (experts == 0 || rows == 0) return 0;
-  const int tile = weight_tile(type, K, N);
+  const int tile = weight_tile(type, gr, K, N);
   const int64_t per = tiles_of(tile, K, N), side = tile == T64 ? 64 : 128;
   const Teams teams = teams_of(tile, gr, per);
   return teams.cuts > 1 && may_be_cut(gr) ? 2 * per * teams.cuts * side * side * (type == TACE_ROW_F64 ? 8 : 4) : 0;
@@ -1432,15 +1434,19 @@ extern "C" int tace_expert_linear_grad(int type, const void* x, const void* g, c
   if (type < 0 || type > TACE_ROW_F16) return tace_fail_msg("expert_linear: unknown row type");
   if (experts == 0) return 0;
   if ((rows && (!x || !g)) || !dw) return tace_fail_msg("expert_linear: null argument");
-  const int tile = weight_tile(type, K, N);
+  const int tile = weight_tile(type, gr, K, N);
   const int64_t per = tiles_of(tile, K, N);
-  if ((int64_t)blocks * experts * per > MOST_WGS / 8) return tace_fail_msg("expert_linear: bad sizes");
+  if ((int64_t)blocks * experts * per > MOST_WGS / 16) return tace_fail_msg("expert_linear: bad sizes");
   const Teams teams = teams_of(tile, gr, per);
   const bool joins = teams.cuts > 1 && may_be_cut(gr);
   if (joins && (!work || !row_aligned(work) ||
                 work_bytes < tace_expert_linear_grad_work(type, rows, experts, blocks, comps, K, N)))
     return tace_fail_msg("expert_linear: the workspace is too small or not 16-byte aligned");
   const unsigned n = grid_of((int64_t)teams.cuts * teams.team);
+  // workgroups of a tile's sums: one move a thread, fewer where there are many tiles (32 tiles of 128 x 128: 15.2 us with
+  // 16, 19.6 with 8, 32.7 with 4; 1,024 tiles: 19.6 with 4, 30.7 with 8)
+  int parts = tile == T64 ? 4 : 16;
+  while (parts > 2 && parts * (int64_t)blocks * experts * per > 4096) parts /= 2;
   const hipStream_t st = (hipStream_t)stream;
   const bool fast = type != TACE_ROW_F64 && K % 8 == 0 && N % 8 == 0 && row_aligned(x) && row_aligned(g) && row_aligned(dw);
   row_dispatch(type, [&](auto zero) {
@@ -1456,8 +1462,8 @@ extern "C" int tace_expert_linear_grad(int type, const void* x, const void* g, c
                              st, (const T*)x, (const T*)g, gr, K, N, (S)scale, (T*)dw, (S*)work, (int)per, cols, teams.cuts, teams.team);
         });
         if (joins)
-          hipLaunchKernelGGL((k_expert_join<T, TM, TN>), dim3((unsigned)(8 * blocks * experts * per)), dim3(WG), 0, st,
-                             (const S*)work, gr, K, N, (S)scale, (T*)dw, (int)per, cols, teams.cuts);
+          hipLaunchKernelGGL((k_expert_join<T, TM, TN>), dim3((unsigned)(parts * blocks * experts * per)), dim3(WG), 0, st,
+                             (const S*)work, gr, K, N, (S)scale, (T*)dw, (int)per, cols, teams.cuts, parts);
       }
     });
   });
@@ -1485,13 +1491,11 @@ extern "C" int tace_expert_linear_e4m3(int out_type, const void* x, const float*
       with_tile(rows_tile(gr, N, false), [&](auto wm, auto wn, auto fm, auto fn) {
         constexpr int WM = decltype(wm)::value, WN = decltype(wn)::value, FM = decltype(fm)::value, FN = decltype(fn)::value;
         constexpr int TM = 16 * WM * FM, TN = 16 * WN * FN;
-        if constexpr (TM != 32) {
         const int64_t cols = (N + TN - 1) / TN, tiles = slots_of(gr, __builtin_ctz(TM)) * cols;
         if (!(fits = tiles <= MOST_WGS)) return;
         hipLaunchKernelGGL((k_expert_codes<O, WM, WN, FM, FN>), dim3(grid_of(tiles)), dim3(WG), 0, (hipStream_t)stream,
                            (const E4m3*)x, x_scale, order, (unsigned)choices, (int)(rows / choices),
                            (const E4m3*)weight, w_scale, gr, K / 2, N, (O*)out, (int)tiles, (int)cols);
-        }
       });
     }
   });

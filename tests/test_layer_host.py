@@ -168,7 +168,8 @@ def test_expert_workspace_covers_every_part():
                 for comps in ((1,), (1, 3, 5, 7)):
                     for K, M in ((16, 8), (128, 128), (1024, 2048), (8192, 8192)):
                         nbytes = L.tace_expert_linear_grad_work(ty, rows, E, len(comps), _ints(*comps), K, M)
-                        side = 64 if ty == 1 or min(K, M) <= 64 else 128
+                        tiles = -(-K // 128) * -(-M // 128)
+                        side = 64 if ty == 1 or min(K, M) <= 64 or rows * sum(comps) // 128 * tiles < 512 else 128
                         tiles = -(-K // side) * -(-M // side)
                         cuts, rest = divmod(nbytes, 2 * tiles * side * side * size)
                         assert rest == 0
