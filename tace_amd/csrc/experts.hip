@@ -8,22 +8,34 @@
 // are one kernel over output tiles: A [M, n] B [n, N] with either operand stored
 // along the summed index or across it.
 //
-// Tiles without a table: every workgroup sums the groups' tiles up to each over its
-// lanes and looks its own up there, so the host launches for a bound (rows /
-// height + groups) and the tiles that exist are shared out evenly.
+// Tiles without a table: every wavefront sums the groups' tiles up to each over its
+// lanes and looks its own up there.  The products of rows are launched for a bound
+// (rows / height + groups) and share out the tiles that exist; the weights'
+// gradients cut the rows into stretches (see Units).
 //
-// Tiles pass through LDS, the next step's loads in registers meanwhile.  An
-// operand stored along the summed index is read from LDS as 16-byte fragments,
-// one stored across it by the transposing read (ds_read_b64_tr_b16).  LDS rows
-// are permuted in 16- or 32-byte pieces so that either read meets every bank
-// once.  bfloat16 and float16 go to the MFMA as they are, float32 as three
-// bfloat16 terms (bf16x3.h, split as it enters LDS), e4m3 codes as the bfloat16
-// of the same value; sums are float32.  (The MFMA of 8-bit codes has twice the
-// rate, but aligns the products it adds to few bits: off by up to 2^-11.9 of the
-// largest product for random codes of all exponents and 2^-17 of the sum of
-// magnitudes for normally distributed ones, 16 x 16 x 128 and 16 x 16 x 32 alike.
-// Few tokens are bound by reading the weights, which either form does once.)
-// float64 has a kernel of its own.
+// 16-bit elements with sizes of multiples of eight and aligned rows are streamed:
+// loads write LDS themselves, a step of 64 ahead, over all tiles of a workgroup
+// without a pause (stream_products).  What else there is goes to LDS through
+// registers (product): float32 as three bfloat16 terms (bf16x3.h, split on the
+// way), e4m3 codes as they are, odd sizes element by element; float64 has its own
+// MFMA (product_f64).  An operand stored along the summed index is read from LDS
+// as 16-byte fragments, one stored across it by the transposing read
+// (ds_read_b64_tr_b16); LDS rows are permuted in 16- or 32-byte pieces so that
+// either read meets every bank once.  Sums are float32 (double for float64).
+//
+// e4m3 codes are multiplied as the bfloat16 of the same value.  The MFMA of 8-bit
+// codes has twice the rate, but aligns the products it adds to few bits: off by up
+// to 2^-11.9 of the largest product for random codes of all exponents and 2^-17 of
+// the sum of magnitudes for normally distributed ones, 16 x 16 x 128 and 16 x 16 x
+// 32 alike.  Few tokens are bound by reading the weights, which either form does
+// once: 24 tokens, 2 of 16 experts each, 1024 x 4096: 15 us, 4.5 TB/s.
+//
+// Measured, us (forward, rows' gradient, weights' gradient): bfloat16, 32,768 rows
+// of 8 experts of 1024 x 2048: 174, 187, 167 + 20 (137 GFLOP each; 790, 735 and 735
+// TFLOP/s, from caches that hold other data; 950 forward from warm ones); 202,752
+// rows of 16 experts of 256 x 512, bound by memory and the latency of four steps a
+// tile: 108, 93, 81 + 14 (311 MB each, 2.9 to 3.3 TB/s).  float32, 196,608 rows of
+// 128 x 128 (its three terms' MFMA takes as long as the memory): 66, 67, 54 + 15.
 #include "bf16x3.h"
 #include "row_types.h"
 
@@ -265,10 +277,9 @@ struct Tile {
   // LDS place (16-bit elements) of a piece of eight
   __device__ __forceinline__ static int lds_at(int line, int piece) {
     if constexpr (ACROSS) {
-      // 32-byte slots: eight (four, two) lines share the banks a transposing read's half wave takes
-      constexpr int SLOTS = TM / 16;
-      const int f = SLOTS >= 8 ? (line & 3) | ((line >> 1) & 4) : SLOTS == 4 ? ((line >> 1) & 1) | ((line >> 2) & 2)
-                                                                            : (line >> 3) & (SLOTS - 1);
+      // 32-byte slots: eight (four) lines share the banks a transposing read's half wave takes
+      static_assert(TM % 64 == 0, "tiles of 64 or 128");
+      const int f = TM >= 128 ? (line & 3) | ((line >> 1) & 4) : ((line >> 1) & 1) | ((line >> 2) & 2);
       return line * TM + (((piece >> 1) ^ f) << 4) + ((piece & 1) << 3);
     } else {
       return line * BK + ((piece ^ (BK == 64 ? (line >> 1) & 7 : (line >> 2) & 3)) << 3);
@@ -354,13 +365,13 @@ struct Tile {
 template <typename T, int TM, bool ACROSS>
 struct WideTile {
   static constexpr int BK = 64, ELEMS = TM * BK;
-  static_assert(sizeof(T) == 2 && TM % 32 == 0, "16-bit tiles of 32");
+  static_assert(sizeof(T) == 2 && TM % 64 == 0, "16-bit tiles");
 
   __device__ __forceinline__ static int lds_at(int line, int piece) {
     if constexpr (ACROSS) {
       // (16 lanes read 32 bytes of four lines; lines 8 apart, and the 32 bytes
       // beside, are read by the other lanes)
-      const int f = (TM >= 128 ? (line & 3) << 1 : TM == 64 ? line & 2 : 0) | ((line >> 3) & 1);
+      const int f = (TM >= 128 ? (line & 3) << 1 : line & 2) | ((line >> 3) & 1);
       return line * TM + (((piece >> 1) ^ f) << 4) + ((piece & 1) << 3);
     } else {
       return line * BK + ((piece ^ ((line >> 1) & 7)) << 3);
@@ -589,13 +600,12 @@ template <typename T, int TM, bool ACROSS, int WAVES>
 struct Stream {
   typedef WideTile<T, TM, ACROSS> L;
   static constexpr int BK = L::BK, LINE = (ACROSS ? TM : BK) * 2, LOADS = TM * BK * 2 / 1024;
-  static constexpr int COUNT = (LOADS + WAVES - 1) / WAVES;   // a wavefront's
+  static constexpr int COUNT = LOADS / WAVES;                 // a wavefront's
   static constexpr int LINES = 1024 / LINE;                   // a load's
-  static constexpr bool EVEN = LOADS % WAVES == 0;
   static constexpr unsigned NONE = 0x80000000u;
   // lines that differ by a multiple of 16 are permuted alike
   static constexpr int KINDS = COUNT < 16 / LINES ? COUNT : 16 / LINES;
-  static_assert(sizeof(T) == 2 && TM * BK * 2 % 1024 == 0 && LINES >= 1 && LINES <= 16, "whole loads");
+  static_assert(sizeof(T) == 2 && LOADS % WAVES == 0 && LINES >= 1 && LINES <= 16, "whole loads, as many for each");
 
   const T* p;
   unsigned ld, range;    // bytes of a line, and up to the end of the last one with values
@@ -640,7 +650,6 @@ struct Stream {
     };
 #pragma unroll
     for (int j = 0; j < COUNT; ++j) {
-      if (!EVEN && first + j >= LOADS) break;
       const unsigned o = at[j % KINDS] + (unsigned)(j / KINDS * KINDS * LINES) * line_bytes;
       load(j, ACROSS || k[j % KINDS] < n ? o : NONE);   // (n may be negative: a step of zeros)
     }
@@ -704,7 +713,7 @@ __device__ __forceinline__ void stream_products(const T* __restrict__ a_base, co
   typedef WideTile<T, TN, BT> TB;
   typedef Stream<T, TM, AT, WM * WN> SA;
   typedef Stream<T, TN, BT, WM * WN> SB;
-  constexpr int NEXT = SA::EVEN && SB::EVEN ? SA::COUNT + SB::COUNT : 0;   // a step's loads of every wavefront
+  constexpr int NEXT = SA::COUNT + SB::COUNT;   // a step's loads of a wavefront
   // (arrays of their own: the compiler then knows which loads a read waits for)
   __shared__ __attribute__((aligned(16))) unsigned short even[TA::ELEMS + TB::ELEMS], odd[TA::ELEMS + TB::ELEMS];
   const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;

@@ -126,6 +126,46 @@ def test_large(cuda, dt, rows, E, K, N):
     _check(cuda, dt, _sizes("skewed", rows, E, 3), E, K, N)
 
 
+@pytest.mark.parametrize("dt", R.TYPES, ids=ids)
+@pytest.mark.parametrize("rows,E,K,N", [(66000, 5, 128, 128), (22000, 4, 264, 264), (33000, 3, 129, 130)])
+def test_full_tiles(cuda, dt, rows, E, K, N):
+    """Enough rows for the largest tiles, in each of the three products."""
+    _check(cuda, dt, _sizes("dropped", rows, E, 4), E, K, N)
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float32], ids=ids)
+def test_every_size_of_a_group_by_full_tiles(cuda, dt):
+    e = torch.repeat_interleave(torch.arange(301), torch.arange(301))
+    _check(cuda, dt, e, 301, 200, 264)
+
+
+def test_many_tiles_for_each_workgroup(cuda):
+    """More than the 64 that a wavefront looks up at once."""
+    rows, E, K, N = 280_000, 3, 8, 2048
+    plan = _plan(cuda, _sizes("dropped", rows, E, 6), E)
+    x, w = _rand((rows, K), torch.bfloat16, 7), _rand((E, K, N), torch.bfloat16, 8)
+    y = ops.expert_linear(x.to(cuda), w.to(cuda), plan)
+    ends = plan.rowptr.tolist()
+    assert not y[ends[-1]:].any()
+    for e in range(E):
+        at = torch.arange(ends[e], ends[e + 1], 499)
+        want, slack = _reference(x[at], w[e:e + 1].unsqueeze(1), [0, len(at)], [1], 1.0)
+        _close(y[at.to(cuda)], want, slack, "y")
+
+
+def test_many_groups_for_each_workgroup(cuda):
+    rows, E, K, N = 21_000, 700, 1024, 1024
+    plan = _plan(cuda, _sizes("dropped", rows, E, 9), E)
+    x, g = _rand((rows, K), torch.bfloat16, 10), _rand((rows, N), torch.bfloat16, 11)
+    lw = torch.zeros(E, K, N, dtype=torch.bfloat16, device=cuda, requires_grad=True)
+    (gw,) = torch.autograd.grad(ops.expert_linear(x.to(cuda), lw, plan), lw, g.to(cuda))
+    ends = plan.rowptr.tolist()
+    for e in range(0, E, 53):
+        i, j = ends[e], ends[e + 1]
+        dw, slack = _weight_reference(x[i:j], g[i:j], [0, j - i], [1], K, N, 1.0)
+        _close(gw[e], dw[0, 0], slack[0, 0], "dw")
+
+
 def test_every_size_of_a_group(cuda):
     """Experts of 0 .. 150 rows, across the tiles' heights."""
     e = torch.repeat_interleave(torch.arange(151), torch.arange(151))
