@@ -14,6 +14,11 @@
 // one block, their weights (and in the backward pass the weights' gradient) in
 // registers.  The gradient's sums leave a workgroup once: groups meet in LDS,
 // a second launch adds the workgroups in order.
+//
+// Measured (forward, backward with the weights' gradient): 12,288 rows of degrees 0
+// to 3 with 128 channels, float32, with residual: 78 + 93 us, 5.2 and 4.6 TB/s;
+// 8,191 rows of 4,096, bfloat16: 24 + 48 us, 5.7 and 4.2 TB/s; 101,306 rows of 256 to
+// 8 bits with residual: 30 to 40 us, 6.0 to 4.6 TB/s (a copy: 5.0).
 #include "row_types.h"
 
 namespace {
@@ -342,6 +347,7 @@ void row_shape(int nvec, F&& f) {
   else f(integral_constant<int, 1024>(), integral_constant<int, V < 8 ? 32 / V : 4>());   // (up to 32,768 elements)
 }
 
+// (twice as many in the backward pass take as long, and the second launch 3 us more)
 constexpr int FWD_WGS = 2048, BWD_WGS = 1024;
 
 int widest(int blocks, const int32_t* comps) {
@@ -350,20 +356,22 @@ int widest(int blocks, const int32_t* comps) {
   return top;
 }
 
-// workgroups of each block, by its share of the elements
+// Workgroups of each block, by its share of the time: a row waits for memory as long
+// as two components more take.  (By its elements alone the blocks of degree 0 were
+// last: 103 instead of 88 us in the backward pass of degrees 0 to 3.)
 NormParts make_parts(int64_t rows, int channels, int blocks, const int32_t* comps, int groups, int most) {
   NormParts pt;
   pt.count = blocks;
   pt.channels = channels;
   int total = 0;
-  for (int b = 0; b < blocks; ++b) total += comps[b];
+  for (int b = 0; b < blocks; ++b) total += comps[b] + 2;
   int before = 0, wgs = 0;
   for (int b = 0; b < blocks; ++b) {
     pt.comps[b] = comps[b];
     pt.before[b] = before;
     pt.first[b] = wgs;
     before += comps[b];
-    const int64_t need = (rows + groups - 1) / groups, share = (int64_t)most * comps[b] / total + 1;
+    const int64_t need = (rows + groups - 1) / groups, share = (int64_t)most * (comps[b] + 2) / total + 1;
     wgs += (int)(need < share ? need : share);
   }
   pt.first[blocks] = wgs;
