@@ -241,16 +241,21 @@ __device__ __forceinline__ Chunk<T> load_chunk(const T* p) {   // 16-byte aligne
   return c;
 }
 
-// the first n of eight elements anywhere, zeros behind them
+// the first n of eight elements anywhere, zeros behind them (eight go as 16-byte
+// loads, which need no alignment but that of the elements)
 template <typename T>
 __device__ __forceinline__ Chunk<T> load_some(const T* p, int n) {
   union {
     T e[8];
     Chunk<T> c;
   } r;
+  if (n >= 8) {
+    __builtin_memcpy(&r.c, p, sizeof(r.c));
+    return r.c;
+  }
   r.c = zero_chunk<T>();
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
+  for (int i = 0; i < 7; ++i)
     if (i < n) r.e[i] = p[i];
   return r.c;
 }
@@ -790,7 +795,6 @@ struct Put {
   int64_t ldo;
   int m, n;
   row_sum_t<O> scale;
-  bool fours;   // rows of a multiple of four, aligned
   const float *row_scale, *col_scale;   // of the tile's rows (by `rows` where given) and columns, or null
   const int* rows;
   __device__ __forceinline__ void one(int i, int j, float v) const {
@@ -804,12 +808,12 @@ struct Put {
     float s = (float)scale;
     if (row_scale) s *= row_scale[rows ? rows[i] : i];
     O* p = out + i * ldo + j;
-    if (fours) {
+    if (j + 4 <= n) {   // (one move, whatever the alignment)
       typedef O o4 __attribute__((ext_vector_type(4)));
       o4 o;
 #pragma unroll
       for (int r = 0; r < 4; ++r) o[r] = (O)(v[r] * (col_scale ? s * col_scale[j + r] : s));
-      *(o4*)p = o;
+      __builtin_memcpy(p, &o, sizeof(o));
     } else {
 #pragma unroll
       for (int r = 0; r < 4; ++r)
@@ -1073,7 +1077,7 @@ __global__ __launch_bounds__(64 * WM * WN, waves_for(FM * FN)) void k_expert_row
                    p.count <= 0 ? NO_TILE : p.expert < gr.experts ? PRODUCT : ZERO_TILE, 1};
       },
       [&](const Job& j) { zero_rows(out + j.out, n, j.m, j.n); },
-      [&](const Job& j) { return Put<T>{out + j.out, n, j.m, j.n, scale, FAST, nullptr, nullptr, nullptr}; });
+      [&](const Job& j) { return Put<T>{out + j.out, n, j.m, j.n, scale, nullptr, nullptr, nullptr}; });
 }
 
 // dW: the groups' rows as one line of units of 128 (a group without rows is one
@@ -1189,8 +1193,8 @@ __global__ __launch_bounds__(64 * WM * WN, waves_for(FM * FN)) void k_expert_wei
       },
       [&](const Job& j) { zero_rows(dw + j.out, N, j.m, j.n); },
       [&](const Job& j) {
-        return PutPart<T>{{dw + j.out, N, j.m, j.n, scale, FAST, nullptr, nullptr, nullptr},
-                          {part + j.out, TN, j.m, j.n, 1, true, nullptr, nullptr, nullptr}, j.whole != 0};
+        return PutPart<T>{{dw + j.out, N, j.m, j.n, scale, nullptr, nullptr, nullptr},
+                          {part + j.out, TN, j.m, j.n, 1, nullptr, nullptr, nullptr}, j.whole != 0};
       });
 }
 
@@ -1273,7 +1277,7 @@ __global__ __launch_bounds__(WG) void k_expert_codes(const E4m3* __restrict__ x,
   const Work<E4m3> w{order ? x : x + p.first * pairs, wt + (int64_t)c0 * pairs, pairs, pairs, pairs, m, nn,
                      order ? rows : nullptr};
   product<E4m3, false, false, WM, WN, FM, FN, true>(
-      w, Put<O>{o, n, m, nn, 1.0f, (n & 3) == 0 && ((uintptr_t)out & 15) == 0, order ? xs : xs + p.first,
+      w, Put<O>{o, n, m, nn, 1.0f, order ? xs : xs + p.first,
                      ws + (int64_t)p.expert * n + c0, order ? rows : nullptr});
 }
 
