@@ -100,16 +100,16 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        launches = [(group, ps) for group in self.param_groups for ps in self._launches(group)]
+        launches = [(k, group, ps) for k, group in enumerate(self.param_groups) for ps in self._launches(group)]
         self.norm = None
         if self.max_norm is not None and launches:
             by_type: Dict[torch.dtype, List[torch.Tensor]] = {}
-            for _, ps in launches:
+            for _, _, ps in launches:
                 by_type.setdefault(ps[0].dtype, []).extend(p.grad for p in ps)
             if len(launches) > 1:
                 norms = [ops.grad_norm(g) for g in by_type.values()]
                 self.norm = norms[0] if len(norms) == 1 else torch.stack([n.double() for n in norms]).square().sum().sqrt()
-        for group, ps in launches:
+        for k, group, ps in launches:
             states = [self.state[p] for p in ps]
             norm = self.norm
             if norm is not None:
@@ -120,7 +120,7 @@ class AdamW(torch.optim.Optimizer):
                 states[0]["step"], lr=group["lr"], betas=group["betas"], eps=group["eps"],
                 weight_decay=group["weight_decay"], scales=[s["scales"] for s in states] if self.bits == 8 else None,
                 masters=[s["master"] for s in states] if "master" in states[0] else None, max_norm=self.max_norm,
-                norm=norm, seed=(self.seed * 1000003 + self.param_groups.index(group) * 8191 + place) % 2 ** 64)
+                norm=norm, seed=(self.seed * 1000003 + k * 8191 + place) % 2 ** 64)
             if self.norm is None:
                 self.norm = got
         return loss

@@ -370,6 +370,23 @@ def test_state_dict_goes_on_where_it_was(cuda, dt, bits, tmp_path):
         other.load_state_dict(oa.state_dict())
 
 
+def test_groups_of_equal_shapes(cuda):
+    shapes = [(16, 8), (16, 8)]
+    a = [torch.nn.Parameter(_rand(s, i).to(cuda)) for i, s in enumerate(shapes * 2)]
+    b = [torch.nn.Parameter(p.detach().clone()) for p in a]
+    groups = lambda ps: [dict(params=ps[:2], lr=1e-2), dict(params=ps[2:], lr=3e-3, weight_decay=0.2)]
+    ours, theirs = optim.AdamW(groups(a), max_norm=0.5), torch.optim.AdamW(groups(b))
+    for k in range(3):
+        for i, (p, q) in enumerate(zip(a, b)):
+            p.grad = _rand(p.shape, 10 * k + i).to(cuda)
+            q.grad = p.grad.clone()
+        ours.step()
+        torch.nn.utils.clip_grad_norm_(b, 0.5)
+        theirs.step()
+    for p, q in zip(a, b):   # (clipping there divides by the norm and 1e-6)
+        assert torch.allclose(p, q, rtol=0, atol=1e-6)
+
+
 def test_recorded_steps_count(cuda):
     c = Case(cuda, torch.bfloat16, [(5000,), (300,)], 8, True, steps=0)
     d = Case(cuda, torch.bfloat16, [(5000,), (300,)], 8, True, steps=0)
