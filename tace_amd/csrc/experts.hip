@@ -938,7 +938,18 @@ struct Results {
 
 template <typename O>
 __device__ __forceinline__ void zero_rows(O* out, int64_t ldo, int m, int n) {
-  for (int u = (int)threadIdx.x; u < m * n; u += (int)blockDim.x) out[(u / n) * ldo + u % n] = (O)0.0f;
+  constexpr int V = 16 / sizeof(O);
+  const int pieces = (n + V - 1) / V;
+  for (int u = (int)threadIdx.x; u < m * pieces; u += (int)blockDim.x) {
+    const int i = u / pieces, j = (u - i * pieces) * V;
+    O* p = out + i * ldo + j;
+    if (j + V <= n) {
+      const u4 z = {0u, 0u, 0u, 0u};
+      __builtin_memcpy(p, &z, sizeof(z));
+    } else {
+      for (int e = 0; j + e < n; ++e) p[e] = (O)0.0f;
+    }
+  }
 }
 
 // ----------------------------------------------------------------- float64 ----
@@ -1355,14 +1366,16 @@ void with_tile(int tile, F&& f) {
 
 // The weight gradient's tiles, by the same rule: 2,048 rows of 128 x 128 in float32
 // take 22 us with 128 x 128 and 16 with 64 x 64, 196,608 rows 72 and 74; 202,752
-// rows of 256 x 512 in bfloat16 96 and 149.
+// rows of 256 x 512 in bfloat16 96 and 149.  Many experts' matrices take the large
+// ones too: most of the time goes to storing them.
 int64_t tiles_of(int tile, int K, int N) {
   const int64_t t = tile == T64 ? 64 : 128;
   return ((K + t - 1) / t) * ((N + t - 1) / t);
 }
 int weight_tile(int type, const Groups& gr, int K, int N) {
   const bool wide = type != TACE_ROW_F64 && K > 64 && N > 64;
-  return wide && fills(gr.rows * total_comps(gr), 128 * tiles_of(T128, K, N)) ? T128 : T64;
+  const bool many = (int64_t)gr.blocks * gr.experts * tiles_of(T64, K, N) > 65536;
+  return wide && (many || fills(gr.rows * total_comps(gr), 128 * tiles_of(T128, K, N))) ? T128 : T64;
 }
 // whether a group may have more than a unit
 bool may_be_cut(const Groups& gr) {
@@ -1449,7 +1462,7 @@ extern "C" int tace_expert_linear_grad(int type, const void* x, const void* g, c
   if ((rows && (!x || !g)) || !dw) return tace_fail_msg("expert_linear: null argument");
   const int tile = weight_tile(type, gr, K, N);
   const int64_t per = tiles_of(tile, K, N);
-  if ((int64_t)blocks * experts * per > MOST_WGS / 16) return tace_fail_msg("expert_linear: bad sizes");
+  if ((int64_t)blocks * experts * per > MOST_WGS / 2) return tace_fail_msg("expert_linear: bad sizes");
   const Teams teams = teams_of(tile, gr, per);
   const bool joins = teams.cuts > 1 && may_be_cut(gr);
   if (joins && (!work || !row_aligned(work) ||

@@ -166,6 +166,21 @@ def test_many_groups_for_each_workgroup(cuda):
         _close(gw[e], dw[0, 0], slack[0, 0], "dw")
 
 
+def test_many_large_matrices(cuda):
+    """300 experts of 4096 x 4096, most of them without a row."""
+    rows, E, K, N = 90, 300, 4096, 4096
+    plan = _plan(cuda, torch.arange(rows) * 3 % 200, E)
+    x, g = _rand((rows, K), torch.bfloat16, 12), _rand((rows, N), torch.bfloat16, 13)
+    lw = torch.zeros(E, K, N, dtype=torch.bfloat16, device=cuda, requires_grad=True)
+    (gw,) = torch.autograd.grad(ops.expert_linear(x.to(cuda), lw, plan), lw, g.to(cuda))
+    ends = plan.rowptr.tolist()
+    for e in (0, 1, 2, 3, 57, 150, 198, 199, 200, 298, 299):
+        i, j = ends[e], ends[e + 1]
+        dw, slack = _weight_reference(x[i:j], g[i:j], [0, j - i], [1], K, N, 1.0)
+        _close(gw[e], dw[0, 0], slack[0, 0], "dw")
+    assert int(gw.view(torch.int16).ne(0).any(2).any(1).sum()) == 90
+
+
 def test_every_size_of_a_group(cuda):
     """Experts of 0 .. 150 rows, across the tiles' heights."""
     e = torch.repeat_interleave(torch.arange(151), torch.arange(151))

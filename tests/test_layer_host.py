@@ -169,7 +169,8 @@ def test_expert_workspace_covers_every_part():
                     for K, M in ((16, 8), (128, 128), (1024, 2048), (8192, 8192)):
                         nbytes = L.tace_expert_linear_grad_work(ty, rows, E, len(comps), _ints(*comps), K, M)
                         tiles = -(-K // 128) * -(-M // 128)
-                        side = 64 if ty == 1 or min(K, M) <= 64 or rows * sum(comps) // 128 * tiles < 512 else 128
+                        side = 64 if ty == 1 or min(K, M) <= 64 or (rows * sum(comps) // 128 * tiles < 512 and
+                            len(comps) * E * (-(-K // 64) * -(-M // 64)) <= 65536) else 128
                         tiles = -(-K // side) * -(-M // side)
                         cuts, rest = divmod(nbytes, 2 * tiles * side * side * size)
                         assert rest == 0
