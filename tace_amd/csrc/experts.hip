@@ -31,10 +31,10 @@
 // once: 24 tokens, 2 of 16 experts each, 1024 x 4096: 15 us, 4.5 TB/s.
 //
 // Measured, us (forward, rows' gradient, weights' gradient): bfloat16, 32,768 rows
-// of 8 experts of 1024 x 2048: 174, 187, 167 + 20 (137 GFLOP each; 790, 735 and 735
+// of 8 experts of 1024 x 2048: 187, 178, 176 + 19 (137 GFLOP each; 735, 772 and 705
 // TFLOP/s, from caches that hold other data; 950 forward from warm ones); 202,752
 // rows of 16 experts of 256 x 512, bound by memory and the latency of four steps a
-// tile: 108, 93, 81 + 14 (311 MB each, 2.9 to 3.3 TB/s).  float32, 196,608 rows of
+// tile: 109, 90, 75 + 14 (311 MB each, 2.9 to 3.5 TB/s).  float32, 196,608 rows of
 // 128 x 128 (its three terms' MFMA takes as long as the memory): 66, 67, 54 + 15.
 #include "bf16x3.h"
 #include "row_types.h"
@@ -67,6 +67,14 @@ struct Groups {
     return v < 0 ? 0 : v > rows ? rows : v;
   }
 };
+
+__host__ __device__ inline int total_comps(const Groups& gr) { return gr.before[gr.blocks - 1] + gr.comps[gr.blocks - 1]; }
+
+// Whether a result of so many bytes is stored past the caches (nt): they hold 256 MB,
+// so the next kernel finds little of as much in them, while it takes the place of
+// what is read again.  202,752 rows of 256 x 512 in bfloat16 (207 MB forward, 104
+// back): a forward and backward pass 271 us, 287 without.
+__device__ __forceinline__ bool large_result(int64_t bytes) { return bytes >= ((int64_t)64 << 20); }
 
 struct Place {
   int64_t first;    // row of the stacked blocks
@@ -853,13 +861,14 @@ struct Results {
   typedef T t4 __attribute__((ext_vector_type(4)));
   typedef unsigned u2 __attribute__((ext_vector_type(2)));
   Make make;
+  bool past;   // (large_result)
   static constexpr int STORES = LATE ? FM * READS : 0;
   static constexpr unsigned NONE = 0x80000000u;
   u4 lined[FM][READS];
   T* base;                  // the tile's first element,
   unsigned range, ld, at;   // and bytes of its rows, of a row, and before this lane's first
 
-  __device__ __forceinline__ explicit Results(Make make) : make(make), base(nullptr), range(0), ld(0), at(NONE) {
+  __device__ __forceinline__ Results(Make make, bool past) : make(make), past(past), base(nullptr), range(0), ld(0), at(NONE) {
 #pragma unroll
     for (int i = 0; i < FM; ++i)
 #pragma unroll
@@ -927,11 +936,16 @@ struct Results {
     const auto rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)q, (short)0, __builtin_amdgcn_readfirstlane((int)range),
                                                         0x00027000);
     const unsigned line = (unsigned)__builtin_amdgcn_readfirstlane((int)ld);
+    auto all = [&](auto aux) {
 #pragma unroll
-    for (int i = 0; i < FM; ++i)
+      for (int i = 0; i < FM; ++i)
 #pragma unroll
-      for (int n = 0; n < READS; ++n)
-        __builtin_amdgcn_raw_buffer_store_b128(lined[i][n], rsrc, (int)(at + (unsigned)(32 * i + n * (128 / SLOTS)) * line), 0, 0);
+        for (int n = 0; n < READS; ++n)
+          __builtin_amdgcn_raw_buffer_store_b128(lined[i][n], rsrc, (int)(at + (unsigned)(32 * i + n * (128 / SLOTS)) * line),
+                                                 0, decltype(aux)::value);
+    };
+    if (past) all(std::integral_constant<int, 2>());   // (nt)
+    else all(std::integral_constant<int, 0>());
     range = 0;
   }
 };
@@ -1043,7 +1057,7 @@ constexpr int waves_for(int fragments) { return fragments > 32 ? 1 : fragments >
 // Walks over a workgroup's tiles: make(t) gives each lane's, zero(job) fills one,
 // put(job) stores a tile's results.
 template <typename T, bool AT, bool BT, int WM, int WN, int FM, int FN, bool FAST, typename Make, typename Zero, typename Store>
-__device__ __forceinline__ void walk(const T* __restrict__ a, const T* __restrict__ b, int64_t lda, int64_t ldb, Share sh,
+__device__ __forceinline__ void walk(const T* __restrict__ a, const T* __restrict__ b, int64_t lda, int64_t ldb, Share sh, bool past,
                                      Make&& make, Zero&& zero, Store&& put) {
   for (int t0 = sh.first; t0 < sh.end; t0 += 64 * sh.step) {
     asm volatile("" : : : "memory");   // (what make() reads is read again)
@@ -1054,7 +1068,7 @@ __device__ __forceinline__ void walk(const T* __restrict__ a, const T* __restric
     unsigned long long mask = __ballot(jobs.kind == PRODUCT);
     if (mask == 0) continue;
     if constexpr (STREAMS<T, FAST>) {
-      Results<T, WM * WN, FM / 2, FN / 2, std::decay_t<Store>> store{put};
+      Results<T, WM * WN, FM / 2, FN / 2, std::decay_t<Store>> store(put, past);
       stream_products<T, AT, BT, WM, WN, FM / 2, FN / 2>(a, b, lda, ldb, jobs, mask, store);
       if (t0 + 64 * sh.step < sh.end) __syncthreads();
     } else {
@@ -1076,7 +1090,7 @@ __global__ __launch_bounds__(64 * WM * WN, waves_for(FM * FN)) void k_expert_row
   constexpr int TM = 16 * WM * FM, TN = 16 * WN * FN;
   const int slots = Places<true, false>(gr, __builtin_ctz(TM)).total();
   walk<T, false, BT, WM, WN, FM, FN, FAST>(
-      x, weight, sum, BT ? n : sum, share_of(slots * cols),
+      x, weight, sum, BT ? n : sum, share_of(slots * cols), large_result(gr.rows * total_comps(gr) * n * (int)sizeof(T)),
       [&](int t) {   // (asked for again for every 64 tiles: nothing of it stays in registers)
         int slot, col;
         blocked(t, slots, cols, &slot, &col);
@@ -1187,7 +1201,7 @@ __global__ __launch_bounds__(64 * WM * WN, waves_for(FM * FN)) void k_expert_wei
     groups = units.group_of(u1 - 1) - g0 + 1;
   }
   walk<T, true, true, WM, WN, FM, FN, FAST>(
-      x, g, K, N, Share{0, groups * rounds, 1},
+      x, g, K, N, Share{0, groups * rounds, 1}, large_result(gr.experts * gr.blocks * size * (int)sizeof(T)),
       [&](int t) {
         const int of = t / rounds, tile = mate + (t - of * rounds) * team, grp = g0 + of;
         const Units::Span s = Units(gr).span(grp);
@@ -1205,7 +1219,7 @@ __global__ __launch_bounds__(64 * WM * WN, waves_for(FM * FN)) void k_expert_wei
       [&](const Job& j) { zero_rows(dw + j.out, N, j.m, j.n); },
       [&](const Job& j) {
         return PutPart<T>{{dw + j.out, N, j.m, j.n, scale, nullptr, nullptr, nullptr},
-                          {part + j.out, TN, j.m, j.n, 1, nullptr, nullptr, nullptr}, j.whole != 0};
+                          {part + j.out, TN, TM, TN, 1, nullptr, nullptr, nullptr}, j.whole != 0};
       });
 }
 
@@ -1317,7 +1331,6 @@ int check_groups(int64_t rows, int experts, int blocks, const int32_t* comps, in
   return 0;
 }
 
-int total_comps(const Groups& gr) { return gr.before[gr.blocks - 1] + gr.comps[gr.blocks - 1]; }
 int64_t slots_of(const Groups& gr, int shift) {
   return ((gr.rows * total_comps(gr)) >> shift) + (int64_t)gr.blocks * (gr.experts + 1);
 }
