@@ -9,6 +9,7 @@
 // Backward, with u_j = gy_j w[j mod C] and gh the gradient of h from elsewhere:
 //   dh_j = q (u_j - h_j q^2 (sum u h) / n) + gh_j
 //   dw_c = sum over rows and components of gy_j h_j q
+// 8 bits: scale = max |y| / 448, code_j = e4m3(448 h_j w_j / max |h w|), y_j's for any q.
 // Bound by HBM.  A group of LPR lanes owns a row and holds it in registers between
 // the sum and the output, so each input is read once; groups walk over rows of
 // one block, their weights (and in the backward pass the weights' gradient) in
@@ -159,23 +160,26 @@ __global__ __launch_bounds__(LPR > WG ? LPR : WG) void k_rms_fwd(
     sum = over_row<LPR, Add>(sum, slots);
     const S q = (S)1 / sqrt(sum / width + eps);
     if (inv && li == 0) inv[r * pt.count + b] = q;
+    // 8 bits: q's power of two alone (over 8), so that h q w of few bits is exact and a
+    // value between two codes is seen to be there, however q was rounded
+    S factor = q;
+    if constexpr (Q) factor = __uint_as_float(__float_as_uint(q) & 0x7f800000u) * 0.125f;
     S top = 0;
 #pragma unroll
     for (int i = 0; i < NV * V; ++i) {
-      a[i] = a[i] * q * w[i];
+      a[i] = a[i] * factor * w[i];
       if constexpr (Q) {
         // (past the row's end: zero times what may be infinite)
         if (li + LPR * (i / V) >= nvec) a[i] = 0;
         top = Top::of(top, (S)fabs(a[i]));
       }
     }
-    S up = 1;
     if constexpr (Q) {
       top = over_row<LPR, Top>(top, slots);
-      // (448 / top overflows below 2^-118: such a row is zeros, as one of zeros)
-      if (top < (S)0x1p-100) top = 0;
-      up = top == 0 ? (S)0 : 448 / top;
-      if (li == 0) scales[r * pt.count + b] = (float)(top / 448);
+      const S full = top * (q / factor);   // the row's largest |y|
+      // (at float32's end quotients lose their bits: such a row is zeros, as one of zeros)
+      if (top == 0 || full < (S)0x1p-100) top = 0;
+      if (li == 0) scales[r * pt.count + b] = top == 0 ? 0.0f : (float)(full / 448);
     }
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -184,7 +188,8 @@ __global__ __launch_bounds__(LPR > WG ? LPR : WG) void k_rms_fwd(
       if constexpr (Q) {
         float v[V];
 #pragma unroll
-        for (int e = 0; e < V; ++e) v[e] = (float)(a[i * V + e] * up);
+        // 448 a / top, rounded once
+        for (int e = 0; e < V; ++e) v[e] = top == 0 ? 0.0f : (float)(a[i * V + e] * 7 / (top * (S)0x1p-6));
         store_codes<V>((unsigned char*)y + at + (int64_t)idx * V, v);
       } else {
         ((Vec*)((T*)y + at))[idx] = row_round<T, V>(a + i * V);

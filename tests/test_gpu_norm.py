@@ -276,3 +276,22 @@ def test_refusals(cuda):
         import torch.autograd.forward_ad as fwd
         with fwd.dual_level():
             ops.rms_norm(fwd.make_dual(x, x), w)
+
+
+@pytest.mark.parametrize("dt,wide", [(torch.bfloat16, False), (torch.bfloat16, True), (torch.float16, True), (torch.float32, False)],
+                         ids=ids)
+@pytest.mark.parametrize("C,comps", [(256, [1]), (100, [1, 3]), (64, [1, 3, 5])])
+def test_codes_on_borders_go_to_even(cuda, dt, wide, C, comps):
+    """A value between two codes is h w 448 / max |h w| of its row, whatever the row's factor was rounded to: products of a
+    few bits lie exactly there, and nowhere else nearer than 2^-22, where no single rounding moves them across."""
+    x = _rand((200, C * sum(comps)), torch.bfloat16, 1).to(dt)
+    w = torch.ones(len(comps), C, dtype=dt) if wide else _rand((len(comps), C), torch.bfloat16, 2).to(dt)
+    q, _ = ops.rms_norm_e4m3(x.to(cuda), (w.float() if wide else w).to(cuda), 1e-6, None, comps)
+    borders = 0
+    for i, (b, got) in enumerate(zip(_blocks(x.double(), comps, C), _blocks(q.cpu().float().double(), comps, C))):
+        p = b * w[i].double().repeat(comps[i])
+        unit = p * 448 / p.abs().amax(1, keepdim=True)
+        steps = unit / _e4m3_step(unit)
+        assert torch.equal(got, torch.round(steps) * _e4m3_step(unit))
+        borders += int((steps.frac().abs() == 0.5).sum())
+    assert borders > 0
