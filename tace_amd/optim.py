@@ -126,29 +126,42 @@ class AdamW(torch.optim.Optimizer):
         return loss
 
     # ------------------------------------------------------------- state ----
+    def _states_of(self, state_dict) -> Dict[torch.Tensor, Dict[str, torch.Tensor]]:
+        """The states that ``state_dict`` holds, checked, for this optimiser's parameters."""
+        groups, given = state_dict["param_groups"], state_dict["state"]
+        if [len(g["params"]) for g in groups] != [len(g["params"]) for g in self.param_groups]:
+            raise ValueError("AdamW: the state's parameter groups are not the optimiser's")
+        counters: Dict[tuple, torch.Tensor] = {}
+        states = {}
+        for k, (theirs, ours) in enumerate(zip(groups, self.param_groups)):
+            for i, p in zip(theirs["params"], ours["params"]):
+                if i not in given:
+                    continue
+                s = {}
+                want = self._init(p, torch.zeros(2, dtype=torch.int64, device=p.device))
+                for name, zero in want.items():
+                    v = given[i].get(name)
+                    if not isinstance(v, torch.Tensor):
+                        raise ValueError(f"AdamW: the state of parameter {i} has no {name}; its states have other bits")
+                    if v.dtype != zero.dtype or v.shape != zero.shape:
+                        raise ValueError(f"AdamW: {name} of parameter {i} is {v.dtype} {tuple(v.shape)}, expected "
+                                         f"{zero.dtype} {tuple(zero.shape)}")
+                    s[name] = v.detach().to(p.device, copy=True, memory_format=torch.contiguous_format)
+                key = (k, p.dtype, p.device, int(s["step"][0]))
+                s["step"] = counters.setdefault(key, s["step"])
+                states[p] = s
+        return states
+
     def load_state_dict(self, state_dict) -> None:
         """As ``Optimizer.load_state_dict``, but states keep their types (masters
         and codes are not cast to the parameters' type) and parameters whose steps
-        are equal share a counter again."""
-        given = state_dict["state"]
-        super().load_state_dict(state_dict)
-        order = [i for g in state_dict["param_groups"] for i in g["params"]]
-        params = [p for g in self.param_groups for p in g["params"]]
-        counters: Dict[tuple, torch.Tensor] = {}
-        group_of = [k for k, g in enumerate(self.param_groups) for _ in g["params"]]
-        for i, p, k in zip(order, params, group_of):
-            if i not in given:
-                continue
-            s = {}
-            want = self._init(p, torch.zeros(2, dtype=torch.int64, device=p.device))
-            for name, zero in want.items():
-                if name not in given[i]:
-                    raise ValueError(f"AdamW: the state of parameter {i} has no {name}; its states have other bits")
-                v = given[i][name]
-                if v.dtype != zero.dtype or v.shape != zero.shape:
-                    raise ValueError(f"AdamW: {name} of parameter {i} is {v.dtype} {tuple(v.shape)}, expected "
-                                     f"{zero.dtype} {tuple(zero.shape)}")
-                s[name] = v.detach().to(p.device, copy=True)
-            key = (k, p.dtype, p.device, int(s["step"][0]))
-            s["step"] = counters.setdefault(key, s["step"])
-            self.state[p] = s
+        are equal share a counter again.  A state that is refused changes nothing."""
+        made: Dict[torch.Tensor, Dict[str, torch.Tensor]] = {}
+        # (between the caller's hooks: after those before the load, before those after it)
+        before = self.register_load_state_dict_pre_hook(lambda _, given: made.update(self._states_of(given)))
+        after = self.register_load_state_dict_post_hook(lambda _: self.state.update(made), prepend=True)
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            before.remove()
+            after.remove()

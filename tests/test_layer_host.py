@@ -179,3 +179,45 @@ def test_expert_workspace_covers_every_part():
                             assert cuts * -(-tiles // 4) <= (1024 if side == 64 else 512)
                         else:
                             assert rows * max(comps) <= 128 or tiles > 512 or rows * sum(comps) // 128 + E * len(comps) < 2
+
+
+def _states(o):
+    return [{k: (v.dtype, v.clone()) for k, v in o.state[p].items()} for g in o.param_groups for p in g["params"]]
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_a_refused_state_dict_changes_nothing(bits):
+    make = lambda b, shapes=((300,), (5, 7)): optim.AdamW([torch.ones(s, requires_grad=True) for s in shapes], bits=b, lr=b / 100)
+    o, other = make(bits), make(40 - bits)
+    for x, v in ((o, 0.5), (other, 2.0)):
+        x.init_states()
+        for s in x.state.values():
+            for k in s:
+                s[k].copy_(torch.full(s[k].shape, v))
+    wrong = other.state_dict(), make(bits, ((300,),)).state_dict(), make(bits, ((301,), (5, 7)))
+    wrong[2].init_states()
+    before = _states(o)
+    for d in (wrong[0], wrong[1], wrong[2].state_dict(), {**o.state_dict(), "state": {0: {"step": torch.zeros(2)}}}):
+        with pytest.raises(ValueError):
+            o.load_state_dict(d)
+        assert o.param_groups[0]["lr"] == bits / 100 and len(o.param_groups[0]["params"]) == 2
+        for a, b in zip(before, _states(o)):
+            assert list(a) == list(b)
+            for k in a:
+                assert a[k][0] == b[k][0] and torch.equal(a[k][1].view(torch.uint8), b[k][1].view(torch.uint8))
+
+
+def test_state_dicts_pass_hooks():
+    """What the hooks before a load make of it is loaded; those after it see the states as they are kept."""
+    p = [torch.ones(9, requires_grad=True)]
+    o, seen = optim.AdamW(p, bits=8), []
+    o.init_states()
+    d = o.state_dict()
+    def double(opt, s):
+        return {**s, "state": {i: {**v, "scales": v["scales"] + 2} for i, v in s["state"].items()}}
+    o.register_load_state_dict_pre_hook(double)
+    o.register_load_state_dict_post_hook(lambda opt: seen.append(opt.state[p[0]]["exp_avg"].dtype))
+    o.load_state_dict(d)
+    assert seen == [torch.float8_e4m3fn] and float(o.state[p[0]]["scales"][0, 0]) == 2
+    o.load_state_dict(d)      # (hooks of a load leave with it)
+    assert float(o.state[p[0]]["scales"][0, 0]) == 2
