@@ -44,6 +44,10 @@ class AdamW(torch.optim.Optimizer):
         self.bits, self.max_norm, self.masters, self.seed = bits, max_norm, masters, int(seed)
         self.norm: Optional[torch.Tensor] = None
 
+    def __getstate__(self):
+        """What copies and pickles hold, the optimiser's own settings among it."""
+        return {**super().__getstate__(), **{k: getattr(self, k) for k in ("bits", "max_norm", "masters", "seed", "norm")}}
+
     # ------------------------------------------------------------ states ----
     def _init(self, p: torch.Tensor, counter: torch.Tensor) -> Dict[str, torch.Tensor]:
         wide = torch.float64 if p.dtype == torch.float64 else torch.float32

@@ -1,6 +1,8 @@
 """The routed layer's operators: boundary and refusals (CPU)."""
 
+import copy
 import ctypes
+import io
 
 import pytest
 import torch
@@ -221,3 +223,24 @@ def test_state_dicts_pass_hooks():
     assert seen == [torch.float8_e4m3fn] and float(o.state[p[0]]["scales"][0, 0]) == 2
     o.load_state_dict(d)      # (hooks of a load leave with it)
     assert float(o.state[p[0]]["scales"][0, 0]) == 2
+
+
+def _saved(o):   # (pickle alone has no tensors of 8 bits)
+    f = io.BytesIO()
+    torch.save(o, f)
+    return torch.load(io.BytesIO(f.getvalue()), weights_only=False)
+
+
+@pytest.mark.parametrize("copied", [copy.deepcopy, _saved])
+def test_copies_of_an_optimiser_are_whole(copied):
+    p = [torch.nn.Parameter(torch.ones(n)) for n in (300, 5)]
+    o = optim.AdamW(p, bits=8, max_norm=2.0, masters=False, seed=77)
+    o.init_states()
+    c = copied(o)
+    assert (c.bits, c.max_norm, c.masters, c.seed, c.norm) == (8, 2.0, False, 77, None)
+    mine = [c.state[q] for q in c.param_groups[0]["params"]]
+    assert mine[0]["step"] is mine[1]["step"] and mine[0]["step"] is not o.state[p[0]]["step"]
+    c.step()                          # nothing has a gradient
+    c.load_state_dict(o.state_dict())
+    c.add_param_group(dict(params=[torch.nn.Parameter(torch.ones(2))]))
+    c.init_states()
