@@ -108,7 +108,9 @@ int tace_rms_norm_bwd(int type, const void* gy, const void* gh, const void* h, c
                       void* dw, void* work, int64_t work_bytes, void* stream);
 
 /* The experts' products.  Rows sorted by expert as tace_route_group's (rowptr
- * [experts + 1]; rows from rowptr[experts] on are dropped) in `blocks` blocks of
+ * [experts + 1], rowptr[0] taken for 0; rows from rowptr[experts] on are dropped;
+ * entries that fall or leave the rows give other groups, with reads and writes
+ * inside the rows all the same) in `blocks` blocks of
  * comps[b] components: a batch is block after block, each [rows, comps[b], K].
  * weight [experts, blocks, K, N].
  * tace_expert_linear: out [.., N] = scale x weight[expert][block], or (transposed;

@@ -60,9 +60,11 @@ struct Groups {
   int experts, blocks;
   int comps[TACE_ROW_MAX_BLOCKS], before[TACE_ROW_MAX_BLOCKS];
 
-  // (rows outside the range and orders that are none give other groups, but rows in range)
+  // (rows outside the range and orders that are none give other groups, but rows in range; from row 0 to the
+  // last in any case, so every row is some group's)
   __device__ __forceinline__ int64_t end_of(int e) const {   // first row of expert e; of the dropped rows for e = experts
     if (e > experts) return rows;
+    if (e == 0) return 0;
     const int64_t v = rowptr[e];
     return v < 0 ? 0 : v > rows ? rows : v;
   }

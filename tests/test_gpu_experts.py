@@ -513,3 +513,74 @@ def test_refusals(cuda):
             (lambda: ops.expert_linear_e4m3(q.cpu(), qs, w8, ws, plan), "GPU tensor")]:
         with pytest.raises(ValueError, match=text):
             call()
+
+
+class Guarded:
+    """A buffer between margins whose bytes are known; nothing in it is a number until it is written."""
+
+    MARGIN = 1 << 16
+
+    def __init__(self, cuda, shape, dt):
+        n = torch.Size(shape).numel() * dt.itemsize
+        self.whole = torch.full((n + 2 * self.MARGIN,), 255, dtype=torch.uint8, device=cuda)
+        self.inner = self.whole[self.MARGIN:self.MARGIN + n].view(dt).view(shape)
+
+    def ptr(self):
+        return self.inner.data_ptr()
+
+    def check(self, written=True):
+        m = self.MARGIN
+        assert bool((self.whole[:m] == 255).all()) and bool((self.whole[-m:] == 255).all())
+        assert not written or not torch.isnan(self.inner).any()
+
+
+NO_ORDERS = [[0, 50, 20, 100], [30, 40, 60, 100], [0, 400, 500, 600], [-5, 10, 20, 30], [100, 0, 0, 0],
+             [7, 7, 7, 7], [99, -1, 200, 50]]
+
+
+@pytest.mark.parametrize("rowptr", NO_ORDERS)
+@pytest.mark.parametrize("dt,K,M,comps", [(torch.bfloat16, 32, 64, [1]), (torch.bfloat16, 33, 17, [1]), (torch.float32, 40, 24, [1, 3]),
+                                          (torch.float32, 7, 9, [1]), (torch.float64, 20, 12, [1]), (torch.float16, 136, 72, [1, 3])],
+                         ids=ids)
+def test_orders_that_are_none_write_every_row_and_nothing_else(cuda, rowptr, dt, K, M, comps):
+    import ctypes
+
+    from tace_amd import _native as N
+
+    rows, E, B, D = 100, 3, len(comps), sum(comps)
+    x, w, g = (_rand(s, dt, i).to(cuda) for i, s in enumerate(((rows, D * K), (E, B, K, M), (rows, D * M))))
+    ptr = torch.tensor(rowptr, dtype=torch.int32, device=cuda)
+    c = (ctypes.c_int32 * B)(*comps)
+    code = {torch.float32: 0, torch.float64: 1, torch.bfloat16: 2, torch.float16: 3}[dt]
+    s = torch.cuda.current_stream().cuda_stream
+    y, dx, dw = (Guarded(cuda, t.shape, dt) for t in (g, x, w))
+    L = N.lib()
+    need = L.tace_expert_linear_grad_work(code, rows, E, B, c, K, M)
+    work = Guarded(cuda, (need,), torch.uint8)
+    for rc in (L.tace_expert_linear(code, 0, x.data_ptr(), w.data_ptr(), ptr.data_ptr(), rows, E, B, c, K, M, 0.5, y.ptr(), s),
+               L.tace_expert_linear(code, 1, g.data_ptr(), w.data_ptr(), ptr.data_ptr(), rows, E, B, c, K, M, 0.5, dx.ptr(), s),
+               L.tace_expert_linear_grad(code, x.data_ptr(), g.data_ptr(), ptr.data_ptr(), rows, E, B, c, K, M, 0.5, dw.ptr(),
+                                         work.ptr(), need, s)):
+        assert rc == 0
+    torch.cuda.synchronize()
+    for t in (y, dx, dw):
+        t.check()
+    work.check(False)
+
+
+@pytest.mark.parametrize("rowptr", NO_ORDERS)
+@pytest.mark.parametrize("gather", [False, True])
+def test_codes_of_orders_that_are_none(cuda, rowptr, gather):
+    from tace_amd import _native as N
+
+    T, k, E, K, M = 50, 2, 3, 48, 40
+    q, qs = (t.to(cuda) for t in _codes(_rand((T if gather else T * k, K), torch.float32, 1)))
+    w, ws = (t.to(cuda) for t in _codes(_rand((E, M, K), torch.float32, 2)))
+    order = (torch.arange(T * k, dtype=torch.int32, device=cuda) - 20) * 1000003     # (few of them are slots)
+    ptr = torch.tensor(rowptr, dtype=torch.int32, device=cuda)
+    y = Guarded(cuda, (T * k, M), torch.bfloat16)
+    assert N.lib().tace_expert_linear_e4m3(2, q.data_ptr(), qs.data_ptr(), order.data_ptr() if gather else None, k, w.data_ptr(),
+                                           ws.data_ptr(), ptr.data_ptr(), T * k, E, K, M, y.ptr(),
+                                           torch.cuda.current_stream().cuda_stream) == 0
+    torch.cuda.synchronize()
+    y.check()
