@@ -584,3 +584,39 @@ def test_codes_of_orders_that_are_none(cuda, rowptr, gather):
                                            torch.cuda.current_stream().cuda_stream) == 0
     torch.cuda.synchronize()
     y.check()
+
+
+def _time(f):
+    f()
+    best = float("inf")
+    for _ in range(3):
+        a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+        a.record()
+        f()
+        b.record()
+        torch.cuda.synchronize()
+        best = min(best, a.elapsed_time(b))
+    return best
+
+
+def test_a_step_of_nan_takes_no_longer(cuda):
+    """Float32 sums that are not finite are made again from the inputs: a diverged step must not stand still there (it took
+    ninety times a step's time when each of a lane's sums ran by itself to its end)."""
+    rows, E, C = 16384, 2, 512
+    plan = _plan(cuda, torch.arange(rows) % E, E)
+    x, w, g = (_rand(s, torch.float32, i).to(cuda) for i, s in enumerate(((rows, C), (E, C, C), (rows, C))))
+    def step(a, b, c):
+        la, lb = a.detach().requires_grad_(True), b.detach().requires_grad_(True)
+        return torch.autograd.grad(ops.expert_linear(la, lb, plan), (la, lb), c)
+    usual = _time(lambda: step(x, w, g))
+    nan = torch.full_like(g, float("nan"))
+    gx, gw = step(x, w, nan)
+    assert torch.isnan(gx).all() and torch.isnan(gw).all()
+    one = g.clone()
+    one[rows // 2] = float("nan")     # half of an expert's sums are run through before they end
+    far = g.clone()
+    far[rows - E:] = float("inf")     # (those of one sign run to their end)
+    for name, args in (("gradient", (x, w, nan)), ("rows", (nan, w, g)), ("row", (x, w, one)), ("infinite rows", (x.abs(), w, far))):
+        took = _time(lambda: step(*args))
+        print(name, took, "of", usual, "ms")
+        assert took < 20 * usual, name
