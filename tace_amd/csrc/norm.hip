@@ -164,7 +164,7 @@ __global__ __launch_bounds__(LPR > WG ? LPR : WG) void k_rms_fwd(
     // value between two codes is seen to be there, however q was rounded
     S factor = q;
     if constexpr (Q) factor = __uint_as_float(__float_as_uint(q) & 0x7f800000u) * 0.125f;
-    S top = 0;
+    S top = 0, den = 0, rcp = 0, seven = 0;
 #pragma unroll
     for (int i = 0; i < NV * V; ++i) {
       a[i] = a[i] * factor * w[i];
@@ -177,9 +177,16 @@ __global__ __launch_bounds__(LPR > WG ? LPR : WG) void k_rms_fwd(
     if constexpr (Q) {
       top = over_row<LPR, Top>(top, slots);
       const S full = top * (q / factor);   // the row's largest |y|
-      // (at float32's end quotients lose their bits: such a row is zeros, as one of zeros)
+      // (below, float32 has no room for what follows: such a row is zeros, as one of zeros)
       if (top == 0 || full < (S)0x1p-100) top = 0;
       if (li == 0) scales[r * pt.count + b] = top == 0 ? 0.0f : (float)(full / 448);
+      // 448 a / top rounded once, by a corrected product with the reciprocal: 7 a over top / 64, both
+      // by top's power of two  (a division of its own for each element: 101,306 rows of 256 in bfloat16 41 instead of 37 us)
+      const unsigned ex = __float_as_uint(top) >> 23;   // (an infinity or NaN: 0, and NaN after)
+      const S one = ex == 255 ? (S)0 : __uint_as_float((254 - ex) << 23);
+      den = top * one * (S)0x1p-6;
+      rcp = top == 0 ? (S)0 : 1 / den;
+      seven = top == 0 ? (S)0 : 7 * one;
     }
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -188,8 +195,10 @@ __global__ __launch_bounds__(LPR > WG ? LPR : WG) void k_rms_fwd(
       if constexpr (Q) {
         float v[V];
 #pragma unroll
-        // 448 a / top, rounded once
-        for (int e = 0; e < V; ++e) v[e] = top == 0 ? 0.0f : (float)(a[i * V + e] * 7 / (top * (S)0x1p-6));
+        for (int e = 0; e < V; ++e) {
+          const float t = (float)(a[i * V + e] * seven), near = t * (float)rcp;
+          v[e] = fmaf(fmaf(-near, (float)den, t), (float)rcp, near);
+        }
         store_codes<V>((unsigned char*)y + at + (int64_t)idx * V, v);
       } else {
         ((Vec*)((T*)y + at))[idx] = row_round<T, V>(a + i * V);
