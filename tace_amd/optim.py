@@ -106,18 +106,18 @@ class AdamW(torch.optim.Optimizer):
                 loss = closure()
         launches = [(k, group, ps) for k, group in enumerate(self.param_groups) for ps in self._launches(group)]
         self.norm = None
-        if self.max_norm is not None and launches:
-            by_type: Dict[torch.dtype, List[torch.Tensor]] = {}
+        if self.max_norm is not None and len(launches) > 1:
+            alike: Dict[tuple, List[torch.Tensor]] = {}
             for _, _, ps in launches:
-                by_type.setdefault(ps[0].dtype, []).extend(p.grad for p in ps)
-            if len(launches) > 1:
-                norms = [ops.grad_norm(g) for g in by_type.values()]
-                self.norm = norms[0] if len(norms) == 1 else torch.stack([n.double() for n in norms]).square().sum().sqrt()
+                alike.setdefault((ps[0].device, ps[0].dtype), []).extend(p.grad for p in ps)
+            norms = [ops.grad_norm(g) for g in alike.values()]
+            self.norm = norms[0] if len(norms) == 1 else torch.stack(
+                [n.to(norms[0].device, torch.float64) for n in norms]).square().sum().sqrt()
         for k, group, ps in launches:
             states = [self.state[p] for p in ps]
             norm = self.norm
             if norm is not None:
-                norm = norm.to(torch.float64 if ps[0].dtype == torch.float64 else torch.float32)
+                norm = norm.to(ps[0].device, torch.float64 if ps[0].dtype == torch.float64 else torch.float32)
             place = next(i for i, p in enumerate(group["params"]) if p is ps[0])
             got = ops.adamw_step(
                 ps, [p.grad for p in ps], [s["exp_avg"] for s in states], [s["exp_avg_sq"] for s in states],

@@ -244,3 +244,42 @@ def test_copies_of_an_optimiser_are_whole(copied):
     c.load_state_dict(o.state_dict())
     c.add_param_group(dict(params=[torch.nn.Parameter(torch.ones(2))]))
     c.init_states()
+
+
+class Recorder:
+    """Stands in for the kernels: notes what they are given and counts steps."""
+
+    def __init__(self, monkeypatch, norm=3.0):
+        self.steps, self.norms = [], []
+
+        def adamw_step(params, grads, ms, ss, counter, *, norm=None, max_norm=None, **more):
+            assert len({(p.device, p.dtype) for p in (*params, *grads)}) == 1
+            self.steps.append(dict(more, params=params, grads=grads, counter=counter, norm=norm))
+            counter[0] += 1
+            if max_norm is not None:
+                return torch.tensor(1.0) if norm is None else norm
+
+        def grad_norm(grads):
+            assert len({(g.device, g.dtype) for g in grads}) == 1
+            self.norms.append(list(grads))
+            return torch.tensor(norm * len(self.norms), dtype=torch.float64 if grads[0].dtype == torch.float64 else torch.float32)
+
+        monkeypatch.setattr(optim.ops, "adamw_step", adamw_step)
+        monkeypatch.setattr(optim.ops, "grad_norm", grad_norm)
+
+
+def _with_grads(*ps):
+    for p in ps:
+        p.grad = torch.ones_like(p)
+    return list(ps)
+
+
+def test_parameters_of_two_devices_are_clipped_together(monkeypatch):
+    r = Recorder(monkeypatch)
+    here = _with_grads(*(torch.ones(n, requires_grad=True) for n in (3, 4)))
+    there = _with_grads(*(torch.ones(n, requires_grad=True, device="meta") for n in (5, 6)))
+    o = optim.AdamW([here[0], there[0], here[1], there[1]], max_norm=1.0)
+    o.step()
+    assert [len(n) for n in r.norms] == [2, 2] and float(o.norm) == 45 ** 0.5 and len(r.steps) == 2
+    for s in r.steps:      # each with the norm of all, where it is read
+        assert s["norm"].device == s["params"][0].device and s["norm"].dtype == torch.float32
