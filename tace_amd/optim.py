@@ -28,7 +28,9 @@ class AdamW(torch.optim.Optimizer):
     one element on the GPU.
 
     A step can be recorded into a graph (its gradients' addresses are part of
-    it) once the states are made, by a first step or ``init_states()``."""
+    it) once the states are made, by a first step or ``init_states()``; a
+    recording that would make states, or part the count of steps of parameters
+    without a gradient from others', is refused."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 0.01,
                  bits: int = 32, max_norm: Optional[float] = None, masters: bool = True, seed: int = 0):
@@ -77,6 +79,18 @@ class AdamW(torch.optim.Optimizer):
         for group in self.param_groups:
             self._init_of([p for p in group["params"] if p.requires_grad])
 
+    def _check_recording(self) -> None:
+        """A recorded step makes no states and parts no counts: each replay would do so again."""
+        for group in self.param_groups:
+            states = [(p.grad is not None, self.state.get(p)) for p in group["params"]]
+            if any(has and not s for has, s in states):
+                raise RuntimeError("AdamW: a step is recorded before its parameters have states; call init_states() or step() "
+                                   "first")
+            moved = {id(s["step"]) for has, s in states if has}
+            if any(s and id(s["step"]) in moved for has, s in states if not has):
+                raise RuntimeError("AdamW: a recorded step has parameters without a gradient whose steps are counted with "
+                                   "others'; step() once with the same gradients missing before")
+
     def _launches(self, group) -> List[List[torch.Tensor]]:
         """Parameters with gradients that take one launch: those of one counter
         (and so of one type).  A counter counts the steps of all that share it, so
@@ -104,6 +118,8 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
+        if torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing():
+            self._check_recording()
         launches = [(k, group, ps) for k, group in enumerate(self.param_groups) for ps in self._launches(group)]
         self.norm = None
         if self.max_norm is not None and len(launches) > 1:

@@ -450,3 +450,30 @@ def test_refusals(cuda):
     f64[0].grad = torch.ones_like(f64[0])
     with pytest.raises(ValueError, match="float64"):
         optim.AdamW(f64, bits=8).step()
+
+
+def test_recorded_steps_of_an_optimiser(cuda):
+    """A step recorded with the optimiser's states goes on as eager ones; one that would make states is refused."""
+    a, b = _params(cuda, torch.float32), _params(cuda, torch.float32)
+    oa, ob = (optim.AdamW(ps, lr=1e-2, max_norm=0.5) for ps in (a, b))
+    _set_grads(a, 0)
+    scratch = torch.zeros(4, device=cuda)
+    with torch.cuda.graph(torch.cuda.CUDAGraph()):
+        scratch.add_(1)
+        with pytest.raises(RuntimeError, match="init_states"):
+            oa.step()
+    assert not oa.state
+    _set_grads(b, 0)
+    a[1].grad = b[1].grad = None
+    for o in (oa, ob):
+        o.init_states()
+        o.step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        oa.step()
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        ob.step()
+        assert all(torch.equal(p, q) for p, q in zip(a, b))
+    assert [int(oa.state[p]["step"][0]) for p in a] == [4, 0, 4, 4, 4] == [int(ob.state[p]["step"][0]) for p in b]

@@ -283,3 +283,26 @@ def test_parameters_of_two_devices_are_clipped_together(monkeypatch):
     assert [len(n) for n in r.norms] == [2, 2] and float(o.norm) == 45 ** 0.5 and len(r.steps) == 2
     for s in r.steps:      # each with the norm of all, where it is read
         assert s["norm"].device == s["params"][0].device and s["norm"].dtype == torch.float32
+
+
+def test_recordings_that_a_replay_would_undo_are_refused(monkeypatch):
+    """States made, or counts parted, inside a recording would be made again by every replay."""
+    r, recording = Recorder(monkeypatch), [True]
+    monkeypatch.setattr(torch.cuda, "is_initialized", lambda: True)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: recording[0])
+    p = _with_grads(*(torch.ones(4, requires_grad=True) for _ in range(3)))
+    o = optim.AdamW(p, max_norm=1.0)
+    with pytest.raises(RuntimeError, match="init_states"):
+        o.step()
+    assert not o.state and not r.steps
+    o.init_states()
+    p[1].grad = None
+    one = o.state[p[0]]["step"]
+    with pytest.raises(RuntimeError, match="without a gradient"):
+        o.step()
+    assert not r.steps and all(o.state[q]["step"] is one for q in p)
+    recording[0] = False
+    o.step()                               # (parts them)
+    recording[0] = True
+    o.step()
+    assert len(r.steps) == 2 and o.state[p[1]]["step"] is not one
