@@ -383,7 +383,7 @@ optional<Tensor> adamw_step(const Tensors& params, const Tensors& grads, const T
                             const Tensor& counter, double lr, const optional<Tensor>& lr_at, double beta1, double beta2,
                             double eps, double decay, const optional<Tensors>& scales,
                             const optional<Tensors>& masters, optional<double> max_norm, const optional<Tensor>& norm_in,
-                            int64_t seed, bool timed) {
+                            int64_t seed, const optional<std::vector<int64_t>>& places, bool timed) {
   const size_t n = params.size();
   TORCH_CHECK_VALUE(n > 0, "adamw_step: no parameters");
   TORCH_CHECK_VALUE(grads.size() == n && ms.size() == n && ss.size() == n && (!scales || scales->size() == n) &&
@@ -399,6 +399,11 @@ optional<Tensor> adamw_step(const Tensors& params, const Tensors& grads, const T
   TORCH_CHECK_VALUE(eps >= 0 && decay >= 0 && (lr_at || lr >= 0), "adamw_step: lr, eps and weight_decay are not negative");
   TORCH_CHECK_VALUE(!max_norm || *max_norm > 0, "adamw_step: max_norm is not positive");
   TORCH_CHECK_VALUE(!norm_in || max_norm, "adamw_step: a norm without max_norm");
+  if (places) {
+    bool ok = places->size() == n && places->front() >= 0 && places->back() < (1 << 20);
+    for (size_t i = 1; i < places->size(); ++i) ok = ok && (*places)[i - 1] < (*places)[i];
+    TORCH_CHECK_VALUE(ok, "adamw_step: places are one for each parameter, each larger than the one before, below 2^20");
+  }
   TORCH_CHECK_VALUE(counter.scalar_type() == at::kLong && counter.dim() == 1 && counter.size(0) == 2 &&
                     counter.is_contiguous() && !counter.is_neg(), "counter must be a contiguous int64 tensor [2]");
   want_device(counter, first, "counter");
@@ -448,9 +453,14 @@ optional<Tensor> adamw_step(const Tensors& params, const Tensors& grads, const T
   } else if (max_norm) {
     norm = norm_of(table, first, counter.data_ptr<int64_t>() + 1, timed);
   }
+  if (places && scales) {   // (draws are numbered by the table's rows: empty ones between)
+    std::vector<tace_adam_tensor> spread((size_t)places->back() + 1);
+    for (size_t i = 0; i < n; ++i) spread[(size_t)(*places)[i]] = table[i];
+    table = std::move(spread);
+  }
   {
     Launch l(first, "adamw", timed);
-    l.done(tace_adamw(type_code(type), scales.has_value(), table.data(), (int64_t)n, counter.data_ptr<int64_t>(), lr,
+    l.done(tace_adamw(type_code(type), scales.has_value(), table.data(), (int64_t)table.size(), counter.data_ptr<int64_t>(), lr,
                       lr_at ? lr_at->const_data_ptr() : nullptr, lr_at && lr_at->scalar_type() == at::kDouble, beta1,
                       beta2, eps, decay, norm.defined() ? norm.const_data_ptr() : nullptr, max_norm.value_or(0),
                       (uint64_t)seed, l.stream), {total});

@@ -1710,7 +1710,8 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
                exp_avg_sqs: Sequence[torch.Tensor], counter: torch.Tensor, *, lr, betas: Tuple[float, float] = (0.9, 0.999),
                eps: float = 1e-8, weight_decay: float = 0.01, scales: Optional[Sequence[torch.Tensor]] = None,
                masters: Optional[Sequence[torch.Tensor]] = None, max_norm: Optional[float] = None,
-               norm: Optional[torch.Tensor] = None, seed: int = 0) -> Optional[torch.Tensor]:
+               norm: Optional[torch.Tensor] = None, seed: int = 0,
+               places: Optional[Sequence[int]] = None) -> Optional[torch.Tensor]:
     """One step of AdamW, in place, over all ``params`` (contiguous, one row type)
     in few launches (56 to 84 tensors each); ``tace_amd.optim.AdamW`` is the optimiser
     around it.
@@ -1719,8 +1720,8 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
     shapes in the type's sums.  With ``scales`` (float32 [ceil(numel / ADAM_BLOCK),
     2] each) they are float8_e4m3fn codes of the average of g and of the ROOT of
     the average of g^2, ``ADAM_BLOCK`` elements to a scale, rounded at random (a
-    function of ``seed``, the step, the parameter's place in the list and the
-    element).  ``masters`` (parameters of 16 bits): float32 weights that are
+    function of ``seed``, the step, the parameter's place and the element; places
+    are those in the list, or ``places``, rising and below 2^20).  ``masters`` (parameters of 16 bits): float32 weights that are
     stepped, the parameters are rounded from them.  ``counter``: int64 [2] on the
     device, the steps done and 0; it counts the step when the kernel runs, so a
     recorded graph goes on counting.  ``lr``: a number, or a tensor of one
@@ -1737,7 +1738,7 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
         raise ValueError("adamw_step: seed has 64 bits")
     return N.rows().adamw_step(params, grads, exp_avgs, exp_avg_sqs, counter, float(lr), lr_at, betas[0], betas[1], eps,
                                weight_decay, scales, masters, max_norm, norm, seed - 2 ** 64 if seed >= 2 ** 63 else seed,
-                               TIMER is not None)
+                               places, TIMER is not None)
 
 
 def _pad4(lst):

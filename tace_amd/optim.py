@@ -24,7 +24,8 @@ class AdamW(torch.optim.Optimizer):
     the states, unless ``masters`` is False.  ``max_norm``: the gradients of all
     groups together are scaled to this norm where it is exceeded, and a step whose
     norm is infinite or NaN changes nothing; ``norm`` is the last step's.
-    ``seed``: of the 8-bit states' rounding.  ``lr`` of a group may be a tensor of
+    ``seed``: of the 8-bit states' rounding, a function of it, a parameter's
+    place among the group's of its type, and its steps.  ``lr`` of a group may be a tensor of
     one element on the GPU.
 
     A step can be recorded into a graph (its gradients' addresses are part of
@@ -111,6 +112,15 @@ class AdamW(torch.optim.Optimizer):
                     s["step"] = copies[id(shared)]
         return list(sets.values())
 
+    def _places(self, group, ps: List[torch.Tensor]):
+        """Where the group's first parameter like ``ps`` is, and the places of ``ps``
+        among those like them: codes are drawn alike however launches divide them."""
+        if self.bits != 8:
+            return 0, None
+        alike = [(i, p) for i, p in enumerate(group["params"]) if p.dtype == ps[0].dtype and p.device == ps[0].device]
+        place = {id(p): n for n, (_, p) in enumerate(alike)}
+        return alike[0][0], [place[id(p)] for p in ps]
+
     # -------------------------------------------------------------- step ----
     @torch.no_grad()
     def step(self, closure=None):
@@ -123,9 +133,11 @@ class AdamW(torch.optim.Optimizer):
         launches = [(k, group, ps) for k, group in enumerate(self.param_groups) for ps in self._launches(group)]
         self.norm = None
         if self.max_norm is not None and len(launches) > 1:
-            alike: Dict[tuple, List[torch.Tensor]] = {}
-            for _, _, ps in launches:
-                alike.setdefault((ps[0].device, ps[0].dtype), []).extend(p.grad for p in ps)
+            alike: Dict[tuple, List[torch.Tensor]] = {}   # (in the parameters' order, whatever the launches)
+            for group in self.param_groups:
+                for p in group["params"]:
+                    if p.grad is not None:
+                        alike.setdefault((p.device, p.dtype), []).append(p.grad)
             norms = [ops.grad_norm(g) for g in alike.values()]
             self.norm = norms[0] if len(norms) == 1 else torch.stack(
                 [n.to(norms[0].device, torch.float64) for n in norms]).square().sum().sqrt()
@@ -134,13 +146,14 @@ class AdamW(torch.optim.Optimizer):
             norm = self.norm
             if norm is not None:
                 norm = norm.to(ps[0].device, torch.float64 if ps[0].dtype == torch.float64 else torch.float32)
-            place = next(i for i, p in enumerate(group["params"]) if p is ps[0])
+            first, places = self._places(group, ps)
             got = ops.adamw_step(
                 ps, [p.grad for p in ps], [s["exp_avg"] for s in states], [s["exp_avg_sq"] for s in states],
                 states[0]["step"], lr=group["lr"], betas=group["betas"], eps=group["eps"],
                 weight_decay=group["weight_decay"], scales=[s["scales"] for s in states] if self.bits == 8 else None,
                 masters=[s["master"] for s in states] if "master" in states[0] else None, max_norm=self.max_norm,
-                norm=norm, seed=(self.seed * 1000003 + k * 8191 + place) % 2 ** 64)
+                norm=norm, seed=(self.seed * 1000003 + k * 8191 + first) % 2 ** 64,
+                places=places)
             if self.norm is None:
                 self.norm = got
         return loss

@@ -477,3 +477,49 @@ def test_recorded_steps_of_an_optimiser(cuda):
         ob.step()
         assert all(torch.equal(p, q) for p, q in zip(a, b))
     assert [int(oa.state[p]["step"][0]) for p in a] == [4, 0, 4, 4, 4] == [int(ob.state[p]["step"][0]) for p in b]
+
+
+def test_resumed_where_gradients_were_missing(cuda, tmp_path):
+    """Parameters with counts of their own draw the same codes after a state has been loaded."""
+    a, b = _params(cuda, torch.float32, 6), _params(cuda, torch.float32, 6)
+    oa, ob = (optim.AdamW(ps, lr=1e-2, bits=8, seed=4, max_norm=0.5) for ps in (a, b))
+    missing = [[], [1], [0, 3], [5], [], [2, 3], [5], []]   # (0, 1, 3 and 5 come to one count on three ways)
+    def run(ps, o, k):
+        _set_grads(ps, k)
+        for i in missing[k]:
+            ps[i].grad = None
+        o.step()
+    for k in range(4):
+        run(a, oa, k)
+    torch.save(oa.state_dict(), tmp_path / "o.pt")
+    with torch.no_grad():
+        for p, q in zip(a, b):
+            q.copy_(p)
+    ob.load_state_dict(torch.load(tmp_path / "o.pt", weights_only=True))
+    for k in range(4, 8):
+        run(a, oa, k)
+        run(b, ob, k)
+        assert torch.equal(oa.norm, ob.norm)
+        for p, q in zip(a, b):
+            assert torch.equal(p, q)
+            for name in ("exp_avg", "exp_avg_sq", "scales"):
+                assert torch.equal(oa.state[p][name].view(torch.uint8), ob.state[q][name].view(torch.uint8))
+
+
+def test_places_of_the_draws(cuda):
+    """A parameter's codes are those of its place, beside others or alone; lists of 130 make holes of several launches."""
+    n, some = 130, [0, 1, 57, 58, 129]
+    whole, parts = (Case(cuda, torch.float32, [(300 + i,) for i in range(n)], 8) for _ in range(2))
+    for c in (whole, parts):
+        c.counter.fill_(0)
+    whole.step(seed=5)
+    pick = lambda l: [l[i] for i in some]
+    ops.adamw_step(*(pick(l) for l in (parts.p, parts.g, parts.m, parts.s)), parts.counter, scales=pick(parts.scales), seed=5,
+                   places=some, **HYPER)
+    for a, b in ((whole.p, parts.p), (whole.m, parts.m), (whole.s, parts.s), (whole.scales, parts.scales)):
+        assert all(torch.equal(x.view(torch.uint8), y.view(torch.uint8)) for x, y in zip(pick(a), pick(b)))
+    assert parts.counter.tolist() == whole.counter.tolist() and parts.counter[1] == 0
+    for bad in ([0], [0, 0], [1, 0], [-1, 0], [0, 1 << 20]):
+        with pytest.raises(ValueError, match="places"):
+            ops.adamw_step(parts.p[:2], parts.g[:2], parts.m[:2], parts.s[:2], parts.counter, scales=parts.scales[:2], lr=0.1,
+                           places=bad)

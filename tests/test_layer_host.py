@@ -306,3 +306,19 @@ def test_recordings_that_a_replay_would_undo_are_refused(monkeypatch):
     recording[0] = True
     o.step()
     assert len(r.steps) == 2 and o.state[p[1]]["step"] is not one
+
+
+def test_codes_are_drawn_by_parameters_not_by_launches(monkeypatch):
+    r = Recorder(monkeypatch)
+    p = [torch.ones(4, requires_grad=True, dtype=torch.bfloat16 if i in (1, 4) else torch.float32) for i in range(6)]
+    o = optim.AdamW([dict(params=p[:5]), dict(params=p[5:])], bits=8, seed=3)
+    _with_grads(*p)
+    o.step()
+    everywhere = [(s["seed"], s["places"]) for s in r.steps]
+    assert everywhere == [(3000009, [0, 1, 2]), (3000010, [0, 1]), (3000009 + 8191, [0])]
+    p[2].grad = p[4].grad = None
+    o.step()
+    assert [(s["seed"], s["places"]) for s in r.steps[3:]] == [(3000009, [0, 2]), (3000010, [0]), (3000009 + 8191, [0])]
+    _with_grads(*p)
+    o.step()
+    assert {(s["seed"], i) for s in r.steps[6:] for i in s["places"]} == {(s, i) for s, l in everywhere for i in l}
