@@ -31,7 +31,11 @@ class AdamW(torch.optim.Optimizer):
     A step can be recorded into a graph (its gradients' addresses are part of
     it) once the states are made, by a first step or ``init_states()``; a
     recording that would make states, or part the count of steps of parameters
-    without a gradient from others', is refused."""
+    without a gradient from others', is refused.
+
+    Parameters of a type in a group take one launch for each count of steps among
+    them: those that miss gradients in turns have counts of their own, which are
+    read back and joined again where a step takes more than 32 launches."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 0.01,
                  bits: int = 32, max_norm: Optional[float] = None, masters: bool = True, seed: int = 0):
@@ -50,6 +54,10 @@ class AdamW(torch.optim.Optimizer):
     def __getstate__(self):
         """What copies and pickles hold, the optimiser's own settings among it."""
         return {**super().__getstate__(), **{k: getattr(self, k) for k in ("bits", "max_norm", "masters", "seed", "norm")}}
+
+    # Launches of a step before counters are looked through for equal ones (twice those that there
+    # are at least), and whether a graph holds their addresses.
+    _apart, _recorded = 32, False
 
     # ------------------------------------------------------------ states ----
     def _init(self, p: torch.Tensor, counter: torch.Tensor) -> Dict[str, torch.Tensor]:
@@ -112,6 +120,22 @@ class AdamW(torch.optim.Optimizer):
                     s["step"] = copies[id(shared)]
         return list(sets.values())
 
+    def _rejoin(self) -> None:
+        """Counters of a group's parameters of a type that are equal become one.  Reads them back:
+        the one place where a step waits for the GPU, where more launches than ``_apart``
+        would take longer."""
+        held = {id(s["step"]): s["step"] for s in self.state.values() if s}
+        count: Dict[int, int] = {}
+        for device in {c.device for c in held.values()}:
+            mine = [c for c in held.values() if c.device == device]
+            count.update(zip(map(id, mine), torch.stack(mine)[:, 0].tolist()))
+        shared: Dict[tuple, torch.Tensor] = {}
+        for k, group in enumerate(self.param_groups):
+            for p in group["params"]:
+                s = self.state.get(p)
+                if s:
+                    s["step"] = shared.setdefault((k, p.device, p.dtype, count[id(s["step"])]), s["step"])
+
     def _places(self, group, ps: List[torch.Tensor]):
         """Where the group's first parameter like ``ps`` is, and the places of ``ps``
         among those like them: codes are drawn alike however launches divide them."""
@@ -130,7 +154,12 @@ class AdamW(torch.optim.Optimizer):
                 loss = closure()
         if torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing():
             self._check_recording()
+            self._recorded = True
         launches = [(k, group, ps) for k, group in enumerate(self.param_groups) for ps in self._launches(group)]
+        if len(launches) > self._apart and not self._recorded:
+            self._rejoin()
+            launches = [(k, group, ps) for k, group in enumerate(self.param_groups) for ps in self._launches(group)]
+            self._apart = max(AdamW._apart, 2 * len(launches))
         self.norm = None
         if self.max_norm is not None and len(launches) > 1:
             alike: Dict[tuple, List[torch.Tensor]] = {}   # (in the parameters' order, whatever the launches)

@@ -3,6 +3,7 @@
 import copy
 import ctypes
 import io
+import random
 
 import pytest
 import torch
@@ -322,3 +323,49 @@ def test_codes_are_drawn_by_parameters_not_by_launches(monkeypatch):
     _with_grads(*p)
     o.step()
     assert {(s["seed"], i) for s in r.steps[6:] for i in s["places"]} == {(s, i) for s, l in everywhere for i in l}
+
+
+def test_counts_that_are_equal_again_share_a_launch(monkeypatch):
+    """Gradients missing in turns part the counts of steps; launches stay few, and each parameter's own count."""
+    r = Recorder(monkeypatch)
+    rng = random.Random(1)
+    p = [torch.ones(4, requires_grad=True) for _ in range(60)]
+    o = optim.AdamW([dict(params=p[:50]), dict(params=p[50:])])
+    o.init_states()
+    counts, most = [0] * len(p), 0
+    for _ in range(40):
+        for i, q in enumerate(p):
+            q.grad = None if rng.random() < 0.2 else torch.ones_like(q)
+            counts[i] += q.grad is not None
+        before = len(r.steps)
+        o.step()
+        most = max(most, len(r.steps) - before)
+        assert [int(o.state[q]["step"][0]) for q in p] == counts
+        kinds = len({(i < 50, c) for i, c in enumerate(counts)})
+        assert len(r.steps) - before <= max(32, 2 * kinds)
+    assert most > 8          # (they did part)
+    for g in o.param_groups:   # no count is of two groups
+        mine = {id(o.state[q]["step"]) for q in g["params"]}
+        assert not mine & {id(o.state[q]["step"]) for h in o.param_groups if h is not g for q in h["params"]}
+
+
+def test_counts_of_a_recorded_step_stay_its_own(monkeypatch):
+    """A graph goes on writing to the counters that it was recorded with."""
+    Recorder(monkeypatch)
+    p = _with_grads(*(torch.ones(4, requires_grad=True) for _ in range(80)))
+    o = optim.AdamW(p)
+    for i in range(80):       # every parameter alone
+        for k, q in enumerate(p):
+            q.grad = torch.ones_like(q) if k == i else None
+        o._apart = 1000
+        o.step()
+    _with_grads(*p)
+    monkeypatch.setattr(torch.cuda, "is_initialized", lambda: True)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    o._apart = 1
+    o.step()
+    held = [o.state[q]["step"] for q in p]
+    assert len({id(c) for c in held}) == 80
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    o.step()
+    assert all(o.state[q]["step"] is c for q, c in zip(p, held))
