@@ -80,11 +80,10 @@ __device__ __forceinline__ int tensor_of(const Tensors<E>& ts, int unit) {
 }
 
 // ------------------------------------------------------------------- norm ----
-// Sums of squares, a workgroup's in double (each thread's of a unit in the
-// type's sums), then the last workgroup to finish adds them in order.
-template <typename S>
-__device__ __forceinline__ double over_wg(S v, double* lds) {
-  double d = (double)v;
+// Sums of squares in double (a float32 square has no room for values past 2^64 or
+// below 2^-63, whose norm has), a workgroup's, then the last workgroup to finish
+// adds them in order.
+__device__ __forceinline__ double over_wg(double d, double* lds) {
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) d += __shfl_xor(d, o, 64);
   __syncthreads();
@@ -109,7 +108,7 @@ __global__ __launch_bounds__(WG) void k_grad_norm(Tensors<Gradient> ts, double* 
     const int64_t i0 = (int64_t)(unit - ts.first[k]) * UNIT, left = ts.t[k].n - i0;
     const int n = (int)(left < UNIT ? left : UNIT);
     g += i0;
-    S s = 0;
+    double s = 0;
     if (((uintptr_t)g & 15) == 0 && n == UNIT) {
       row_vec_t<T, W> v[UNIT / WG / W];
 #pragma unroll
@@ -119,12 +118,12 @@ __global__ __launch_bounds__(WG) void k_grad_norm(Tensors<Gradient> ts, double* 
         S a[W];
         row_widen<T, W>(v[i], a);
 #pragma unroll
-        for (int e = 0; e < W; ++e) s += a[e] * a[e];
+        for (int e = 0; e < W; ++e) s += (double)a[e] * (double)a[e];
       }
     } else {
-      for (int i = (int)threadIdx.x; i < n; i += WG) s += (S)g[i] * (S)g[i];
+      for (int i = (int)threadIdx.x; i < n; i += WG) s += (double)g[i] * (double)g[i];
     }
-    sum += (double)s;
+    sum += s;
   }
   const double total = over_wg(sum, lds);
   if (threadIdx.x == 0) {

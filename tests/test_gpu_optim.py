@@ -523,3 +523,16 @@ def test_places_of_the_draws(cuda):
         with pytest.raises(ValueError, match="places"):
             ops.adamw_step(parts.p[:2], parts.g[:2], parts.m[:2], parts.s[:2], parts.counter, scales=parts.scales[:2], lr=0.1,
                            places=bad)
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16], ids=ids)
+@pytest.mark.parametrize("size", [1e30, 1e-30])
+def test_norms_whose_squares_have_no_float32(cuda, dt, size):
+    g = [(_rand((n,), n) * size).to(dt).to(cuda) for n in (4096, 5000, 3)]
+    want = torch.cat([t.cpu().double() for t in g]).norm()
+    # squares and sums are doubles': the norm is rounded once
+    R.assert_within(ops.grad_norm(g), want, want * (1 + 2.0 ** -20) * 2.0 ** -24, "norm")
+    c = Case(cuda, torch.float32, [(4096,)])
+    c.g[0].fill_(1e30)
+    before = c.p[0].clone()
+    assert torch.isfinite(c.step(max_norm=1.0)) and not torch.equal(before, c.p[0]) and torch.isfinite(c.p[0]).all()
