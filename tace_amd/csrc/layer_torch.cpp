@@ -379,6 +379,35 @@ Tensor grad_norm(const Tensors& grads, bool timed) {
   return norm_of(table, grads[0], ticket.data_ptr<int64_t>(), timed);
 }
 
+// What a step writes shares no memory, and none with what it reads.
+void want_apart(const std::vector<tace_adam_tensor>& table, at::ScalarType type, at::ScalarType wide, bool eight) {
+  typedef std::pair<uintptr_t, uintptr_t> Span;   // first byte, end
+  std::vector<Span> written;
+  written.reserve(table.size() * 4);
+  const int64_t b = (int64_t)c10::elementSize(type), state = eight ? 1 : (int64_t)c10::elementSize(wide);
+  auto add = [&](const void* p, int64_t bytes) {
+    if (p && bytes) written.emplace_back((uintptr_t)p, (uintptr_t)p + (uintptr_t)bytes);
+  };
+  for (const auto& t : table) {
+    add(t.p, t.n * b);
+    add(t.m, t.n * state);
+    add(t.s, t.n * state);
+    add(t.master, t.n * 4);
+    add(t.scales, (t.n + TACE_ADAM_BLOCK - 1) / TACE_ADAM_BLOCK * 8);
+  }
+  std::sort(written.begin(), written.end());
+  for (size_t i = 1; i < written.size(); ++i)
+    TORCH_CHECK_VALUE(written[i - 1].second <= written[i].first,
+                      "adamw_step: parameters or states overlap (or one is given twice)");
+  for (const auto& t : table) {
+    if (t.n == 0) continue;
+    const uintptr_t g = (uintptr_t)t.g;
+    const auto after = std::lower_bound(written.begin(), written.end(), Span(g + (uintptr_t)(t.n * b), 0));
+    TORCH_CHECK_VALUE(after == written.begin() || std::prev(after)->second <= g,
+                      "adamw_step: a gradient overlaps a parameter or state");
+  }
+}
+
 optional<Tensor> adamw_step(const Tensors& params, const Tensors& grads, const Tensors& ms, const Tensors& ss,
                             const Tensor& counter, double lr, const optional<Tensor>& lr_at, double beta1, double beta2,
                             double eps, double decay, const optional<Tensors>& scales,
@@ -414,8 +443,6 @@ optional<Tensor> adamw_step(const Tensors& params, const Tensors& grads, const T
   }
   Tensors held;
   std::vector<tace_adam_tensor> table(n);
-  std::vector<const void*> seen;
-  seen.reserve(n);
   int64_t total = 0;
   for (size_t i = 0; i < n; ++i) {
     const Tensor& p = params[i];
@@ -437,11 +464,9 @@ optional<Tensor> adamw_step(const Tensors& params, const Tensors& grads, const T
     const Tensor g = gradient_of(grads[i], p, held, i);
     table[i] = {p.data_ptr(), g.const_data_ptr(), ms[i].data_ptr(), ss[i].data_ptr(),
                 masters ? (*masters)[i].data_ptr() : nullptr, scales ? (*scales)[i].data_ptr() : nullptr, count};
-    if (count) seen.push_back(table[i].p);
     total += count;
   }
-  std::sort(seen.begin(), seen.end());
-  TORCH_CHECK_VALUE(std::adjacent_find(seen.begin(), seen.end()) == seen.end(), "adamw_step: a parameter is given twice");
+  want_apart(table, type, wide, scales.has_value());
   if (total == 0) return max_norm ? optional<Tensor>(at::zeros({}, first.options().dtype(wide).requires_grad(false)))
                                   : std::nullopt;
   Tensor norm;

@@ -536,3 +536,19 @@ def test_norms_whose_squares_have_no_float32(cuda, dt, size):
     c.g[0].fill_(1e30)
     before = c.p[0].clone()
     assert torch.isfinite(c.step(max_norm=1.0)) and not torch.equal(before, c.p[0]) and torch.isfinite(c.p[0]).all()
+
+
+def test_tensors_that_overlap_are_refused(cuda):
+    c = Case(cuda, torch.float32, [(300,), (300,)])
+    flat = torch.zeros(1000, device=cuda)
+    def call(**over):
+        a = {**dict(params=c.p, grads=c.g, exp_avgs=c.m, exp_avg_sqs=c.s), **over}
+        return ops.adamw_step(*(a[k] for k in ("params", "grads", "exp_avgs", "exp_avg_sqs")), c.counter, lr=1e-3)
+    pair = [flat[:300], flat[299:599]]
+    for over in (dict(params=pair), dict(exp_avgs=pair), dict(exp_avg_sqs=pair), dict(exp_avgs=c.s), dict(exp_avgs=[c.m[0], c.m[0]]),
+                 dict(exp_avg_sqs=c.p), dict(grads=[c.m[0], c.g[1]]), dict(params=[flat[:300], c.p[1]], grads=[flat[1:301], c.g[1]])):
+        with pytest.raises(ValueError, match="overlap|given twice"):
+            call(**over)
+    assert c.counter.tolist() == [6, 0] and not flat.any()
+    call(grads=[c.g[0], c.g[0]])                                       # (gradients are read only)
+    call(params=[flat[:300], flat[300:600]], grads=[flat[600:900], flat[600:900]])
