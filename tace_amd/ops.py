@@ -1676,10 +1676,13 @@ def expert_linear(x: torch.Tensor, weight: torch.Tensor, plan: RoutePlan, scale:
 def expert_weights_e4m3(weight: torch.Tensor, scale: float = 1.0) -> Tuple[torch.Tensor, torch.Tensor]:
     """``scale weight`` [E, K, N] as ``expert_linear_e4m3`` reads it, laid out
     once: codes float8_e4m3fn [E, N, K] and their scales float32 [E, N]
-    (largest magnitude of a column / 448)."""
+    (largest magnitude of a column / 448).  A column with a NaN or an infinity is
+    NaN; one below 2^-100 is zeros under scale 0."""
     w = weight.detach().float().transpose(1, 2) * scale
     top = w.abs().amax(2)
-    codes = (w * torch.where(top > 0, 448 / top, torch.zeros_like(top)).unsqueeze(2)).to(torch.float8_e4m3fn)
+    zeros = torch.zeros_like(top)
+    top = torch.where(top < 2.0 ** -100, zeros, top)   # (a NaN stays)
+    codes = (w * torch.where(top == 0, zeros, 448 / top).unsqueeze(2)).to(torch.float8_e4m3fn)
     return codes.contiguous(), top / 448
 
 

@@ -369,3 +369,16 @@ def test_counts_of_a_recorded_step_stay_its_own(monkeypatch):
     monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
     o.step()
     assert all(o.state[q]["step"] is c for q, c in zip(p, held))
+
+
+def test_weights_of_8_bits_below_float32s_quotients_are_zeros():
+    """448 / top overflows below 2^-118: codes were NaN. Such a column is zeros under scale 0, as a normed row is."""
+    w = torch.zeros(2, 4, 3)
+    w[0, 1:, 0], w[0, 2, 1], w[0, 3, 2] = 2.0 ** -125, -(2.0 ** -101), 2.0 ** -100
+    w[1, 0, 0], w[1, :, 1] = float("nan"), float("inf")
+    codes, scales = ops.expert_weights_e4m3(w)
+    least = torch.tensor(2.0 ** -100 / 448).item()     # (rounded to float32, as scales are)
+    assert not codes[0, :2].float().any() and scales[0].tolist() == [0, 0, least]
+    assert codes[0, 2].float().tolist() == [0, 0, 0, 448]
+    assert torch.isnan(codes[1, 0].float() * scales[1, 0]).all() and torch.isnan(codes[1, 1].float() * scales[1, 1]).all()
+    assert not codes[1, 2].float().any() and scales[1, 2] == 0
