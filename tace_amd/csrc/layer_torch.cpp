@@ -269,8 +269,9 @@ Tensor expert_linear(const Tensor& x, const Tensor& weight, const Tensor& rowptr
   TORCH_CHECK_VALUE(ok, "expert_linear: components ", components, " are not 1 to ", TACE_ROW_MAX_BLOCKS,
                     " blocks of 1 to 1024");
   const int64_t B = a.blocks();
-  TORCH_CHECK_VALUE(weight.scalar_type() == x.scalar_type() && weight.size(0) == a.experts &&
-                    ((B == 1 && weight.dim() == 3) || (weight.dim() == 4 && weight.size(1) == B)),
+  TORCH_CHECK_VALUE(weight.scalar_type() == x.scalar_type() &&
+                    ((B == 1 && weight.dim() == 3) || (weight.dim() == 4 && weight.size(1) == B)) &&
+                    weight.size(0) == a.experts,
                     "weight is ", weight.scalar_type(), " ", weight.sizes(), ", expected ", x.scalar_type(), " [",
                     a.experts, ", ", B, ", K, N]", B == 1 ? " or [E, K, N]" : "");
   want_device(weight, x, "weight");
@@ -299,7 +300,8 @@ Tensor expert_linear_e4m3(const Tensor& q, const Tensor& q_scale, const Tensor& 
   const int64_t N = w.size(1), K = w.size(2);
   TORCH_CHECK_VALUE(q.scalar_type() == at::kFloat8_e4m3fn && q.dim() == 2 && q.size(0) == from && q.size(1) == K, "q is ",
                     q.scalar_type(), " ", q.sizes(), ", expected float8_e4m3fn [", from, ", ", K, "]");
-  TORCH_CHECK_VALUE(q_scale.scalar_type() == at::kFloat && q_scale.numel() == from && q_scale.size(0) == from,
+  TORCH_CHECK_VALUE(q_scale.scalar_type() == at::kFloat && q_scale.dim() >= 1 && q_scale.numel() == from &&
+                    q_scale.size(0) == from,
                     "q_scale is ", q_scale.scalar_type(), " ", q_scale.sizes(), ", expected float32 [", from, "]");
   TORCH_CHECK_VALUE(w_scale.scalar_type() == at::kFloat && w_scale.dim() == 2 && w_scale.size(0) == E &&
                     w_scale.size(1) == N, "w_scale is ", w_scale.scalar_type(), " ", w_scale.sizes(),

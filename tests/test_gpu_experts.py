@@ -620,3 +620,17 @@ def test_a_step_of_nan_takes_no_longer(cuda):
         took = _time(lambda: step(*args))
         print(name, took, "of", usual, "ms")
         assert took < 20 * usual, name
+
+
+def test_tensors_without_axes_are_refused_by_name(cuda):
+    plan = _plan(cuda, torch.tensor([0]), 1)
+    one = torch.ones((), device=cuda)
+    q, qs = (t.to(cuda) for t in _codes(torch.ones(1, 16)))
+    w8, ws = (t.to(cuda) for t in _codes(torch.ones(1, 8, 16)))
+    for call, text in [(lambda: ops.expert_linear(one.view(1, 1), one, plan), "weight is"),
+                       (lambda: ops.expert_linear(one, one.view(1, 1, 1), plan), "x has shape"),
+                       (lambda: ops.expert_linear_e4m3(q, one, w8, ws, plan), "q_scale is"),
+                       (lambda: ops.rms_norm(one, one.view(1)), "x has shape"),
+                       (lambda: ops.rms_norm(one.view(1), one), "weight is")]:
+        with pytest.raises(ValueError, match=text):
+            call()
