@@ -81,7 +81,6 @@ __device__ __forceinline__ bool large_result(int64_t bytes) { return bytes >= ((
 struct Place {
   int64_t first;    // row of the stacked blocks
   int64_t count;    // rows of the group from there on
-  int64_t part;     // slots of the group before this one
   int expert, block;
 };
 
@@ -120,9 +119,7 @@ __device__ __forceinline__ int up_to_lane(int v) {
 
 // Numbers the slots of 2^shift rows of all groups without gaps and finds a slot's
 // group, a slot a lane: 64 groups at a time are in the lanes, with the sum of their
-// slots up to each.  Groups of a block: the experts and, with DROPPED, the
-// dropped rows as one more; EMPTY: a group without rows has a slot all the same.
-template <bool DROPPED, bool EMPTY>
+// slots up to each.  Groups of a block: the experts and the dropped rows.
 struct Places {
   const Groups& gr;
   int shift, n, base;   // base: the first group in the lanes
@@ -130,11 +127,11 @@ struct Places {
   int upto;             // slots of the lanes' groups up to this one
 
   __device__ __forceinline__ Places(const Groups& gr, int shift)
-      : gr(gr), shift(shift), n((gr.experts + (DROPPED ? 1 : 0)) * gr.blocks) {
+      : gr(gr), shift(shift), n((gr.experts + 1) * gr.blocks) {
     take(0);
   }
   __device__ __forceinline__ void take(int at) {
-    const int lane = (int)threadIdx.x & 63, per = gr.experts + (DROPPED ? 1 : 0), g = at + lane;
+    const int lane = (int)threadIdx.x & 63, per = gr.experts + 1, g = at + lane;
     base = at;
     from = to = 0;
     int slots = 0;
@@ -143,7 +140,7 @@ struct Places {
       const int64_t block0 = gr.rows * gr.before[b];
       from = block0 + gr.comps[b] * gr.end_of(e);
       to = block0 + gr.comps[b] * gr.end_of(e + 1);
-      slots = to > from ? (int)((to - from + ((int64_t)1 << shift) - 1) >> shift) : EMPTY ? 1 : 0;
+      slots = to > from ? (int)((to - from + ((int64_t)1 << shift) - 1) >> shift) : 0;
     }
     upto = up_to_lane(slots);
   }
@@ -159,8 +156,8 @@ struct Places {
     return sum;
   }
   __device__ __forceinline__ Place place(int g, int64_t part, int64_t f, int64_t t) const {
-    const int per = gr.experts + (DROPPED ? 1 : 0), b = g / per;
-    return Place{f + (part << shift), t - f - (part << shift), part, g - b * per, b};
+    const int per = gr.experts + 1, b = g / per;
+    return Place{f + (part << shift), t - f - (part << shift), g - b * per, b};
   }
   // a slot that is the same in all lanes
   __device__ __forceinline__ Place find_one(int slot) {
@@ -173,11 +170,11 @@ struct Places {
       }
       before += last();
     }
-    return Place{0, 0, 0, gr.experts, 0};
+    return Place{0, 0, gr.experts, 0};
   }
   // each lane's own (every lane of the wavefront calls it); slots behind the last give a place without rows
   __device__ __forceinline__ Place find(int slot) {
-    Place p{0, 0, 0, gr.experts, 0};
+    Place p{0, 0, gr.experts, 0};
     int before = 0;
     for (int at = 0; at < n; at += 64) {
       if (n > 64) take(at);
@@ -1102,13 +1099,13 @@ __global__ __launch_bounds__(64 * WM * WN, waves_for(FM * FN)) void k_expert_row
     const T* __restrict__ x, const T* __restrict__ weight, Groups gr, int64_t wsize, int sum, int n, row_sum_t<T> scale,
     T* __restrict__ out, int cols) {
   constexpr int TM = 16 * WM * FM, TN = 16 * WN * FN;
-  const int slots = Places<true, false>(gr, __builtin_ctz(TM)).total();
+  const int slots = Places(gr, __builtin_ctz(TM)).total();
   walk<T, false, BT, WM, WN, FM, FN, FAST>(
       x, weight, sum, BT ? n : sum, share_of(slots * cols), large_result(gr.rows * total_comps(gr) * n * (int)sizeof(T)),
       [&](int t) {   // (asked for again for every 64 tiles: nothing of it stays in registers)
         int slot, col;
         blocked(t, slots, cols, &slot, &col);
-        const Place p = Places<true, false>(gr, __builtin_ctz(TM)).find(slot);
+        const Place p = Places(gr, __builtin_ctz(TM)).find(slot);
         const int c0 = col * TN;
         return Job{p.first * sum,
                    ((int64_t)p.expert * gr.blocks + p.block) * wsize + (BT ? (int64_t)c0 : (int64_t)c0 * sum),
@@ -1297,7 +1294,7 @@ __global__ __launch_bounds__(WG) void k_expert_codes(const E4m3* __restrict__ x,
   __shared__ int rows[TM];
   const int t = tile_of(tiles);
   if (t < 0) return;
-  const Place p = Places<true, false>(gr, __builtin_ctz(TM)).find_one(t / cols);
+  const Place p = Places(gr, __builtin_ctz(TM)).find_one(t / cols);
   if (p.count <= 0) return;
   const int c0 = t % cols * TN, m = (int)min(p.count, (int64_t)TM), nn = n - c0;
   O* o = out + p.first * n + c0;
