@@ -7,10 +7,11 @@
 //   p = p (1 - lr decay) - lr / (1 - b1^t) m / (sqrt(v / (1 - b2^t)) + eps)
 //
 // Bound by HBM: each operand is read once and written once (a gradient twice
-// where it is clipped).  The tensors' addresses travel with the launch, as many as
-// its 4 KB of arguments hold (56; 84 without masters and scales, 160 for norms), so
-// a step over new gradients copies nothing ahead of it and a recorded one replays;
-// a workgroup finds its tensor by ballots over the tensors' first units.
+// where it is clipped).  The tensors' addresses travel with the launch, within its 4
+// KB of arguments (84 tensors come near them; 56 with masters and scales and 160 for
+// norms leave 600 and 800 bytes), so a step over new gradients copies nothing ahead of
+// it and a recorded one replays; a workgroup finds its tensor by ballots over the
+// tensors' first units.
 //
 // States of 8 bits: m and r = sqrt(v) as e4m3 codes, 256 elements to a float32
 // scale (the block's largest magnitude / 448): r has half the range of v, and
@@ -19,7 +20,9 @@
 // stay where it is under rounding to nearest, so codes are rounded up with the
 // probability of the value's distance from the one below: from 16 bits of
 // Philox-4x32 on (position / 4, tensor, step), half a word for each of m and r.
-// A positive r never becomes code zero (it is divided by).
+// A positive r never becomes code zero (it is divided by).  The draw has r's mean, so
+// v = r^2 gains r's variance: under normal gradients and b2 = 0.999 v settles 5.5 %
+// above its exact average (steps 2.7 % shorter), one element in a hundred at twice it.
 #include "philox.h"
 #include "row_types.h"
 

@@ -24,15 +24,19 @@
 // either read meets every bank once.  Sums are float32 (double for float64).
 //
 // e4m3 codes are multiplied as the bfloat16 of the same value.  The MFMA of 8-bit
-// codes has twice the rate, but aligns the products it adds to few bits: off by up
-// to 2^-11.9 of the largest product for random codes of all exponents and 2^-17 of
-// the sum of magnitudes for normally distributed ones, 16 x 16 x 128 and 16 x 16 x
-// 32 alike.  Few tokens are bound by reading the weights, which either form does
-// once: 24 tokens, 2 of 16 experts each, 1024 x 4096: 15 us, 4.5 TB/s.
+// codes has up to three times the rate (library products of 8192 cubed: 3,214 and 1,066
+// TFLOP/s), but aligns the products it adds to few bits: off by up to 2^-11.9 of the
+// largest product for random codes of all exponents and 2^-17 of the sum of magnitudes
+// for normally distributed ones, 16 x 16 x 128 and 16 x 16 x 32 alike.  An output of
+// float32 would show either, one of 16 bits the first; prompts pay for it: 8,000
+// tokens, 2 of 16 experts each, 1024 x 4096, 243 us (552 TFLOP/s, registers in between).
+// Few tokens are bound by reading the weights, which either form does once: 24 tokens
+// there 15.5 us, 16.4 as calls in a row with the weights in the caches, 17.5 (3.9
+// TB/s) where ten layers' weights take turns.
 //
 // Measured, us (forward, rows' gradient, weights' gradient): bfloat16, 32,768 rows
 // of 8 experts of 1024 x 2048: 187, 178, 176 + 19 (137 GFLOP each; 735, 772 and 705
-// TFLOP/s, from caches that hold other data; 950 forward from warm ones); 202,752
+// TFLOP/s, from caches that hold other data; 950 forward from warm ones); 202,612
 // rows of 16 experts of 256 x 512, bound by memory and the latency of four steps a
 // tile: 109, 90, 75 + 14 (311 MB each, 2.9 to 3.5 TB/s).  float32, 196,608 rows of
 // 128 x 128 (its three terms' MFMA takes as long as the memory): 66, 67, 54 + 15.
@@ -72,9 +76,10 @@ struct Groups {
 
 __host__ __device__ inline int total_comps(const Groups& gr) { return gr.before[gr.blocks - 1] + gr.comps[gr.blocks - 1]; }
 
-// Whether a result of so many bytes is stored past the caches (nt): they hold 256 MB,
-// so the next kernel finds little of as much in them, while it takes the place of
-// what is read again.  202,752 rows of 256 x 512 in bfloat16 (207 MB forward, 104
+// Whether a result of so many bytes is stored past the caches (nt; streamed products
+// alone): they hold 256 MB, so the next kernel finds little of as much in them, while it
+// takes the place of what is read again.  (Measured at 104 and 207 MB; a quarter of the
+// caches is a guess for what is between.)  202,612 rows of 256 x 512 in bfloat16 (207 MB forward, 104
 // back): a forward and backward pass 271 us, 287 without.
 __device__ __forceinline__ bool large_result(int64_t bytes) { return bytes >= ((int64_t)64 << 20); }
 
@@ -1389,7 +1394,7 @@ void with_tile(int tile, F&& f) {
 }
 
 // The weight gradient's tiles, by the same rule: 2,048 rows of 128 x 128 in float32
-// take 22 us with 128 x 128 and 16 with 64 x 64, 196,608 rows 72 and 74; 202,752
+// take 22 us with 128 x 128 and 16 with 64 x 64, 196,608 rows 72 and 74; 202,612
 // rows of 256 x 512 in bfloat16 96 and 149.  Many experts' matrices take the large
 // ones too: most of the time goes to storing them.
 int64_t tiles_of(int tile, int K, int N) {
