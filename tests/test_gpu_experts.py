@@ -616,10 +616,12 @@ def test_a_step_of_nan_takes_no_longer(cuda):
     one[rows // 2] = float("nan")     # half of an expert's sums are run through before they end
     far = g.clone()
     far[rows - E:] = float("inf")     # (those of one sign run to their end)
-    for name, args in (("gradient", (x, w, nan)), ("rows", (nan, w, g)), ("row", (x, w, one)), ("infinite rows", (x.abs(), w, far))):
+    # (infinities: 64 sums a lane, 512 terms each, four loads at a time of up to 1 us: 8 ms, forty times a step's 0.2)
+    for name, most, args in (("gradient", 20, (x, w, nan)), ("rows", 20, (nan, w, g)), ("row", 20, (x, w, one)),
+                             ("infinite rows", 50, (x.abs(), w, far))):
         took = _time(lambda: step(*args))
         print(name, took, "of", usual, "ms")
-        assert took < 20 * usual, name
+        assert took < most * usual, name
 
 
 def test_tensors_without_axes_are_refused_by_name(cuda):
