@@ -68,6 +68,13 @@ __device__ __forceinline__ S over_row(S v, S* lds) {
   return v;
 }
 
+// Waves a SIMD of rows to 8 bits, where the compiler would take a few registers more
+// than they leave (one is spilled at most): 60,000 float32 rows of degrees 0 to 3, 128
+// channels, with residual 304 us, 336 without.
+constexpr int code_waves(int V, int LPR, int NV) {
+  return LPR == 64 && NV == 4 ? (V == 4 ? 5 : V == 8 ? 4 : 1) : 1;
+}
+
 // V values as e4m3 codes, to nearest even (|v| <= 448 but for rounding; NaN stays)
 template <int V>
 __device__ __forceinline__ void store_codes(unsigned char* p, const float* v) {
@@ -111,7 +118,7 @@ __device__ __forceinline__ void lane_weights(const void* weight, bool wide, int 
 
 // Q: y as e4m3 codes with scales [rows, blocks]
 template <typename T, int V, int LPR, int NV, bool Q>
-__global__ __launch_bounds__(LPR > WG ? LPR : WG) void k_rms_fwd(
+__global__ __launch_bounds__(LPR > WG ? LPR : WG, Q ? code_waves(V, LPR, NV) : 1) void k_rms_fwd(
     const T* __restrict__ x, const T* __restrict__ res, const void* __restrict__ weight, bool wide, int64_t rows,
     NormParts pt, row_sum_t<T> eps, T* __restrict__ h, void* __restrict__ y, float* __restrict__ scales,
     row_sum_t<T>* __restrict__ inv) {
@@ -164,11 +171,15 @@ __global__ __launch_bounds__(LPR > WG ? LPR : WG) void k_rms_fwd(
     sum = over_row<LPR, Add>(sum, slots);
     const S q = (S)1 / sqrt(sum / width + eps);
     if (inv && li == 0) inv[r * pt.count + b] = q;
-    // 8 bits: q's power of two alone (over 8), so that h q w of few bits is exact and a
-    // value between two codes is seen to be there, however q was rounded
-    S factor = q;
-    if constexpr (Q) factor = __uint_as_float(__float_as_uint(q) & 0x7f800000u) * 0.125f;
-    S top = 0, den = 0, rcp = 0, seven = 0;
+    // 8 bits: instead of q a power of two near q / 1024, times 448: h w of few bits stays
+    // exact, and a value between two codes is seen to be there, however q was rounded
+    // (but in rows below 2^-60, whose quotients' remainders float32 does not hold).
+    S factor = q, two = 0;
+    if constexpr (Q) {
+      two = __uint_as_float(__float_as_uint(q) & 0x7f800000u) * 0x1p-10f;
+      factor = two * 448;
+    }
+    S top = 0, most = 0, per = 0;
 #pragma unroll
     for (int i = 0; i < NV * V; ++i) {
       a[i] = a[i] * factor * w[i];
@@ -180,17 +191,14 @@ __global__ __launch_bounds__(LPR > WG ? LPR : WG) void k_rms_fwd(
     }
     if constexpr (Q) {
       top = over_row<LPR, Top>(top, slots);
-      const S full = top * (q / factor);   // the row's largest |y|
-      // (below, float32 has no room for what follows: such a row is zeros, as one of zeros)
-      if (top == 0 || full < (S)0x1p-100) top = 0;
-      if (li == 0) scales[r * pt.count + b] = top == 0 ? 0.0f : (float)(full / 448);
-      // 448 a / top rounded once, by a corrected product with the reciprocal: 7 a over top / 64, both
-      // by top's power of two  (a division of its own for each element: 101,306 rows of 256 in bfloat16 41 instead of 37 us)
-      const unsigned ex = __float_as_uint(top) >> 23;   // (an infinity or NaN: 0, and NaN after)
-      const S one = ex == 255 ? (S)0 : __uint_as_float((254 - ex) << 23);
-      den = top * one * (S)0x1p-6;
-      rcp = top == 0 ? (S)0 : 1 / den;
-      seven = top == 0 ? (S)0 : 7 * one;
+      const S full = top * (q / two);   // 448 times the row's largest |y|
+      // (smaller rows are zeros, as those of zeros: near float32's end quotients lose their bits)
+      const bool none = top == 0 || full < (S)(448 * 0x1p-100);
+      if (li == 0) scales[r * pt.count + b] = none ? 0.0f : (float)(full / (448 * 448));
+      // a code is that of a / most, rounded once: by a corrected product with the reciprocal.  (A
+      // division for each element: 101,306 rows of 256 in bfloat16 41 instead of 37 us.)
+      most = none ? (S)0 : top / 448;
+      per = none ? (S)0 : 1 / most;
     }
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -200,8 +208,8 @@ __global__ __launch_bounds__(LPR > WG ? LPR : WG) void k_rms_fwd(
         float v[V];
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-          const float t = (float)(a[i * V + e] * seven), near = t * (float)rcp;
-          v[e] = fmaf(fmaf(-near, (float)den, t), (float)rcp, near);
+          const float t = (float)a[i * V + e], near = t * (float)per;
+          v[e] = fmaf(fmaf(-near, (float)most, t), (float)per, near);
         }
         store_codes<V>((unsigned char*)y + at + (int64_t)idx * V, v);
       } else {
