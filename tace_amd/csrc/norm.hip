@@ -191,10 +191,10 @@ __global__ __launch_bounds__(LPR > WG ? LPR : WG, Q ? code_waves(V, LPR, NV) : 1
     }
     if constexpr (Q) {
       top = over_row<LPR, Top>(top, slots);
-      const S full = top * (q / two);   // 448 times the row's largest |y|
+      const S scale = top / (448 * 448) * (q / two);   // the row's largest |y| / 448
       // (smaller rows are zeros, as those of zeros: near float32's end quotients lose their bits)
-      const bool none = top == 0 || full < (S)(448 * 0x1p-100);
-      if (li == 0) scales[r * pt.count + b] = none ? 0.0f : (float)(full / (448 * 448));
+      const bool none = top == 0 || scale < (S)(0x1p-100 / 448);
+      if (li == 0) scales[r * pt.count + b] = none ? 0.0f : (float)scale;
       // a code is that of a / most, rounded once: by a corrected product with the reciprocal.  (A
       // division for each element: 101,306 rows of 256 in bfloat16 41 instead of 37 us.)
       most = none ? (S)0 : top / 448;

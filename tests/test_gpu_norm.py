@@ -295,3 +295,21 @@ def test_codes_on_borders_go_to_even(cuda, dt, wide, C, comps):
         assert torch.equal(got, torch.round(steps) * _e4m3_step(unit))
         borders += int((steps.frac().abs() == 0.5).sum())
     assert borders > 0
+
+
+def test_codes_of_the_largest_and_smallest_rows(cuda):
+    """Rows at float32's ends: scales are max |y| / 448 as long as those are numbers of 2^-100 and more."""
+    x = _rand((50, 72), torch.bfloat16, 1).float()
+    for size in (2.0 ** 126, 1e37, 1.0, 1e-20, 2.0 ** -98):
+        w = (_rand((72,), torch.float32, 2).abs() + 0.5).clamp(max=1.0) * size
+        x = x / x.abs().amax(1, keepdim=True)
+        x[:, 0], w[0] = 1.0, size               # (the largest |y|: size by a row's factor of 1 to 4)
+        ref = Reference(x, None, w, 1e-6, [1])
+        q, s = ops.rms_norm_e4m3(x.to(cuda), w.to(cuda), 1e-6)
+        top = ref.y.abs().amax(1)
+        held = top < 3.4e38
+        R.assert_within(s[held.to(cuda), 0], (top / 448)[held], (top / 448 * (FACTOR + 4) * 2.0 ** -24)[held], size)
+        unit = ref.y / (s.cpu().double())
+        slack = unit.abs() * (2 * FACTOR + 8) * 2.0 ** -24
+        R.assert_within(q[held.to(cuda)].float(), unit[held], (_e4m3_step(unit + slack) / 2 + slack)[held], size)
+        assert int(held.sum()) >= 10
